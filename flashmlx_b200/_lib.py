@@ -59,6 +59,24 @@ class AttnConfig(C.Structure):
                 ("rope_theta", C.c_float), ("scale", C.c_float), ("norm_eps", C.c_float), ("qkv_ld", C.c_int)]
 
 
+FM_ROPE_UNSCALED, FM_ROPE_LINEAR, FM_ROPE_NTK, FM_ROPE_YARN, FM_ROPE_BANDED = 0, 1, 2, 3, 4
+
+
+class RopeConfig(C.Structure):
+    _fields_ = [("head_dim", C.c_int), ("rotary_dim", C.c_int), ("traditional", C.c_int), ("scaling", C.c_int),
+                ("theta", C.c_float), ("factor", C.c_float), ("original_len", C.c_float), ("low", C.c_float),
+                ("high", C.c_float), ("attn_factor", C.c_float)]
+
+
+class CacheAttnConfig(C.Structure):
+    _fields_ = [("n_heads", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("max_len", C.c_int),
+                ("prefix_max", C.c_int), ("q_ld", C.c_int), ("scale", C.c_float)]
+
+
+class EvictConfig(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("n_kv_heads", "head_dim", "max_len", "out_max_len", "budget", "sinks", "recent")]
+
+
 class KernelTime(C.Structure):
     _fields_ = [("name", C.c_char_p), ("launches", C.c_int64), ("total_ms", C.c_double)]
 
@@ -102,6 +120,13 @@ SIGNATURES = {
     "fm_attention": (_i, [_p, C.POINTER(AttnConfig), _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _p]),
     "fm_swiglu": (_i, [_p, _p, _p, _i64, _p]),
     "fm_argmax": (_i, [_p, _p, _i64, _i64, _p]),
+    "fm_rope": (_i, [_p, C.POINTER(RopeConfig), _p, _i64, _i, _p, _i64, _p, _i64]),
+    "fm_rope_append": (_i, [_p, C.POINTER(RopeConfig), _p, _i64, _i, _p, _p, _i64, _i, _p, _p, _i, _i, _p, _p, _i, _p,
+                            _i64]),
+    "fm_attention_prefix": (_i, [_p, C.POINTER(CacheAttnConfig), _p, _p, _p, _i, _p, _p, _p, _i, _i, _p]),
+    "fm_attention_scored": (_i, [_p, C.POINTER(CacheAttnConfig), _p, _p, _p, _p, _i, _i, _p, _p]),
+    "fm_cache_evict": (_i, [_p, C.POINTER(EvictConfig), _p, _p, _p, _p, _p, _i, _p, _p, _p, _p, _p]),
+    "fm_serve_reserve": (_i, [_p, C.POINTER(CacheAttnConfig), _i, _i]),
 }
 
 _lib = None

@@ -20,6 +20,7 @@
 
 #include "flashmoe.h"
 #include "fm_internal.cuh"
+#include "fm_serve.cuh"
 
 namespace fm {
 __global__ void route_kernel(const RouteArgs a);
@@ -116,6 +117,13 @@ struct fm_handle {
     uint32_t epoch = 0;
     int coop_blocks = 0;  // co-resident blocks of the dispatch kernel
   } p2p;
+  // workspace of the serving calls (fm_attention_prefix, ...): blocks are only added, so a
+  // captured call's pointers stay valid; the first block begins with their error word
+  std::vector<uint8_t*> sv_blocks;
+  uint8_t* sv_ws = nullptr;   // the largest block, past the control bytes
+  size_t sv_bytes = 0;
+  size_t sv_total = 0;        // bytes of all blocks
+  bool sv_ready = false;      // shared-memory opt-in done
   // kernel timing (fm_profile_enable)
   bool profile = false;
   struct Pending {
@@ -234,6 +242,60 @@ int ensure_ws(fm_handle* h, size_t bytes) {
   if (e != cudaSuccess) return cuda_err(h, e, "cudaMemsetAsync");
   return FM_OK;
 }
+
+// the status of a non-zero device error word
+int device_status(fm_handle* h, uint32_t word) {
+  if (word & fm::DEVERR_TIMEOUT) return set_err(h, FM_ETIMEOUT, "a bounded device-side wait ran out");
+  if (word & fm::DEVERR_BOUNDS) return set_err(h, FM_EDEVICE, "an index failed its device-side bounds check");
+  return set_err(h, FM_EDEVICE, "device-side check failed");
+}
+
+// Makes the handle's device current for a call, and the caller's again after it.
+struct OnDevice {
+  int before = -1;
+  explicit OnDevice(const fm_handle* h) {
+    int cur = -1;
+    if (cudaGetDevice(&cur) == cudaSuccess && cur != h->device && cudaSetDevice(h->device) == cudaSuccess) before = cur;
+  }
+  ~OnDevice() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+// The serving calls' workspace: at least `bytes`, and their error word (sv_err).  Blocks are
+// never freed before fm_destroy, and each is at least half as large again as the last.
+int ensure_sv(fm_handle* h, size_t bytes) {
+  if (!h->sv_blocks.empty() && bytes <= h->sv_bytes) return FM_OK;
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(h->stream, &cap);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return cuda_err(h, e, "cudaStreamIsCapturing");
+  }
+  if (cap != cudaStreamCaptureStatusNone)
+    return set_err(h, FM_EINVAL, "the workspace would have to grow during a capture: reserve it first");
+  const size_t want = ws_alloc_bytes(std::max(bytes, h->sv_bytes + h->sv_bytes / 2) + kCtrlBytes);
+  uint8_t* p = nullptr;
+  e = cudaMalloc(&p, want);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_err(h, FM_ENOMEM, std::string("workspace allocation failed: ") + cudaGetErrorString(e));
+  }
+  if (h->sv_blocks.empty()) {
+    e = cudaMemset(p, 0, kCtrlBytes);
+    if (e != cudaSuccess) {
+      cudaFree(p);
+      return cuda_err(h, e, "cudaMemset");
+    }
+  }
+  h->sv_blocks.push_back(p);
+  h->sv_ws = p + kCtrlBytes;
+  h->sv_bytes = want - kCtrlBytes;
+  h->sv_total += want;
+  return FM_OK;
+}
+
+uint32_t* sv_err(fm_handle* h) { return reinterpret_cast<uint32_t*>(h->sv_blocks[0]); }
 
 cudaEvent_t take_event(fm_handle* h) {
   if (!h->event_pool.empty()) {
@@ -828,6 +890,7 @@ int fm_destroy(fm_handle* h) {
   p2p_close(h);
   if (h->ws) cudaFree(h->ws);
   if (h->ep_ws) cudaFree(h->ep_ws);
+  for (uint8_t* b : h->sv_blocks) cudaFree(b);
   delete h;
   return FM_OK;
 }
@@ -858,7 +921,7 @@ int fm_set_route_mode(fm_handle* h, int mode) {
   return FM_OK;
 }
 
-size_t fm_workspace_bytes(const fm_handle* h) { return h ? h->ws_bytes : 0; }
+size_t fm_workspace_bytes(const fm_handle* h) { return h ? h->ws_bytes + h->sv_total : 0; }
 
 int fm_profile_enable(fm_handle* h, int on) {
   if (!h) return FM_EINVAL;
@@ -917,11 +980,17 @@ int fm_sync_status(fm_handle* h) {
   uint32_t word = 0;
   e = cudaMemcpy(&word, h->ws, sizeof(word), cudaMemcpyDeviceToHost);
   if (e != cudaSuccess) return cuda_err(h, e, "cudaMemcpy(error word)");
+  if (!h->sv_blocks.empty()) {
+    uint32_t sv = 0;
+    e = cudaMemcpy(&sv, h->sv_blocks[0], sizeof(sv), cudaMemcpyDeviceToHost);
+    if (e != cudaSuccess) return cuda_err(h, e, "cudaMemcpy(error word)");
+    if (sv) cudaMemset(h->sv_blocks[0], 0, kCtrlBytes);
+    if (sv && !word) return device_status(h, sv);
+    word |= sv;
+  }
   if (word == 0) return FM_OK;
   cudaMemset(h->ws, 0, kCtrlBytes);  // clear the error word and the grid-sync counters
-  if (word & fm::DEVERR_TIMEOUT) return set_err(h, FM_ETIMEOUT, "a bounded device-side wait ran out");
-  if (word & fm::DEVERR_BOUNDS) return set_err(h, FM_EDEVICE, "an index failed its device-side bounds check");
-  return set_err(h, FM_EDEVICE, "device-side check failed");
+  return device_status(h, word);
 }
 
 int fm_reserve(fm_handle* h, const fm_moe_config* c, int64_t max_tokens) {
@@ -1954,6 +2023,313 @@ int fm_argmax(fm_handle* h, const uint16_t* logits, int64_t T, int64_t V, int32_
   const cudaError_t e = fm::launch_argmax(logits, T, V, ids, h->stream);
   prof_end(h);
   return e == cudaSuccess ? FM_OK : cuda_err(h, e, "argmax launch");
+}
+
+// ---------------------------------------------------------------- serving calls (serve.cu)
+
+}  // extern "C"
+
+namespace {
+
+// cfg's frequencies in full turns per position, and the factor on cos and sin
+int rope_args(fm_handle* h, const fm_rope_config* c, fm::RopeArgs* a) {
+  std::memset(a, 0, sizeof(*a));
+  if (!c) return set_err(h, FM_EINVAL, "null config");
+  const int r = c->rotary_dim ? c->rotary_dim : c->head_dim;
+  if (c->head_dim <= 0 || r <= 0 || r % 2 || r > c->head_dim)
+    return set_err(h, FM_EINVAL, "rotary_dim must be even and at most head_dim");
+  if (c->head_dim % 8 || c->head_dim > fm::kRopeMaxDim)
+    return set_err(h, FM_EUNSUPPORTED, "head_dim must be a multiple of 8, at most 256");
+  if (!(c->theta > 0.f) || !std::isfinite(c->theta)) return set_err(h, FM_EINVAL, "theta must be positive");
+  if (c->scaling < FM_ROPE_UNSCALED || c->scaling > FM_ROPE_BANDED) return set_err(h, FM_EINVAL, "unknown scaling");
+  const bool scaled = c->scaling != FM_ROPE_UNSCALED, parts = c->scaling >= FM_ROPE_YARN;
+  if (scaled && !(c->factor >= 1.f && std::isfinite(c->factor))) return set_err(h, FM_EINVAL, "factor must be at least 1");
+  if (parts && !(c->original_len > 0.f && std::isfinite(c->original_len) && c->low > 0.f && c->low < c->high &&
+                 std::isfinite(c->high)))
+    return set_err(h, FM_EINVAL, "original_len and 0 < low < high are needed");
+  if (c->scaling == FM_ROPE_YARN && !(c->theta > 1.f)) return set_err(h, FM_EINVAL, "theta must be above 1");
+  if (c->scaling == FM_ROPE_NTK && r <= 2) return set_err(h, FM_EINVAL, "rotary_dim must be above 2");
+  if (!(c->attn_factor >= 0.f) || !std::isfinite(c->attn_factor)) return set_err(h, FM_EINVAL, "bad attn_factor");
+  const double kTau = 6.283185307179586476925286766559, f = c->factor, n = c->original_len;
+  double base = c->theta;
+  if (c->scaling == FM_ROPE_NTK) base *= std::pow(f, r / (r - 2.0));
+  // FM_ROPE_YARN: the pair that turns `turns` times over original_len
+  auto pair_of = [&](double turns) { return r * std::log(n / (turns * kTau)) / (2 * std::log(base)); };
+  double first = 0, last = 0;
+  if (c->scaling == FM_ROPE_YARN) {
+    first = std::max(std::floor(pair_of(c->high)), 0.0);
+    last = std::min(std::ceil(pair_of(c->low)), r - 1.0);
+  }
+  for (int i = 0; i < r / 2; ++i) {
+    double inv = std::pow(base, -2.0 * i / r);
+    if (c->scaling == FM_ROPE_LINEAR) {
+      inv /= f;
+    } else if (parts) {
+      const double keep = c->scaling == FM_ROPE_YARN ? 1 - (i - first) / std::max(last - first, 0.001)
+                                                     : (n * inv / kTau - c->low) / (c->high - c->low);
+      const double k = std::min(std::max(keep, 0.0), 1.0);
+      inv *= k + (1 - k) / f;
+    }
+    a->turns[i] = inv / kTau;
+  }
+  a->factor = c->attn_factor != 0.f ? c->attn_factor
+              : c->scaling == FM_ROPE_YARN ? static_cast<float>(0.1 * std::log(f) + 1) : 1.f;
+  a->d = c->head_dim;
+  a->rotary = r;
+  a->traditional = c->traditional != 0;
+  a->L = 1;
+  return FM_OK;
+}
+
+bool rows_ok(const void* p, int64_t ld, int64_t cols) { return aligned16(p) && ld >= cols && ld % 8 == 0; }
+
+// the bytes [p, p + n) and [q, q + m) overlap
+bool overlap(const void* p, int64_t n, const void* q, int64_t m) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a < b + m && b < a + n;
+}
+
+size_t evict_bytes(int64_t heads, int64_t budget) { return align_up(sizeof(int32_t) * heads * 2 * budget, 256) + sizeof(int32_t) * heads * 2; }
+
+int check_cache_attn(fm_handle* h, const fm_cache_attn_config* c, int B, int L, int prefix_len) {
+  if (!c) return set_err(h, FM_EINVAL, "null config");
+  if (c->n_heads <= 0 || c->n_kv_heads <= 0 || c->n_heads % c->n_kv_heads || c->max_len < 0 || c->prefix_max < 0)
+    return set_err(h, FM_EINVAL, "bad attention config");
+  if (c->head_dim != 64 && c->head_dim != 128) return set_err(h, FM_EUNSUPPORTED, "head_dim must be 64 or 128");
+  if (!std::isfinite(c->scale)) return set_err(h, FM_EINVAL, "bad scale");
+  if (c->q_ld < 0 || c->q_ld % 8 || (c->q_ld > 0 && c->q_ld < static_cast<int64_t>(c->n_heads) * c->head_dim))
+    return set_err(h, FM_EINVAL, "q_ld must be 0 or a multiple of 8 of at least n_heads * head_dim");
+  if (B < 0 || L < 0 || prefix_len < 0) return set_err(h, FM_EINVAL, "negative B, L or prefix_len");
+  if (prefix_len > c->prefix_max) return set_err(h, FM_EINVAL, "prefix_len exceeds prefix_max");
+  if (static_cast<int64_t>(B) * L > 0x7fffffffLL / c->n_heads || c->n_kv_heads > 65535 || B > 65535)
+    return set_err(h, FM_EUNSUPPORTED, "too many tokens or heads");
+  return FM_OK;
+}
+
+int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, const uint16_t* pk, const uint16_t* pv,
+               int prefix_len, const uint16_t* ck, const uint16_t* cv, const int32_t* lens, int B, int L, float* acc,
+               bool scored, uint16_t* out) {
+  if (!h) return FM_EINVAL;
+  int rc = check_cache_attn(h, c, B, L, prefix_len);
+  if (rc != FM_OK) return rc;
+  if (B == 0 || L == 0) return FM_OK;
+  if (!q || !out || (prefix_len > 0 && (!pk || !pv)) || (lens && (!ck || !cv)) || (scored && (!acc || !lens)))
+    return set_err(h, FM_EINVAL, "null pointer");
+  if (!aligned16(q) || !aligned16(out) || (prefix_len > 0 && (!aligned16(pk) || !aligned16(pv))) ||
+      (lens && (!aligned16(ck) || !aligned16(cv))))
+    return set_err(h, FM_EINVAL, "q, the caches and out must be 16-byte aligned");
+  const int64_t q_ld = c->q_ld ? c->q_ld : static_cast<int64_t>(c->n_heads) * c->head_dim;
+  const int64_t T = static_cast<int64_t>(B) * L, cols = static_cast<int64_t>(c->n_heads) * c->head_dim;
+  if (overlap(q, 2 * ((T - 1) * q_ld + cols), out, 2 * T * cols)) return set_err(h, FM_EINVAL, "out may not overlap q");
+  const OnDevice on(h);
+  if (!h->sv_ready) {
+    const cudaError_t e = fm::cache_attn_init();
+    if (e != cudaSuccess) return cuda_err(h, e, "cache attention kernel set-up");
+    h->sv_ready = true;
+  }
+  const fm::CacheAttnPlan p =
+      fm::cache_attn_plan(B, L, c->n_heads, c->n_kv_heads, c->head_dim, prefix_len, scored, h->num_sms);
+  rc = ensure_sv(h, p.bytes);
+  if (rc != FM_OK) return rc;
+  fm::CacheAttnArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.q = q;
+  a.q_ld = q_ld;
+  a.pk = pk;
+  a.pv = pv;
+  a.p_head = static_cast<int64_t>(c->prefix_max) * c->head_dim;
+  a.ck = ck;
+  a.cv = cv;
+  a.lens = lens;
+  a.out = out;
+  a.acc = scored ? acc : nullptr;
+  a.B = B;
+  a.L = L;
+  a.nh = c->n_heads;
+  a.nkv = c->n_kv_heads;
+  a.group = c->n_heads / c->n_kv_heads;
+  a.max_len = c->max_len;
+  a.prefix_len = prefix_len;
+  const double scale = c->scale != 0.f ? c->scale : 1.0 / std::sqrt(static_cast<double>(c->head_dim));
+  a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  a.rt_p = static_cast<int>(p.rt_p);
+  a.rt_s = static_cast<int>(p.rt_s);
+  a.workers = p.workers;
+  a.part_o = reinterpret_cast<float*>(h->sv_ws);
+  a.part_ml = reinterpret_cast<float2*>(h->sv_ws + p.off_ml);
+  a.lse2 = scored ? reinterpret_cast<float*>(h->sv_ws + p.off_lse) : nullptr;
+  a.err = sv_err(h);
+  prof_begin(h, scored ? "attention_scored" : "attention_prefix");
+  const cudaError_t e = fm::launch_cache_attn(a, c->head_dim, h->stream);
+  prof_end(h);
+  return e == cudaSuccess ? FM_OK : cuda_err(h, e, "cache attention launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+int fm_rope(fm_handle* h, const fm_rope_config* cfg, const uint16_t* x, int64_t x_ld, int n_heads,
+            const int32_t* positions, int64_t T, uint16_t* y, int64_t y_ld) {
+  if (!h) return FM_EINVAL;
+  fm::RopeArgs a;
+  const int rc = rope_args(h, cfg, &a);
+  if (rc != FM_OK) return rc;
+  if (n_heads <= 0 || T < 0) return set_err(h, FM_EINVAL, "bad sizes");
+  if (T > 0x7fffffffLL || n_heads > 65535) return set_err(h, FM_EUNSUPPORTED, "too many tokens or heads");
+  if (T == 0) return FM_OK;
+  if (!x || !positions || !y) return set_err(h, FM_EINVAL, "null pointer");
+  const int64_t cols = static_cast<int64_t>(n_heads) * a.d;
+  if (!rows_ok(x, x_ld, cols) || !rows_ok(y, y_ld, cols))
+    return set_err(h, FM_EINVAL, "rows must be 16-byte aligned, their strides multiples of 8 of at least n_heads * head_dim");
+  if (!(x == y && x_ld == y_ld) && overlap(x, 2 * ((T - 1) * x_ld + cols), y, 2 * ((T - 1) * y_ld + cols)))
+    return set_err(h, FM_EINVAL, "y must be x or not overlap it");
+  const OnDevice on(h);
+  a.q = x;
+  a.q_ld = x_ld;
+  a.q_out = y;
+  a.qo_ld = y_ld;
+  a.positions = positions;
+  a.T = T;
+  a.nq = n_heads;
+  prof_begin(h, "rope");
+  const cudaError_t e = fm::launch_rope(a, h->num_sms, h->stream);
+  prof_end(h);
+  return e == cudaSuccess ? FM_OK : cuda_err(h, e, "rope launch");
+}
+
+int fm_rope_append(fm_handle* h, const fm_rope_config* cfg, const uint16_t* q, int64_t q_ld, int n_heads,
+                   const uint16_t* k, const uint16_t* v, int64_t kv_ld, int n_kv_heads, const int32_t* positions,
+                   const int32_t* slots, int B, int L, uint16_t* cache_k, uint16_t* cache_v, int max_len,
+                   uint16_t* q_out, int64_t q_out_ld) {
+  if (!h) return FM_EINVAL;
+  fm::RopeArgs a;
+  int rc = rope_args(h, cfg, &a);
+  if (rc != FM_OK) return rc;
+  if (n_heads <= 0 || n_kv_heads <= 0 || max_len <= 0 || B < 0 || L < 0) return set_err(h, FM_EINVAL, "bad sizes");
+  const int64_t T = static_cast<int64_t>(B) * L;
+  if (T > 0x7fffffffLL || n_heads > 65535 || n_kv_heads > 65535)
+    return set_err(h, FM_EUNSUPPORTED, "too many tokens or heads");
+  if (T == 0) return FM_OK;
+  if (!q || !k || !v || !positions || !slots || !cache_k || !cache_v || !q_out)
+    return set_err(h, FM_EINVAL, "null pointer");
+  const int64_t cols = static_cast<int64_t>(n_heads) * a.d, kv_cols = static_cast<int64_t>(n_kv_heads) * a.d;
+  if (!rows_ok(q, q_ld, cols) || !rows_ok(q_out, q_out_ld, cols) || !rows_ok(k, kv_ld, kv_cols) ||
+      !rows_ok(v, kv_ld, kv_cols) || !aligned16(cache_k) || !aligned16(cache_v))
+    return set_err(h, FM_EINVAL, "rows must be 16-byte aligned, their strides multiples of 8 of at least their heads * head_dim");
+  const int64_t out_bytes = 2 * ((T - 1) * q_out_ld + cols);
+  if (!(q == q_out && q_ld == q_out_ld) && overlap(q, 2 * ((T - 1) * q_ld + cols), q_out, out_bytes))
+    return set_err(h, FM_EINVAL, "q_out must be q or not overlap it");
+  rc = ensure_sv(h, 0);
+  if (rc != FM_OK) return rc;
+  const OnDevice on(h);
+  a.q = q;
+  a.q_ld = q_ld;
+  a.q_out = q_out;
+  a.qo_ld = q_out_ld;
+  a.k = k;
+  a.v = v;
+  a.kv_ld = kv_ld;
+  a.cache_k = cache_k;
+  a.cache_v = cache_v;
+  a.positions = positions;
+  a.slots = slots;
+  a.T = T;
+  a.nq = n_heads;
+  a.nkv = n_kv_heads;
+  a.L = L;
+  a.max_len = max_len;
+  a.err = sv_err(h);
+  prof_begin(h, "rope_append");
+  const cudaError_t e = fm::launch_rope(a, h->num_sms, h->stream);
+  prof_end(h);
+  return e == cudaSuccess ? FM_OK : cuda_err(h, e, "rope_append launch");
+}
+
+int fm_attention_prefix(fm_handle* h, const fm_cache_attn_config* cfg, const uint16_t* q, const uint16_t* prefix_k,
+                        const uint16_t* prefix_v, int prefix_len, const uint16_t* cache_k, const uint16_t* cache_v,
+                        const int32_t* lens, int B, int L, uint16_t* out) {
+  return cache_attn(h, cfg, q, prefix_k, prefix_v, prefix_len, cache_k, cache_v, lens, B, L, nullptr, false, out);
+}
+
+int fm_attention_scored(fm_handle* h, const fm_cache_attn_config* cfg, const uint16_t* q, const uint16_t* cache_k,
+                        const uint16_t* cache_v, const int32_t* lens, int B, int L, float* acc, uint16_t* out) {
+  return cache_attn(h, cfg, q, nullptr, nullptr, 0, cache_k, cache_v, lens, B, L, acc, true, out);
+}
+
+int fm_cache_evict(fm_handle* h, const fm_evict_config* c, const uint16_t* cache_k, const uint16_t* cache_v,
+                   const float* acc, const int32_t* positions, const int32_t* lens, int B, uint16_t* out_k,
+                   uint16_t* out_v, float* out_acc, int32_t* out_positions, int32_t* out_lens) {
+  if (!h) return FM_EINVAL;
+  if (!c) return set_err(h, FM_EINVAL, "null config");
+  if (c->n_kv_heads <= 0 || c->max_len <= 0 || c->head_dim <= 0 || c->budget < 1 || c->sinks < 0 || c->recent < 0 ||
+      static_cast<int64_t>(c->sinks) + c->recent > c->budget || B < 0)
+    return set_err(h, FM_EINVAL, "bad eviction config (budget >= 1, 0 <= sinks + recent <= budget)");
+  if (c->head_dim % 8 || c->head_dim > 256)
+    return set_err(h, FM_EUNSUPPORTED, "head_dim must be a multiple of 8, at most 256");
+  const int budget = std::min(c->budget, c->max_len);
+  if (c->out_max_len < budget) return set_err(h, FM_EINVAL, "out_max_len is below the budget");
+  const int64_t heads = static_cast<int64_t>(B) * c->n_kv_heads;
+  if (heads > 65535) return set_err(h, FM_EUNSUPPORTED, "too many sequences and heads");
+  if (B == 0) return FM_OK;
+  if (!cache_k || !cache_v || !acc || !lens || !out_k || !out_v || !out_acc || !out_lens || (positions && !out_positions))
+    return set_err(h, FM_EINVAL, "null pointer");
+  if (!aligned16(cache_k) || !aligned16(cache_v) || !aligned16(out_k) || !aligned16(out_v))
+    return set_err(h, FM_EINVAL, "caches must be 16-byte aligned");
+  const bool in_place = out_k == cache_k;
+  const int64_t in = heads * c->max_len, to = heads * c->out_max_len, d2 = 2 * static_cast<int64_t>(c->head_dim);
+  if (in_place) {
+    if (out_v != cache_v || out_acc != acc || out_positions != positions || c->out_max_len != c->max_len)
+      return set_err(h, FM_EINVAL, "in place, every output must be its input and out_max_len max_len");
+  } else {
+    const struct { const void* p; int64_t n; } src[] = {{cache_k, in * d2}, {cache_v, in * d2}, {acc, in * 4},
+                                                        {positions, positions ? in * 4 : 0}},
+        dst[] = {{out_k, to * d2}, {out_v, to * d2}, {out_acc, to * 4}, {out_positions, out_positions ? to * 4 : 0}};
+    for (const auto& s : src)
+      for (const auto& t : dst)
+        if (s.n && t.n && overlap(s.p, s.n, t.p, t.n)) return set_err(h, FM_EINVAL, "the outputs may not overlap the inputs");
+  }
+  const OnDevice on(h);
+  const int rc = ensure_sv(h, evict_bytes(heads, budget));
+  if (rc != FM_OK) return rc;
+  fm::EvictArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.cache_k = cache_k;
+  a.cache_v = cache_v;
+  a.acc = acc;
+  a.positions = positions;
+  a.lens = lens;
+  a.out_k = out_k;
+  a.out_v = out_v;
+  a.out_acc = out_acc;
+  a.out_positions = out_positions;
+  a.out_lens = out_lens;
+  a.B = B;
+  a.nkv = c->n_kv_heads;
+  a.d = c->head_dim;
+  a.max_len = c->max_len;
+  a.out_max_len = c->out_max_len;
+  a.budget = budget;
+  a.sinks = c->sinks;
+  a.recent = c->recent;
+  a.in_place = in_place;
+  a.list = reinterpret_cast<int32_t*>(h->sv_ws);
+  a.counts = reinterpret_cast<int32_t*>(h->sv_ws + align_up(sizeof(int32_t) * heads * 2 * budget, 256));
+  a.err = sv_err(h);
+  prof_begin(h, "cache_evict");
+  const cudaError_t e = fm::launch_evict(a, h->num_sms, h->stream);
+  prof_end(h);
+  return e == cudaSuccess ? FM_OK : cuda_err(h, e, "cache_evict launch");
+}
+
+int fm_serve_reserve(fm_handle* h, const fm_cache_attn_config* cfg, int B, int L) {
+  if (!h) return FM_EINVAL;
+  const int rc = check_cache_attn(h, cfg, B, L, 0);
+  if (rc != FM_OK) return rc;
+  const OnDevice on(h);
+  const fm::CacheAttnPlan p =
+      fm::cache_attn_plan(B, L, cfg->n_heads, cfg->n_kv_heads, cfg->head_dim, cfg->prefix_max, true, h->num_sms);
+  return ensure_sv(h, std::max(p.bytes, evict_bytes(static_cast<int64_t>(B) * cfg->n_kv_heads, cfg->max_len)));
 }
 
 }  // extern "C"

@@ -1,0 +1,794 @@
+// serve.cu -- serving over long and shared KV caches: rotary positions per token (and into
+// the cache), attention of a batch over a shared prefix and its own ragged caches, the
+// attention weight each cache slot receives, and eviction by that weight.
+//
+// What the reference does in this place (server/src): one RoPE offset for the batch
+// (model.cpp:588-606), a prefix cache that copies the prefix's K / V into every request's
+// own cache (scheduler.cpp:121-168), caches bounded by max_context_len.
+#include <algorithm>
+#include <cmath>
+
+#include "fm_serve.cuh"
+
+namespace fm {
+
+// ------------------------------------------------------------------ rotary positions
+// Pair i of a head turns by pos * turns[i] full turns; the product and its reduction to
+// [-1/2, 1/2] are fp64 (at position 1e6 an fp32 product is off by 0.06 rad), the sine and
+// cosine of the reduced turn fp32.  A CTA takes `tpb` tokens: their cos / sin are computed
+// once into shared memory, then shared by all heads.  Bound: HBM, every element read and
+// written once.
+constexpr int kRopeThreads = 256;
+
+namespace {
+
+FM_DEV void rotate(float x1, float x2, float2 cs, float& o1, float& o2) {
+  o1 = x1 * cs.x - x2 * cs.y;
+  o2 = x1 * cs.y + x2 * cs.x;
+}
+
+FM_DEV float lo_f(uint32_t v) { return __uint_as_float(v << 16); }
+FM_DEV float hi_f(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+// source and destination rows of head slot `hs` of token t; false: no destination
+struct RopeRow {
+  const uint16_t* src;
+  uint16_t* dst;
+  bool rot;
+};
+
+FM_DEV bool rope_row(const RopeArgs& a, int64_t t, int hs, RopeRow& r) {
+  if (hs < a.nq) {
+    r.src = a.q + t * a.q_ld + static_cast<int64_t>(hs) * a.d;
+    r.dst = a.q_out + t * a.qo_ld + static_cast<int64_t>(hs) * a.d;
+    r.rot = true;
+    return true;
+  }
+  const int slot = a.slots[t];
+  if (slot < 0) return false;
+  if (slot >= a.max_len) {
+    if (hs == a.nq) report(a.err, DEVERR_BOUNDS);
+    return false;
+  }
+  const int64_t b = t / a.L;
+  hs -= a.nq;
+  r.rot = hs < a.nkv;
+  if (!r.rot) hs -= a.nkv;
+  const int64_t row = ((b * a.nkv + hs) * a.max_len + slot) * a.d;
+  r.src = (r.rot ? a.k : a.v) + t * a.kv_ld + static_cast<int64_t>(hs) * a.d;
+  r.dst = (r.rot ? a.cache_k : a.cache_v) + row;
+  return true;
+}
+
+}  // namespace
+
+// VEC: the rotated part splits into whole 16-byte chunks (half: rotary / 2 a multiple of 8,
+// traditional: rotary a multiple of 8); otherwise elements are taken pair by pair.
+template <bool TRADITIONAL, bool VEC>
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
+  extern __shared__ float2 s_cs[];  // [tpb][rotary / 2]
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tpb;
+  const int nt = static_cast<int>(min(static_cast<int64_t>(a.tpb), a.T - t0));
+  const int half = a.rotary / 2;
+  for (int i = threadIdx.x; i < nt * half; i += kRopeThreads) {
+    const int tt = i / half, p = i - tt * half;
+    double u = static_cast<double>(a.positions[t0 + tt]) * a.turns[p];
+    u -= rint(u);
+    float sn, cs;
+    sincospif(static_cast<float>(2.0 * u), &sn, &cs);
+    s_cs[i] = make_float2(cs * a.factor, sn * a.factor);
+  }
+  __syncthreads();
+  const int slots = a.nq + 2 * a.nkv;
+  const int d = a.d;
+  if (VEC) {
+    // items of a head: half layout: rotary / 16 chunk pairs; traditional: rotary / 8 chunks;
+    // then the (d - rotary) / 8 chunks that are copied.  A v head takes the same items.
+    const int rot_items = TRADITIONAL ? a.rotary / 8 : a.rotary / 16;
+    const int items = rot_items + (d - a.rotary) / 8;
+    const int total = nt * slots * items;
+    for (int i = threadIdx.x; i < total; i += kRopeThreads) {
+      const int it = i % items, hs_t = i / items;
+      const int hs = hs_t % slots, tt = hs_t / slots;
+      RopeRow r;
+      if (!rope_row(a, t0 + tt, hs, r)) continue;
+      const float2* cs = s_cs + tt * half;
+      if (it >= rot_items) {
+        const int c = a.rotary + 8 * (it - rot_items);
+        *reinterpret_cast<uint4*>(r.dst + c) = *reinterpret_cast<const uint4*>(r.src + c);
+        continue;
+      }
+      if (TRADITIONAL) {
+        uint4 v = *reinterpret_cast<const uint4*>(r.src + 8 * it);
+        if (r.rot) {
+          uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float o1, o2;
+            rotate(lo_f(w[e]), hi_f(w[e]), cs[4 * it + e], o1, o2);
+            w[e] = pack_bf16x2(o1, o2);
+          }
+          v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        *reinterpret_cast<uint4*>(r.dst + 8 * it) = v;
+      } else {
+        uint4 v1 = *reinterpret_cast<const uint4*>(r.src + 8 * it);
+        uint4 v2 = *reinterpret_cast<const uint4*>(r.src + half + 8 * it);
+        if (r.rot) {
+          uint32_t w1[4] = {v1.x, v1.y, v1.z, v1.w}, w2[4] = {v2.x, v2.y, v2.z, v2.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float a1, a2, b1, b2;
+            rotate(lo_f(w1[e]), lo_f(w2[e]), cs[8 * it + 2 * e], a1, a2);
+            rotate(hi_f(w1[e]), hi_f(w2[e]), cs[8 * it + 2 * e + 1], b1, b2);
+            w1[e] = pack_bf16x2(a1, b1);
+            w2[e] = pack_bf16x2(a2, b2);
+          }
+          v1 = make_uint4(w1[0], w1[1], w1[2], w1[3]);
+          v2 = make_uint4(w2[0], w2[1], w2[2], w2[3]);
+        }
+        *reinterpret_cast<uint4*>(r.dst + 8 * it) = v1;
+        *reinterpret_cast<uint4*>(r.dst + half + 8 * it) = v2;
+      }
+    }
+  } else {
+    const int items = half + (d - a.rotary);
+    const int total = nt * slots * items;
+    for (int i = threadIdx.x; i < total; i += kRopeThreads) {
+      const int it = i % items, hs_t = i / items;
+      const int hs = hs_t % slots, tt = hs_t / slots;
+      RopeRow r;
+      if (!rope_row(a, t0 + tt, hs, r)) continue;
+      if (it >= half) {
+        const int c = a.rotary + it - half;
+        r.dst[c] = r.src[c];
+        continue;
+      }
+      const int e1 = TRADITIONAL ? 2 * it : it, e2 = TRADITIONAL ? 2 * it + 1 : it + half;
+      const uint16_t h1 = r.src[e1], h2 = r.src[e2];
+      if (r.rot) {
+        float o1, o2;
+        rotate(bf2f(h1), bf2f(h2), s_cs[tt * half + it], o1, o2);
+        r.dst[e1] = f2bf(o1);
+        r.dst[e2] = f2bf(o2);
+      } else {
+        r.dst[e1] = h1;
+        r.dst[e2] = h2;
+      }
+    }
+  }
+}
+
+cudaError_t launch_rope(RopeArgs a, int num_sms, cudaStream_t st) {
+  // few tokens: one per CTA (latency); many: four share the cos / sin set-up's barrier
+  a.tpb = a.T >= 8ll * num_sms ? 4 : 1;
+  const unsigned grid = static_cast<unsigned>((a.T + a.tpb - 1) / a.tpb);
+  const size_t smem = sizeof(float2) * a.tpb * (a.rotary / 2);
+  const bool vec = a.traditional ? a.rotary % 8 == 0 : (a.rotary / 2) % 8 == 0;
+  if (a.traditional) {
+    if (vec) rope_kernel<true, true><<<grid, kRopeThreads, smem, st>>>(a);
+    else rope_kernel<true, false><<<grid, kRopeThreads, smem, st>>>(a);
+  } else {
+    if (vec) rope_kernel<false, true><<<grid, kRopeThreads, smem, st>>>(a);
+    else rope_kernel<false, false><<<grid, kRopeThreads, smem, st>>>(a);
+  }
+  return cudaGetLastError();
+}
+
+// ------------------------------------------------------------------ attention, split over keys
+// Work is counted in tiles of 16 keys.  The prefix gives nkv * rt_p items (a kv head, 16 of
+// all sequences' query rows) of ceil(prefix_len / 16) tiles; sequence b gives nkv * rt_s
+// items (a kv head, 16 of its L * group rows) of ceil(lens[b] / 16) tiles.  All tiles in
+// this order are cut into one contiguous range per worker (a warp), so ragged lengths
+// balance.  A worker's piece of an item leaves an unnormalised fp32 output, its maximum
+// (log2 units) and its sum in slot worker + item -- both only grow along the order, so no
+// two pieces share a slot -- and attn_merge_kernel joins an output row's pieces.
+namespace {
+
+struct Span {  // a worker's place in the order
+  int64_t per, t0, t1;
+};
+
+FM_DEV int seq_len(const CacheAttnArgs& a, int b) {
+  const int n = a.lens ? a.lens[b] : 0;
+  return n < 0 || n > a.max_len ? 0 : n;  // reported by the merge
+}
+
+FM_DEV int64_t warp_sum64(int64_t v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// tiles of one item of sequences [0, b), summed; whole warp, B <= a few thousand
+FM_DEV int64_t tiles_before(const CacheAttnArgs& a, int b) {
+  const int lane = threadIdx.x & 31;
+  int64_t s = 0;
+  for (int i = lane; i < b; i += 32) s += (seq_len(a, i) + kAttnTile - 1) / kAttnTile;
+  return warp_sum64(s);
+}
+
+FM_DEV int64_t tiles_per_worker(const CacheAttnArgs& a, int64_t total) {
+  const int64_t per = (total + a.workers - 1) / a.workers;
+  return per < kAttnMinTiles ? kAttnMinTiles : per;
+}
+
+FM_DEV void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr)
+               : "memory");
+}
+
+FM_DEV void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr)
+               : "memory");
+}
+
+// 16 bytes, or zeros when n is 0 (nothing is read then)
+FM_DEV void cp_async16_or_zero(uint32_t dst, const void* src, int n) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
+}  // namespace
+
+template <int D>
+__global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const CacheAttnArgs a) {
+  constexpr int CH = D / 8;                          // 16-byte chunks of a row
+  constexpr int KS = D / 16;                         // k-steps of Q K^T
+  constexpr int NT = D / 8;                          // n-tiles of O
+  constexpr uint32_t ROW = D * 2;                    // bytes of a row
+  constexpr uint32_t TILE = kAttnTile * ROW;         // bytes of a K (or V) tile
+  constexpr uint32_t STAGE = 2 * TILE;
+  extern __shared__ __align__(128) uint8_t s_kv[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+  const uint32_t ring = smem_u32(s_kv) + warp * (kAttnStages * STAGE);
+  const int64_t worker = static_cast<int64_t>(blockIdx.x) * kAttnWarps + warp;
+
+  const int64_t tp = (a.prefix_len + kAttnTile - 1) / kAttnTile;  // tiles of a prefix item
+  const int np = a.nkv * a.rt_p, ns = a.nkv * a.rt_s;             // items of the prefix / of a sequence
+  const int64_t total_p = tp * np;
+  const int64_t total = total_p + ns * tiles_before(a, a.B);
+  const int64_t per = tiles_per_worker(a, total);
+  int64_t t = worker * per;
+  const int64_t t_end = min(total, t + per);
+  if (t >= t_end) return;
+
+  // the item of tile t: sequence (-1: the prefix), item of it, tile of the item
+  int b = -1, item, tiles;
+  int tile;
+  if (t < total_p) {
+    item = static_cast<int>(t / tp);
+    tile = static_cast<int>(t - item * tp);
+    tiles = static_cast<int>(tp);
+  } else {
+    int64_t rest = t - total_p;
+    b = 0;
+    while (true) {  // 32 sequences at a time
+      const int i = b + lane;
+      const int64_t mine = i < a.B ? static_cast<int64_t>(ns) * ((seq_len(a, i) + kAttnTile - 1) / kAttnTile) : 0;
+      int64_t incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, incl > rest);
+      if (past) {  // the first sequence whose tiles reach beyond `rest`
+        const int f = __ffs(past) - 1;
+        rest -= __shfl_sync(0xffffffffu, incl - mine, f);
+        b += f;
+        break;
+      }
+      rest -= __shfl_sync(0xffffffffu, incl, 31);
+      b += 32;
+      if (b >= a.B) return;  // t < total makes this unreachable
+    }
+    tiles = (seq_len(a, b) + kAttnTile - 1) / kAttnTile;
+    item = static_cast<int>(rest / tiles);
+    tile = static_cast<int>(rest - static_cast<int64_t>(item) * tiles);
+  }
+
+  while (t < t_end) {
+    const int cnt = static_cast<int>(min(static_cast<int64_t>(tiles - tile), t_end - t));
+    const bool pre = b < 0;
+    const int rts = pre ? a.rt_p : a.rt_s;
+    const int kvh = item / rts, row0 = (item - kvh * rts) * kAttnRowTile;
+    const int rows = pre ? a.B * a.L * a.group : a.L * a.group;
+    const int len = pre ? a.prefix_len : seq_len(a, b);
+    const int64_t tok0 = pre ? 0 : static_cast<int64_t>(b) * a.L;
+    const int64_t base = pre ? kvh * a.p_head : (static_cast<int64_t>(b) * a.nkv + kvh) * a.max_len * D;
+    const uint16_t* kb = (pre ? a.pk : a.ck) + base;
+    const uint16_t* vb = (pre ? a.pv : a.cv) + base;
+
+    auto load = [&](int j) {  // tile + j of the item into stage j
+      if (j < cnt) {
+        const uint32_t sk = ring + (j % kAttnStages) * STAGE, sv = sk + TILE;
+        const int key0 = (tile + j) * kAttnTile;
+#pragma unroll
+        for (int i = 0; i < kAttnTile * CH / 32; ++i) {
+          const int e = i * 32 + lane, r = e / CH, ch = e % CH;
+          const int key = key0 + r;
+          const uint32_t off = r * ROW + ((ch ^ (r & 7)) << 4);
+          const int64_t src = static_cast<int64_t>(min(key, len - 1)) * D + ch * 8;
+          const int n = key < len ? 16 : 0;  // rows past the length count as zeros
+          cp_async16_or_zero(sk + off, kb + src, n);
+          cp_async16_or_zero(sv + off, vb + src, n);
+        }
+      }
+      cp_async_commit();
+    };
+    __syncwarp();  // the previous item's last reads of the ring are done
+#pragma unroll
+    for (int j = 0; j < kAttnStages - 1; ++j) load(j);
+
+    // Q fragments of rows row0 + g and row0 + g + 8 (zeros past the last row), and the last
+    // slot each of them sees
+    uint32_t qa[KS][4];
+    int lim[2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int r = row0 + g + 8 * hf;
+      const bool on = r < rows;
+      const int tk = on ? r / a.group : 0;
+      lim[hf] = !on ? -1 : pre ? len - 1 : len - a.L + tk;
+      const uint16_t* q = a.q + (tok0 + tk) * a.q_ld + static_cast<int64_t>(kvh * a.group + (on ? r - tk * a.group : 0)) * D;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        qa[ks][hf] = on ? *reinterpret_cast<const uint32_t*>(q + 16 * ks + 2 * c) : 0u;
+        qa[ks][hf + 2] = on ? *reinterpret_cast<const uint32_t*>(q + 16 * ks + 2 * c + 8) : 0u;
+      }
+    }
+    float o[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (int j = 0; j < cnt; ++j) {
+      load(j + kAttnStages - 1);
+      cp_async_wait<kAttnStages - 1>();
+      __syncwarp();
+      const uint32_t sk = ring + (j % kAttnStages) * STAGE, sv = sk + TILE;
+      const int mi = lane >> 3, rr = lane & 7;
+      float s[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int r = (mi >> 1) * 8 + rr, ch = 2 * ks + (mi & 1);
+        uint32_t b0, b1, b2, b3;
+        ldsm_x4(sk + r * ROW + ((ch ^ (r & 7)) << 4), b0, b1, b2, b3);
+        mma_bf16_16816(s[0], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b0, b1);
+        mma_bf16_16816(s[1], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b2, b3);
+      }
+      // scale, visibility, online softmax; rows g (hf 0) and g + 8 (hf 1)
+      uint32_t pa[2][2];
+      float al[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int key = (tile + j) * kAttnTile + 8 * n + 2 * c + e;
+            float& v = s[n][2 * hf + e];
+            v = key <= lim[hf] ? v * a.scale_log2 : -INFINITY;
+            mx = fmaxf(mx, v);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = fmaxf(m[hf], mx);
+        const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every term is 0
+        al[hf] = exp2f(m[hf] - ref);
+        m[hf] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float p0 = exp2f(s[n][2 * hf] - ref), p1 = exp2f(s[n][2 * hf + 1] - ref);
+          sum += p0 + p1;
+          pa[n][hf] = pack_bf16x2(p0, p1);  // the tensor product's operand: one rounding to bf16
+        }
+        l[hf] = l[hf] * al[hf] + sum;
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        o[n][0] *= al[0];
+        o[n][1] *= al[0];
+        o[n][2] *= al[1];
+        o[n][3] *= al[1];
+      }
+#pragma unroll
+      for (int n = 0; n < NT; n += 2) {
+        const int r = (mi & 1) * 8 + rr, ch = n + (mi >> 1);
+        uint32_t b0, b1, b2, b3;
+        ldsm_x4_t(sv + r * ROW + ((ch ^ (r & 7)) << 4), b0, b1, b2, b3);
+        mma_bf16_16816(o[n], pa[0][0], pa[0][1], pa[1][0], pa[1][1], b0, b1);
+        mma_bf16_16816(o[n + 1], pa[0][0], pa[0][1], pa[1][0], pa[1][1], b2, b3);
+      }
+      __syncwarp();  // the next iteration's load overwrites a stage read one step ago
+    }
+    cp_async_wait<0>();
+
+    const int64_t gi = pre ? item : np + static_cast<int64_t>(b) * ns + item;
+    const int64_t slot = worker + gi;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
+      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
+      if (row0 + g + 8 * hf < rows) {
+        const int64_t pr = slot * kAttnRowTile + g + 8 * hf;
+        float* po = a.part_o + pr * D;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          *reinterpret_cast<float2*>(po + 8 * n + 2 * c) = make_float2(o[n][2 * hf], o[n][2 * hf + 1]);
+        if (c == 0) a.part_ml[pr] = make_float2(m[hf], l[hf]);
+      }
+    }
+    t += cnt;
+    if (t >= t_end) break;
+    tile = 0;
+    ++item;
+    if (item >= (pre ? np : ns)) {
+      ++b;
+      item = 0;
+      while (seq_len(a, b) == 0) ++b;  // tiles are left, so a sequence that has some follows
+    }
+    tiles = b < 0 ? static_cast<int>(tp) : (seq_len(a, b) + kAttnTile - 1) / kAttnTile;
+  }
+}
+
+// Joins the pieces of one output row (one warp): out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i,
+// zeros when nothing was seen; lse2 = M + log2(sum) for the slot weights.
+template <int D>
+__global__ void __launch_bounds__(128) attn_merge_kernel(const CacheAttnArgs a) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + warp;  // (b, l, h)
+  if (row >= static_cast<int64_t>(a.B) * a.L * a.nh) return;
+  const int64_t tok = row / a.nh;
+  const int h = static_cast<int>(row - tok * a.nh);
+  const int b = static_cast<int>(tok / a.L), l = static_cast<int>(tok - static_cast<int64_t>(b) * a.L);
+  const int kvh = h / a.group, gq = h - kvh * a.group;
+  if (a.lens && lane == 0 && l == 0 && h == 0 && (a.lens[b] < 0 || a.lens[b] > a.max_len)) report(a.err, DEVERR_BOUNDS);
+  const int64_t tp = (a.prefix_len + kAttnTile - 1) / kAttnTile;
+  const int np = a.nkv * a.rt_p, ns = a.nkv * a.rt_s;
+  const int64_t total_p = tp * np;
+  const int64_t per = tiles_per_worker(a, total_p + ns * tiles_before(a, a.B));
+  constexpr int V = D / 32;  // columns of a lane
+  float acc[V] = {};
+  float M = -INFINITY, S = 0.f;
+  auto join = [&](int64_t first, int64_t tiles, int64_t item, int rr) {
+    if (tiles <= 0) return;
+    const int64_t w1 = (first + tiles - 1) / per;
+    for (int64_t w = first / per; w <= w1; ++w) {
+      const int64_t pr = (w + item) * kAttnRowTile + rr;
+      const float2 ml = a.part_ml[pr];
+      const float* po = a.part_o + pr * D + lane * V;
+      float v[V];
+      if (V == 4) {
+        const float4 t4 = *reinterpret_cast<const float4*>(po);
+        v[0] = t4.x; v[1] = t4.y; v[2 % V] = t4.z; v[3 % V] = t4.w;
+      } else {
+        const float2 t2 = *reinterpret_cast<const float2*>(po);
+        v[0] = t2.x; v[1] = t2.y;
+      }
+      if (ml.x == -INFINITY) continue;  // the piece's keys are all hidden from this row
+      const float mn = fmaxf(M, ml.x);
+      const float wa = exp2f(M - mn), wb = exp2f(ml.x - mn);
+      M = mn;
+      S = S * wa + ml.y * wb;
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = acc[i] * wa + v[i] * wb;
+    }
+  };
+  if (tp > 0) {
+    const int64_t r = tok * a.group + gq;
+    const int64_t item = kvh * a.rt_p + r / kAttnRowTile;
+    join(item * tp, tp, item, static_cast<int>(r % kAttnRowTile));
+  }
+  const int64_t ts = (seq_len(a, b) + kAttnTile - 1) / kAttnTile;
+  if (ts > 0) {
+    const int r = l * a.group + gq;
+    const int64_t in = kvh * a.rt_s + r / kAttnRowTile;
+    join(total_p + ns * tiles_before(a, b) + in * ts, ts, np + static_cast<int64_t>(b) * ns + in, r % kAttnRowTile);
+  }
+  const float inv = M == -INFINITY ? 0.f : 1.f / S;
+  uint16_t* out = a.out + row * D + lane * V;
+#pragma unroll
+  for (int i = 0; i < V; i += 2)
+    *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
+  if (a.lse2 && lane == 0) a.lse2[row] = M == -INFINITY ? INFINITY : M + log2f(S);
+}
+
+// ------------------------------------------------------------------ slot weights
+// acc[b, kvh, j] += sum over the kv head's query rows of 2^(s_rj - lse2_r), recomputing the
+// scores with keys as the product's rows: a warp holds 16 keys' fragments and walks the query
+// rows 8 at a time, so a key's sum over rows stays in a lane quad.
+template <int D>
+__global__ void __launch_bounds__(128) slot_weight_kernel(const CacheAttnArgs a) {
+  constexpr int KS = D / 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+  const int b = blockIdx.z, kvh = blockIdx.y;
+  const int len = seq_len(a, b);
+  const int key0 = (blockIdx.x * 4 + warp) * 16;
+  if (key0 >= len) return;
+  const uint16_t* kb = a.ck + (static_cast<int64_t>(b) * a.nkv + kvh) * a.max_len * D;
+  uint32_t ka[KS][4];
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf) {
+    const int key = key0 + g + 8 * hf;
+    const uint16_t* kr = kb + static_cast<int64_t>(min(key, len - 1)) * D;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      ka[ks][hf] = *reinterpret_cast<const uint32_t*>(kr + 16 * ks + 2 * c);
+      ka[ks][hf + 2] = *reinterpret_cast<const uint32_t*>(kr + 16 * ks + 2 * c + 8);
+    }
+  }
+  const int rows = a.L * a.group;
+  float sum[2] = {0.f, 0.f};
+  // token l sees slot j iff j <= len - L + l: rows of earlier tokens see none of these keys
+  const int first = max(0, key0 - (len - a.L)) * a.group;
+  for (int r0 = first / 8 * 8; r0 < rows; r0 += 8) {
+    const int rq = min(r0 + g, rows - 1);
+    const int tk = rq / a.group;
+    const uint16_t* q = a.q + (static_cast<int64_t>(b) * a.L + tk) * a.q_ld +
+                        static_cast<int64_t>(kvh * a.group + rq - tk * a.group) * D;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      mma_bf16_16816(s, ka[ks][0], ka[ks][1], ka[ks][2], ka[ks][3],
+                     *reinterpret_cast<const uint32_t*>(q + 16 * ks + 2 * c),
+                     *reinterpret_cast<const uint32_t*>(q + 16 * ks + 2 * c + 8));
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = r0 + 2 * c + e;
+      if (r >= rows) continue;
+      const int tr = r / a.group;
+      const float lse = a.lse2[(static_cast<int64_t>(b) * a.L + tr) * a.nh + kvh * a.group + r - tr * a.group];
+      const int lim = len - a.L + tr;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+        if (key0 + g + 8 * hf <= lim) sum[hf] += exp2f(s[2 * hf + e] * a.scale_log2 - lse);
+    }
+  }
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf) {
+    sum[hf] += __shfl_xor_sync(0xffffffffu, sum[hf], 1);
+    sum[hf] += __shfl_xor_sync(0xffffffffu, sum[hf], 2);
+    const int key = key0 + g + 8 * hf;
+    if (c == 0 && key < len) a.acc[(static_cast<int64_t>(b) * a.nkv + kvh) * a.max_len + key] += sum[hf];
+  }
+}
+
+template <int D>
+static cudaError_t attn_opt_in() {
+  return cudaFuncSetAttribute(attn_split_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_split_smem(D));
+}
+
+cudaError_t cache_attn_init() {
+  const cudaError_t e = attn_opt_in<128>();
+  return e == cudaSuccess ? attn_opt_in<64>() : e;
+}
+
+CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_len, bool scored, int num_sms) {
+  CacheAttnPlan p;
+  const int64_t group = nh / nkv;
+  p.rt_p = prefix_len > 0 ? (static_cast<int64_t>(B) * L * group + kAttnRowTile - 1) / kAttnRowTile : 0;
+  p.rt_s = (L * group + kAttnRowTile - 1) / kAttnRowTile;
+  p.workers = num_sms * kAttnBlocksPerSm * kAttnWarps;
+  const int64_t slots = p.workers + nkv * (p.rt_p + B * p.rt_s);
+  p.off_ml = static_cast<size_t>(slots) * kAttnRowTile * d * sizeof(float);
+  p.off_lse = p.off_ml + static_cast<size_t>(slots) * kAttnRowTile * sizeof(float2);
+  p.bytes = p.off_lse + (scored ? sizeof(float) * B * L * nh : 0);
+  return p;
+}
+
+template <int D>
+static cudaError_t launch_cache_attn_d(const CacheAttnArgs& a, cudaStream_t st) {
+  attn_split_kernel<D><<<a.workers / kAttnWarps, kAttnWarps * 32, attn_split_smem(D), st>>>(a);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const int64_t rows = static_cast<int64_t>(a.B) * a.L * a.nh;
+  attn_merge_kernel<D><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, st>>>(a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || !a.acc) return e;
+  const dim3 grid((a.max_len + 63) / 64, a.nkv, a.B);
+  slot_weight_kernel<D><<<grid, 128, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_cache_attn(const CacheAttnArgs& a, int d, cudaStream_t st) {
+  return d == 128 ? launch_cache_attn_d<128>(a, st) : launch_cache_attn_d<64>(a, st);
+}
+
+// ------------------------------------------------------------------ eviction
+// evict_select_kernel (one CTA per sequence and kv head) finds the n = min(len, budget) slots
+// that stay: a radix select over 32-bit keys (protected slots the largest, then the weight's
+// order-preserving bits, NaN as -inf), 8 bits a pass, ties to the lower slot.  It leaves the
+// list of rows that move as (destination, source) pairs; evict_move_kernel moves them.
+// In place only the holes below n are filled, by the kept slots from n on, both in ascending
+// order: sources >= n, destinations < n, so no move reads what another writes.
+constexpr int kEvictThreads = 1024;
+
+namespace {
+
+FM_DEV uint32_t order_bits(float v) {
+  if (v != v) v = -INFINITY;
+  if (v == 0.f) v = 0.f;  // -0 ranks as 0
+  const uint32_t u = __float_as_uint(v);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;  // [0x007fffff, 0xff800000]
+}
+
+// inclusive scan over the CTA of one value a thread; s_w: 32 ints of shared memory
+FM_DEV int block_scan(int v, int* s_w, int* sum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += up;
+  }
+  if (lane == 31) s_w[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    int w = s_w[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += up;
+    }
+    s_w[lane] = w;
+  }
+  __syncthreads();
+  const int before = warp ? s_w[warp - 1] : 0;
+  *sum = s_w[31];
+  __syncthreads();  // s_w may be written again
+  return v + before;
+}
+
+}  // namespace
+
+__global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const EvictArgs a) {
+  __shared__ int s_hist[256 * 32];  // [bin][lane]: a lane's own bank, no conflicts
+  __shared__ int s_w[32];
+  __shared__ int s_pick[2];
+  const int lane = threadIdx.x & 31;
+  const int64_t bh = blockIdx.x;
+  const int b = static_cast<int>(bh / a.nkv);
+  int len = a.lens[b];
+  if (len < 0 || len > a.max_len) {
+    if (threadIdx.x == 0) report(a.err, DEVERR_BOUNDS);
+    len = 0;
+  }
+  const int n = min(len, a.budget);
+  const float* acc = a.acc + bh * a.max_len;
+  const int32_t* pos = a.positions ? a.positions + bh * a.max_len : nullptr;
+  int32_t* list_dst = a.list + bh * 2 * a.budget;
+  int32_t* list_src = list_dst + a.budget;
+  if (n == len) {  // all stay
+    if (!a.in_place)
+      for (int i = threadIdx.x; i < n; i += kEvictThreads) list_dst[i] = list_src[i] = i;
+    if (threadIdx.x == 0) {
+      a.counts[2 * bh] = a.in_place ? 0 : n;
+      a.counts[2 * bh + 1] = n;
+    }
+    return;
+  }
+  // the newest position held
+  int64_t newest = len - 1;
+  if (pos) {
+    int mx = INT32_MIN;
+    for (int i = threadIdx.x; i < len; i += kEvictThreads) mx = max(mx, pos[i]);
+    mx = __reduce_max_sync(0xffffffffu, mx);
+    if (lane == 0) s_w[threadIdx.x >> 5] = mx;
+    __syncthreads();
+    newest = __reduce_max_sync(0xffffffffu, s_w[lane]);
+    __syncthreads();
+  }
+  auto key_of = [&](int i) -> uint32_t {
+    const int64_t p = pos ? pos[i] : i;
+    if (p < a.sinks || p > newest - a.recent) return 0xffffffffu;
+    return order_bits(acc[i]);
+  };
+  // radix select: the n-th largest key and how many keys equal to it stay
+  uint32_t prefix = 0;
+  int want = n;  // of the keys that match the prefix so far
+#pragma unroll 1
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    for (int i = threadIdx.x; i < 256 * 32; i += kEvictThreads) s_hist[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < len; i += kEvictThreads) {
+      const uint32_t k = key_of(i);
+      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
+        atomicAdd(&s_hist[((k >> shift) & 255u) * 32 + lane], 1);
+    }
+    __syncthreads();
+    // bins from the largest down: thread t < 256 holds bin 255 - t
+    int cnt = 0;
+    if (threadIdx.x < 256)
+      for (int i = 0; i < 32; ++i) cnt += s_hist[(255 - threadIdx.x) * 32 + ((i + lane) & 31)];
+    int all;
+    const int incl = block_scan(cnt, s_w, &all);
+    if (threadIdx.x < 256 && incl >= want && incl - cnt < want) {
+      s_pick[0] = 255 - threadIdx.x;
+      s_pick[1] = want - (incl - cnt);
+    }
+    __syncthreads();
+    prefix |= static_cast<uint32_t>(s_pick[0]) << shift;
+    want = s_pick[1];
+    __syncthreads();
+  }
+  // `want` of the keys equal to `prefix` stay, the lowest slots first.  Slots in order, 1024
+  // at a time, with running counts of equals, holes and kept tails; the heads that stay are
+  // listed after the m moves when rows are copied elsewhere.
+  int eq0 = 0, hole0 = 0, tail0 = 0;
+  // holes below n: n minus the kept below n, so m is known only at the end; heads are listed
+  // from the back of the list
+  int head0 = 0;
+  for (int base = 0; base < len; base += kEvictThreads) {
+    const int i = base + threadIdx.x;
+    const uint32_t k = i < len ? key_of(i) : 0u;
+    const bool eq = i < len && k == prefix;
+    int all;
+    const int eq_incl = block_scan(eq ? 1 : 0, s_w, &all);
+    const bool kept = i < len && (k > prefix || (eq && eq0 + eq_incl <= want));
+    eq0 += all;
+    const bool hole = i < n && !kept, tail = i >= n && kept, head = i < n && kept;
+    const int hi = block_scan(hole ? 1 : 0, s_w, &all);
+    if (hole) list_dst[hole0 + hi - 1] = i;
+    hole0 += all;
+    const int ti = block_scan(tail ? 1 : 0, s_w, &all);
+    if (tail) list_src[tail0 + ti - 1] = i;
+    tail0 += all;
+    if (!a.in_place) {
+      const int ci = block_scan(head ? 1 : 0, s_w, &all);
+      if (head) list_dst[n - (head0 + ci)] = list_src[n - (head0 + ci)] = i;
+      head0 += all;
+    }
+  }
+  if (threadIdx.x == 0) {
+    a.counts[2 * bh] = a.in_place ? hole0 : n;
+    a.counts[2 * bh + 1] = n;
+  }
+}
+
+// One warp a row pair: K and V rows, weight and position.
+__global__ void __launch_bounds__(256) evict_move_kernel(const EvictArgs a) {
+  const int64_t bh = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cnt = a.counts[2 * bh];
+  if (blockIdx.x == 0 && threadIdx.x == 0 && bh % a.nkv == 0) a.out_lens[bh / a.nkv] = a.counts[2 * bh + 1];
+  const int32_t* list_dst = a.list + bh * 2 * a.budget;
+  const int32_t* list_src = list_dst + a.budget;
+  const int ch = a.d / 8;
+  for (int i = blockIdx.x * 8 + warp; i < cnt; i += gridDim.x * 8) {
+    const int dst = list_dst[i], src = list_src[i];
+    const int64_t from = (bh * a.max_len + src) * a.d, to = (bh * a.out_max_len + dst) * a.d;
+    for (int e = lane; e < 2 * ch; e += 32) {
+      const bool v = e >= ch;
+      const int c = (v ? e - ch : e) * 8;
+      *reinterpret_cast<uint4*>((v ? a.out_v : a.out_k) + to + c) =
+          *reinterpret_cast<const uint4*>((v ? a.cache_v : a.cache_k) + from + c);
+    }
+    if (lane == 0) a.out_acc[bh * a.out_max_len + dst] = a.acc[bh * a.max_len + src];
+    if (lane == 1 && a.out_positions)
+      a.out_positions[bh * a.out_max_len + dst] = a.positions ? a.positions[bh * a.max_len + src] : src;
+  }
+}
+
+cudaError_t launch_evict(const EvictArgs& a, int num_sms, cudaStream_t st) {
+  const int64_t heads = static_cast<int64_t>(a.B) * a.nkv;
+  evict_select_kernel<<<static_cast<unsigned>(heads), kEvictThreads, 0, st>>>(a);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const int64_t most = a.in_place ? std::min<int64_t>(a.budget, std::max(0, a.max_len - a.budget)) : a.budget;
+  const int64_t want = std::max<int64_t>(1, (num_sms * 8 + heads - 1) / heads);
+  const unsigned gx = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((most + 7) / 8, want)));
+  evict_move_kernel<<<dim3(gx, static_cast<unsigned>(heads)), 256, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace fm

@@ -540,3 +540,237 @@ def argmax(logits, handle=None) -> torch.Tensor:
     h.bind_stream()
     h.check(h.lib.fm_argmax(h.h, _ptr(logits), logits.numel() // V, V, _ptr(out)))
     return out
+
+
+# ---------------------------------------------------------------- serving over long and shared caches
+
+_BF16, _I32, _F32 = (torch.bfloat16,), (torch.int32,), (torch.float32,)
+_ROPE_SCALINGS = {"linear": _lib.FM_ROPE_LINEAR, "ntk": _lib.FM_ROPE_NTK, "yarn": _lib.FM_ROPE_YARN,
+                  "banded": _lib.FM_ROPE_BANDED}
+
+
+def _rope_config(d, theta, rotary_dim, traditional, scaling) -> _lib.RopeConfig:
+    c = _lib.RopeConfig(int(d), int(rotary_dim or 0), int(traditional), _lib.FM_ROPE_UNSCALED, float(theta))
+    if rotary_dim is not None and not 0 < rotary_dim <= d:
+        raise ValueError("rotary_dim must be between 2 and the head size")
+    if scaling is not None:
+        s = dict(scaling)
+        kind = s.pop("type", None)
+        if kind not in _ROPE_SCALINGS:
+            raise ValueError(f"unknown rope scaling {kind!r}, expected one of {sorted(_ROPE_SCALINGS)}")
+        c.scaling, c.factor = _ROPE_SCALINGS[kind], float(s.pop("factor"))
+        c.attn_factor = float(s.pop("attn_factor", 0.0))
+        if kind in ("yarn", "banded"):
+            lo, hi = ("beta_slow", "beta_fast") if kind == "yarn" else ("low_freq", "high_freq")
+            c.original_len = float(s.pop("original_len"))
+            c.low, c.high = float(s.pop(lo, 1.0)), float(s.pop(hi, 32.0 if kind == "yarn" else 4.0))
+        if s:
+            raise ValueError(f"unknown {kind} scaling entries {sorted(s)}")
+    return c
+
+
+def _need_heads(t, name, device):
+    """[..., heads, d] bf16 whose heads lie side by side in each token's row: the elements
+    from one token's row to the next (leading axes must be one stride apart in order)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor")
+    if t.device.type != "cuda" or (device is not None and t.device != device):
+        raise ValueError(f"{name} must live on {device or 'a CUDA device'}")
+    if t.dtype != torch.bfloat16:
+        raise ValueError(f"{name} has dtype {t.dtype}, expected torch.bfloat16")
+    if t.dim() < 3:
+        raise ValueError(f"{name} must be [..., heads, head size]")
+    h, d = t.shape[-2:]
+    if t.numel() == 0:
+        return h * d
+    if (d > 1 and t.stride(-1) != 1) or (h > 1 and t.stride(-2) != d):
+        raise ValueError(f"the heads of {name} must lie side by side")
+    ld, n = None, 1
+    for size, step in zip(reversed(t.shape[:-2]), reversed(t.stride()[:-2])):
+        if size > 1:
+            if ld is None:
+                ld = step
+            elif step != ld * n:
+                raise ValueError(f"the tokens of {name} must be one stride apart")
+            n *= size
+    return h * d if ld is None else ld
+
+
+def rope(x, positions, theta, rotary_dim=None, traditional=False, scaling=None, out=None, handle=None) -> torch.Tensor:
+    """Rotary positions (mx::fast::rope with one position per token): x [..., heads, d] bf16,
+    positions int32 [...] (any int32; negative ones rotate back) -> x rotated, in `out` if given
+    (it may be x).  rotary_dim leading elements of a head rotate (default all), in pairs
+    (i, i + rotary_dim / 2) or, traditional, (2i, 2i + 1).  scaling: None or a dict with
+    "type" and "factor": "linear", "ntk", "yarn" (original_len, beta_slow, beta_fast) or
+    "banded" (original_len, low_freq, high_freq), and optionally attn_factor.  x and out may
+    be views of wider rows (a fused projection's)."""
+    ld = _need_heads(x, "x", None)
+    dev = x.device
+    _need(positions, "positions", _I32, dev)
+    if tuple(positions.shape) != tuple(x.shape[:-2]):
+        raise ValueError("positions must have x's shape without heads and head size")
+    cfg = _rope_config(x.shape[-1], theta, rotary_dim, traditional, scaling)
+    y = out if out is not None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y_ld = _need_heads(y, "out", dev)
+    if y.shape != x.shape:
+        raise ValueError("out has another shape than x")
+    h = handle or default_handle(dev.index)
+    h.bind_stream()
+    h.check(h.lib.fm_rope(h.h, C.byref(cfg), _ptr(x), ld, x.shape[-2], _ptr(positions), positions.numel(), _ptr(y), y_ld))
+    return y
+
+
+def _need_caches(cache_k, cache_v, dev, what="cache"):
+    _need(cache_k, what + "_k", _BF16, dev)
+    _need(cache_v, what + "_v", _BF16, dev)
+    if cache_v.shape != cache_k.shape:
+        raise ValueError(f"{what}_k and {what}_v must be alike")
+
+
+def rope_append(q, k, v, positions, slots, cache_k, cache_v, theta, traditional=False, scaling=None, rotary_dim=None,
+                out=None, handle=None) -> torch.Tensor:
+    """A step's q [T, nh, d], k and v [T, n_kv, d] (views of a fused projection's rows, or
+    separate) with T = B * L tokens in sequence order: returns q rotated at positions [T] (in
+    `out` if given, which may be q); k rotated and v go into the caches [B, n_kv, max_len, d]
+    at slots [T] (a negative slot writes nothing; a sequence's slots must differ)."""
+    ld = _need_heads(q, "q", None)
+    dev = q.device
+    kv_ld = _need_heads(k, "k", dev)
+    if _need_heads(v, "v", dev) != kv_ld or v.shape != k.shape:
+        raise ValueError("k and v must have the same shape and strides")
+    _need_caches(cache_k, cache_v, dev)
+    _need(positions, "positions", _I32, dev)
+    _need(slots, "slots", _I32, dev)
+    T, d = positions.numel(), q.shape[-1]
+    if cache_k.dim() != 4 or cache_k.shape[3] != d or k.shape[-1] != d or k.shape[-2] != cache_k.shape[1]:
+        raise ValueError("caches must be [B, n_kv, max_len, d] with k's heads and q's head size")
+    B = cache_k.shape[0]
+    if B == 0 or T % B or slots.numel() != T or q.numel() != T * q.shape[-2] * d or k.numel() != T * k.shape[-2] * d:
+        raise ValueError("q, k, v, positions and slots must hold the same T = B * L tokens")
+    cfg = _rope_config(d, theta, rotary_dim, traditional, scaling)
+    y = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=dev)
+    y_ld = _need_heads(y, "out", dev)
+    if y.shape != q.shape:
+        raise ValueError("out has another shape than q")
+    h = handle or default_handle(dev.index)
+    h.bind_stream()
+    h.check(h.lib.fm_rope_append(h.h, C.byref(cfg), _ptr(q), ld, q.shape[-2], _ptr(k), _ptr(v), kv_ld, k.shape[-2],
+                                 _ptr(positions), _ptr(slots), B, T // B, _ptr(cache_k), _ptr(cache_v),
+                                 cache_k.shape[2], _ptr(y), y_ld))
+    return y
+
+
+def _cache_attn(q, cache_k, lens, prefix_k, scale):
+    """Checked sizes of an attention over caches: (config, B, L, device)."""
+    ld = _need_heads(q, "q", None)
+    if q.dim() != 4:
+        raise ValueError("q must be [B, L, n_heads, d]")
+    B, L, nh, d = q.shape
+    some = cache_k if cache_k is not None else prefix_k
+    if some is None:
+        raise ValueError("a prefix or caches are needed")
+    nkv = some.shape[1] if cache_k is not None else some.shape[0]
+    if cache_k is not None:
+        if cache_k.dim() != 4 or cache_k.shape[0] != B or cache_k.shape[3] != d:
+            raise ValueError("caches must be [B, n_kv, max_len, d] with q's batch and head size")
+        if lens is None:
+            raise ValueError("lens is required with caches")
+        _need(lens, "lens", _I32, q.device)
+        if tuple(lens.shape) != (B,):
+            raise ValueError("lens must be [B]")
+    elif lens is not None:
+        raise ValueError("lens without caches")
+    if prefix_k is not None and (prefix_k.dim() != 3 or prefix_k.shape[0] != nkv or prefix_k.shape[2] != d):
+        raise ValueError("the prefix must be [n_kv, length, d] with the caches' heads and q's head size")
+    if nkv == 0 or nh % nkv:
+        raise ValueError("n_heads must be a multiple of n_kv")
+    return _lib.CacheAttnConfig(nh, nkv, d, cache_k.shape[2] if cache_k is not None else 0,
+                                prefix_k.shape[1] if prefix_k is not None else 0, ld, float(scale)), B, L
+
+
+def attention_prefix(q, prefix_k, prefix_v, cache_k=None, cache_v=None, lens=None, prefix_len=None, scale=0.0,
+                     handle=None) -> torch.Tensor:
+    """Attention of a batch whose sequences share a prefix, read once for all: q [B, L, nh, d]
+    (rotated; a view of wider rows may be given), prefix_k / prefix_v [n_kv, P, d] of which the
+    first prefix_len rows count (default all), and each sequence's own caches
+    [B, n_kv, max_len, d] with lens [B] int32 filled slots, the L new tokens' among them:
+    token l sees the prefix and the slots j <= lens[b] - L + l.  Returns [B, L, nh, d]."""
+    cfg, B, L = _cache_attn(q, cache_k, lens, prefix_k, scale)
+    dev = q.device
+    if prefix_k is not None:
+        _need_caches(prefix_k, prefix_v, dev, "prefix")
+    if cache_k is not None:
+        _need_caches(cache_k, cache_v, dev)
+    n = cfg.prefix_max if prefix_len is None else int(prefix_len)
+    if not 0 <= n <= cfg.prefix_max:
+        raise ValueError("prefix_len is not within the prefix")
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    h = handle or default_handle(dev.index)
+    h.bind_stream()
+    h.check(h.lib.fm_attention_prefix(h.h, C.byref(cfg), _ptr(q), _ptr(prefix_k), _ptr(prefix_v), n, _ptr(cache_k),
+                                      _ptr(cache_v), _ptr(lens), B, L, _ptr(out)))
+    return out
+
+
+def attention_scored(q, cache_k, cache_v, lens, acc, scale=0.0, handle=None) -> torch.Tensor:
+    """attention_prefix without a prefix that also adds to acc [B, n_kv, max_len] fp32 each
+    slot's attention probabilities, summed over the kv head's query heads and the L tokens."""
+    cfg, B, L = _cache_attn(q, cache_k, lens, None, scale)
+    dev = q.device
+    _need_caches(cache_k, cache_v, dev)
+    _need(acc, "acc", _F32, dev)
+    if acc.shape != cache_k.shape[:3]:
+        raise ValueError("acc must be [B, n_kv, max_len]")
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    h = handle or default_handle(dev.index)
+    h.bind_stream()
+    h.check(h.lib.fm_attention_scored(h.h, C.byref(cfg), _ptr(q), _ptr(cache_k), _ptr(cache_v), _ptr(lens), B, L,
+                                      _ptr(acc), _ptr(out)))
+    return out
+
+
+def cache_evict(cache_k, cache_v, acc, lens, budget, sinks=0, recent=0, positions=None, out=None, lens_out=None,
+                handle=None) -> torch.Tensor:
+    """Cuts every (sequence, kv head) of the caches [B, n_kv, max_len, d] down to
+    n = min(lens[b], budget) slots, those of the largest acc [B, n_kv, max_len]; positions
+    below `sinks` and above the newest - `recent` stay whatever their weight (positions
+    [B, n_kv, max_len] int32, a slot's index without them).  In place, or into
+    out = (k, v, acc, positions) of [B, n_kv, M >= budget, ...] (positions may be None when
+    `positions` is).  Slots that stay below n keep their places, the others below n take those
+    from n on in order.  Returns the new lengths [B] (lens_out if given; it may be lens)."""
+    _need(cache_k, "cache_k", _BF16, None)
+    dev = cache_k.device
+    _need_caches(cache_k, cache_v, dev)
+    if cache_k.dim() != 4:
+        raise ValueError("caches must be [B, n_kv, max_len, d]")
+    B, nkv, max_len, d = cache_k.shape
+
+    def beside(a, p, name, rows):
+        _need(a, name + "acc", _F32, dev)
+        if tuple(a.shape) != (B, nkv, rows):
+            raise ValueError(name + "acc must be [B, n_kv, max_len]")
+        if p is not None:
+            _need(p, name + "positions", _I32, dev)
+            if p.shape != a.shape:
+                raise ValueError(name + "positions must be [B, n_kv, max_len]")
+
+    beside(acc, positions, "", max_len)
+    if out is None:
+        out = (cache_k, cache_v, acc, positions)
+    ok, ov, oacc, opos = out
+    _need_caches(ok, ov, dev, "out")
+    if ok.dim() != 4 or (ok.shape[0], ok.shape[1], ok.shape[3]) != (B, nkv, d):
+        raise ValueError("the output caches must be [B, n_kv, length, d]")
+    beside(oacc, opos, "out ", ok.shape[2])
+    if lens_out is None:
+        lens_out = torch.empty_like(lens)
+    for t, n in ((lens, "lens"), (lens_out, "lens_out")):
+        _need(t, n, _I32, dev)
+        if tuple(t.shape) != (B,):
+            raise ValueError(f"{n} must be [B]")
+    cfg = _lib.EvictConfig(nkv, d, max_len, ok.shape[2], int(budget), int(sinks), int(recent))
+    h = handle or default_handle(dev.index)
+    h.bind_stream()
+    h.check(h.lib.fm_cache_evict(h.h, C.byref(cfg), _ptr(cache_k), _ptr(cache_v), _ptr(acc), _ptr(positions),
+                                 _ptr(lens), B, _ptr(ok), _ptr(ov), _ptr(oacc), _ptr(opos), _ptr(lens_out)))
+    return lens_out

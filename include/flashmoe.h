@@ -326,6 +326,122 @@ FM_API int fm_swiglu(fm_handle* h, const uint16_t* gate, const uint16_t* up, int
  * Replaces sample_token at temperature 0, mx::argmax(logits, -1) (sampling.cpp:5-7). */
 FM_API int fm_argmax(fm_handle* h, const uint16_t* logits, int64_t T, int64_t V, int32_t* ids);
 
+/* Serving over long and shared caches ---------------------------------------------
+ * What a server with long conversations needs around fm_attention, whose batch has one
+ * offset and whose caches only grow: positions per token, a prefix that the batch shares
+ * without copies (the reference copies it into every request's cache,
+ * scheduler.cpp:121-168), caches of ragged lengths, and caches that give up their lightest
+ * slots.  A decode step is fm_rope_append, then fm_attention_prefix or
+ * fm_attention_scored, then from time to time fm_cache_evict.
+ *
+ * bf16 rows are 16-byte aligned, and the strides given in elements are multiples of 8.
+ * Caches are [B, n_kv_heads, max_len, head_dim] as for fm_attention; lens, positions and
+ * slots are int32 in device memory.  An entry of them that is out of range is reported by
+ * FM_EDEVICE at the next fm_sync_status and its memory is not touched.
+ *
+ * These calls keep their partial results in a workspace of the handle that grows with the
+ * largest call and whose earlier blocks stay until fm_destroy, so a captured call stays
+ * valid when a later one needs more; a call that would have to grow it on a capturing
+ * stream returns FM_EINVAL and leaves the capture intact (fm_serve_reserve, or one call
+ * before the capture).  Calls of one handle share the workspace: calls, and replays of graphs
+ * captured from it, must not overlap on the GPU. */
+#define FM_ROPE_UNSCALED 0 /* theta^(-2i/r) */
+#define FM_ROPE_LINEAR 1   /* every frequency / factor (position interpolation) */
+#define FM_ROPE_NTK 2      /* base theta * factor^(r / (r - 2)) */
+#define FM_ROPE_YARN 3     /* by parts: pairs that turn more than `high` times over
+                              original_len keep their frequency, below `low` times take
+                              frequency / factor, linear in the pair's index between (the two
+                              indices rounded outwards); cos and sin times 0.1 ln(factor) + 1 */
+#define FM_ROPE_BANDED 4   /* the same two ends, blended linearly in the pair's turns over
+                              original_len, without a factor on cos and sin */
+
+typedef struct fm_rope_config {
+  int head_dim;        /* a multiple of 8, at most 256 */
+  int rotary_dim;      /* r: the leading elements of a head that rotate (even); 0 = head_dim.  The
+                          others are copied */
+  int traditional;     /* 1: pairs (2i, 2i + 1), mx::fast::rope's traditional form; 0: (i, i + r/2) */
+  int scaling;         /* FM_ROPE_* */
+  float theta;         /* base */
+  float factor;        /* of the scalings, >= 1 */
+  float original_len;  /* FM_ROPE_YARN, FM_ROPE_BANDED: the trained length */
+  float low, high;     /* their turns over original_len, low < high */
+  float attn_factor;   /* on cos and sin; 0 = 1, or FM_ROPE_YARN's own */
+} fm_rope_config;
+
+/* y[t, h] = x[t, h] rotated at positions[t], for n_heads heads lying side by side in rows x_ld
+ * (y_ld) apart.  Positions may be any int32; negative ones rotate back, so keys in a cache
+ * can be moved to other positions.  y may be x (with y_ld == x_ld).  Angles are reduced in
+ * 64 bits, so far positions keep their precision.  Replaces mx::fast::rope
+ * (model.cpp:588-589) where fm_attention's fused form does not fit. */
+FM_API int fm_rope(fm_handle* h, const fm_rope_config* cfg, const uint16_t* x, int64_t x_ld, int n_heads,
+                   const int32_t* positions, int64_t T, uint16_t* y, int64_t y_ld);
+
+/* A step's q, k and v, T = B * L tokens: q_out[t] = q[t] rotated at positions[t] (q_out may be q),
+ * k[t] rotated and v[t] as it is into slot slots[t] of sequence t / L's caches.  slots[t] < 0
+ * writes nothing to the caches (a padding token).  The slots of one sequence must differ. */
+FM_API int fm_rope_append(fm_handle* h, const fm_rope_config* cfg, const uint16_t* q, int64_t q_ld, int n_heads,
+                          const uint16_t* k, const uint16_t* v, int64_t kv_ld, int n_kv_heads,
+                          const int32_t* positions, const int32_t* slots, int B, int L, uint16_t* cache_k,
+                          uint16_t* cache_v, int max_len, uint16_t* q_out, int64_t q_out_ld);
+
+typedef struct fm_cache_attn_config {
+  int n_heads;
+  int n_kv_heads;  /* divides n_heads */
+  int head_dim;    /* 64 or 128 */
+  int max_len;     /* slots per (sequence, kv head) of the caches */
+  int prefix_max;  /* rows per kv head of the prefix buffers */
+  int q_ld;        /* elements from one token's q row to the next; 0 = n_heads * head_dim */
+  float scale;     /* softmax scale; 0 = 1/sqrt(head_dim) */
+} fm_cache_attn_config;
+
+/* Attention of L new tokens of each of B sequences (rotated q rows [B * L, q_ld], their k and v
+ * already in the caches) over a prefix that all share, prefix_k / prefix_v
+ * [n_kv_heads, prefix_max, head_dim] rows [0, prefix_len), and each sequence's own cache:
+ * token l of sequence b sees the whole prefix and the slots j <= lens[b] - L + l, lens[b]
+ * counting the new tokens.  A token that sees nothing (no prefix, and lens[b] too short) gives
+ * zeros.  out is [B * L, n_heads * head_dim].  prefix_len may be 0 (prefix pointers NULL); lens
+ * NULL means no own caches (cache pointers NULL). */
+FM_API int fm_attention_prefix(fm_handle* h, const fm_cache_attn_config* cfg, const uint16_t* q,
+                               const uint16_t* prefix_k, const uint16_t* prefix_v, int prefix_len,
+                               const uint16_t* cache_k, const uint16_t* cache_v, const int32_t* lens, int B, int L,
+                               uint16_t* out);
+
+/* The same without a prefix, and acc[b, kvh, j] += the sum, over kv head kvh's query heads and
+ * the L tokens, of the attention probability of slot j (fp32 [B, n_kv_heads, max_len]; slots
+ * at or past lens[b] are left as they were). */
+FM_API int fm_attention_scored(fm_handle* h, const fm_cache_attn_config* cfg, const uint16_t* q,
+                               const uint16_t* cache_k, const uint16_t* cache_v, const int32_t* lens, int B, int L,
+                               float* acc, uint16_t* out);
+
+typedef struct fm_evict_config {
+  int n_kv_heads;
+  int head_dim;     /* a multiple of 8, at most 256 */
+  int max_len;      /* slots per (sequence, kv head) of the caches, acc and positions */
+  int out_max_len;  /* the same of the outputs */
+  int budget;       /* slots that stay, >= 1 */
+  int sinks;        /* positions below it stay */
+  int recent;       /* so do the positions above newest - recent; sinks + recent <= budget */
+} fm_evict_config;
+
+/* Cuts each (sequence, kv head) down to n = min(lens[b], budget) slots.  The n that stay: first
+ * the protected ones (sinks and recent, by positions [B, n_kv_heads, max_len], or by slot
+ * index when NULL; lower slots first), then by acc descending (NaN as -inf, equal weights the
+ * lower slot first).  A slot that stays and lies below n keeps its place; the places left
+ * below n take the slots that stay from n on, both in ascending order -- so a step that is
+ * one slot over moves one row.  k, v, acc and position of a slot move together; out_lens[b]
+ * = n (out_lens may be lens).  In place when the outputs are the inputs (out_max_len ==
+ * max_len then); otherwise every slot that stays is copied into the outputs, which may not
+ * overlap the inputs.  Slots from n on are left as they were.  out_positions may be NULL when
+ * positions is. */
+FM_API int fm_cache_evict(fm_handle* h, const fm_evict_config* cfg, const uint16_t* cache_k, const uint16_t* cache_v,
+                          const float* acc, const int32_t* positions, const int32_t* lens, int B, uint16_t* out_k,
+                          uint16_t* out_v, float* out_acc, int32_t* out_positions, int32_t* out_lens);
+
+/* Sizes the workspace for fm_attention_prefix / fm_attention_scored calls of up to B sequences
+ * of L tokens over cfg's caches and prefix_max, and for fm_cache_evict of such a batch, so
+ * that later calls do not allocate. */
+FM_API int fm_serve_reserve(fm_handle* h, const fm_cache_attn_config* cfg, int B, int L);
+
 /* Expert parallelism ------------------------------------------------------------
  * No reference counterpart: the reference runs the whole MoE layer in one process
  * (model.cpp:750-807).  These calls split fm_moe_block into the three stages of an

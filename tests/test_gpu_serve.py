@@ -1,0 +1,519 @@
+"""The serving operators (fm_rope, fm_rope_append, fm_attention_prefix, fm_attention_scored,
+fm_cache_evict) on a B200 against the plain 64-bit implementations of tests/serve_util.py,
+with the tolerances derived there; moves and lengths are exact."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests import serve_util as R
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+
+
+@pytest.fixture(autouse=True)
+def _clean_status():
+    """No call leaves a device-side report unless its test expects and reads it."""
+    yield
+    from flashmlx_b200 import ops
+    ops.synchronize()
+
+
+def rnd(seed, *shape, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * std).to(BF).cuda()
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def held(got, want, tol, what=""):
+    err = (got.double().cpu() - want).abs()
+    assert torch.isfinite(got).all(), what
+    bad = err > tol
+    assert not bad.any(), f"{what}: {int(bad.sum())} outside, worst {float((err / tol.clamp_min(1e-300)).max()):.2f} times the tolerance"
+
+
+# ------------------------------------------------------------------ refusals (host side, nothing launched)
+def refused(call, status=None):
+    from flashmlx_b200 import _lib
+    with pytest.raises((ValueError, TypeError, NotImplementedError, _lib.FlashMoEError)) as e:
+        call()
+    if isinstance(e.value, _lib.FlashMoEError) and status is not None:
+        assert e.value.status == status
+
+
+def test_rope_refusals():
+    from flashmlx_b200 import _lib, ops
+    x, p = rnd(1, 3, 2, 64), i32([0, 1, 2])
+    bad = [
+        lambda: ops.rope(x.float(), p, 1e4), lambda: ops.rope(x.half(), p, 1e4), lambda: ops.rope(x, p.long(), 1e4),
+        lambda: ops.rope(x, p[:2], 1e4), lambda: ops.rope(x, p, 1e4, rotary_dim=3),
+        lambda: ops.rope(x, p, 1e4, rotary_dim=66), lambda: ops.rope(x, p, 0.0), lambda: ops.rope(x, p, float("nan")),
+        lambda: ops.rope(x, p, 1e4, scaling={"type": "linear", "factor": 0.5}),
+        lambda: ops.rope(x, p, 1e4, rotary_dim=2, scaling={"type": "ntk", "factor": 2.0}),
+        lambda: ops.rope(x, p, 1e4, scaling={"type": "yarn", "factor": 2.0, "original_len": 0}),
+        lambda: ops.rope(x, p, 1e4, scaling={"type": "banded", "factor": 2.0, "original_len": 64, "low_freq": 4.0,
+                                             "high_freq": 4.0}),
+        lambda: ops.rope(rnd(1, 3, 2, 60), p, 1e4),            # head size not a multiple of 8
+        lambda: ops.rope(x.transpose(1, 2).contiguous().transpose(1, 2), p, 1e4),  # heads not side by side
+        lambda: ops.rope(x, p, 1e4, out=torch.empty(3, 2, 32, dtype=BF, device="cuda")),
+        lambda: ops.rope(rnd(1, 4, 2, 64)[:3], p, 1e4, out=rnd(1, 3, 2, 64).float()),
+    ]
+    base = rnd(2, 4, 2, 64)
+    bad.append(lambda: ops.rope(base[:3], p, 1e4, out=base[1:]))  # partly overlapping
+    wide = rnd(3, 3 * 140)[: 3 * 132].view(3, 132)
+    bad.append(lambda: ops.rope(wide[:, :128].view(3, 2, 64), p, 1e4))  # a row stride that is no multiple of 8
+    for call in bad:
+        refused(call, _lib.FM_EINVAL if call is not bad[12] else _lib.FM_EUNSUPPORTED)
+
+
+def test_attention_refusals():
+    from flashmlx_b200 import _lib, ops
+    q, ck, lens = rnd(4, 2, 1, 4, 64), rnd(5, 2, 2, 16, 64), i32([3, 4])
+    pk = rnd(6, 2, 8, 64)
+    acc = torch.zeros(2, 2, 16, device="cuda")
+    h = ops.default_handle()
+    cfg = _lib.CacheAttnConfig(4, 2, 64, 16, 8, 0, 0.0)
+    for call in [
+        lambda: ops.attention_prefix(q, None, None), lambda: ops.attention_prefix(q, pk, pk, ck, ck, None),
+        lambda: ops.attention_prefix(q, pk, pk[:1], ck, ck, lens), lambda: ops.attention_prefix(q, pk, pk, prefix_len=9),
+        lambda: ops.attention_prefix(q, pk, pk, prefix_len=-1), lambda: ops.attention_prefix(q, pk, pk, lens=lens),
+        lambda: ops.attention_prefix(q[:1], pk, pk, ck, ck, lens), lambda: ops.attention_prefix(q.half(), pk, pk, ck, ck, lens),
+        lambda: ops.attention_prefix(rnd(7, 2, 1, 4, 32), rnd(7, 2, 8, 32), rnd(7, 2, 8, 32)),  # head size 32
+        lambda: ops.attention_prefix(rnd(7, 2, 1, 3, 64), pk, pk, ck, ck, lens),                # 3 heads over 2
+        lambda: ops.attention_prefix(q, pk, pk, ck, ck, lens, scale=float("nan")),
+        lambda: ops.attention_scored(q, ck, ck, lens.long(), acc), lambda: ops.attention_scored(q, ck, ck, lens, acc[:1]),
+        lambda: ops.attention_scored(q, ck, ck, lens, acc.half()), lambda: ops.attention_scored(q, ck, ck[:, :1], lens, acc),
+        lambda: h.check(h.lib.fm_attention_prefix(h.h, _lib.C.byref(cfg), q.data_ptr(), None, None, 4, None, None, None, 2, 1,
+                                                  q.data_ptr())),
+        lambda: h.check(h.lib.fm_attention_prefix(h.h, _lib.C.byref(cfg), q.data_ptr(), pk.data_ptr(), pk.data_ptr(), 4, None,
+                                                  None, None, 2, 1, q.data_ptr())),  # out is q
+        lambda: h.check(h.lib.fm_attention_prefix(h.h, _lib.C.byref(cfg), q.data_ptr() + 2, pk.data_ptr(), pk.data_ptr(), 4,
+                                                  None, None, None, 2, 1, ck.data_ptr())),
+        lambda: h.check(h.lib.fm_serve_reserve(h.h, _lib.C.byref(cfg), -1, 1)),
+    ]:
+        refused(call)
+
+
+def test_evict_refusals():
+    from flashmlx_b200 import ops
+    ck, cv, acc, lens = rnd(8, 2, 2, 16, 64), rnd(9, 2, 2, 16, 64), torch.zeros(2, 2, 16, device="cuda"), i32([9, 16])
+    pos = torch.zeros(2, 2, 16, dtype=torch.int32, device="cuda")
+    small = (rnd(1, 2, 2, 3, 64), rnd(1, 2, 2, 3, 64), torch.zeros(2, 2, 3, device="cuda"), None)
+    other = torch.zeros_like(acc)
+    for call in [
+        lambda: ops.cache_evict(ck, cv, acc, lens, 0), lambda: ops.cache_evict(ck, cv, acc, lens, 4, sinks=3, recent=2),
+        lambda: ops.cache_evict(ck, cv, acc, lens, 4, sinks=-1), lambda: ops.cache_evict(ck, cv, acc, lens, 4, out=small),
+        lambda: ops.cache_evict(ck, cv, acc, lens, 4, out=(ck, cv, other, None)),      # half in place
+        lambda: ops.cache_evict(ck, cv, acc, lens, 4, out=(cv, ck, acc, None)),        # crosswise
+        lambda: ops.cache_evict(ck, cv, acc, lens, 4, positions=pos, out=(ck, cv, acc, None)),
+        lambda: ops.cache_evict(ck, cv, acc.double(), lens, 4), lambda: ops.cache_evict(ck, cv, acc, lens[:1], 4),
+        lambda: ops.cache_evict(ck, cv[:1], acc, lens, 4),
+        lambda: ops.cache_evict(ck[:, :, ::2], cv[:, :, ::2], acc[:, :, :8].contiguous(), lens, 4),
+    ]:
+        refused(call)
+
+
+# ------------------------------------------------------------------ rotary positions
+YARN = {"type": "yarn", "factor": 4.0, "original_len": 4096, "beta_slow": 1.0, "beta_fast": 32.0}
+BANDED = {"type": "banded", "factor": 8.0, "original_len": 8192, "low_freq": 1.0, "high_freq": 4.0}
+
+
+@pytest.mark.parametrize("T,heads,d,rotary,traditional,scaling", [
+    (1, 1, 8, None, False, None),
+    (1, 36, 128, None, False, None),
+    (5, 4, 64, 32, True, {"type": "linear", "factor": 4.0}),
+    (3, 2, 64, 20, False, YARN),                       # half of 10: pair by pair
+    (3, 3, 24, 6, True, {"type": "ntk", "factor": 2.0}),
+    (7, 2, 128, 64, True, BANDED),
+    (129, 5, 256, 2, False, None),
+    (1300, 6, 64, None, False, YARN),                  # several tokens a block, a ragged last block
+    (1301, 2, 128, 96, True, {"type": "yarn", "factor": 2.0, "original_len": 512, "beta_slow": 1.0, "beta_fast": 32.0,
+                              "attn_factor": 1.25}),
+])
+def test_rope(T, heads, d, rotary, traditional, scaling):
+    from flashmlx_b200 import ops
+    x = rnd(10 + T, T, heads, d)
+    g = torch.Generator().manual_seed(T)
+    pos = torch.randint(-2000000, 2000000, (T,), generator=g, dtype=torch.int32)
+    pos[0] = 2 ** 31 - 1
+    if T > 2:
+        pos[1], pos[2] = -2 ** 31, 0
+    want, tol = R.rope(x, pos, 1e4, rotary, traditional, scaling)
+    kw = dict(rotary_dim=rotary, traditional=traditional, scaling=scaling)
+    y = ops.rope(x, pos.cuda(), 1e4, **kw)
+    held(y, want, tol)
+    # in place inside a wider row (a fused projection's), whose other columns stay
+    wide = rnd(11, T, (heads + 2) * d)
+    before = wide.clone()
+    view = wide[:, d:(heads + 1) * d].view(T, heads, d)
+    view.copy_(x)
+    assert ops.rope(view, pos.cuda(), 1e4, out=view, **kw) is view
+    assert torch.equal(view, y)
+    assert torch.equal(wide[:, :d], before[:, :d]) and torch.equal(wide[:, (heads + 1) * d:], before[:, (heads + 1) * d:])
+
+
+def test_rope_turns_back():
+    """Negated positions undo a rotation but for the two roundings."""
+    from flashmlx_b200 import ops
+    x, pos = rnd(12, 40, 3, 128), torch.arange(1000, 1040, dtype=torch.int32, device="cuda")
+    back = ops.rope(ops.rope(x, pos, 1e6), -pos, 1e6)
+    f = x.double().cpu()
+    size = f.abs() + torch.cat((f[..., 64:], f[..., :64]), -1).abs()
+    held(back, f, size * (3 * R.U16))
+
+
+def test_rope_no_tokens():
+    from flashmlx_b200 import ops
+    assert ops.rope(rnd(1, 0, 2, 64), i32([]), 1e4).shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("B,L,nh,nkv,d,traditional,rotary", [
+    (1, 1, 4, 4, 128, False, None), (3, 5, 4, 2, 64, True, 32), (2, 7, 6, 2, 40, False, 12), (2, 600, 2, 1, 64, False, None)])
+def test_rope_append(B, L, nh, nkv, d, traditional, rotary):
+    from flashmlx_b200 import ops
+    M, T = L + 9, B * L
+    qkv = rnd(20, T, nh + 2 * nkv, d)
+    q, k, v = qkv[:, :nh], qkv[:, nh:nh + nkv], qkv[:, nh + nkv:]
+    ck, cv = rnd(21, B, nkv, M, d), rnd(22, B, nkv, M, d)
+    ck0, cv0 = ck.clone(), cv.clone()
+    slots = torch.stack([torch.randperm(M, generator=torch.Generator().manual_seed(b))[:L] for b in range(B)]).int()
+    slots[-1, L // 2] = -1  # a padding token
+    pos = torch.arange(100, 100 + T, dtype=torch.int32)
+    before = qkv.clone()
+    got = ops.rope_append(q, k, v, pos.cuda(), slots.reshape(-1).cuda(), ck, cv, 1e6, traditional=traditional,
+                          rotary_dim=rotary)
+    assert torch.equal(qkv, before)
+    held(got, *R.rope(q, pos, 1e6, rotary, traditional), what="q")
+    rot = ops.rope(k, pos.cuda(), 1e6, rotary_dim=rotary, traditional=traditional)  # held to the formula above
+    for t in range(T):
+        s = int(slots.reshape(-1)[t])
+        if s >= 0:
+            ck0[t // L, :, s], cv0[t // L, :, s] = rot[t], v[t]
+    assert torch.equal(ck, ck0) and torch.equal(cv, cv0)
+    assert ops.rope_append(q, k, v, pos.cuda(), slots.reshape(-1).cuda(), ck, cv, 1e6, traditional=traditional,
+                           rotary_dim=rotary, out=q) is q
+    assert torch.equal(q, got)
+
+
+def test_rope_append_reports_a_slot_past_the_cache():
+    from flashmlx_b200 import _lib, ops
+    ck, cv = rnd(23, 1, 2, 8, 64), rnd(24, 1, 2, 8, 64)
+    k0, x = ck.clone(), rnd(25, 2, 2, 64)
+    ops.rope_append(x, x, x, i32([0, 1]), i32([8, 3]), ck, cv, 1e4)
+    with pytest.raises(_lib.FlashMoEError) as e:
+        ops.synchronize()
+    assert e.value.status == _lib.FM_EDEVICE
+    k0[:, :, 3] = ck[:, :, 3]
+    assert torch.equal(ck, k0) and torch.equal(cv[0, :, 3], x[1])
+
+
+# ------------------------------------------------------------------ attention
+def caches(seed, B, nkv, M, d, lens):
+    """Random caches whose slots past each length are NaN (K) and infinite (V)."""
+    ck, cv = rnd(seed, B, nkv, M, d), rnd(seed + 1, B, nkv, M, d)
+    for b, n in enumerate(lens):
+        ck[b, :, max(n, 0):] = float("nan")
+        cv[b, :, max(n, 0):] = float("inf")
+    return ck, cv
+
+
+@pytest.mark.parametrize("B,L,nh,nkv,d,P,lens,M", [
+    (1, 1, 1, 1, 64, 1, [0], 1),
+    (1, 1, 4, 4, 128, 0, [1], 3),
+    (3, 1, 4, 2, 64, 97, [1, 17, 41], 41),
+    (2, 1, 32, 4, 128, 300, [0, 129], 130),
+    (4, 3, 8, 2, 64, 63, [3, 2, 0, 70], 75),            # fewer slots than tokens: early ones see the prefix alone
+    (3, 2, 6, 2, 128, 0, [1, 0, 33], 40),               # rows that see nothing
+    (5, 1, 16, 16, 128, 129, [5, 128, 16, 127, 255], 256),
+    (2, 17, 8, 2, 64, 40, [17, 64], 64),
+    (1, 70, 6, 2, 128, 31, [200], 207),
+    (40, 1, 8, 2, 64, 1000, list(range(0, 80, 2)), 80),
+    (2, 1, 4, 2, 128, 5000, [7, 3], 9),
+    (1, 300, 4, 1, 64, 10, [300], 300),
+    (33, 5, 8, 2, 128, 517, [5 + 9 * (i % 7) for i in range(33)], 60),
+])
+def test_attention_prefix(B, L, nh, nkv, d, P, lens, M):
+    from flashmlx_b200 import ops
+    q = rnd(30 + B + L, B, L, nh, d)
+    ck, cv = caches(31, B, nkv, M, d, lens)
+    pk = pv = None
+    if P:
+        pk, pv = rnd(33, nkv, P, d), rnd(34, nkv, P, d)
+    out = ops.attention_prefix(q, pk, pv, ck, cv, i32(lens))
+    want, tol, _, _ = R.attention(q, ck, cv, lens, pk, pv)
+    held(out, want, tol)
+    # q rows of a fused projection, the prefix in a longer buffer
+    wide = rnd(35, B, L, nh + 2 * nkv, d)
+    wide[:, :, :nh] = q
+    long = [None, None]
+    if P:
+        long = [torch.full((nkv, P + 21, d), float("nan"), dtype=BF, device="cuda") for _ in range(2)]
+        long[0][:, :P], long[1][:, :P] = pk, pv
+    again = ops.attention_prefix(wide[:, :, :nh], long[0], long[1], ck, cv, i32(lens), prefix_len=P if P else None)
+    assert torch.equal(again, out)
+
+
+def test_attention_prefix_alone():
+    from flashmlx_b200 import ops
+    q, pk, pv = rnd(40, 9, 2, 8, 64), rnd(41, 4, 130, 64), rnd(42, 4, 130, 64)
+    want, tol, _, _ = R.attention(q, None, None, None, pk, pv)
+    held(ops.attention_prefix(q, pk, pv), want, tol)
+    assert torch.equal(ops.attention_prefix(q, pk, pv, prefix_len=0), torch.zeros_like(q))
+
+
+def test_attention_prefix_large_scores():
+    """Scores of several hundred: the running maximum, not the exponent's range, carries them."""
+    from flashmlx_b200 import ops
+    q, lens = rnd(43, 2, 1, 4, 64, std=30.0), [200, 90]
+    ck, cv = caches(44, 2, 2, 200, 64, lens)
+    pk, pv = rnd(46, 2, 100, 64, std=10.0), rnd(47, 2, 100, 64)
+    want, tol, _, _ = R.attention(q, ck, cv, lens, pk, pv)
+    held(ops.attention_prefix(q, pk, pv, ck, cv, i32(lens)), want, tol)
+
+
+@pytest.mark.parametrize("scale", [0.25, -0.1])
+def test_attention_scale(scale):
+    from flashmlx_b200 import ops
+    q, lens = rnd(48, 2, 3, 4, 64), [30, 5]
+    ck, cv = caches(49, 2, 2, 33, 64, lens)
+    acc = torch.zeros(2, 2, 33, device="cuda")
+    want, tol, a, at = R.attention(q, ck, cv, lens, acc=acc, scale=scale)
+    held(ops.attention_scored(q, ck, cv, i32(lens), acc, scale=scale), want, tol)
+    held(acc, a, at)
+
+
+@pytest.mark.parametrize("B,L,nh,nkv,d,lens,M", [
+    (1, 1, 1, 1, 64, [1], 1),
+    (2, 1, 4, 4, 128, [0, 37], 40),
+    (3, 1, 32, 4, 128, [1, 700, 129], 700),
+    (2, 4, 8, 2, 64, [2, 100], 101),
+    (1, 130, 8, 2, 64, [130], 131),
+    (2, 200, 6, 2, 128, [333, 200], 340),
+    (1, 513, 4, 1, 64, [600], 600),
+    (17, 1, 16, 16, 64, [3 * i for i in range(17)], 64),
+])
+def test_attention_scored(B, L, nh, nkv, d, lens, M):
+    from flashmlx_b200 import ops
+    q = rnd(50 + L, B, L, nh, d)
+    ck, cv = caches(51, B, nkv, M, d, lens)
+    acc = torch.rand(B, nkv, M, generator=torch.Generator().manual_seed(5)).cuda()
+    first = acc.clone()
+    want, tol, a, at = R.attention(q, ck, cv, lens, acc=acc)
+    out = ops.attention_scored(q, ck, cv, i32(lens), acc)
+    held(out, want, tol, "out")
+    held(acc, a, at, "acc")
+    for b, n in enumerate(lens):
+        assert torch.equal(acc[b, :, n:], first[b, :, n:])
+    twice = first.clone()  # the same sums in the same order every time
+    assert torch.equal(ops.attention_scored(q, ck, cv, i32(lens), twice), out) and torch.equal(twice, acc)
+
+
+def test_lengths_out_of_range_are_reported():
+    from flashmlx_b200 import _lib, ops
+    q = rnd(60, 3, 1, 4, 64)
+    ck, cv = rnd(61, 3, 2, 16, 64), rnd(62, 3, 2, 16, 64)
+    acc = torch.zeros(3, 2, 16, device="cuda")
+    lens = [17, 9, -1]
+    out = ops.attention_scored(q, ck, cv, i32(lens), acc)
+    with pytest.raises(_lib.FlashMoEError) as e:
+        ops.synchronize()
+    assert e.value.status == _lib.FM_EDEVICE
+    want, tol, a, at = R.attention(q, ck, cv, [0, 9, 0], acc=torch.zeros(3, 2, 16))
+    held(out, want, tol)
+    held(acc, a, at)
+
+
+def test_attention_far_into_a_large_cache():
+    """Element offsets past 2^31."""
+    from flashmlx_b200 import ops
+    B, nkv, M, d = 34, 8, 65536, 128
+    ck = torch.empty(B, nkv, M, d, dtype=BF, device="cuda")
+    cv = torch.empty_like(ck)
+    lens = [0] * B
+    lens[-1] = 200
+    ck[-1, :, :200], cv[-1, :, :200] = rnd(63, nkv, 200, d), rnd(64, nkv, 200, d)
+    q = rnd(65, B, 1, 8, d)
+    out = ops.attention_prefix(q, None, None, ck, cv, i32(lens))
+    want, tol, _, _ = R.attention(q[-1:], ck[-1:, :, :200], cv[-1:, :, :200], [200])
+    held(out[-1:], want, tol)
+    assert not out[:-1].any()
+    acc = torch.rand(B, nkv, M, device="cuda")
+    acc[-1, :, 50] = 9.0
+    k50 = ck[-1, :, 50].clone()
+    ops.cache_evict(ck, cv, acc, i32(lens), 10)
+    assert (ck[-1, :, :10] == k50[:, None]).all(-1).any(-1).all()
+
+
+# ------------------------------------------------------------------ eviction
+@pytest.mark.parametrize("B,nkv,d,M,lens,budget,sinks,recent,weights", [
+    (1, 1, 64, 1, [1], 1, 0, 0, "rand"),
+    (2, 2, 64, 20, [20, 3], 7, 0, 0, "rand"),
+    (2, 2, 128, 41, [0, 41], 40, 4, 8, "rand"),
+    (3, 1, 64, 70, [70, 64, 33], 32, 2, 30, "ties"),
+    (2, 2, 8, 33, [33, 20], 5, 0, 0, "zeros"),
+    (2, 3, 40, 50, [50, 49], 16, 1, 3, "odd"),          # NaN, infinities, negative zeros
+    (1, 2, 256, 3000, [2999], 1500, 4, 100, "rand"),
+    (2, 2, 64, 5000, [5000, 1025], 1024, 0, 512, "ties"),
+    (1, 1, 64, 100, [100], 200, 0, 0, "rand"),           # nothing to evict
+])
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("given", [True, False])
+def test_cache_evict(B, nkv, d, M, lens, budget, sinks, recent, weights, in_place, given):
+    from flashmlx_b200 import ops
+    ck, cv = rnd(70, B, nkv, M, d), rnd(71, B, nkv, M, d)
+    g = torch.Generator().manual_seed(M + budget)
+    acc = torch.rand(B, nkv, M, generator=g)
+    if weights == "ties":
+        acc = (acc * 4).floor()
+    elif weights == "zeros":
+        acc.zero_()
+    elif weights == "odd":
+        acc[..., ::3], acc[..., 1::7], acc[..., 2::11], acc[..., 5::9] = float("nan"), float("inf"), -float("inf"), -0.0
+        acc[..., 6::9] = 0.0
+    pos = None
+    if given:  # positions in an order of their own, as after earlier evictions
+        pos = torch.stack([torch.randperm(3 * M, generator=g)[:M] for _ in range(B * nkv)]).view(B, nkv, M).int()
+    host = [ck.cpu(), cv.cpu(), acc.clone(), pos.clone() if given else None]
+    n = M if in_place else min(budget, M) + 3
+    to = host if in_place else [torch.zeros(B, nkv, n, d, dtype=BF), torch.zeros(B, nkv, n, d, dtype=BF),
+                                torch.zeros(B, nkv, n), torch.zeros(B, nkv, n, dtype=torch.int32)]
+    dev = [ck, cv, acc.cuda(), pos.cuda() if given else None]
+    out = dev if in_place else [t.cuda() for t in to]
+    source = [t.clone() if t is not None else None for t in host]
+    want = R.evict(host[0], host[1], host[2], host[3], lens, budget, sinks, recent, to)
+    lens_t = i32(lens)
+    got = ops.cache_evict(dev[0], dev[1], dev[2], lens_t, budget, sinks=sinks, recent=recent, positions=dev[3],
+                          out=None if in_place else tuple(out), lens_out=lens_t if in_place else None)
+    assert got.tolist() == want
+    for a, b in zip(out, to):
+        if b is not None:
+            assert torch.equal(a.cpu().nan_to_num(nan=-7.0), b.nan_to_num(nan=-7.0))
+    if not in_place:
+        for a, b in zip(dev, source):
+            if b is not None:
+                assert torch.equal(a.cpu().nan_to_num(nan=-7.0), b.nan_to_num(nan=-7.0))
+        assert lens_t.tolist() == lens
+
+
+def test_evict_reports_a_length_past_the_cache():
+    from flashmlx_b200 import _lib, ops
+    ck, cv, acc = rnd(72, 2, 1, 16, 64), rnd(73, 2, 1, 16, 64), torch.rand(2, 1, 16, device="cuda")
+    k0 = ck.clone()
+    got = ops.cache_evict(ck, cv, acc, i32([17, 16]), 8)
+    with pytest.raises(_lib.FlashMoEError) as e:
+        ops.synchronize()
+    assert e.value.status == _lib.FM_EDEVICE
+    assert got.tolist() == [0, 8] and torch.equal(ck[0], k0[0])
+
+
+# ------------------------------------------------------------------ together
+def test_a_conversation_that_evicts():
+    """Steps as a server makes them: append, attend and weigh, evict when over the budget; every
+    output, weight and cache against the plain forms carried along in 64 bits (the caches' bf16
+    rows are taken over, so that each step's error is its own)."""
+    from flashmlx_b200 import ops
+    B, nh, nkv, d, M, budget, sinks, recent, theta = 3, 4, 2, 64, 40, 32, 2, 6, 1e6
+    ck, cv = (torch.full((B, nkv, M, d), float("nan"), dtype=BF, device="cuda") for _ in range(2))
+    acc = torch.zeros(B, nkv, M, device="cuda")
+    positions = torch.zeros(B, nkv, M, dtype=torch.int32, device="cuda")
+    lens, seen = [0] * B, [0] * B
+    for step, new in enumerate([20, 1, 1, 9, 1, 1, 1, 7, 1, 1]):
+        qkv = rnd(80 + step, B * new, nh + 2 * nkv, d)
+        slots = torch.tensor([[lens[b] + i for i in range(new)] for b in range(B)], dtype=torch.int32)
+        pos = torch.tensor([[seen[b] + 10 * b + i for i in range(new)] for b in range(B)], dtype=torch.int32)
+        q = ops.rope_append(qkv[:, :nh], qkv[:, nh:nh + nkv], qkv[:, nh + nkv:], pos.view(-1).cuda(),
+                            slots.view(-1).cuda(), ck, cv, theta)
+        for b in range(B):
+            positions[b, :, lens[b]:lens[b] + new] = pos[b].cuda()
+            acc[b, :, lens[b]:lens[b] + new] = 0
+            lens[b] += new
+            seen[b] += new
+        before = acc.clone()
+        q = q.view(B, new, nh, d)
+        want, tol, a, at = R.attention(q, ck, cv, lens, acc=before)
+        out = ops.attention_scored(q, ck, cv, i32(lens), acc)
+        held(out, want, tol, f"step {step}")
+        held(acc, a, at, f"step {step} acc")
+        host = [t.cpu().clone() for t in (ck, cv, acc, positions)]
+        to = R.evict(*host, lens, budget, sinks, recent, host)
+        lens_t = i32(lens)
+        ops.cache_evict(ck, cv, acc, lens_t, budget, sinks=sinks, recent=recent, positions=positions, lens_out=lens_t)
+        assert lens_t.tolist() == to
+        lens = to
+        for x, y in zip((ck, cv, acc, positions), host):
+            assert torch.equal(x.cpu().nan_to_num(nan=-7.0), y.nan_to_num(nan=-7.0)), f"step {step}"
+
+
+def test_a_captured_step_follows_its_lengths():
+    """One graph of append + attention, replayed as the caches grow; a call that would grow the
+    workspace inside a capture is refused and the capture goes on."""
+    from flashmlx_b200 import _lib, ops
+    B, nh, nkv, d, M, P = 4, 8, 2, 64, 96, 50
+    h = ops.Handle()
+    pk, pv = rnd(90, nkv, P, d), rnd(91, nkv, P, d)
+    ck, cv = (torch.full((B, nkv, M, d), float("nan"), dtype=BF, device="cuda") for _ in range(2))
+    start = [0, 7, 30, 64]
+    for b, n in enumerate(start):
+        ck[b, :, :n], cv[b, :, :n] = rnd(92 + b, nkv, n, d), rnd(96 + b, nkv, n, d)
+    qkv = torch.zeros(B, nh + 2 * nkv, d, dtype=BF, device="cuda")
+    slots, lens = i32(start), i32([n + 1 for n in start])
+
+    def step():
+        q = ops.rope_append(qkv[:, :nh], qkv[:, nh:nh + nkv], qkv[:, nh + nkv:], slots, slots, ck, cv, 1e6, handle=h)
+        return ops.attention_prefix(q.view(B, 1, nh, d), pk, pv, ck, cv, lens, handle=h)
+
+    cfg = _lib.CacheAttnConfig(nh, nkv, d, M, P, 0, 0.0)
+    h.check(h.lib.fm_serve_reserve(h.h, _lib.C.byref(cfg), B, 1))
+    keep = ck.clone(), cv.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    ck.copy_(keep[0]), cv.copy_(keep[1])
+    many = rnd(99, 4000, 1, nh, d)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+        with pytest.raises(_lib.FlashMoEError) as e:
+            ops.attention_prefix(many, pk, pv, handle=h)
+        assert e.value.status == _lib.FM_EINVAL
+    big = ops.attention_prefix(many, pk, pv, handle=h)  # now it grows; the graph's block stays
+    want, tol, _, _ = R.attention(many[:3], None, None, None, pk, pv)
+    held(big[:3], want, tol)
+    for i in range(3):
+        qkv.copy_(rnd(100 + i, B, nh + 2 * nkv, d))
+        g.replay()
+        torch.cuda.synchronize()
+        q = ops.rope(qkv[:, :nh], slots, 1e6)  # held to the formula in test_rope
+        n = [s + 1 + i for s in start]
+        assert not torch.isnan(ck[0, :, :n[0]]).any()
+        want, tol, _, _ = R.attention(q.view(B, 1, nh, d), ck, cv, n, pk, pv)
+        held(out, want, tol, f"replay {i}")
+        slots += 1
+        lens += 1
+    h.sync()
+
+
+def test_two_streams_with_their_own_handles():
+    from flashmlx_b200 import ops
+    q, lens = rnd(110, 4, 1, 8, 128), [300, 20, 150, 77]
+    ck, cv = caches(111, 4, 2, 300, 128, lens)
+    one = ops.attention_prefix(q, None, None, ck, cv, i32(lens))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    handles = [ops.Handle() for _ in range(2)]
+    n = i32(lens)
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for s, h in zip(streams, handles):
+            with torch.cuda.stream(s):
+                got.append(ops.attention_prefix(q, None, None, ck, cv, n, handle=h))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, one) for x in got)
