@@ -2127,8 +2127,11 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
     if (e != cudaSuccess) return cuda_err(h, e, "cache attention kernel set-up");
     h->sv_ready = true;
   }
-  const fm::CacheAttnPlan p =
-      fm::cache_attn_plan(B, L, c->n_heads, c->n_kv_heads, c->head_dim, prefix_len, scored, h->num_sms);
+  const int nh = c->n_heads, nkv = c->n_kv_heads, d = c->head_dim;
+  const fm::CacheAttnPlan p = fm::cache_attn_plan(B, L, nh, nkv, d, prefix_len, lens != nullptr, scored, h->num_sms);
+  const int64_t own_rows = static_cast<int64_t>(B) * nkv * c->max_len, prefix_rows = static_cast<int64_t>(nkv) * c->prefix_max;
+  if ((p.tc_s && own_rows > 0x7fffff00LL) || (p.tc_p && prefix_rows > 0x7fffff00LL))
+    return set_err(h, FM_EUNSUPPORTED, "too many cache rows");
   rc = ensure_sv(h, p.bytes);
   if (rc != FM_OK) return rc;
   fm::CacheAttnArgs a;
@@ -2137,7 +2140,7 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
   a.q_ld = q_ld;
   a.pk = pk;
   a.pv = pv;
-  a.p_head = static_cast<int64_t>(c->prefix_max) * c->head_dim;
+  a.p_head = static_cast<int64_t>(c->prefix_max) * d;
   a.ck = ck;
   a.cv = cv;
   a.lens = lens;
@@ -2145,22 +2148,57 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
   a.acc = scored ? acc : nullptr;
   a.B = B;
   a.L = L;
-  a.nh = c->n_heads;
-  a.nkv = c->n_kv_heads;
-  a.group = c->n_heads / c->n_kv_heads;
+  a.nh = nh;
+  a.nkv = nkv;
+  a.group = nh / nkv;
   a.max_len = c->max_len;
-  a.prefix_len = prefix_len;
-  const double scale = c->scale != 0.f ? c->scale : 1.0 / std::sqrt(static_cast<double>(c->head_dim));
+  a.split_prefix = p.rt_p ? prefix_len : 0;
+  a.split_own = p.rt_s > 0;
+  const double scale = c->scale != 0.f ? c->scale : 1.0 / std::sqrt(static_cast<double>(d));
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-  a.rt_p = static_cast<int>(p.rt_p);
-  a.rt_s = static_cast<int>(p.rt_s);
+  a.rt_p = p.rt_p;
+  a.rt_s = p.rt_s;
   a.workers = p.workers;
   a.part_o = reinterpret_cast<float*>(h->sv_ws);
   a.part_ml = reinterpret_cast<float2*>(h->sv_ws + p.off_ml);
   a.lse2 = scored ? reinterpret_cast<float*>(h->sv_ws + p.off_lse) : nullptr;
   a.err = sv_err(h);
+  fm::TcAttnArgs t[2];
+  fm::TcMapsKV maps[2];
+  std::memset(t, 0, sizeof(t));
+  std::memset(maps, 0, sizeof(maps));
+  for (int i = 0; i < 2; ++i) {  // the prefix, the own caches
+    if (!(i ? p.tc_s : p.tc_p)) continue;
+    fm::TcAttnArgs& s = t[i];
+    s.q = q;
+    s.q_ld = q_ld;
+    s.lens = i ? lens : nullptr;
+    s.nseq = i ? B : 1;
+    s.L = i ? L : B * L;
+    s.nh = nh;
+    s.nkv = nkv;
+    s.group = a.group;
+    s.max_len = i ? c->max_len : prefix_len;
+    s.const_len = prefix_len;
+    s.causal = i;
+    s.head_rows = i ? c->max_len : c->prefix_max;
+    s.rps = i ? p.rps_s : p.rps_p;
+    s.workers = i ? p.workers_s : p.workers_p;
+    s.direct = i && prefix_len == 0;
+    s.scale_log2 = std::fabs(a.scale_log2);
+    s.q_sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+    s.part_o = reinterpret_cast<float*>(h->sv_ws + (i ? p.off_so : p.off_po));
+    s.part_ml = reinterpret_cast<float2*>(h->sv_ws + (i ? p.off_sml : p.off_pml));
+    s.out = out;
+    s.lse2 = a.lse2;
+    s.err = a.err;
+    const uint64_t rows = i ? own_rows : prefix_rows;
+    if (!encode_2d(&maps[i].k, false, i ? ck : pk, d, rows, 64, fm::kTcKeys) ||
+        !encode_2d(&maps[i].v, false, i ? cv : pv, d, rows, 64, fm::kTcKeys))
+      return set_err(h, FM_ECUDA, "cuTensorMapEncodeTiled failed");
+  }
   prof_begin(h, scored ? "attention_scored" : "attention_prefix");
-  const cudaError_t e = fm::launch_cache_attn(a, c->head_dim, h->stream);
+  const cudaError_t e = fm::launch_cache_attn(a, t[0], maps[0], t[1], maps[1], d, h->stream);
   prof_end(h);
   return e == cudaSuccess ? FM_OK : cuda_err(h, e, "cache attention launch");
 }
@@ -2328,7 +2366,7 @@ int fm_serve_reserve(fm_handle* h, const fm_cache_attn_config* cfg, int B, int L
   if (rc != FM_OK) return rc;
   const OnDevice on(h);
   const fm::CacheAttnPlan p =
-      fm::cache_attn_plan(B, L, cfg->n_heads, cfg->n_kv_heads, cfg->head_dim, cfg->prefix_max, true, h->num_sms);
+      fm::cache_attn_plan(B, L, cfg->n_heads, cfg->n_kv_heads, cfg->head_dim, cfg->prefix_max, true, true, h->num_sms);
   return ensure_sv(h, std::max(p.bytes, evict_bytes(static_cast<int64_t>(B) * cfg->n_kv_heads, cfg->max_len)));
 }
 

@@ -26,6 +26,18 @@ struct RopeArgs {
   double turns[kRopeMaxDim / 2];  // full turns per position of each pair
 };
 
+// Attention over caches is split over keys.  A source of keys -- the shared prefix, or the
+// sequences' own caches -- is read by one of two kernels:
+//
+//   attn_split_kernel (serve.cu), a worker a warp, for few query rows per key: items of 16 query
+//     rows, tiles of 16 keys, mma.sync.  Bound by HBM.
+//   attn_tc_kernel (attn_tc.cu), a worker a CTA, for many: items of 256 query rows (of the heads
+//     that share a kv head, neighbouring tokens together), tiles of 128 keys, tcgen05.
+//
+// Either way the tiles of all items, in order, are cut into one contiguous range per worker, so
+// ragged lengths balance.  A worker's piece of an item leaves an unnormalised fp32 output,
+// its maximum (log2 units) and its sum in slot worker + item -- both only grow along the
+// order, so no two pieces share a slot -- and attn_merge_kernel joins an output row's pieces.
 constexpr int kAttnTile = 16;        // keys of a tile
 constexpr int kAttnRowTile = 16;     // query rows of an item
 constexpr int kAttnMinTiles = 4;     // least tiles of a worker's range
@@ -33,6 +45,9 @@ constexpr int kAttnWarps = 4;        // workers of a CTA
 constexpr int kAttnBlocksPerSm = 2;
 constexpr int kAttnStages = 3;       // ring of K / V tiles of a worker
 constexpr int attn_split_smem(int d) { return kAttnWarps * kAttnStages * 2 * kAttnTile * d * 2; }
+
+constexpr int kTcKeys = 128;         // keys of a tile, rows of a TMEM tile
+constexpr int kTcRows = 256;         // query rows of an item
 
 struct CacheAttnArgs {
   const uint16_t* q;        // [B * L, q_ld]: nh heads of d
@@ -45,7 +60,9 @@ struct CacheAttnArgs {
   const int32_t* lens;      // [B] or null: no own caches
   uint16_t* out;            // [B * L, nh * d]
   float* acc;               // [B, nkv, max_len] or null
-  int B, L, nh, nkv, group, max_len, prefix_len;
+  int B, L, nh, nkv, group, max_len;
+  int split_prefix;         // prefix rows the split kernel reads (0: none, or the other kernel's)
+  int split_own;            // 1: it reads the own caches
   float scale_log2;         // softmax scale * log2(e)
   int rt_p, rt_s;           // row tiles of the prefix items / of a sequence's items, per kv head
   int workers;
@@ -55,12 +72,119 @@ struct CacheAttnArgs {
   uint32_t* err;
 };
 
-struct CacheAttnPlan {
-  int64_t rt_p = 0, rt_s = 0;
-  int workers = 0;
-  size_t off_ml = 0, off_lse = 0, bytes = 0;
+// One source of keys for attn_tc_kernel: nseq sequences of L query tokens.
+struct TcAttnArgs {
+  const uint16_t* q;        // [nseq * L, q_ld]
+  int64_t q_ld;
+  const int32_t* lens;      // [nseq], or null: const_len keys each
+  int nseq, L, nh, nkv, group, max_len, const_len;
+  int causal;               // token l sees the keys j <= len - L + l; 0: all
+  int head_rows;            // rows of K / V from one (sequence, kv head) to the next
+  int rps;                  // items per (sequence, kv head)
+  int workers;              // 0: this source is not read here
+  int direct;               // the only source: an unsplit item's rows go to out
+  float scale_log2;         // >= 0
+  uint32_t q_sign;          // 0x80008000: q is negated (a negative scale)
+  float* part_o;            // [workers + items][256][d]; with one tile of rows, stream 1's piece
+  float2* part_ml;          //   in rows 128 ..
+  uint16_t* out;
+  float* lse2;
+  uint32_t* err;
 };
-CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_len, bool scored, int num_sms);
+
+#ifdef __CUDACC__
+FM_DEV int tc_len(const TcAttnArgs& a, int b) {
+  const int n = a.lens ? a.lens[b] : a.const_len;
+  return n < 0 || n > a.max_len ? 0 : n;  // reported by the merge
+}
+
+// tiles of item flat = b * rps + rp: up to the last key that its last token sees
+FM_DEV int tc_item_tiles(const TcAttnArgs& a, int flat) {
+  const int b = flat / a.rps, rp = flat - b * a.rps;
+  const int len = tc_len(a, b);
+  int seen = len;
+  if (a.causal) {
+    const int64_t last = (static_cast<int64_t>(rp) * kTcRows + kTcRows - 1) / a.group;
+    seen = len - a.L + static_cast<int>(last < a.L - 1 ? last : a.L - 1) + 1;
+  }
+  return seen <= 0 ? 0 : (seen + kTcKeys - 1) / kTcKeys;
+}
+
+// tiles of one kv head of items [0, n), summed by the whole warp
+FM_DEV int64_t tc_tiles_before(const TcAttnArgs& a, int n) {
+  int64_t s = 0;
+  for (int i = threadIdx.x & 31; i < n; i += 32) s += tc_item_tiles(a, i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+FM_DEV int64_t tc_tiles_per_worker(const TcAttnArgs& a, int64_t total) {
+  const int64_t per = (total + a.workers - 1) / a.workers;
+  return per < 1 ? 1 : per;
+}
+
+// A worker's place in the order (item, kv head, tile); cnt: tiles of the piece, 0 at the end.
+struct TcPiece {
+  int flat, kvh, tile, tiles, cnt;
+  int64_t left;  // tiles of the worker's range, this piece's included
+};
+
+FM_DEV void tc_set(TcPiece& p) {
+  p.cnt = static_cast<int>(p.left < p.tiles - p.tile ? p.left : p.tiles - p.tile);
+}
+
+FM_DEV void tc_first(const TcAttnArgs& a, int worker, int64_t per, TcPiece& p) {  // whole warp
+  const int lane = threadIdx.x & 31;
+  int64_t rest = worker * per;
+  p.left = per;
+  p.cnt = 0;
+  for (int base = 0; base < a.nseq * a.rps; base += 32) {
+    const int i = base + lane;
+    const int64_t mine = i < a.nseq * a.rps ? static_cast<int64_t>(tc_item_tiles(a, i)) * a.nkv : 0;
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, incl > rest);
+    if (past) {
+      const int f = __ffs(past) - 1;
+      rest -= __shfl_sync(0xffffffffu, incl - mine, f);
+      p.flat = base + f;
+      p.tiles = tc_item_tiles(a, p.flat);
+      p.kvh = static_cast<int>(rest / p.tiles);
+      p.tile = static_cast<int>(rest - static_cast<int64_t>(p.kvh) * p.tiles);
+      tc_set(p);
+      return;
+    }
+    rest -= __shfl_sync(0xffffffffu, incl, 31);
+  }
+}
+
+FM_DEV void tc_next(const TcAttnArgs& a, TcPiece& p) {
+  p.left -= p.cnt;
+  p.tile = 0;
+  if (++p.kvh == a.nkv) {
+    p.kvh = 0;
+    do {
+      ++p.flat;
+      p.tiles = p.flat < a.nseq * a.rps ? tc_item_tiles(a, p.flat) : 0;
+    } while (p.tiles == 0 && p.flat < a.nseq * a.rps);
+  }
+  tc_set(p);
+}
+#endif
+
+// Which kernel reads what, and the workspace.
+struct CacheAttnPlan {
+  bool tc_p = false, tc_s = false;  // the prefix / the own caches by attn_tc_kernel
+  int rt_p = 0, rt_s = 0, rps_p = 0, rps_s = 0;
+  int workers = 0, workers_p = 0, workers_s = 0;
+  size_t off_ml = 0, off_po = 0, off_pml = 0, off_so = 0, off_sml = 0, off_lse = 0, bytes = 0;
+};
+CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_len, bool own, bool scored, int num_sms);
 
 struct EvictArgs {
   const uint16_t* cache_k;  // [B, nkv, max_len, d]
@@ -82,7 +206,14 @@ struct EvictArgs {
 
 cudaError_t launch_rope(RopeArgs a, int num_sms, cudaStream_t st);
 cudaError_t cache_attn_init();
-cudaError_t launch_cache_attn(const CacheAttnArgs& a, int d, cudaStream_t st);
+// p, s: the prefix / own caches by attn_tc_kernel where their workers are set, with its maps
+struct TcMapsKV {
+  CUtensorMap k, v;
+};
+cudaError_t launch_cache_attn(const CacheAttnArgs& a, const TcAttnArgs& p, const TcMapsKV& mp, const TcAttnArgs& s,
+                              const TcMapsKV& ms, int d, cudaStream_t st);
+cudaError_t attn_tc_init();
+cudaError_t launch_attn_tc(const TcAttnArgs& a, int d, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st);
 cudaError_t launch_evict(const EvictArgs& a, int num_sms, cudaStream_t st);
 
 }  // namespace fm

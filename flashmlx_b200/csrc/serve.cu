@@ -176,21 +176,10 @@ cudaError_t launch_rope(RopeArgs a, int num_sms, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------ attention, split over keys
-// Work is counted in tiles of 16 keys.  The prefix gives nkv * rt_p items (a kv head, 16 of
-// all sequences' query rows) of ceil(prefix_len / 16) tiles; sequence b gives nkv * rt_s
-// items (a kv head, 16 of its L * group rows) of ceil(lens[b] / 16) tiles.  All tiles in
-// this order are cut into one contiguous range per worker (a warp), so ragged lengths
-// balance.  A worker's piece of an item leaves an unnormalised fp32 output, its maximum
-// (log2 units) and its sum in slot worker + item -- both only grow along the order, so no
-// two pieces share a slot -- and attn_merge_kernel joins an output row's pieces.
 namespace {
 
-struct Span {  // a worker's place in the order
-  int64_t per, t0, t1;
-};
-
 FM_DEV int seq_len(const CacheAttnArgs& a, int b) {
-  const int n = a.lens ? a.lens[b] : 0;
+  const int n = a.split_own ? a.lens[b] : 0;
   return n < 0 || n > a.max_len ? 0 : n;  // reported by the merge
 }
 
@@ -248,7 +237,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
   const uint32_t ring = smem_u32(s_kv) + warp * (kAttnStages * STAGE);
   const int64_t worker = static_cast<int64_t>(blockIdx.x) * kAttnWarps + warp;
 
-  const int64_t tp = (a.prefix_len + kAttnTile - 1) / kAttnTile;  // tiles of a prefix item
+  const int64_t tp = (a.split_prefix + kAttnTile - 1) / kAttnTile;  // tiles of a prefix item
   const int np = a.nkv * a.rt_p, ns = a.nkv * a.rt_s;             // items of the prefix / of a sequence
   const int64_t total_p = tp * np;
   const int64_t total = total_p + ns * tiles_before(a, a.B);
@@ -298,7 +287,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
     const int rts = pre ? a.rt_p : a.rt_s;
     const int kvh = item / rts, row0 = (item - kvh * rts) * kAttnRowTile;
     const int rows = pre ? a.B * a.L * a.group : a.L * a.group;
-    const int len = pre ? a.prefix_len : seq_len(a, b);
+    const int len = pre ? a.split_prefix : seq_len(a, b);
     const int64_t tok0 = pre ? 0 : static_cast<int64_t>(b) * a.L;
     const int64_t base = pre ? kvh * a.p_head : (static_cast<int64_t>(b) * a.nkv + kvh) * a.max_len * D;
     const uint16_t* kb = (pre ? a.pk : a.ck) + base;
@@ -441,66 +430,115 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
   }
 }
 
-// Joins the pieces of one output row (one warp): out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i,
-// zeros when nothing was seen; lse2 = M + log2(sum) for the slot weights.
+// Joins the pieces of output rows: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, zeros when
+// nothing was seen; lse2 = M + log2(sum) for the slot weights.  A block takes up to 64 of a
+// (sequence, kv head)'s rows, a warp every fourth of them.
+constexpr int kMergeRows = 64;
+
 template <int D>
-__global__ void __launch_bounds__(128) attn_merge_kernel(const CacheAttnArgs a) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + warp;  // (b, l, h)
-  if (row >= static_cast<int64_t>(a.B) * a.L * a.nh) return;
-  const int64_t tok = row / a.nh;
-  const int h = static_cast<int>(row - tok * a.nh);
-  const int b = static_cast<int>(tok / a.L), l = static_cast<int>(tok - static_cast<int64_t>(b) * a.L);
-  const int kvh = h / a.group, gq = h - kvh * a.group;
-  if (a.lens && lane == 0 && l == 0 && h == 0 && (a.lens[b] < 0 || a.lens[b] > a.max_len)) report(a.err, DEVERR_BOUNDS);
-  const int64_t tp = (a.prefix_len + kAttnTile - 1) / kAttnTile;
-  const int np = a.nkv * a.rt_p, ns = a.nkv * a.rt_s;
-  const int64_t total_p = tp * np;
-  const int64_t per = tiles_per_worker(a, total_p + ns * tiles_before(a, a.B));
+__global__ void __launch_bounds__(128) attn_merge_kernel(const CacheAttnArgs a, const TcAttnArgs tp, const TcAttnArgs ts) {
   constexpr int V = D / 32;  // columns of a lane
-  float acc[V] = {};
-  float M = -INFINITY, S = 0.f;
-  auto join = [&](int64_t first, int64_t tiles, int64_t item, int rr) {
-    if (tiles <= 0) return;
-    const int64_t w1 = (first + tiles - 1) / per;
-    for (int64_t w = first / per; w <= w1; ++w) {
-      const int64_t pr = (w + item) * kAttnRowTile + rr;
-      const float2 ml = a.part_ml[pr];
-      const float* po = a.part_o + pr * D + lane * V;
-      float v[V];
-      if (V == 4) {
-        const float4 t4 = *reinterpret_cast<const float4*>(po);
-        v[0] = t4.x; v[1] = t4.y; v[2 % V] = t4.z; v[3 % V] = t4.w;
-      } else {
-        const float2 t2 = *reinterpret_cast<const float2*>(po);
-        v[0] = t2.x; v[1] = t2.y;
+  constexpr int U = 4;       // pieces whose loads are in flight together
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.z, kvh = blockIdx.y;
+  const int rows = a.L * a.group, first_row = blockIdx.x * kMergeRows;
+  if (a.lens && threadIdx.x == 0 && blockIdx.x == 0 && kvh == 0 && (a.lens[b] < 0 || a.lens[b] > a.max_len))
+    report(a.err, DEVERR_BOUNDS);
+  // the split kernel's cut
+  const int64_t tp16 = (a.split_prefix + kAttnTile - 1) / kAttnTile;
+  const int np = a.nkv * a.rt_p, ns = a.nkv * a.rt_s;
+  int64_t per = 1, own_first = 0, own_tiles = 0;
+  if (a.workers) {
+    per = tiles_per_worker(a, tp16 * np + ns * tiles_before(a, a.B));
+    own_tiles = (seq_len(a, b) + kAttnTile - 1) / kAttnTile;
+    own_first = tp16 * np + ns * tiles_before(a, b) + static_cast<int64_t>(kvh) * a.rt_s * own_tiles;
+  }
+  // the tcgen05 kernel's cuts
+  int64_t per_p = 1, tiles_p = 0, per_s = 1, first_s = 0, tiles_s = 0;
+  int flat_s = 0;
+  if (tp.workers) {
+    tiles_p = tc_item_tiles(tp, 0);
+    per_p = tc_tiles_per_worker(tp, tiles_p * tp.rps * tp.nkv);
+  }
+  if (ts.workers) {
+    flat_s = b * ts.rps + first_row / kTcRows;
+    tiles_s = tc_item_tiles(ts, flat_s);
+    per_s = tc_tiles_per_worker(ts, tc_tiles_before(ts, ts.nseq * ts.rps) * ts.nkv);
+    first_s = tc_tiles_before(ts, flat_s) * ts.nkv + kvh * tiles_s;
+    // written by the kernel itself when one worker had the item whole and one piece
+    const bool pair = rows - first_row / kTcRows * kTcRows > kTcKeys;
+    if (ts.direct && tiles_s > 0 && first_s / per_s == (first_s + tiles_s - 1) / per_s && (pair || tiles_s == 1)) return;
+  }
+  for (int r = first_row + warp; r < min(rows, first_row + kMergeRows); r += 4) {
+    float acc[V] = {};
+    float M = -INFINITY, S = 0.f;
+    // n pieces, piece i in row row0 + i * step of a part buffer
+    auto join = [&](const float* part_o, const float2* part_ml, int64_t row0, int64_t step, int n) {
+      for (int i0 = 0; i0 < n; i0 += U) {
+        float2 ml[U];
+        float v[U][V];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t pr = row0 + min(i0 + u, n - 1) * step;
+          ml[u] = part_ml[pr];
+          const float* po = part_o + pr * D + lane * V;
+          if (V == 4) {
+            const float4 t4 = *reinterpret_cast<const float4*>(po);
+            v[u][0] = t4.x; v[u][1] = t4.y; v[u][2 % V] = t4.z; v[u][3 % V] = t4.w;
+          } else {
+            const float2 t2 = *reinterpret_cast<const float2*>(po);
+            v[u][0] = t2.x; v[u][1] = t2.y;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (i0 + u >= n || ml[u].y == 0.f) continue;  // the piece's keys are all hidden from this row
+          const float mn = fmaxf(M, ml[u].x);
+          const float wa = exp2f(M - mn), wb = exp2f(ml[u].x - mn);
+          M = mn;
+          S = S * wa + ml[u].y * wb;
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[e] = acc[e] * wa + v[u][e] * wb;
+        }
       }
-      if (ml.x == -INFINITY) continue;  // the piece's keys are all hidden from this row
-      const float mn = fmaxf(M, ml.x);
-      const float wa = exp2f(M - mn), wb = exp2f(ml.x - mn);
-      M = mn;
-      S = S * wa + ml.y * wb;
-#pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] = acc[i] * wa + v[i] * wb;
+    };
+    auto split_join = [&](int64_t first, int64_t tiles, int64_t item, int rr) {
+      if (tiles <= 0) return;
+      const int64_t w0 = first / per, w1 = (first + tiles - 1) / per;
+      join(a.part_o, a.part_ml, (w0 + item) * kAttnRowTile + rr, kAttnRowTile, static_cast<int>(w1 - w0 + 1));
+    };
+    auto tc_join = [&](const TcAttnArgs& t, int64_t pr, int64_t first, int64_t tiles, int64_t item, int rr, bool pair) {
+      if (tiles <= 0) return;
+      const int64_t w0 = first / pr, w1 = (first + tiles - 1) / pr;
+      // pair: a row is one stream's; otherwise both streams hold a piece of it
+      join(t.part_o, t.part_ml, (w0 + item) * kTcRows + rr, pair ? kTcRows : kTcKeys,
+           static_cast<int>(w1 - w0 + 1) * (pair ? 1 : 2));
+    };
+    const int64_t rp = static_cast<int64_t>(b) * rows + r;  // the row among all sequences'
+    if (tp16 > 0) {
+      const int64_t item = kvh * a.rt_p + rp / kAttnRowTile;
+      split_join(item * tp16, tp16, item, static_cast<int>(rp % kAttnRowTile));
     }
-  };
-  if (tp > 0) {
-    const int64_t r = tok * a.group + gq;
-    const int64_t item = kvh * a.rt_p + r / kAttnRowTile;
-    join(item * tp, tp, item, static_cast<int>(r % kAttnRowTile));
-  }
-  const int64_t ts = (seq_len(a, b) + kAttnTile - 1) / kAttnTile;
-  if (ts > 0) {
-    const int r = l * a.group + gq;
-    const int64_t in = kvh * a.rt_s + r / kAttnRowTile;
-    join(total_p + ns * tiles_before(a, b) + in * ts, ts, np + static_cast<int64_t>(b) * ns + in, r % kAttnRowTile);
-  }
-  const float inv = M == -INFINITY ? 0.f : 1.f / S;
-  uint16_t* out = a.out + row * D + lane * V;
+    if (tiles_p > 0) {
+      const int64_t flat = rp / kTcRows, item = flat * tp.nkv + kvh;
+      tc_join(tp, per_p, item * tiles_p, tiles_p, item, static_cast<int>(rp % kTcRows),
+              static_cast<int64_t>(a.B) * rows - flat * kTcRows > kTcKeys);
+    }
+    if (own_tiles > 0)
+      split_join(own_first + r / kAttnRowTile * own_tiles, own_tiles,
+                 np + static_cast<int64_t>(b) * ns + kvh * a.rt_s + r / kAttnRowTile, r % kAttnRowTile);
+    if (tiles_s > 0)
+      tc_join(ts, per_s, first_s, tiles_s, static_cast<int64_t>(flat_s) * ts.nkv + kvh, r % kTcRows,
+              rows - r / kTcRows * kTcRows > kTcKeys);
+    const float inv = S == 0.f ? 0.f : 1.f / S;
+    const int tk = r / a.group;
+    const int64_t row = (static_cast<int64_t>(b) * a.L + tk) * a.nh + kvh * a.group + (r - tk * a.group);
+    uint16_t* out = a.out + row * D + lane * V;
 #pragma unroll
-  for (int i = 0; i < V; i += 2)
-    *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
-  if (a.lse2 && lane == 0) a.lse2[row] = M == -INFINITY ? INFINITY : M + log2f(S);
+    for (int i = 0; i < V; i += 2)
+      *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
+    if (a.lse2 && lane == 0) a.lse2[row] = S == 0.f ? INFINITY : M + log2f(S);
+  }
 }
 
 // ------------------------------------------------------------------ slot weights
@@ -513,7 +551,8 @@ __global__ void __launch_bounds__(128) slot_weight_kernel(const CacheAttnArgs a)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int b = blockIdx.z, kvh = blockIdx.y;
-  const int len = seq_len(a, b);
+  int len = a.lens[b];
+  if (len < 0 || len > a.max_len) len = 0;  // reported by the merge
   const int key0 = (blockIdx.x * 4 + warp) * 16;
   if (key0 >= len) return;
   const uint16_t* kb = a.ck + (static_cast<int64_t>(b) * a.nkv + kvh) * a.max_len * D;
@@ -570,30 +609,57 @@ static cudaError_t attn_opt_in() {
 }
 
 cudaError_t cache_attn_init() {
-  const cudaError_t e = attn_opt_in<128>();
-  return e == cudaSuccess ? attn_opt_in<64>() : e;
+  cudaError_t e = attn_opt_in<128>();
+  if (e == cudaSuccess) e = attn_opt_in<64>();
+  return e == cudaSuccess ? attn_tc_init() : e;
 }
 
-CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_len, bool scored, int num_sms) {
+CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_len, bool own, bool scored, int num_sms) {
   CacheAttnPlan p;
-  const int64_t group = nh / nkv;
-  p.rt_p = prefix_len > 0 ? (static_cast<int64_t>(B) * L * group + kAttnRowTile - 1) / kAttnRowTile : 0;
-  p.rt_s = (L * group + kAttnRowTile - 1) / kAttnRowTile;
-  p.workers = num_sms * kAttnBlocksPerSm * kAttnWarps;
-  const int64_t slots = p.workers + nkv * (p.rt_p + B * p.rt_s);
-  p.off_ml = static_cast<size_t>(slots) * kAttnRowTile * d * sizeof(float);
-  p.off_lse = p.off_ml + static_cast<size_t>(slots) * kAttnRowTile * sizeof(float2);
-  p.bytes = p.off_lse + (scored ? sizeof(float) * B * L * nh : 0);
+  const int64_t group = nh / nkv, rows_s = L * group, rows_p = B * rows_s;
+  // up to one warp tile of rows the split kernel reads each key once with no row to spare for
+  // the tensor pipe's 128; above it attn_tc_kernel does
+  p.tc_p = prefix_len > 0 && rows_p > kAttnRowTile;
+  p.tc_s = own && rows_s > kAttnRowTile;
+  if (prefix_len > 0 && !p.tc_p) p.rt_p = static_cast<int>((rows_p + kAttnRowTile - 1) / kAttnRowTile);
+  if (own && !p.tc_s) p.rt_s = static_cast<int>((rows_s + kAttnRowTile - 1) / kAttnRowTile);
+  if (p.rt_p || p.rt_s) p.workers = num_sms * kAttnBlocksPerSm * kAttnWarps;
+  auto add = [&](size_t bytes) {
+    const size_t off = p.bytes;
+    p.bytes = (p.bytes + bytes + 255) / 256 * 256;
+    return off;
+  };
+  const size_t rows = p.workers ? (p.workers + static_cast<size_t>(nkv) * (p.rt_p + static_cast<size_t>(B) * p.rt_s)) * kAttnRowTile : 0;
+  add(rows * d * sizeof(float));
+  p.off_ml = add(rows * sizeof(float2));
+  auto tc = [&](bool on, int64_t nseq, int64_t item_rows, int& rps, int& workers, size_t& off_o, size_t& off_ml) {
+    if (!on) return;
+    rps = static_cast<int>((item_rows + kTcRows - 1) / kTcRows);
+    workers = num_sms;
+    const size_t n = (workers + static_cast<size_t>(nseq) * rps * nkv) * kTcRows;
+    off_o = add(n * d * sizeof(float));
+    off_ml = add(n * sizeof(float2));
+  };
+  tc(p.tc_p, 1, rows_p, p.rps_p, p.workers_p, p.off_po, p.off_pml);
+  tc(p.tc_s, B, rows_s, p.rps_s, p.workers_s, p.off_so, p.off_sml);
+  p.off_lse = add(scored ? sizeof(float) * B * L * nh : 0);
   return p;
 }
 
 template <int D>
-static cudaError_t launch_cache_attn_d(const CacheAttnArgs& a, cudaStream_t st) {
-  attn_split_kernel<D><<<a.workers / kAttnWarps, kAttnWarps * 32, attn_split_smem(D), st>>>(a);
-  cudaError_t e = cudaGetLastError();
+static cudaError_t launch_cache_attn_d(const CacheAttnArgs& a, const TcAttnArgs& p, const TcMapsKV& mp,
+                                       const TcAttnArgs& s, const TcMapsKV& ms, cudaStream_t st) {
+  cudaError_t e = cudaSuccess;
+  if (p.workers) e = launch_attn_tc(p, D, mp.k, mp.v, st);
+  if (e == cudaSuccess && s.workers) e = launch_attn_tc(s, D, ms.k, ms.v, st);
   if (e != cudaSuccess) return e;
-  const int64_t rows = static_cast<int64_t>(a.B) * a.L * a.nh;
-  attn_merge_kernel<D><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, st>>>(a);
+  if (a.workers) {
+    attn_split_kernel<D><<<a.workers / kAttnWarps, kAttnWarps * 32, attn_split_smem(D), st>>>(a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  const dim3 rows((a.L * a.group + kMergeRows - 1) / kMergeRows, a.nkv, a.B);
+  attn_merge_kernel<D><<<rows, 128, 0, st>>>(a, p, s);
   e = cudaGetLastError();
   if (e != cudaSuccess || !a.acc) return e;
   const dim3 grid((a.max_len + 63) / 64, a.nkv, a.B);
@@ -601,8 +667,9 @@ static cudaError_t launch_cache_attn_d(const CacheAttnArgs& a, cudaStream_t st) 
   return cudaGetLastError();
 }
 
-cudaError_t launch_cache_attn(const CacheAttnArgs& a, int d, cudaStream_t st) {
-  return d == 128 ? launch_cache_attn_d<128>(a, st) : launch_cache_attn_d<64>(a, st);
+cudaError_t launch_cache_attn(const CacheAttnArgs& a, const TcAttnArgs& p, const TcMapsKV& mp, const TcAttnArgs& s,
+                              const TcMapsKV& ms, int d, cudaStream_t st) {
+  return d == 128 ? launch_cache_attn_d<128>(a, p, mp, s, ms, st) : launch_cache_attn_d<64>(a, p, mp, s, ms, st);
 }
 
 // ------------------------------------------------------------------ eviction
