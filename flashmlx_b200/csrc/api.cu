@@ -2156,6 +2156,7 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
   a.split_own = p.rt_s > 0;
   const double scale = c->scale != 0.f ? c->scale : 1.0 / std::sqrt(static_cast<double>(d));
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  a.merge_rows = p.merge_rows;
   a.rt_p = p.rt_p;
   a.rt_s = p.rt_s;
   a.workers = p.workers;

@@ -48,6 +48,7 @@ constexpr int attn_split_smem(int d) { return kAttnWarps * kAttnStages * 2 * kAt
 
 constexpr int kTcKeys = 128;         // keys of a tile, rows of a TMEM tile
 constexpr int kTcRows = 256;         // query rows of an item
+constexpr int kTcItemCost = 2;       // what an item costs beside its tiles, in tiles
 
 struct CacheAttnArgs {
   const uint16_t* q;        // [B * L, q_ld]: nh heads of d
@@ -64,6 +65,7 @@ struct CacheAttnArgs {
   int split_prefix;         // prefix rows the split kernel reads (0: none, or the other kernel's)
   int split_own;            // 1: it reads the own caches
   float scale_log2;         // softmax scale * log2(e)
+  int merge_rows;           // rows of a merge block: 4 or 16
   int rt_p, rt_s;           // row tiles of the prefix items / of a sequence's items, per kv head
   int workers;
   float* part_o;            // [slots][16][d]
@@ -110,28 +112,55 @@ FM_DEV int tc_item_tiles(const TcAttnArgs& a, int flat) {
   return seen <= 0 ? 0 : (seen + kTcKeys - 1) / kTcKeys;
 }
 
-// tiles of one kv head of items [0, n), summed by the whole warp
-FM_DEV int64_t tc_tiles_before(const TcAttnArgs& a, int n) {
+// An item's start and end (Q in, O out) cost a worker about as much as kTcItemCost tiles, so the
+// order has that many empty places before each item's tiles and ranges are cut by places.
+FM_DEV int tc_item_places(const TcAttnArgs& a, int flat) {
+  const int n = tc_item_tiles(a, flat);
+  return n ? n + kTcItemCost : 0;
+}
+
+// places of one kv head of items [0, n), summed by the whole warp
+FM_DEV int64_t tc_places_before(const TcAttnArgs& a, int n) {
   int64_t s = 0;
-  for (int i = threadIdx.x & 31; i < n; i += 32) s += tc_item_tiles(a, i);
+  for (int i = threadIdx.x & 31; i < n; i += 32) s += tc_item_places(a, i);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
 
-FM_DEV int64_t tc_tiles_per_worker(const TcAttnArgs& a, int64_t total) {
+FM_DEV int64_t tc_places_per_worker(const TcAttnArgs& a, int64_t total) {
   const int64_t per = (total + a.workers - 1) / a.workers;
   return per < 1 ? 1 : per;
 }
 
-// A worker's place in the order (item, kv head, tile); cnt: tiles of the piece, 0 at the end.
+// A worker's piece in hand: tiles [tile, tile + cnt) of item (flat, kvh); cnt 0 at the end.
 struct TcPiece {
   int flat, kvh, tile, tiles, cnt;
-  int64_t left;  // tiles of the worker's range, this piece's included
+  int64_t left;  // places of the worker's range from the item's first (or the range's) on
 };
 
-FM_DEV void tc_set(TcPiece& p) {
-  p.cnt = static_cast<int>(p.left < p.tiles - p.tile ? p.left : p.tiles - p.tile);
+// the piece of the range that begins at place `at` of item (flat, kvh)
+FM_DEV void tc_cut(TcPiece& p, int at) {
+  const int64_t end = at + p.left;  // in the item's places
+  p.tile = at > kTcItemCost ? at - kTcItemCost : 0;
+  const int64_t last = end - kTcItemCost < p.tiles ? end - kTcItemCost : p.tiles;
+  p.cnt = last > p.tile ? static_cast<int>(last - p.tile) : 0;
+  p.left -= p.tiles + kTcItemCost - at;
+}
+
+// the next item's piece; ends with cnt 0
+FM_DEV void tc_next(const TcAttnArgs& a, TcPiece& p) {
+  p.cnt = 0;
+  while (p.left > 0 && p.cnt == 0) {
+    if (++p.kvh == a.nkv) {
+      p.kvh = 0;
+      do {
+        if (++p.flat >= a.nseq * a.rps) return;
+        p.tiles = tc_item_tiles(a, p.flat);
+      } while (p.tiles == 0);
+    }
+    tc_cut(p, 0);
+  }
 }
 
 FM_DEV void tc_first(const TcAttnArgs& a, int worker, int64_t per, TcPiece& p) {  // whole warp
@@ -141,7 +170,7 @@ FM_DEV void tc_first(const TcAttnArgs& a, int worker, int64_t per, TcPiece& p) {
   p.cnt = 0;
   for (int base = 0; base < a.nseq * a.rps; base += 32) {
     const int i = base + lane;
-    const int64_t mine = i < a.nseq * a.rps ? static_cast<int64_t>(tc_item_tiles(a, i)) * a.nkv : 0;
+    const int64_t mine = i < a.nseq * a.rps ? static_cast<int64_t>(tc_item_places(a, i)) * a.nkv : 0;
     int64_t incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -154,33 +183,21 @@ FM_DEV void tc_first(const TcAttnArgs& a, int worker, int64_t per, TcPiece& p) {
       rest -= __shfl_sync(0xffffffffu, incl - mine, f);
       p.flat = base + f;
       p.tiles = tc_item_tiles(a, p.flat);
-      p.kvh = static_cast<int>(rest / p.tiles);
-      p.tile = static_cast<int>(rest - static_cast<int64_t>(p.kvh) * p.tiles);
-      tc_set(p);
+      const int places = p.tiles + kTcItemCost;
+      p.kvh = static_cast<int>(rest / places);
+      tc_cut(p, static_cast<int>(rest - static_cast<int64_t>(p.kvh) * places));
+      if (p.cnt == 0) tc_next(a, p);
       return;
     }
     rest -= __shfl_sync(0xffffffffu, incl, 31);
   }
-}
-
-FM_DEV void tc_next(const TcAttnArgs& a, TcPiece& p) {
-  p.left -= p.cnt;
-  p.tile = 0;
-  if (++p.kvh == a.nkv) {
-    p.kvh = 0;
-    do {
-      ++p.flat;
-      p.tiles = p.flat < a.nseq * a.rps ? tc_item_tiles(a, p.flat) : 0;
-    } while (p.tiles == 0 && p.flat < a.nseq * a.rps);
-  }
-  tc_set(p);
 }
 #endif
 
 // Which kernel reads what, and the workspace.
 struct CacheAttnPlan {
   bool tc_p = false, tc_s = false;  // the prefix / the own caches by attn_tc_kernel
-  int rt_p = 0, rt_s = 0, rps_p = 0, rps_s = 0;
+  int rt_p = 0, rt_s = 0, rps_p = 0, rps_s = 0, merge_rows = 16;
   int workers = 0, workers_p = 0, workers_s = 0;
   size_t off_ml = 0, off_po = 0, off_pml = 0, off_so = 0, off_sml = 0, off_lse = 0, bytes = 0;
 };

@@ -431,17 +431,17 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
 }
 
 // Joins the pieces of output rows: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, zeros when
-// nothing was seen; lse2 = M + log2(sum) for the slot weights.  A block takes up to 64 of a
-// (sequence, kv head)'s rows, a warp every fourth of them.
-constexpr int kMergeRows = 64;
+// nothing was seen; lse2 = M + log2(sum) for the slot weights.  A block takes a.merge_rows of
+// a (sequence, kv head)'s rows (fewer when there are few in all: a row's pieces are read one
+// after the other), a warp every fourth of them.
 
 template <int D>
 __global__ void __launch_bounds__(128) attn_merge_kernel(const CacheAttnArgs a, const TcAttnArgs tp, const TcAttnArgs ts) {
   constexpr int V = D / 32;  // columns of a lane
-  constexpr int U = 4;       // pieces whose loads are in flight together
+  constexpr int U = 8;       // pieces whose loads are in flight together
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z, kvh = blockIdx.y;
-  const int rows = a.L * a.group, first_row = blockIdx.x * kMergeRows;
+  const int rows = a.L * a.group, first_row = blockIdx.x * a.merge_rows;
   if (a.lens && threadIdx.x == 0 && blockIdx.x == 0 && kvh == 0 && (a.lens[b] < 0 || a.lens[b] > a.max_len))
     report(a.err, DEVERR_BOUNDS);
   // the split kernel's cut
@@ -454,22 +454,22 @@ __global__ void __launch_bounds__(128) attn_merge_kernel(const CacheAttnArgs a, 
     own_first = tp16 * np + ns * tiles_before(a, b) + static_cast<int64_t>(kvh) * a.rt_s * own_tiles;
   }
   // the tcgen05 kernel's cuts
-  int64_t per_p = 1, tiles_p = 0, per_s = 1, first_s = 0, tiles_s = 0;
+  int64_t per_p = 1, tiles_p = 0, per_s = 1, first_s = 0, tiles_s = 0;  // first_s: a place
   int flat_s = 0;
   if (tp.workers) {
     tiles_p = tc_item_tiles(tp, 0);
-    per_p = tc_tiles_per_worker(tp, tiles_p * tp.rps * tp.nkv);
+    per_p = tc_places_per_worker(tp, (tiles_p + kTcItemCost) * tp.rps * tp.nkv);
   }
   if (ts.workers) {
     flat_s = b * ts.rps + first_row / kTcRows;
     tiles_s = tc_item_tiles(ts, flat_s);
-    per_s = tc_tiles_per_worker(ts, tc_tiles_before(ts, ts.nseq * ts.rps) * ts.nkv);
-    first_s = tc_tiles_before(ts, flat_s) * ts.nkv + kvh * tiles_s;
-    // written by the kernel itself when one worker had the item whole and one piece
+    per_s = tc_places_per_worker(ts, tc_places_before(ts, ts.nseq * ts.rps) * ts.nkv);
+    first_s = tc_places_before(ts, flat_s) * ts.nkv + kvh * (tiles_s + kTcItemCost) + kTcItemCost;
+    // written by the kernel itself when one worker had the item whole and a row is one stream's
     const bool pair = rows - first_row / kTcRows * kTcRows > kTcKeys;
-    if (ts.direct && tiles_s > 0 && first_s / per_s == (first_s + tiles_s - 1) / per_s && (pair || tiles_s == 1)) return;
+    if (ts.direct && pair && tiles_s > 0 && first_s / per_s == (first_s + tiles_s - 1) / per_s) return;
   }
-  for (int r = first_row + warp; r < min(rows, first_row + kMergeRows); r += 4) {
+  for (int r = first_row + warp; r < min(rows, first_row + a.merge_rows); r += 4) {
     float acc[V] = {};
     float M = -INFINITY, S = 0.f;
     // n pieces, piece i in row row0 + i * step of a part buffer
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(128) attn_merge_kernel(const CacheAttnArgs a, 
     }
     if (tiles_p > 0) {
       const int64_t flat = rp / kTcRows, item = flat * tp.nkv + kvh;
-      tc_join(tp, per_p, item * tiles_p, tiles_p, item, static_cast<int>(rp % kTcRows),
+      tc_join(tp, per_p, item * (tiles_p + kTcItemCost) + kTcItemCost, tiles_p, item, static_cast<int>(rp % kTcRows),
               static_cast<int64_t>(a.B) * rows - flat * kTcRows > kTcKeys);
     }
     if (own_tiles > 0)
@@ -642,6 +642,7 @@ CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_l
   };
   tc(p.tc_p, 1, rows_p, p.rps_p, p.workers_p, p.off_po, p.off_pml);
   tc(p.tc_s, B, rows_s, p.rps_s, p.workers_s, p.off_so, p.off_sml);
+  if (B * nkv * ((rows_s + 15) / 16) < 8ll * num_sms) p.merge_rows = 4;
   p.off_lse = add(scored ? sizeof(float) * B * L * nh : 0);
   return p;
 }
@@ -658,7 +659,7 @@ static cudaError_t launch_cache_attn_d(const CacheAttnArgs& a, const TcAttnArgs&
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
-  const dim3 rows((a.L * a.group + kMergeRows - 1) / kMergeRows, a.nkv, a.B);
+  const dim3 rows((a.L * a.group + a.merge_rows - 1) / a.merge_rows, a.nkv, a.B);
   attn_merge_kernel<D><<<rows, 128, 0, st>>>(a, p, s);
   e = cudaGetLastError();
   if (e != cudaSuccess || !a.acc) return e;
