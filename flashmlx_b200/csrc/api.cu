@@ -2128,7 +2128,7 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
     h->sv_ready = true;
   }
   const int nh = c->n_heads, nkv = c->n_kv_heads, d = c->head_dim;
-  const fm::CacheAttnPlan p = fm::cache_attn_plan(B, L, nh, nkv, d, prefix_len, lens != nullptr, scored, h->num_sms);
+  const fm::CacheAttnPlan p = fm::cache_attn_plan(B, L, nh, nkv, d, prefix_len, lens != nullptr, scored, c->max_len, h->num_sms);
   const int64_t own_rows = static_cast<int64_t>(B) * nkv * c->max_len, prefix_rows = static_cast<int64_t>(nkv) * c->prefix_max;
   if ((p.tc_s && own_rows > 0x7fffff00LL) || (p.tc_p && prefix_rows > 0x7fffff00LL))
     return set_err(h, FM_EUNSUPPORTED, "too many cache rows");
@@ -2198,8 +2198,28 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
         !encode_2d(&maps[i].v, false, i ? cv : pv, d, rows, 64, fm::kTcKeys))
       return set_err(h, FM_ECUDA, "cuTensorMapEncodeTiled failed");
   }
+  fm::TcWeightArgs w;
+  std::memset(&w, 0, sizeof(w));
+  if (scored && p.tc_s) {
+    w.q = q;
+    w.q_ld = q_ld;
+    w.lens = lens;
+    w.lse2 = a.lse2;
+    w.acc = acc;
+    w.part = reinterpret_cast<float*>(h->sv_ws + p.off_w);
+    w.B = B;
+    w.L = L;
+    w.nh = nh;
+    w.nkv = nkv;
+    w.group = a.group;
+    w.max_len = c->max_len;
+    w.key_tiles = (c->max_len + fm::kTcKeys - 1) / fm::kTcKeys;
+    w.workers = h->num_sms;
+    w.scale_log2 = a.scale_log2;
+    w.err = a.err;
+  }
   prof_begin(h, scored ? "attention_scored" : "attention_prefix");
-  const cudaError_t e = fm::launch_cache_attn(a, t[0], maps[0], t[1], maps[1], d, h->stream);
+  const cudaError_t e = fm::launch_cache_attn(a, t[0], maps[0], t[1], maps[1], w, d, h->stream);
   prof_end(h);
   return e == cudaSuccess ? FM_OK : cuda_err(h, e, "cache attention launch");
 }
@@ -2367,7 +2387,7 @@ int fm_serve_reserve(fm_handle* h, const fm_cache_attn_config* cfg, int B, int L
   if (rc != FM_OK) return rc;
   const OnDevice on(h);
   const fm::CacheAttnPlan p =
-      fm::cache_attn_plan(B, L, cfg->n_heads, cfg->n_kv_heads, cfg->head_dim, cfg->prefix_max, true, true, h->num_sms);
+      fm::cache_attn_plan(B, L, cfg->n_heads, cfg->n_kv_heads, cfg->head_dim, cfg->prefix_max, true, true, cfg->max_len, h->num_sms);
   return ensure_sv(h, std::max(p.bytes, evict_bytes(static_cast<int64_t>(B) * cfg->n_kv_heads, cfg->max_len)));
 }
 

@@ -1,0 +1,858 @@
+// attn_tc.cu -- attention of many query rows over a key range on tcgen05 (sm_100a): the shared
+// prefix of a batch, and the new tokens' rows of a sequence when they are more than a warp's
+// tile.  fm_serve.cuh describes the order of the work and its split over workers.
+//
+// A worker is a CTA, one per SM.  An item is a kv head's keys and up to 256 query rows (the
+// group's heads of neighbouring tokens, so that every head that shares the keys shares the
+// loads), two 128-row tiles.  Two streams of 128 softmax threads, a row each, share the tensor
+// pipe and every K / V tile: with more than 128 rows a stream has its own row tile and all keys,
+// with fewer both have the same rows and a stream takes half of each tile's keys; those halves
+// are joined like any two pieces.
+//
+//   warps 0-3, 4-7  stream 0, 1: Q rows to shared memory (the next piece's are already in
+//                   registers when a piece ends); per 64 keys S out of TMEM, scale and
+//                   visibility, online softmax, P back into TMEM over S (bf16 pairs); at the
+//                   end O out of TMEM, through the warp's own Q rows so that the stores are
+//                   whole lines
+//   warp 8          MMA issuer: S = Q K^T (both operands K-major in shared memory) and
+//                   O += P V (P in TMEM, V as loaded: keys x head, i.e. MN-major)
+//   warp 9          TMA loads of K / V tiles of 128 keys into a ring
+//
+// TMEM: per stream two S / P buffers of 64 columns and head_dim columns of O.  A step is 64 keys
+// of a stream; S of step n + 2 is issued right after P V of step n, into the buffer that step
+// n's P leaves, so S of step n + 1 is there before the stream is done with step n and the streams
+// never wait for the pipe's latency.  (With one S of 128 keys a stream -- all that fits next to
+// O -- the chain S, softmax, P V, S took 3950 cycles a tile where the products take 2048.)
+//
+// A stream's running maximum is only a reference: P is 2^(s - ref) with ref moved (and O
+// rescaled, by the stream itself) when a row's maximum passes it by more than 8, so that O
+// in TMEM is rarely touched; P stays below 2^8 and keeps its relative precision.  Past an item's
+// first step the exponentials do not wait for the maximum: it is taken alongside, and in the
+// rare case that ref has to move they are done again.  The special-function units (4
+// exponentials a cycle and scheduler) alone would take as long as the products, so a share
+// of the exponentials is computed with fused multiply-adds instead.
+#include "fm_serve.cuh"
+
+namespace fm {
+namespace {
+
+constexpr int kThreads = 320;
+constexpr int kMmaWarp = 8;      // warp 9 loads
+constexpr int kStep = 64;        // keys of a stream's step
+constexpr int kPolyEvery = 4;    // one pair of exponentials in so many by fused multiply-adds
+
+template <int D>
+struct Shape {
+  static constexpr int kHalf = D / 64;                       // 64-column halves of a row
+  static constexpr uint32_t kTileBytes = kTcKeys * D * 2;    // a K, V or 128-row Q tile
+  static constexpr int kSlots = D == 128 ? 5 : 8;            // ring of K / V tiles
+  static constexpr uint32_t kSmem = 1024 + (2 + kSlots) * kTileBytes;
+};
+
+struct Bars {
+  uint64_t qfull[2], sfull[2][2], pfull[2][2], ofull, tail, done;
+  uint64_t kvfull[8], kvempty[8];
+  uint32_t tmem;
+  int abort_flag;
+};
+
+FM_DEV void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accum)
+      : "memory");
+}
+
+// descriptor of a [K rows x 64 N columns] tile in the 128-byte swizzle read as the N x K operand
+// (MN-major): 8 K rows 1024 B apart, the next 64 columns `cols` bytes on
+FM_DEV uint64_t sdesc_mn_sw128(uint32_t saddr, uint32_t cols) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(cols >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+
+FM_DEV float ex2(float x) {  // 2^x, 2 ulp; results below 2^-126 are 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// two fp32 operations an instruction
+FM_DEV uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+FM_DEV void unpack2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+FM_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+FM_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+FM_DEV float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 2^x for both halves without the special-function unit: x = n + f with n the nearest whole
+// number (the low bits of x + 1.5 * 2^23) and |f| <= 1/2, 2^f by a polynomial of degree 5 fitted
+// for the least relative error with p(0) = 1 (9e-8, 1.7e-7 with fp32 sums), n added to the
+// exponent.  x is at least -127, where the exponent's bits give exactly 0: a hidden key's
+// weight is 0 here too, and a row that sees nothing sums to 0.
+FM_DEV uint64_t ex2_poly2(uint64_t x) {
+  float lo, hi;
+  unpack2(x, lo, hi);
+  x = pack2(max_nan(lo, -127.f), max_nan(hi, -127.f));
+  const float kMagic = 12582912.f;
+  const uint64_t t = add2(x, pack2(kMagic, kMagic));
+  const uint64_t n = add2(t, pack2(-kMagic, -kMagic));
+  const uint64_t f = fma2(n, pack2(-1.f, -1.f), x);
+  uint64_t p = pack2(0.0013264727302716457f, 0.0013264727302716457f);
+  p = fma2(p, f, pack2(0.009671512728706911f, 0.009671512728706911f));
+  p = fma2(p, f, pack2(0.05550733743810932f, 0.05550733743810932f));
+  p = fma2(p, f, pack2(0.24022242084016385f, 0.24022242084016385f));
+  p = fma2(p, f, pack2(0.6931469775983554f, 0.6931469775983554f));
+  p = fma2(p, f, pack2(1.f, 1.f));
+  float pl, ph, tl, th;
+  unpack2(p, pl, ph);
+  unpack2(t, tl, th);
+  return pack2(__uint_as_float(__float_as_uint(pl) + (__float_as_uint(tl) << 23)),
+               __uint_as_float(__float_as_uint(ph) + (__float_as_uint(th) << 23)));
+}
+
+// 32 columns of this lane's row, without waiting for them
+FM_DEV void tmem_ld32_async(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+FM_DEV void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+FM_DEV void tmem_st16(uint32_t taddr, const float (&v)[16]) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+FM_DEV void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// bounded wait that ignores the abort flag: drains copies and products in flight
+FM_DEV bool wait_drained(uint64_t* bar, uint32_t parity, uint32_t* err) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (clock64() - t0 > kWaitBudgetCycles) {
+      report(err, DEVERR_TIMEOUT);
+      return false;
+    }
+  }
+  return true;
+}
+
+}  // namespace
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ TcAttnArgs a,
+                                                             const __grid_constant__ CUtensorMap map_k,
+                                                             const __grid_constant__ CUtensorMap map_v) {
+  using S = Shape<D>;
+  constexpr int NS = S::kSlots;
+  extern __shared__ uint8_t s_raw[];
+  __shared__ Bars bars;
+  // tiles on 1024-byte boundaries, as the swizzle's pattern needs
+  const uint32_t pad = (1024u - (smem_u32(s_raw) & 1023u)) & 1023u;
+  uint8_t* s_q = s_raw + pad;                        // [2][kTileBytes]
+  uint8_t* s_kv = s_q + 2 * S::kTileBytes;           // [NS][kTileBytes]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &bars.abort_flag;
+  const int64_t per = tc_places_per_worker(a, tc_places_before(a, a.items()) * a.nkv);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.qfull[i], 4);  // a warp's arrival each
+      for (int j = 0; j < 2; ++j) {
+        mbar_init(&bars.sfull[i][j], 1);
+        mbar_init(&bars.pfull[i][j], 4);
+      }
+    }
+    mbar_init(&bars.ofull, 1);
+    mbar_init(&bars.tail, 1);
+    mbar_init(&bars.done, 1);
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&bars.kvfull[i], 1);
+      mbar_init(&bars.kvempty[i], 1);
+    }
+    bars.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(&bars.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+
+  TcPiece it;
+  tc_first(a, blockIdx.x, per, it);
+  const int rows = a.L * a.group;
+
+  if (warp < kMmaWarp) {
+    // ---------------------------------------------------------------- softmax streams
+    const int s = warp >> 2;
+    const int quad = warp & 3;
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t t_s = tmem + lanes + s * kTcKeys, t_o = tmem + lanes + 2 * kTcKeys + s * D;
+    uint8_t* q_tile = s_q + s * S::kTileBytes;
+    uint8_t* stage = q_tile + quad * 32 * 128;  // the warp's own Q rows (their first 64 columns)
+    constexpr int CPR = D / 8, RPI = 32 / CPR;  // 16-byte chunks of a row, rows a warp brings at once
+    uint4 qv[32 / RPI];
+    // ---- Q: stream s brings tile s (with one tile of rows stream 0 alone)
+    auto fetch_q = [&](const TcPiece& p) {
+      const int b = p.flat / a.rps, row_base = (p.flat - b * a.rps) * kTcRows;
+      const bool mine = p.cnt > 0 && (s == 0 || rows - row_base > kTcKeys);
+      const uint16_t* q = a.q + static_cast<int64_t>(b) * a.L * a.q_ld + static_cast<int64_t>(p.kvh) * a.group * D + lane % CPR * 8;
+      int r = row_base + s * kTcKeys + quad * 32 + lane / CPR;
+      int tk = r / a.group, gq = r - tk * a.group;
+#pragma unroll
+      for (int i = 0; i < 32 / RPI; ++i) {
+        qv[i] = make_uint4(0, 0, 0, 0);
+        if (mine && r < rows) qv[i] = *reinterpret_cast<const uint4*>(q + tk * a.q_ld + gq * D);
+        r += RPI;
+        gq += RPI;
+        while (gq >= a.group) {
+          gq -= a.group;
+          ++tk;
+        }
+      }
+    };
+    // both streams arrive for every piece, so that neither falls behind by a phase of `ofull`
+    auto store_q = [&](const TcPiece& p) {
+      if (p.cnt <= 0) return;
+      if (s == 0 || rows - p.flat % a.rps * kTcRows > kTcKeys) {
+        const int ch = lane % CPR;
+#pragma unroll
+        for (int i = 0; i < 32 / RPI; ++i) {
+          uint4 v = qv[i];
+          v.x ^= a.q_sign;  // a negative scale is taken as its size, with -q
+          v.y ^= a.q_sign;
+          v.z ^= a.q_sign;
+          v.w ^= a.q_sign;
+          *reinterpret_cast<uint4*>(q_tile + (ch >> 3) * (kTcKeys * 128) +
+                                    sw128_off(quad * 32 + i * RPI + lane / CPR, ch & 7)) = v;
+        }
+        fence_proxy_async();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.qfull[s]);
+    };
+    uint32_t g = 0;  // steps of this stream: step g is in buffer g % 2
+    int oph = 0;
+    bool ok = true;
+    fetch_q(it);
+    store_q(it);
+    const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2);
+    while (it.cnt > 0) {
+      const int b = it.flat / a.rps, row_base = (it.flat - b * a.rps) * kTcRows;
+      const bool pair = rows - row_base > kTcKeys;
+      const int len = tc_len(a, b);
+      const int64_t tok0 = static_cast<int64_t>(b) * a.L;
+      const int rl = quad * 32 + lane;
+      const int r = row_base + (pair ? s * kTcKeys : 0) + rl;
+      const bool on = r < rows;
+      const int tk = on ? r / a.group : 0;
+      const int lim = !on ? -1 : a.causal ? len - a.L + tk : len - 1;  // the last key this row sees
+      const bool live = row_base + (pair ? s * kTcKeys : 0) + quad * 32 < rows;
+      const int steps = pair ? 2 * it.cnt : it.cnt;
+      float ref = -INFINITY, l = 0.f;
+      int key0 = it.tile * kTcKeys + (pair ? 0 : s * kStep);
+#pragma unroll 1
+      for (int n = 0; n < steps; ++n, ++g, key0 += pair ? kStep : kTcKeys) {
+        const uint32_t buf = g & 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars.sfull[s][buf], g >> 1 & 1, abort_flag, a.err))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (live) {
+          const uint32_t t_b = t_s + buf * kStep;
+          float v[kStep];
+#pragma unroll
+          for (int c = 0; c < kStep; c += 32) tmem_ld32_async(t_b + c, v + c);
+          tmem_wait_ld();
+          if (__any_sync(0xffffffffu, lim < key0 + kStep - 1)) {
+#pragma unroll
+            for (int c = 0; c < kStep; ++c) v[c] = key0 + c <= lim ? v[c] : -INFINITY;
+          }
+          float mx;
+          auto maximum = [&]() {
+            float m4[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+            for (int c = 4; c < kStep; ++c) m4[c & 3] = fmaxf(m4[c & 3], v[c]);
+            mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
+          };
+          float sum;
+          auto exponentials = [&]() {
+            const float base = ref == -INFINITY ? 0.f : -ref;
+            const uint64_t base2 = pack2(base, base);
+            uint64_t sum2[2] = {0ull, 0ull};
+            uint4 w[8];
+            uint32_t* pw = reinterpret_cast<uint32_t*>(w);
+#pragma unroll
+            for (int c = 0; c < kStep / 2; ++c) {
+              uint64_t x = fma2(pack2(v[2 * c], v[2 * c + 1]), scale2, base2);
+              float p0, p1;
+              if (c % kPolyEvery == kPolyEvery - 1) {
+                x = ex2_poly2(x);
+                unpack2(x, p0, p1);
+              } else {
+                unpack2(x, p0, p1);
+                p0 = ex2(p0);
+                p1 = ex2(p1);
+                x = pack2(p0, p1);
+              }
+              sum2[c & 1] = add2(sum2[c & 1], x);
+              pw[c] = pack_bf16x2(p0, p1);  // the tensor product's operand: one rounding to bf16
+            }
+            tmem_st32(t_b, w);
+            float s0, s1;
+            unpack2(add2(sum2[0], sum2[1]), s0, s1);
+            sum = s0 + s1;
+          };
+          // the first step's maximum is needed before its exponentials; later ones' alongside
+          bool done = false;
+          if (n == 0) {
+            maximum();
+            ref = mx;
+            done = true;
+          }
+#pragma unroll 1
+          while (true) {
+            exponentials();
+            if (done) break;
+            maximum();
+            if (!__any_sync(0xffffffffu, mx > ref + 8.f)) break;
+            const float nref = mx > ref + 8.f ? mx : ref;
+            // the product that last wrote O is complete (this step's S was issued after it)
+            const float f = ref == -INFINITY ? 0.f : ex2(ref - nref);
+            l *= f;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              float o[16];
+              tmem_ld16(t_o + c, o);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] *= f;
+              tmem_st16(t_o + c, o);
+            }
+            ref = nref;
+            done = true;
+          }
+          l += sum;
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.pfull[s][buf]);
+      }
+      TcPiece nx = it;
+      tc_next(a, nx);
+      fetch_q(nx);
+      if (!ok || !__all_sync(0xffffffffu, mbar_wait(&bars.ofull, oph & 1, abort_flag, a.err))) break;
+      ++oph;
+      tc_fence_after();
+      const bool whole = a.direct && it.cnt == it.tiles && pair;
+      if (live) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int64_t row = (tok0 + tk) * a.nh + it.kvh * a.group + (r - tk * a.group);
+        const int64_t pr = (static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(it.flat) * a.nkv + it.kvh) * kTcRows +
+                           s * kTcKeys + quad * 32;
+        const uint32_t on_rows = __ballot_sync(0xffffffffu, on);
+        const int rsub = lane >> 3, csub = lane & 7;
+        {
+          // a 128-byte line of each row at a time: 32 fp32 or 64 bf16 columns
+#pragma unroll 1
+          for (int c = 0; c < D; c += whole ? 64 : 32) {
+            __syncwarp();
+            if (whole) {
+#pragma unroll 1
+              for (int hh = 0; hh < 2; ++hh) {
+                float o[32];
+                tmem_ld32(t_o + c + 32 * hh, o);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  *reinterpret_cast<uint4*>(stage + sw128_off(lane, 4 * hh + e)) =
+                      make_uint4(pack_bf16x2(o[8 * e] * inv, o[8 * e + 1] * inv), pack_bf16x2(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                                 pack_bf16x2(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack_bf16x2(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+              }
+            } else {
+              float o[32];
+              tmem_ld32(t_o + c, o);
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                *reinterpret_cast<float4*>(stage + sw128_off(lane, e)) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int rr = 4 * i + rsub;
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + sw128_off(rr, csub));
+              const int64_t out_row = __shfl_sync(0xffffffffu, row, rr);
+              if (!(on_rows >> rr & 1)) continue;
+              if (whole) *reinterpret_cast<uint4*>(a.out + out_row * D + c + 8 * csub) = v;
+              else *reinterpret_cast<uint4*>(a.part_o + (pr + rr) * D + c + 4 * csub) = v;
+            }
+          }
+        }
+        if (on) {
+          if (!whole) a.part_ml[pr + lane] = make_float2(ref, l);
+          else if (a.lse2) a.lse2[row] = l == 0.f ? INFINITY : ref + log2f(l);
+        }
+        __syncwarp();
+      }
+      it = nx;
+      store_q(it);
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------------- MMA issuer
+    // elect.sync, not a lane test: one lane chosen so lets the compiler hold the operands in uniform
+    // registers (65 to 90 cycles a product otherwise, where the pipe takes 48)
+    if (elect_one()) {
+      const uint64_t q_desc = sdesc_sw128(smem_u32(s_q)), k_desc = sdesc_sw128(smem_u32(s_kv));
+      const uint64_t v_desc = sdesc_mn_sw128(smem_u32(s_kv), kTcKeys * 128);
+      constexpr uint32_t kTile16 = S::kTileBytes >> 4;      // in descriptor units
+      constexpr uint32_t kHalf16 = kTcKeys * 128 >> 4;      // the next 64 columns of a tile
+      constexpr uint32_t kStep16 = kStep * 128 >> 4;        // the next 64 keys
+      const uint32_t id_s = idesc_bf16(kTcKeys, kStep), id_o = idesc_bf16(kTcKeys, D) | (1u << 16);  // B MN-major
+      int qph = 0, kslot = 0, vslot = 0, ring = 0;
+      uint32_t ring_ph = 0, g = 0;  // g: steps done by a stream, as in the streams
+      bool ok = true;
+      auto next_slot = [&](int& slot) {
+        slot = ring;
+        const bool got = mbar_wait(&bars.kvfull[slot], ring_ph, abort_flag, a.err);
+        if (++ring == NS) {
+          ring = 0;
+          ring_ph ^= 1;
+        }
+        return got;
+      };
+      for (; ok && it.cnt > 0; tc_next(a, it)) {
+        const bool pair = rows - it.flat % a.rps * kTcRows > kTcKeys;
+        const int steps = pair ? 2 * it.cnt : it.cnt;
+        // S of step n: with one row tile a tile is one step (a half of its keys per stream)
+        auto issue_s = [&](int n, int s) {
+          if (s == 0 && !(pair && (n & 1))) {
+            if (!next_slot(kslot)) return false;
+            tc_fence_after();
+          }
+          const uint64_t ad = q_desc + (pair ? s : 0) * kTile16;
+          const uint64_t bd = k_desc + kslot * kTile16 + (pair ? n & 1 : s) * kStep16;
+          const uint32_t buf = (g + n) & 1;
+          const uint32_t d = tmem + s * kTcKeys + buf * kStep;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_bf16(d, ad + (kk >> 2) * kHalf16 + 2 * (kk & 3), bd + (kk >> 2) * kHalf16 + 2 * (kk & 3), id_s, kk != 0);
+          umma_commit(&bars.sfull[s][buf]);
+          if (s == 1 && !(pair && !(n & 1))) umma_commit(&bars.kvempty[kslot]);
+          return true;
+        };
+        for (int s = 0; ok && s < 2; ++s) ok = mbar_wait(&bars.qfull[s], qph & 1, abort_flag, a.err);
+        ++qph;
+        tc_fence_after();
+        for (int n = 0; ok && n < min(2, steps); ++n)
+          for (int s = 0; ok && s < 2; ++s) ok = issue_s(n, s);
+#pragma unroll 1
+        for (int n = 0; ok && n < steps; ++n) {
+          const uint32_t buf = (g + n) & 1, ph = (g + n) >> 1 & 1;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if (s == 0 && !(pair && (n & 1))) ok = next_slot(vslot);
+            ok = ok && mbar_wait(&bars.pfull[s][buf], ph, abort_flag, a.err);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t bd = v_desc + vslot * kTile16 + (pair ? n & 1 : s) * kStep16;
+            const uint32_t d = tmem + 2 * kTcKeys + s * D, at = tmem + s * kTcKeys + buf * kStep;
+#pragma unroll
+            for (int kk = 0; kk < kStep / 16; ++kk) umma_bf16_ts(d, at + 8 * kk, bd + kk * 128, id_o, n != 0 || kk != 0);
+            if (s == 1 && !(pair && !(n & 1))) umma_commit(&bars.kvempty[vslot]);
+            if (n + 2 < steps) ok = issue_s(n + 2, s);
+            if (!ok) break;
+          }
+        }
+        if (ok) umma_commit(&bars.ofull);
+        g += steps;
+      }
+      // every product and commit of this CTA has landed before it frees TMEM and leaves
+      umma_commit(&bars.done);
+      wait_drained(&bars.done, 0, a.err);
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- K / V loader
+    int kc = 0, tph = 0;
+    bool ok = true;
+    for (; ok && it.cnt > 0; tc_next(a, it)) {
+      const int b = it.flat / a.rps;
+      const bool pair = rows - (it.flat - b * a.rps) * kTcRows > kTcKeys;
+      const int len = tc_len(a, b);
+      const int y0 = (b * a.nkv + it.kvh) * a.head_rows;
+      auto load = [&](const CUtensorMap* map, int j, bool v) {
+        const int slot = kc % NS;
+        if (!mbar_wait_lane0(&bars.kvempty[slot], ((kc / NS) & 1) ^ 1, abort_flag, a.err)) return false;
+        ++kc;
+        uint8_t* dst = s_kv + slot * S::kTileBytes;
+        const int key0 = (it.tile + j) * kTcKeys;
+        // rows of V past the length may hold anything, and 0 * NaN is NaN: they become zeros
+        const bool ragged = v && key0 + kTcKeys > len;
+        uint64_t* bar = ragged ? &bars.tail : &bars.kvfull[slot];
+        if (elect_one()) {
+          mbar_arrive_expect_tx(bar, S::kTileBytes);
+#pragma unroll
+          for (int h = 0; h < S::kHalf; ++h)
+            tma_load_2d(smem_u32(dst) + h * (kTcKeys * 128), map, h * 64, y0 + key0, bar);
+        }
+        __syncwarp();
+        if (ragged) {
+          if (!__all_sync(0xffffffffu, wait_drained(&bars.tail, tph & 1, a.err))) return false;
+          ++tph;
+          const int first = len - key0;
+          for (int e = lane; e < (kTcKeys - first) * 8; e += 32)
+#pragma unroll
+            for (int h = 0; h < S::kHalf; ++h)
+              *reinterpret_cast<uint4*>(dst + h * (kTcKeys * 128) + (first + (e >> 3)) * 128 + (e & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.kvfull[slot]);
+        }
+        return true;
+      };
+      // in the order of their first use: K0 V0 K1 V1 .. (pair), K0 K1 V0 K2 V1 .. (one tile)
+      if (!pair) {
+        ok = load(&map_k, 0, false);
+        if (ok && it.cnt > 1) ok = load(&map_k, 1, false);
+      }
+      for (int j = 0; ok && j < it.cnt; ++j) {
+        if (pair) ok = load(&map_k, j, false);
+        ok = ok && load(&map_v, j, true);
+        if (ok && !pair && j + 2 < it.cnt) ok = load(&map_k, j + 2, false);
+      }
+    }
+    // copies in flight land before the CTA leaves (all did unless a wait ran out)
+    if (!ok)
+      for (int j = max(0, kc - NS); j < kc; ++j)
+        if (!wait_drained(&bars.kvfull[j % NS], (j / NS) & 1, a.err)) break;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------ slot weights
+// acc[j] of a kv head's 128 keys: S^T = K Q^T for 128 query rows at a time (keys are the TMEM
+// lanes, rows the columns), so a thread's sum over its columns of 2^(s - lse of the row) is its
+// key's weight and needs no other thread.  The two groups of 128 threads take every other row
+// tile.  Bound by the exponentials (128 x 128 a tile: 1024 cycles of the special-function units
+// against 512 of the tensor pipe), of which a third go to fused multiply-adds here.
+//   warps 0-3, 4-7  groups 0, 1     warp 8  MMA issuer     warps 9-12  K (TMA) and Q (cp.async)
+namespace {
+constexpr int kWThreads = 416;
+constexpr int kWStages = 4;    // Q tiles, their rows' lse, TMEM buffers
+constexpr int kWPolyEvery = 3;
+
+template <int D>
+struct WShape {
+  static constexpr uint32_t kTileBytes = kTcKeys * D * 2;
+  static constexpr uint32_t kSmem = 1024 + (2 + kWStages) * kTileBytes;
+};
+
+struct WBars {
+  uint64_t qfull[kWStages], sfull[kWStages], sempty[kWStages], kfull[2], kempty[2], done;
+  uint32_t tmem;
+  int abort_flag;
+};
+}  // namespace
+
+template <int D>
+__global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __grid_constant__ TcWeightArgs a,
+                                                                     const __grid_constant__ CUtensorMap map_k) {
+  using S = WShape<D>;
+  extern __shared__ uint8_t s_raw[];
+  __shared__ WBars bars;
+  __shared__ __align__(16) float s_lse[kWStages][kTcKeys];  // negated; -inf: no such row
+  const uint32_t pad = (1024u - (smem_u32(s_raw) & 1023u)) & 1023u;
+  uint8_t* s_k = s_raw + pad;                    // [2][kTileBytes]
+  uint8_t* s_q = s_k + 2 * S::kTileBytes;        // [kWStages][kTileBytes]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &bars.abort_flag;
+  const int64_t per = tc_places_per_worker(a, tc_places_before(a, a.items()) * a.nkv);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kWStages; ++i) {
+      mbar_init(&bars.qfull[i], 4);
+      mbar_init(&bars.sfull[i], 1);
+      mbar_init(&bars.sempty[i], 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.kfull[i], 1);
+      mbar_init(&bars.kempty[i], 1);
+    }
+    mbar_init(&bars.done, 1);
+    bars.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async();
+  }
+  if (warp == 8) {
+    tmem_alloc(&bars.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+  TcPiece it;
+  tc_first(a, blockIdx.x, per, it);
+  const int rows = a.L * a.group;
+  uint32_t t = 0;  // tiles of this CTA: tile t is in stage t % 4
+
+  if (warp < 8) {
+    // ---------------------------------------------------------------- sums
+    const int grp = warp >> 2;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int kl = (warp & 3) * 32 + lane;
+    const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2);
+    bool ok = true;
+    for (; ok && it.cnt > 0; tc_next(a, it)) {
+      const int b = it.flat / a.key_tiles, key0 = (it.flat - b * a.key_tiles) * kTcKeys;
+      const int len = a.lens[b];
+      const int row0 = (a.first_tile(b, key0, len) + it.tile) * kTcKeys;
+      // the first row that sees this lane's key; the item's last key's bounds the masked tiles
+      const int tk = max(key0 + kl - (len - a.L), 0), tk_last = max(min(key0 + kTcKeys, len) - 1 - (len - a.L), 0);
+      const int rmin = key0 + kl < len ? tk * a.group : 0x7fffffff, rmin_last = tk_last * a.group;
+      float total = 0.f, low = 0.f;  // a compensated sum over tiles
+      for (int i = 0; i < it.cnt; ++i, ++t) {
+        if ((t & 1) != static_cast<uint32_t>(grp)) continue;
+        const uint32_t st = t % kWStages;
+        // qfull (complete by then) for the loaders' s_lse, sfull for the product
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars.sfull[st], t / kWStages & 1, abort_flag, a.err) &&
+                                         mbar_wait(&bars.qfull[st], t / kWStages & 1, abort_flag, a.err))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int r0 = row0 + i * kTcKeys;
+        const bool masked = r0 < rmin_last;
+        uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll 1
+        for (int c = 0; c < kTcKeys; c += 32) {
+          float v[32];
+          tmem_ld32_async(tmem + lanes + st * kTcKeys + c, v);
+          tmem_wait_ld();
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = r0 + c + e >= rmin ? v[e] * a.scale_log2 : -INFINITY;
+          }
+          const uint64_t mul = masked ? pack2(1.f, 1.f) : scale2;
+          const float4* nl = reinterpret_cast<const float4*>(&s_lse[st][c]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float4 n4 = nl[e];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint64_t x = fma2(pack2(v[4 * e + 2 * h], v[4 * e + 2 * h + 1]), mul, h ? pack2(n4.z, n4.w) : pack2(n4.x, n4.y));
+              if ((2 * e + h) % kWPolyEvery == kWPolyEvery - 1) {
+                x = ex2_poly2(x);
+              } else {
+                float p0, p1;
+                unpack2(x, p0, p1);
+                x = pack2(ex2(p0), ex2(p1));
+              }
+              sum2[h] = add2(sum2[h], x);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.sempty[st]);
+        float s0, s1;
+        unpack2(add2(sum2[0], sum2[1]), s0, s1);
+        const float y = (s0 + s1) - low, u = total + y;
+        low = (u - total) - y;
+        total = u;
+      }
+      if (!ok) break;
+      a.part[((static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(it.flat) * a.nkv + it.kvh) * 2 + grp) * kTcKeys + kl] = total;
+    }
+  } else if (warp == 8) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (elect_one()) {
+      const uint64_t k_desc = sdesc_sw128(smem_u32(s_k)), q_desc = sdesc_sw128(smem_u32(s_q));
+      constexpr uint32_t kTile16 = S::kTileBytes >> 4, kHalf16 = kTcKeys * 128 >> 4;
+      const uint32_t id = idesc_bf16(kTcKeys, kTcKeys);
+      bool ok = true;
+      uint32_t n = 0;  // items
+      for (; ok && it.cnt > 0; tc_next(a, it), ++n) {
+        ok = mbar_wait(&bars.kfull[n & 1], n >> 1 & 1, abort_flag, a.err);
+#pragma unroll 1
+        for (int i = 0; ok && i < it.cnt; ++i, ++t) {
+          const uint32_t st = t % kWStages;
+          ok = mbar_wait(&bars.qfull[st], t / kWStages & 1, abort_flag, a.err);  // and its buffer is free
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t ad = k_desc + (n & 1) * kTile16, bd = q_desc + st * kTile16;
+          const uint32_t d = tmem + st * kTcKeys;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_bf16(d, ad + (kk >> 2) * kHalf16 + 2 * (kk & 3), bd + (kk >> 2) * kHalf16 + 2 * (kk & 3), id, kk != 0);
+          umma_commit(&bars.sfull[st]);
+        }
+        if (ok) umma_commit(&bars.kempty[n & 1]);
+      }
+      umma_commit(&bars.done);
+      wait_drained(&bars.done, 0, a.err);
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- loaders
+    const int lt = threadIdx.x - 9 * 32;  // 0..127
+    constexpr int CPR = D / 8, RPI = kTcKeys / CPR;  // chunks of a row, rows a pass brings
+    const int ch = lt % CPR;
+    bool ok = true;
+    uint32_t n = 0, sent = 0;  // items; tiles whose copies were reported complete
+    auto publish = [&](uint32_t upto) {  // this thread's copies of tiles [sent, upto) are complete
+      fence_proxy_async();
+      __syncwarp();
+      for (; sent < upto; ++sent)
+        if (lane == 0) mbar_arrive(&bars.qfull[sent % kWStages]);
+    };
+    for (; ok && it.cnt > 0; tc_next(a, it), ++n) {
+      const int b = it.flat / a.key_tiles, key0 = (it.flat - b * a.key_tiles) * kTcKeys;
+      const int row0 = (a.first_tile(b, key0, a.lens[b]) + it.tile) * kTcKeys;
+      if (warp == 9) {
+        if (!mbar_wait_lane0(&bars.kempty[n & 1], (n >> 1 & 1) ^ 1, abort_flag, a.err)) {
+          ok = false;
+        } else if (elect_one()) {
+          mbar_arrive_expect_tx(&bars.kfull[n & 1], S::kTileBytes);
+#pragma unroll
+          for (int h = 0; h < D / 64; ++h)
+            tma_load_2d(smem_u32(s_k + (n & 1) * S::kTileBytes) + h * (kTcKeys * 128), &map_k, h * 64,
+                        (b * a.nkv + it.kvh) * a.max_len + key0, &bars.kfull[n & 1]);
+        }
+        __syncwarp();
+        if (!ok) break;
+      }
+      const uint16_t* q = a.q + static_cast<int64_t>(b) * a.L * a.q_ld + static_cast<int64_t>(it.kvh) * a.group * D + ch * 8;
+      const float* lse = a.lse2 + static_cast<int64_t>(b) * a.L * a.nh + it.kvh * a.group;
+      for (int i = 0; i < it.cnt; ++i, ++t) {
+        const uint32_t st = t % kWStages;
+        const int r0 = row0 + i * kTcKeys;
+        int r = r0 + lt;
+        float nl = -INFINITY;
+        if (r < rows) {
+          const int tk = r / a.group;
+          nl = -lse[static_cast<int64_t>(tk) * a.nh + r - tk * a.group];
+        }
+        // the sums of tile t - 4 were taken, so its product is complete: its stage is free
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars.sempty[st], (t / kWStages & 1) ^ 1, abort_flag, a.err))) {
+          ok = false;
+          break;
+        }
+        s_lse[st][lt] = nl;
+        const uint32_t dst = smem_u32(s_q + st * S::kTileBytes) + (ch >> 3) * (kTcKeys * 128);
+        r = r0 + lt / CPR;
+        int tk = r / a.group, gq = r - tk * a.group;
+#pragma unroll 4
+        for (int e = 0; e < CPR; ++e) {
+          const bool on = r < rows;
+          const uint16_t* src = q + (on ? tk * a.q_ld + gq * D : 0);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + sw128_off(r - r0, ch & 7)), "l"(src),
+                       "r"(on ? 16 : 0)
+                       : "memory");
+          r += RPI;
+          gq += RPI;
+          while (gq >= a.group) {
+            gq -= a.group;
+            ++tk;
+          }
+        }
+        cp_async_commit();
+        cp_async_wait<1>();  // all but this tile's
+        publish(t);
+      }
+      if (!ok) break;
+    }
+    cp_async_wait<0>();
+    publish(t);
+    // a K tile in flight lands before the CTA leaves (its item's products waited for it unless a
+    // wait ran out)
+    if (warp == 9 && !ok && n > 0) wait_drained(&bars.kfull[(n - 1) & 1], (n - 1) >> 1 & 1, a.err);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int D>
+static cudaError_t tc_opt_in() {
+  const cudaError_t e = cudaFuncSetAttribute(attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
+  if (e != cudaSuccess) return e;
+  return cudaFuncSetAttribute(slot_weight_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, WShape<D>::kSmem);
+}
+
+cudaError_t attn_tc_init() {
+  const cudaError_t e = tc_opt_in<128>();
+  return e == cudaSuccess ? tc_opt_in<64>() : e;
+}
+
+cudaError_t launch_slot_weight_tc(const TcWeightArgs& a, int d, const CUtensorMap& k, cudaStream_t st) {
+  if (d == 128)
+    slot_weight_tc_kernel<128><<<a.workers, kWThreads, WShape<128>::kSmem, st>>>(a, k);
+  else
+    slot_weight_tc_kernel<64><<<a.workers, kWThreads, WShape<64>::kSmem, st>>>(a, k);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_attn_tc(const TcAttnArgs& a, int d, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
+  if (d == 128)
+    attn_tc_kernel<128><<<a.workers, kThreads, Shape<128>::kSmem, st>>>(a, k, v);
+  else
+    attn_tc_kernel<64><<<a.workers, kThreads, Shape<64>::kSmem, st>>>(a, k, v);
+  return cudaGetLastError();
+}
+
+}  // namespace fm

@@ -48,7 +48,6 @@ constexpr int attn_split_smem(int d) { return kAttnWarps * kAttnStages * 2 * kAt
 
 constexpr int kTcKeys = 128;         // keys of a tile, rows of a TMEM tile
 constexpr int kTcRows = 256;         // query rows of an item
-constexpr int kTcItemCost = 2;       // what an item costs beside its tiles, in tiles
 
 struct CacheAttnArgs {
   const uint16_t* q;        // [B * L, q_ld]: nh heads of d
@@ -92,6 +91,36 @@ struct TcAttnArgs {
   uint16_t* out;
   float* lse2;
   uint32_t* err;
+
+  static constexpr int kItemCost = 2;  // what an item costs beside its tiles, in tiles
+#ifdef __CUDACC__
+  __device__ int items() const { return nseq * rps; }
+  // tiles of item flat = b * rps + rp: up to the last key that its last token sees
+  __device__ int tiles(int flat) const;
+#endif
+};
+
+// The slot weights by slot_weight_tc_kernel (attn_tc.cu): an item is a kv head's 128 keys, its
+// tiles the query rows that see any of them, 128 at a time.
+struct TcWeightArgs {
+  const uint16_t* q;        // [B * L, q_ld]
+  int64_t q_ld;
+  const int32_t* lens;
+  const float* lse2;        // [B * L, nh]
+  float* acc;               // [B, nkv, max_len]
+  float* part;              // [workers + items][2][128] sums of a piece's even and odd tiles
+  int B, L, nh, nkv, group, max_len;
+  int key_tiles;            // of max_len
+  int workers;
+  float scale_log2;
+  uint32_t* err;
+
+  static constexpr int kItemCost = 2;
+#ifdef __CUDACC__
+  __device__ int items() const { return B * key_tiles; }
+  __device__ int first_tile(int b, int key0, int len) const;  // of the rows that see key0
+  __device__ int tiles(int flat) const;
+#endif
 };
 
 #ifdef __CUDACC__
@@ -100,27 +129,40 @@ FM_DEV int tc_len(const TcAttnArgs& a, int b) {
   return n < 0 || n > a.max_len ? 0 : n;  // reported by the merge
 }
 
-// tiles of item flat = b * rps + rp: up to the last key that its last token sees
-FM_DEV int tc_item_tiles(const TcAttnArgs& a, int flat) {
-  const int b = flat / a.rps, rp = flat - b * a.rps;
-  const int len = tc_len(a, b);
+__device__ __forceinline__ int TcAttnArgs::tiles(int flat) const {
+  const int b = flat / rps, rp = flat - b * rps;
+  const int len = tc_len(*this, b);
   int seen = len;
-  if (a.causal) {
-    const int64_t last = (static_cast<int64_t>(rp) * kTcRows + kTcRows - 1) / a.group;
-    seen = len - a.L + static_cast<int>(last < a.L - 1 ? last : a.L - 1) + 1;
+  if (causal) {
+    const int64_t last = (static_cast<int64_t>(rp) * kTcRows + kTcRows - 1) / group;
+    seen = len - L + static_cast<int>(last < L - 1 ? last : L - 1) + 1;
   }
   return seen <= 0 ? 0 : (seen + kTcKeys - 1) / kTcKeys;
 }
 
-// An item's start and end (Q in, O out) cost a worker about as much as kTcItemCost tiles, so the
-// order has that many empty places before each item's tiles and ranges are cut by places.
-FM_DEV int tc_item_places(const TcAttnArgs& a, int flat) {
-  const int n = tc_item_tiles(a, flat);
-  return n ? n + kTcItemCost : 0;
+__device__ __forceinline__ int TcWeightArgs::first_tile(int b, int key0, int len) const {
+  const int tk = key0 - (len - L);  // the first token that sees key0
+  return tk > 0 ? static_cast<int>(static_cast<int64_t>(tk) * group / kTcKeys) : 0;
+}
+
+__device__ __forceinline__ int TcWeightArgs::tiles(int flat) const {
+  const int b = flat / key_tiles, key0 = (flat - b * key_tiles) * kTcKeys;
+  const int len = lens[b];
+  if (len < 0 || len > max_len || key0 >= len) return 0;
+  return (L * group + kTcKeys - 1) / kTcKeys - first_tile(b, key0, len);
+}
+
+// An item's start and end cost a worker about as much as kItemCost tiles, so the order has that
+// many empty places before each item's tiles and ranges are cut by places.
+template <class A>
+FM_DEV int tc_item_places(const A& a, int flat) {
+  const int n = a.tiles(flat);
+  return n ? n + A::kItemCost : 0;
 }
 
 // places of one kv head of items [0, n), summed by the whole warp
-FM_DEV int64_t tc_places_before(const TcAttnArgs& a, int n) {
+template <class A>
+FM_DEV int64_t tc_places_before(const A& a, int n) {
   int64_t s = 0;
   for (int i = threadIdx.x & 31; i < n; i += 32) s += tc_item_places(a, i);
 #pragma unroll
@@ -128,7 +170,8 @@ FM_DEV int64_t tc_places_before(const TcAttnArgs& a, int n) {
   return s;
 }
 
-FM_DEV int64_t tc_places_per_worker(const TcAttnArgs& a, int64_t total) {
+template <class A>
+FM_DEV int64_t tc_places_per_worker(const A& a, int64_t total) {
   const int64_t per = (total + a.workers - 1) / a.workers;
   return per < 1 ? 1 : per;
 }
@@ -140,37 +183,40 @@ struct TcPiece {
 };
 
 // the piece of the range that begins at place `at` of item (flat, kvh)
-FM_DEV void tc_cut(TcPiece& p, int at) {
+template <class A>
+FM_DEV void tc_cut(const A&, TcPiece& p, int at) {
   const int64_t end = at + p.left;  // in the item's places
-  p.tile = at > kTcItemCost ? at - kTcItemCost : 0;
-  const int64_t last = end - kTcItemCost < p.tiles ? end - kTcItemCost : p.tiles;
+  p.tile = at > A::kItemCost ? at - A::kItemCost : 0;
+  const int64_t last = end - A::kItemCost < p.tiles ? end - A::kItemCost : p.tiles;
   p.cnt = last > p.tile ? static_cast<int>(last - p.tile) : 0;
-  p.left -= p.tiles + kTcItemCost - at;
+  p.left -= p.tiles + A::kItemCost - at;
 }
 
 // the next item's piece; ends with cnt 0
-FM_DEV void tc_next(const TcAttnArgs& a, TcPiece& p) {
+template <class A>
+FM_DEV void tc_next(const A& a, TcPiece& p) {
   p.cnt = 0;
   while (p.left > 0 && p.cnt == 0) {
     if (++p.kvh == a.nkv) {
       p.kvh = 0;
       do {
-        if (++p.flat >= a.nseq * a.rps) return;
-        p.tiles = tc_item_tiles(a, p.flat);
+        if (++p.flat >= a.items()) return;
+        p.tiles = a.tiles(p.flat);
       } while (p.tiles == 0);
     }
-    tc_cut(p, 0);
+    tc_cut(a, p, 0);
   }
 }
 
-FM_DEV void tc_first(const TcAttnArgs& a, int worker, int64_t per, TcPiece& p) {  // whole warp
+template <class A>
+FM_DEV void tc_first(const A& a, int worker, int64_t per, TcPiece& p) {  // whole warp
   const int lane = threadIdx.x & 31;
   int64_t rest = worker * per;
   p.left = per;
   p.cnt = 0;
-  for (int base = 0; base < a.nseq * a.rps; base += 32) {
+  for (int base = 0; base < a.items(); base += 32) {
     const int i = base + lane;
-    const int64_t mine = i < a.nseq * a.rps ? static_cast<int64_t>(tc_item_places(a, i)) * a.nkv : 0;
+    const int64_t mine = i < a.items() ? static_cast<int64_t>(tc_item_places(a, i)) * a.nkv : 0;
     int64_t incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -182,10 +228,10 @@ FM_DEV void tc_first(const TcAttnArgs& a, int worker, int64_t per, TcPiece& p) {
       const int f = __ffs(past) - 1;
       rest -= __shfl_sync(0xffffffffu, incl - mine, f);
       p.flat = base + f;
-      p.tiles = tc_item_tiles(a, p.flat);
-      const int places = p.tiles + kTcItemCost;
+      p.tiles = a.tiles(p.flat);
+      const int places = p.tiles + A::kItemCost;
       p.kvh = static_cast<int>(rest / places);
-      tc_cut(p, static_cast<int>(rest - static_cast<int64_t>(p.kvh) * places));
+      tc_cut(a, p, static_cast<int>(rest - static_cast<int64_t>(p.kvh) * places));
       if (p.cnt == 0) tc_next(a, p);
       return;
     }
@@ -199,9 +245,10 @@ struct CacheAttnPlan {
   bool tc_p = false, tc_s = false;  // the prefix / the own caches by attn_tc_kernel
   int rt_p = 0, rt_s = 0, rps_p = 0, rps_s = 0, merge_rows = 16;
   int workers = 0, workers_p = 0, workers_s = 0;
-  size_t off_ml = 0, off_po = 0, off_pml = 0, off_so = 0, off_sml = 0, off_lse = 0, bytes = 0;
+  size_t off_ml = 0, off_po = 0, off_pml = 0, off_so = 0, off_sml = 0, off_lse = 0, off_w = 0, bytes = 0;
 };
-CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_len, bool own, bool scored, int num_sms);
+CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_len, bool own, bool scored, int max_len,
+                              int num_sms);
 
 struct EvictArgs {
   const uint16_t* cache_k;  // [B, nkv, max_len, d]
@@ -228,9 +275,10 @@ struct TcMapsKV {
   CUtensorMap k, v;
 };
 cudaError_t launch_cache_attn(const CacheAttnArgs& a, const TcAttnArgs& p, const TcMapsKV& mp, const TcAttnArgs& s,
-                              const TcMapsKV& ms, int d, cudaStream_t st);
+                              const TcMapsKV& ms, const TcWeightArgs& w, int d, cudaStream_t st);
 cudaError_t attn_tc_init();
 cudaError_t launch_attn_tc(const TcAttnArgs& a, int d, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st);
+cudaError_t launch_slot_weight_tc(const TcWeightArgs& a, int d, const CUtensorMap& k, cudaStream_t st);
 cudaError_t launch_evict(const EvictArgs& a, int num_sms, cudaStream_t st);
 
 }  // namespace fm

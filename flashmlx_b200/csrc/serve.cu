@@ -457,14 +457,14 @@ __global__ void __launch_bounds__(128) attn_merge_kernel(const CacheAttnArgs a, 
   int64_t per_p = 1, tiles_p = 0, per_s = 1, first_s = 0, tiles_s = 0;  // first_s: a place
   int flat_s = 0;
   if (tp.workers) {
-    tiles_p = tc_item_tiles(tp, 0);
-    per_p = tc_places_per_worker(tp, (tiles_p + kTcItemCost) * tp.rps * tp.nkv);
+    tiles_p = tp.tiles(0);
+    per_p = tc_places_per_worker(tp, (tiles_p + TcAttnArgs::kItemCost) * tp.rps * tp.nkv);
   }
   if (ts.workers) {
     flat_s = b * ts.rps + first_row / kTcRows;
-    tiles_s = tc_item_tiles(ts, flat_s);
-    per_s = tc_places_per_worker(ts, tc_places_before(ts, ts.nseq * ts.rps) * ts.nkv);
-    first_s = tc_places_before(ts, flat_s) * ts.nkv + kvh * (tiles_s + kTcItemCost) + kTcItemCost;
+    tiles_s = ts.tiles(flat_s);
+    per_s = tc_places_per_worker(ts, tc_places_before(ts, ts.items()) * ts.nkv);
+    first_s = tc_places_before(ts, flat_s) * ts.nkv + kvh * (tiles_s + TcAttnArgs::kItemCost) + TcAttnArgs::kItemCost;
     // written by the kernel itself when one worker had the item whole and a row is one stream's
     const bool pair = rows - first_row / kTcRows * kTcRows > kTcKeys;
     if (ts.direct && pair && tiles_s > 0 && first_s / per_s == (first_s + tiles_s - 1) / per_s) return;
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(128) attn_merge_kernel(const CacheAttnArgs a, 
     }
     if (tiles_p > 0) {
       const int64_t flat = rp / kTcRows, item = flat * tp.nkv + kvh;
-      tc_join(tp, per_p, item * (tiles_p + kTcItemCost) + kTcItemCost, tiles_p, item, static_cast<int>(rp % kTcRows),
+      tc_join(tp, per_p, item * (tiles_p + TcAttnArgs::kItemCost) + TcAttnArgs::kItemCost, tiles_p, item, static_cast<int>(rp % kTcRows),
               static_cast<int64_t>(a.B) * rows - flat * kTcRows > kTcKeys);
     }
     if (own_tiles > 0)
@@ -603,6 +603,23 @@ __global__ void __launch_bounds__(128) slot_weight_kernel(const CacheAttnArgs a)
   }
 }
 
+// Adds the pieces of a key tile's weights, in the workers' order.
+__global__ void __launch_bounds__(kTcKeys) slot_weight_sum_kernel(const TcWeightArgs a) {
+  const int b = blockIdx.z, kvh = blockIdx.y, flat = b * a.key_tiles + blockIdx.x;
+  const int tiles = a.tiles(flat);
+  if (tiles == 0) return;
+  const int64_t per = tc_places_per_worker(a, tc_places_before(a, a.items()) * a.nkv);
+  const int64_t first = tc_places_before(a, flat) * a.nkv + kvh * (tiles + TcWeightArgs::kItemCost) + TcWeightArgs::kItemCost;
+  const int64_t item = static_cast<int64_t>(flat) * a.nkv + kvh;
+  float sum = 0.f;
+  for (int64_t w = first / per; w <= (first + tiles - 1) / per; ++w) {
+    const float* p = a.part + (w + item) * 2 * kTcKeys + threadIdx.x;
+    sum += p[0] + p[kTcKeys];
+  }
+  const int key = blockIdx.x * kTcKeys + threadIdx.x;
+  if (key < a.lens[b]) a.acc[(static_cast<int64_t>(b) * a.nkv + kvh) * a.max_len + key] += sum;
+}
+
 template <int D>
 static cudaError_t attn_opt_in() {
   return cudaFuncSetAttribute(attn_split_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_split_smem(D));
@@ -614,7 +631,8 @@ cudaError_t cache_attn_init() {
   return e == cudaSuccess ? attn_tc_init() : e;
 }
 
-CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_len, bool own, bool scored, int num_sms) {
+CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_len, bool own, bool scored, int max_len,
+                              int num_sms) {
   CacheAttnPlan p;
   const int64_t group = nh / nkv, rows_s = L * group, rows_p = B * rows_s;
   // up to one warp tile of rows the split kernel reads each key once with no row to spare for
@@ -644,12 +662,14 @@ CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_l
   tc(p.tc_s, B, rows_s, p.rps_s, p.workers_s, p.off_so, p.off_sml);
   if (B * nkv * ((rows_s + 15) / 16) < 8ll * num_sms) p.merge_rows = 4;
   p.off_lse = add(scored ? sizeof(float) * B * L * nh : 0);
+  const size_t key_items = static_cast<size_t>(B) * nkv * ((max_len + kTcKeys - 1) / kTcKeys);
+  p.off_w = add(scored && p.tc_s ? (num_sms + key_items) * 2 * kTcKeys * sizeof(float) : 0);
   return p;
 }
 
 template <int D>
 static cudaError_t launch_cache_attn_d(const CacheAttnArgs& a, const TcAttnArgs& p, const TcMapsKV& mp,
-                                       const TcAttnArgs& s, const TcMapsKV& ms, cudaStream_t st) {
+                                       const TcAttnArgs& s, const TcMapsKV& ms, const TcWeightArgs& w, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
   if (p.workers) e = launch_attn_tc(p, D, mp.k, mp.v, st);
   if (e == cudaSuccess && s.workers) e = launch_attn_tc(s, D, ms.k, ms.v, st);
@@ -663,14 +683,20 @@ static cudaError_t launch_cache_attn_d(const CacheAttnArgs& a, const TcAttnArgs&
   attn_merge_kernel<D><<<rows, 128, 0, st>>>(a, p, s);
   e = cudaGetLastError();
   if (e != cudaSuccess || !a.acc) return e;
+  if (w.workers) {
+    e = launch_slot_weight_tc(w, D, ms.k, st);
+    if (e != cudaSuccess) return e;
+    slot_weight_sum_kernel<<<dim3(w.key_tiles, a.nkv, a.B), kTcKeys, 0, st>>>(w);
+    return cudaGetLastError();
+  }
   const dim3 grid((a.max_len + 63) / 64, a.nkv, a.B);
   slot_weight_kernel<D><<<grid, 128, 0, st>>>(a);
   return cudaGetLastError();
 }
 
 cudaError_t launch_cache_attn(const CacheAttnArgs& a, const TcAttnArgs& p, const TcMapsKV& mp, const TcAttnArgs& s,
-                              const TcMapsKV& ms, int d, cudaStream_t st) {
-  return d == 128 ? launch_cache_attn_d<128>(a, p, mp, s, ms, st) : launch_cache_attn_d<64>(a, p, mp, s, ms, st);
+                              const TcMapsKV& ms, const TcWeightArgs& w, int d, cudaStream_t st) {
+  return d == 128 ? launch_cache_attn_d<128>(a, p, mp, s, ms, w, st) : launch_cache_attn_d<64>(a, p, mp, s, ms, w, st);
 }
 
 // ------------------------------------------------------------------ eviction

@@ -236,6 +236,11 @@ def caches(seed, B, nkv, M, d, lens):
     (2, 1, 4, 2, 128, 5000, [7, 3], 9),
     (1, 300, 4, 1, 64, 10, [300], 300),
     (33, 5, 8, 2, 128, 517, [5 + 9 * (i % 7) for i in range(33)], 60),
+    (3, 40, 8, 2, 64, 0, [10, 40, 0], 64),              # many rows that see nothing
+    (2, 100, 8, 2, 128, 0, [7, 333], 340),
+    (1, 129, 4, 4, 128, 0, [500], 512),                 # one head a kv head, a ragged second row tile
+    (2, 50, 7, 1, 128, 0, [256, 50], 256),              # 350 rows in groups of 7
+    (1, 9, 64, 1, 64, 1500, [9], 9),                    # 64 heads on one kv head
 ])
 def test_attention_prefix(B, L, nh, nkv, d, P, lens, M):
     from flashmlx_b200 import ops
@@ -295,6 +300,10 @@ def test_attention_scale(scale):
     (1, 130, 8, 2, 64, [130], 131),
     (2, 200, 6, 2, 128, [333, 200], 340),
     (1, 513, 4, 1, 64, [600], 600),
+    (3, 60, 8, 2, 128, [20, 60, 0], 64),
+    (2, 37, 7, 1, 64, [300, 129], 300),
+    (1, 1100, 8, 2, 128, [1100], 1100),
+    (1, 300, 2, 2, 128, [1000], 1024),
     (17, 1, 16, 16, 64, [3 * i for i in range(17)], 64),
 ])
 def test_attention_scored(B, L, nh, nkv, d, lens, M):
