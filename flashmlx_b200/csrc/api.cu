@@ -419,6 +419,21 @@ bool encode_2d(CUtensorMap* m, bool u32, const void* base, uint64_t inner, uint6
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// bf16 [tokens][heads][d] rows of tokens `ld` elements apart, 128B-swizzled boxes of 64 columns of
+// box_heads heads of box_tokens tokens
+bool encode_heads(CUtensorMap* m, const uint16_t* x, int d, int heads, int64_t tokens, int64_t ld, int box_heads,
+                  int box_tokens) {
+  auto fn = tensor_map_encoder();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  const cuuint64_t strides[2] = {2u * static_cast<cuuint64_t>(d), 2u * static_cast<cuuint64_t>(ld)};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
+  const cuuint32_t es[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint16_t*>(x), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // codes of a [rows, K] 4-bit matrix: uint32 words, box {4 k-steps, box_rows rows}
 bool encode_codes(CUtensorMap* m, const uint32_t* w, int64_t rows, int K, uint32_t box_rows) {
   return encode_2d(m, true, w, static_cast<uint64_t>(K / 8), static_cast<uint64_t>(rows), 32, box_rows);
@@ -2130,8 +2145,12 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
   const int nh = c->n_heads, nkv = c->n_kv_heads, d = c->head_dim;
   const fm::CacheAttnPlan p = fm::cache_attn_plan(B, L, nh, nkv, d, prefix_len, lens != nullptr, scored, c->max_len, h->num_sms);
   const int64_t own_rows = static_cast<int64_t>(B) * nkv * c->max_len, prefix_rows = static_cast<int64_t>(nkv) * c->prefix_max;
-  if ((p.tc_s && own_rows > 0x7fffff00LL) || (p.tc_p && prefix_rows > 0x7fffff00LL))
-    return set_err(h, FM_EUNSUPPORTED, "too many cache rows");
+  // the kernels count rows and tiles in 32 bits
+  const double group = nh / nkv, tiles = (c->max_len / 128 + 3.0) * nkv * B * (L * group / 256 + 1) +
+                                         (prefix_len / 128 + 3.0) * nkv * (static_cast<double>(B) * L * group / 256 + 1) +
+                                         (c->max_len + 16.0) * nkv * B / 8 + prefix_len / 8.0 * nkv;
+  if (own_rows > 0x7fffff00LL || prefix_rows > 0x7fffff00LL || tiles > 1e9)
+    return set_err(h, FM_EUNSUPPORTED, "too many rows");
   rc = ensure_sv(h, p.bytes);
   if (rc != FM_OK) return rc;
   fm::CacheAttnArgs a;
@@ -2200,7 +2219,7 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
   }
   fm::TcWeightArgs w;
   std::memset(&w, 0, sizeof(w));
-  if (scored && p.tc_s) {
+  if (scored && p.tc_s && a.group <= fm::kTcKeys) {
     w.q = q;
     w.q_ld = q_ld;
     w.lens = lens;
@@ -2215,6 +2234,9 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
     w.max_len = c->max_len;
     w.key_tiles = (c->max_len + fm::kTcKeys - 1) / fm::kTcKeys;
     w.workers = h->num_sms;
+    w.tile_tokens = fm::kTcKeys / a.group;
+    if (!encode_heads(&maps[1].q, q, d, nh, T, q_ld, a.group, w.tile_tokens))
+      return set_err(h, FM_ECUDA, "cuTensorMapEncodeTiled failed");
     w.scale_log2 = a.scale_log2;
     w.err = a.err;
   }

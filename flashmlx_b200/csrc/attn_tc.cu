@@ -6,8 +6,8 @@
 // group's heads of neighbouring tokens, so that every head that shares the keys shares the
 // loads), two 128-row tiles.  Two streams of 128 softmax threads, a row each, share the tensor
 // pipe and every K / V tile: with more than 128 rows a stream has its own row tile and all keys,
-// with fewer both have the same rows and a stream takes half of each tile's keys; those halves
-// are joined like any two pieces.
+// with fewer both have the same rows and a stream takes half of each tile's keys; their halves
+// are joined in shared memory when the piece ends.
 //
 //   warps 0-3, 4-7  stream 0, 1: Q rows to shared memory (the next piece's are already in
 //                   registers when a piece ends); per 64 keys S out of TMEM, scale and
@@ -133,6 +133,14 @@ FM_DEV uint64_t ex2_poly2(uint64_t x) {
                __uint_as_float(__float_as_uint(ph) + (__float_as_uint(th) << 23)));
 }
 
+FM_DEV void tma_load_3d(uint32_t dst, const void* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
 // 32 columns of this lane's row, without waiting for them
 FM_DEV void tmem_ld32_async(uint32_t taddr, float* v) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -194,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   uint8_t* s_kv = s_q + 2 * S::kTileBytes;           // [NS][kTileBytes]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &bars.abort_flag;
-  const int64_t per = tc_places_per_worker(a, tc_places_before(a, a.items()) * a.nkv);
+  const int per = tc_places_per_worker(a, tc_places_before(a, a.items()) * a.nkv);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -391,58 +399,98 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       if (!ok || !__all_sync(0xffffffffu, mbar_wait(&bars.ofull, oph & 1, abort_flag, a.err))) break;
       ++oph;
       tc_fence_after();
-      const bool whole = a.direct && it.cnt == it.tiles && pair;
+      const bool whole = a.direct && it.cnt == it.tiles;
       if (live) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
         const int64_t row = (tok0 + tk) * a.nh + it.kvh * a.group + (r - tk * a.group);
         const int64_t pr = (static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(it.flat) * a.nkv + it.kvh) * kTcRows +
-                           s * kTcKeys + quad * 32;
+                           (pair ? s * kTcKeys : 0) + quad * 32;
         const uint32_t on_rows = __ballot_sync(0xffffffffu, on);
         const int rsub = lane >> 3, csub = lane & 7;
-        {
-          // a 128-byte line of each row at a time: 32 fp32 or 64 bf16 columns
+        float fac = 1.f;  // on this stream's O
+        if (!pair) {      // one reference for both streams' halves
+          const int other = s == 0 ? static_cast<int>(S::kTileBytes) : -static_cast<int>(S::kTileBytes);
+          reinterpret_cast<float2*>(stage)[lane] = make_float2(ref, l);
+          named_bar_sync(1 + quad, 64);
+          const float2 o = reinterpret_cast<const float2*>(stage + other)[lane];
+          named_bar_sync(1 + quad, 64);
+          const float top = fmaxf(ref, o.x);
+          fac = ref == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2(ref - top);
+          l = l * fac + (o.x == -INFINITY ? o.y : o.y * ex2(o.x - top));
+          ref = top;
+        }
+        const float mul = whole ? (l == 0.f ? 0.f : fac / l) : fac;
+        // a 128-byte line of each row at a time: 32 fp32 or 64 bf16 columns
 #pragma unroll 1
-          for (int c = 0; c < D; c += whole ? 64 : 32) {
-            __syncwarp();
-            if (whole) {
-#pragma unroll 1
-              for (int hh = 0; hh < 2; ++hh) {
-                float o[32];
-                tmem_ld32(t_o + c + 32 * hh, o);
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          __syncwarp();
+          tmem_ld32(t_o + c, o);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  *reinterpret_cast<uint4*>(stage + sw128_off(lane, 4 * hh + e)) =
-                      make_uint4(pack_bf16x2(o[8 * e] * inv, o[8 * e + 1] * inv), pack_bf16x2(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
-                                 pack_bf16x2(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack_bf16x2(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
-              }
-            } else {
-              float o[32];
-              tmem_ld32(t_o + c, o);
+          for (int e = 0; e < 32; ++e) o[e] *= mul;
+          if (!pair) {  // stream 1 hands its half over
+            if (s == 1) {
 #pragma unroll
               for (int e = 0; e < 8; ++e)
                 *reinterpret_cast<float4*>(stage + sw128_off(lane, e)) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
-            __syncwarp();
+            named_bar_sync(1 + quad, 64);
+            if (s == 0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int rr = 4 * i + rsub;
-              const uint4 v = *reinterpret_cast<const uint4*>(stage + sw128_off(rr, csub));
-              const int64_t out_row = __shfl_sync(0xffffffffu, row, rr);
-              if (!(on_rows >> rr & 1)) continue;
-              if (whole) *reinterpret_cast<uint4*>(a.out + out_row * D + c + 8 * csub) = v;
-              else *reinterpret_cast<uint4*>(a.part_o + (pr + rr) * D + c + 4 * csub) = v;
+              for (int e = 0; e < 8; ++e) {
+                const float4 h = *reinterpret_cast<const float4*>(stage + S::kTileBytes + sw128_off(lane, e));
+                o[4 * e] += h.x;
+                o[4 * e + 1] += h.y;
+                o[4 * e + 2] += h.z;
+                o[4 * e + 3] += h.w;
+              }
             }
+            named_bar_sync(1 + quad, 64);
+            if (s == 1) continue;
+          }
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(stage + sw128_off(lane, (c >> 3 & 4) + e)) =
+                  make_uint4(pack_bf16x2(o[8 * e], o[8 * e + 1]), pack_bf16x2(o[8 * e + 2], o[8 * e + 3]),
+                             pack_bf16x2(o[8 * e + 4], o[8 * e + 5]), pack_bf16x2(o[8 * e + 6], o[8 * e + 7]));
+            if (!(c & 32)) continue;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<float4*>(stage + sw128_off(lane, e)) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int rr = 4 * i + rsub;
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + sw128_off(rr, csub));
+            const int64_t out_row = __shfl_sync(0xffffffffu, row, rr);
+            if (!(on_rows >> rr & 1)) continue;
+            if (whole) *reinterpret_cast<uint4*>(a.out + out_row * D + (c & ~63) + 8 * csub) = v;
+            else *reinterpret_cast<uint4*>(a.part_o + (pr + rr) * D + c + 4 * csub) = v;
           }
         }
-        if (on) {
+        if (on && (pair || s == 0)) {
           if (!whole) a.part_ml[pr + lane] = make_float2(ref, l);
-          else if (a.lse2) a.lse2[row] = l == 0.f ? INFINITY : ref + log2f(l);
+          else if (a.lse2) a.lse2[(static_cast<int64_t>(b) * a.nkv + it.kvh) * rows + r] = l == 0.f ? INFINITY : ref + log2f(l);
         }
         __syncwarp();
       }
       it = nx;
       store_q(it);
     }
+    // items whose rows see nothing are in no worker's range
+    if (ok && a.direct)
+      for (int f = blockIdx.x; f < a.items(); f += gridDim.x) {
+        if (a.tiles(f) > 0) continue;
+        const int b = f / a.rps, row_base = (f - b * a.rps) * kTcRows, n = min(rows - row_base, kTcRows);
+        for (int i = threadIdx.x; i < n * a.nkv * (D / 8); i += kMmaWarp * 32) {
+          const int ch = i % (D / 8), rk = i / (D / 8), kvh = rk / n, r = row_base + rk - kvh * n, tk = r / a.group;
+          *reinterpret_cast<uint4*>(a.out + ((static_cast<int64_t>(b) * a.L + tk) * a.nh + kvh * a.group + r - tk * a.group) * D +
+                                    8 * ch) = make_uint4(0, 0, 0, 0);
+          if (ch == 0 && a.lse2) a.lse2[(static_cast<int64_t>(b) * a.nkv + kvh) * rows + r] = INFINITY;
+        }
+      }
   } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------------- MMA issuer
     // elect.sync, not a lane test: one lane chosen so lets the compiler hold the operands in uniform
@@ -587,9 +635,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 // key's weight and needs no other thread.  The two groups of 128 threads take every other row
 // tile.  Bound by the exponentials (128 x 128 a tile: 1024 cycles of the special-function units
 // against 512 of the tensor pipe), of which a third go to fused multiply-adds here.
-//   warps 0-3, 4-7  groups 0, 1     warp 8  MMA issuer     warps 9-12  K (TMA) and Q (cp.async)
+//   warps 0-3, 4-7  groups 0, 1     warp 8  MMA issuer     warp 9  TMA loads of K and Q
 namespace {
-constexpr int kWThreads = 416;
+constexpr int kWThreads = 320;
 constexpr int kWStages = 4;    // Q tiles, their rows' lse, TMEM buffers
 constexpr int kWPolyEvery = 3;
 
@@ -608,7 +656,8 @@ struct WBars {
 
 template <int D>
 __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __grid_constant__ TcWeightArgs a,
-                                                                     const __grid_constant__ CUtensorMap map_k) {
+                                                                     const __grid_constant__ CUtensorMap map_k,
+                                                                     const __grid_constant__ CUtensorMap map_q) {
   using S = WShape<D>;
   extern __shared__ uint8_t s_raw[];
   __shared__ WBars bars;
@@ -618,10 +667,10 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
   uint8_t* s_q = s_k + 2 * S::kTileBytes;        // [kWStages][kTileBytes]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &bars.abort_flag;
-  const int64_t per = tc_places_per_worker(a, tc_places_before(a, a.items()) * a.nkv);
+  const int per = tc_places_per_worker(a, tc_places_before(a, a.items()) * a.nkv);
   if (threadIdx.x == 0) {
     for (int i = 0; i < kWStages; ++i) {
-      mbar_init(&bars.qfull[i], 4);
+      mbar_init(&bars.qfull[i], 2);  // the copy, and the rows' lse
       mbar_init(&bars.sfull[i], 1);
       mbar_init(&bars.sempty[i], 4);
     }
@@ -634,6 +683,10 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
   }
+  // rows past a Q tile's whole tokens are never copied: zeros
+  for (uint32_t i = threadIdx.x; i < kWStages * S::kTileBytes / 16; i += kWThreads)
+    reinterpret_cast<uint4*>(s_q)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async();
   if (warp == 8) {
     tmem_alloc(&bars.tmem, 512);
     tmem_relinquish();
@@ -657,7 +710,8 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
     for (; ok && it.cnt > 0; tc_next(a, it)) {
       const int b = it.flat / a.key_tiles, key0 = (it.flat - b * a.key_tiles) * kTcKeys;
       const int len = a.lens[b];
-      const int row0 = (a.first_tile(b, key0, len) + it.tile) * kTcKeys;
+      const int tile_rows = a.tile_tokens * a.group;
+      const int row0 = (a.first_tile(key0, len) + it.tile) * tile_rows;
       // the first row that sees this lane's key; the item's last key's bounds the masked tiles
       const int tk = max(key0 + kl - (len - a.L), 0), tk_last = max(min(key0 + kTcKeys, len) - 1 - (len - a.L), 0);
       const int rmin = key0 + kl < len ? tk * a.group : 0x7fffffff, rmin_last = tk_last * a.group;
@@ -672,8 +726,9 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
           break;
         }
         tc_fence_after();
-        const int r0 = row0 + i * kTcKeys;
-        const bool masked = r0 < rmin_last;
+        const int r0 = row0 + i * tile_rows;
+        // a copy past the sequence's tokens brings another's rows
+        const bool masked = r0 < rmin_last || r0 + tile_rows > rows;
         uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll 1
         for (int c = 0; c < kTcKeys; c += 32) {
@@ -682,7 +737,7 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
           tmem_wait_ld();
           if (masked) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = r0 + c + e >= rmin ? v[e] * a.scale_log2 : -INFINITY;
+            for (int e = 0; e < 32; ++e) v[e] = r0 + c + e >= rmin && r0 + c + e < rows ? v[e] * a.scale_log2 : -INFINITY;
           }
           const uint64_t mul = masked ? pack2(1.f, 1.f) : scale2;
           const float4* nl = reinterpret_cast<const float4*>(&s_lse[st][c]);
@@ -745,79 +800,60 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
     }
     __syncwarp();
   } else {
-    // ---------------------------------------------------------------- loaders
-    const int lt = threadIdx.x - 9 * 32;  // 0..127
-    constexpr int CPR = D / 8, RPI = kTcKeys / CPR;  // chunks of a row, rows a pass brings
-    const int ch = lt % CPR;
+    // ---------------------------------------------------------------- loader
+    const int tile_rows = a.tile_tokens * a.group;
+    const uint32_t tile_bytes = static_cast<uint32_t>(tile_rows) * 128;  // of a 64-column half
     bool ok = true;
-    uint32_t n = 0, sent = 0;  // items; tiles whose copies were reported complete
-    auto publish = [&](uint32_t upto) {  // this thread's copies of tiles [sent, upto) are complete
-      fence_proxy_async();
-      __syncwarp();
-      for (; sent < upto; ++sent)
-        if (lane == 0) mbar_arrive(&bars.qfull[sent % kWStages]);
-    };
+    uint32_t n = 0;  // items
     for (; ok && it.cnt > 0; tc_next(a, it), ++n) {
       const int b = it.flat / a.key_tiles, key0 = (it.flat - b * a.key_tiles) * kTcKeys;
-      const int row0 = (a.first_tile(b, key0, a.lens[b]) + it.tile) * kTcKeys;
-      if (warp == 9) {
-        if (!mbar_wait_lane0(&bars.kempty[n & 1], (n >> 1 & 1) ^ 1, abort_flag, a.err)) {
-          ok = false;
-        } else if (elect_one()) {
-          mbar_arrive_expect_tx(&bars.kfull[n & 1], S::kTileBytes);
+      const int tile0 = a.first_tile(key0, a.lens[b]) + it.tile;
+      if (!mbar_wait_lane0(&bars.kempty[n & 1], (n >> 1 & 1) ^ 1, abort_flag, a.err)) break;
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&bars.kfull[n & 1], S::kTileBytes);
 #pragma unroll
-          for (int h = 0; h < D / 64; ++h)
-            tma_load_2d(smem_u32(s_k + (n & 1) * S::kTileBytes) + h * (kTcKeys * 128), &map_k, h * 64,
-                        (b * a.nkv + it.kvh) * a.max_len + key0, &bars.kfull[n & 1]);
-        }
-        __syncwarp();
-        if (!ok) break;
+        for (int h = 0; h < D / 64; ++h)
+          tma_load_2d(smem_u32(s_k + (n & 1) * S::kTileBytes) + h * (kTcKeys * 128), &map_k, h * 64,
+                      (b * a.nkv + it.kvh) * a.max_len + key0, &bars.kfull[n & 1]);
       }
-      const uint16_t* q = a.q + static_cast<int64_t>(b) * a.L * a.q_ld + static_cast<int64_t>(it.kvh) * a.group * D + ch * 8;
-      const float* lse = a.lse2 + static_cast<int64_t>(b) * a.L * a.nh + it.kvh * a.group;
+      __syncwarp();
+      const float* lse = a.lse2 + (static_cast<int64_t>(b) * a.nkv + it.kvh) * rows;
+      float nl[4];
+      auto fetch = [&](int i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = 32 * e + lane, r = (tile0 + i) * tile_rows + c;
+          nl[e] = c < tile_rows && r < rows ? -lse[r] : -INFINITY;
+        }
+      };
+      fetch(0);
       for (int i = 0; i < it.cnt; ++i, ++t) {
         const uint32_t st = t % kWStages;
-        const int r0 = row0 + i * kTcKeys;
-        int r = r0 + lt;
-        float nl = -INFINITY;
-        if (r < rows) {
-          const int tk = r / a.group;
-          nl = -lse[static_cast<int64_t>(tk) * a.nh + r - tk * a.group];
-        }
         // the sums of tile t - 4 were taken, so its product is complete: its stage is free
-        if (!__all_sync(0xffffffffu, mbar_wait(&bars.sempty[st], (t / kWStages & 1) ^ 1, abort_flag, a.err))) {
+        if (!mbar_wait_lane0(&bars.sempty[st], (t / kWStages & 1) ^ 1, abort_flag, a.err)) {
           ok = false;
           break;
         }
-        s_lse[st][lt] = nl;
-        const uint32_t dst = smem_u32(s_q + st * S::kTileBytes) + (ch >> 3) * (kTcKeys * 128);
-        r = r0 + lt / CPR;
-        int tk = r / a.group, gq = r - tk * a.group;
-#pragma unroll 4
-        for (int e = 0; e < CPR; ++e) {
-          const bool on = r < rows;
-          const uint16_t* src = q + (on ? tk * a.q_ld + gq * D : 0);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + sw128_off(r - r0, ch & 7)), "l"(src),
-                       "r"(on ? 16 : 0)
-                       : "memory");
-          r += RPI;
-          gq += RPI;
-          while (gq >= a.group) {
-            gq -= a.group;
-            ++tk;
-          }
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&bars.qfull[st], tile_bytes * (D / 64));
+#pragma unroll
+          for (int h = 0; h < D / 64; ++h)
+            tma_load_3d(smem_u32(s_q + st * S::kTileBytes) + h * (kTcKeys * 128), &map_q, h * 64, it.kvh * a.group,
+                        b * a.L + (tile0 + i) * a.tile_tokens, &bars.qfull[st]);
         }
-        cp_async_commit();
-        cp_async_wait<1>();  // all but this tile's
-        publish(t);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s_lse[st][32 * e + lane] = nl[e];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.qfull[st]);
+        if (i + 1 < it.cnt) fetch(i + 1);
       }
-      if (!ok) break;
     }
-    cp_async_wait<0>();
-    publish(t);
-    // a K tile in flight lands before the CTA leaves (its item's products waited for it unless a
-    // wait ran out)
-    if (warp == 9 && !ok && n > 0) wait_drained(&bars.kfull[(n - 1) & 1], (n - 1) >> 1 & 1, a.err);
+    // copies in flight land before the CTA leaves (their products waited for them unless a wait
+    // ran out)
+    if (*abort_flag) {
+      for (uint32_t j = t > kWStages ? t - kWStages : 0; j < t; ++j) wait_drained(&bars.qfull[j % kWStages], j / kWStages & 1, a.err);
+      if (n > 0) wait_drained(&bars.kfull[(n - 1) & 1], (n - 1) >> 1 & 1, a.err);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -839,11 +875,11 @@ cudaError_t attn_tc_init() {
   return e == cudaSuccess ? tc_opt_in<64>() : e;
 }
 
-cudaError_t launch_slot_weight_tc(const TcWeightArgs& a, int d, const CUtensorMap& k, cudaStream_t st) {
+cudaError_t launch_slot_weight_tc(const TcWeightArgs& a, int d, const CUtensorMap& k, const CUtensorMap& q, cudaStream_t st) {
   if (d == 128)
-    slot_weight_tc_kernel<128><<<a.workers, kWThreads, WShape<128>::kSmem, st>>>(a, k);
+    slot_weight_tc_kernel<128><<<a.workers, kWThreads, WShape<128>::kSmem, st>>>(a, k, q);
   else
-    slot_weight_tc_kernel<64><<<a.workers, kWThreads, WShape<64>::kSmem, st>>>(a, k);
+    slot_weight_tc_kernel<64><<<a.workers, kWThreads, WShape<64>::kSmem, st>>>(a, k, q);
   return cudaGetLastError();
 }
 

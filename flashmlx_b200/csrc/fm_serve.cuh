@@ -34,6 +34,7 @@ struct RopeArgs {
 //   attn_tc_kernel (attn_tc.cu), a worker a CTA, for many: items of 256 query rows (of the heads
 //     that share a kv head, neighbouring tokens together), tiles of 128 keys, tcgen05.
 //
+// The host refuses calls of 2^31 / 2 tiles or rows.
 // Either way the tiles of all items, in order, are cut into one contiguous range per worker, so
 // ragged lengths balance.  A worker's piece of an item leaves an unnormalised fp32 output,
 // its maximum (log2 units) and its sum in slot worker + item -- both only grow along the
@@ -69,7 +70,7 @@ struct CacheAttnArgs {
   int workers;
   float* part_o;            // [slots][16][d]
   float2* part_ml;          // [slots][16] (maximum in log2 units, sum)
-  float* lse2;              // [B * L, nh] or null
+  float* lse2;              // [B, nkv, L * group] or null
   uint32_t* err;
 };
 
@@ -83,11 +84,11 @@ struct TcAttnArgs {
   int head_rows;            // rows of K / V from one (sequence, kv head) to the next
   int rps;                  // items per (sequence, kv head)
   int workers;              // 0: this source is not read here
-  int direct;               // the only source: an unsplit item's rows go to out
+  int direct;               // the only source: an item that one worker has whole goes to out
   float scale_log2;         // >= 0
   uint32_t q_sign;          // 0x80008000: q is negated (a negative scale)
-  float* part_o;            // [workers + items][256][d]; with one tile of rows, stream 1's piece
-  float2* part_ml;          //   in rows 128 ..
+  float* part_o;            // [workers + items][256][d]
+  float2* part_ml;
   uint16_t* out;
   float* lse2;
   uint32_t* err;
@@ -101,16 +102,18 @@ struct TcAttnArgs {
 };
 
 // The slot weights by slot_weight_tc_kernel (attn_tc.cu): an item is a kv head's 128 keys, its
-// tiles the query rows that see any of them, 128 at a time.
+// tiles the query rows that see any of them, tile_tokens whole tokens (at most 128 rows) at a
+// time.
 struct TcWeightArgs {
   const uint16_t* q;        // [B * L, q_ld]
   int64_t q_ld;
   const int32_t* lens;
-  const float* lse2;        // [B * L, nh]
+  const float* lse2;        // [B, nkv, L * group]
   float* acc;               // [B, nkv, max_len]
   float* part;              // [workers + items][2][128] sums of a piece's even and odd tiles
   int B, L, nh, nkv, group, max_len;
   int key_tiles;            // of max_len
+  int tile_tokens;          // 128 / group
   int workers;
   float scale_log2;
   uint32_t* err;
@@ -118,7 +121,7 @@ struct TcWeightArgs {
   static constexpr int kItemCost = 2;
 #ifdef __CUDACC__
   __device__ int items() const { return B * key_tiles; }
-  __device__ int first_tile(int b, int key0, int len) const;  // of the rows that see key0
+  __device__ int first_tile(int key0, int len) const;  // of the rows that see key0
   __device__ int tiles(int flat) const;
 #endif
 };
@@ -134,22 +137,20 @@ __device__ __forceinline__ int TcAttnArgs::tiles(int flat) const {
   const int len = tc_len(*this, b);
   int seen = len;
   if (causal) {
-    const int64_t last = (static_cast<int64_t>(rp) * kTcRows + kTcRows - 1) / group;
-    seen = len - L + static_cast<int>(last < L - 1 ? last : L - 1) + 1;
+    seen = len - L + min((rp * kTcRows + kTcRows - 1) / group, L - 1) + 1;
   }
   return seen <= 0 ? 0 : (seen + kTcKeys - 1) / kTcKeys;
 }
 
-__device__ __forceinline__ int TcWeightArgs::first_tile(int b, int key0, int len) const {
-  const int tk = key0 - (len - L);  // the first token that sees key0
-  return tk > 0 ? static_cast<int>(static_cast<int64_t>(tk) * group / kTcKeys) : 0;
+__device__ __forceinline__ int TcWeightArgs::first_tile(int key0, int len) const {
+  return max(key0 - (len - L), 0) / tile_tokens;  // token key0 - (len - L) is the first that sees key0
 }
 
 __device__ __forceinline__ int TcWeightArgs::tiles(int flat) const {
   const int b = flat / key_tiles, key0 = (flat - b * key_tiles) * kTcKeys;
   const int len = lens[b];
   if (len < 0 || len > max_len || key0 >= len) return 0;
-  return (L * group + kTcKeys - 1) / kTcKeys - first_tile(b, key0, len);
+  return (L + tile_tokens - 1) / tile_tokens - first_tile(key0, len);
 }
 
 // An item's start and end cost a worker about as much as kItemCost tiles, so the order has that
@@ -162,33 +163,59 @@ FM_DEV int tc_item_places(const A& a, int flat) {
 
 // places of one kv head of items [0, n), summed by the whole warp
 template <class A>
-FM_DEV int64_t tc_places_before(const A& a, int n) {
-  int64_t s = 0;
+FM_DEV int tc_places_before(const A& a, int n) {
+  int s = 0;
   for (int i = threadIdx.x & 31; i < n; i += 32) s += tc_item_places(a, i);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  return s;
+  return __reduce_add_sync(0xffffffffu, s);
 }
 
 template <class A>
-FM_DEV int64_t tc_places_per_worker(const A& a, int64_t total) {
-  const int64_t per = (total + a.workers - 1) / a.workers;
-  return per < 1 ? 1 : per;
+FM_DEV int tc_places_per_worker(const A& a, int total) {
+  return max(1, (total + a.workers - 1) / a.workers);
+}
+
+// The item (flat, kvh) that place `place` falls into, and which of its places; false past the
+// end.  Whole warp.
+template <class A>
+FM_DEV bool tc_locate(const A& a, int place, int& flat, int& kvh, int& at) {
+  const int lane = threadIdx.x & 31;
+  int rest = place;
+  for (int base = 0; base < a.items(); base += 32) {
+    const int i = base + lane;
+    const int mine = i < a.items() ? tc_item_places(a, i) * a.nkv : 0;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, incl > rest);
+    if (past) {
+      const int f = __ffs(past) - 1;
+      rest -= __shfl_sync(0xffffffffu, incl - mine, f);
+      const int places = __shfl_sync(0xffffffffu, mine, f) / a.nkv;
+      flat = base + f;
+      kvh = rest / places;
+      at = rest - kvh * places;
+      return true;
+    }
+    rest -= __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return false;
 }
 
 // A worker's piece in hand: tiles [tile, tile + cnt) of item (flat, kvh); cnt 0 at the end.
 struct TcPiece {
   int flat, kvh, tile, tiles, cnt;
-  int64_t left;  // places of the worker's range from the item's first (or the range's) on
+  int left;  // places of the worker's range from the item's first (or the range's) on
 };
 
 // the piece of the range that begins at place `at` of item (flat, kvh)
 template <class A>
 FM_DEV void tc_cut(const A&, TcPiece& p, int at) {
-  const int64_t end = at + p.left;  // in the item's places
-  p.tile = at > A::kItemCost ? at - A::kItemCost : 0;
-  const int64_t last = end - A::kItemCost < p.tiles ? end - A::kItemCost : p.tiles;
-  p.cnt = last > p.tile ? static_cast<int>(last - p.tile) : 0;
+  const int end = at + p.left;  // in the item's places
+  p.tile = max(at - A::kItemCost, 0);
+  p.cnt = max(min(end - A::kItemCost, p.tiles) - p.tile, 0);
   p.left -= p.tiles + A::kItemCost - at;
 }
 
@@ -209,34 +236,14 @@ FM_DEV void tc_next(const A& a, TcPiece& p) {
 }
 
 template <class A>
-FM_DEV void tc_first(const A& a, int worker, int64_t per, TcPiece& p) {  // whole warp
-  const int lane = threadIdx.x & 31;
-  int64_t rest = worker * per;
+FM_DEV void tc_first(const A& a, int worker, int per, TcPiece& p) {  // whole warp
+  int at;
   p.left = per;
   p.cnt = 0;
-  for (int base = 0; base < a.items(); base += 32) {
-    const int i = base + lane;
-    const int64_t mine = i < a.items() ? static_cast<int64_t>(tc_item_places(a, i)) * a.nkv : 0;
-    int64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
-    const uint32_t past = __ballot_sync(0xffffffffu, incl > rest);
-    if (past) {
-      const int f = __ffs(past) - 1;
-      rest -= __shfl_sync(0xffffffffu, incl - mine, f);
-      p.flat = base + f;
-      p.tiles = a.tiles(p.flat);
-      const int places = p.tiles + A::kItemCost;
-      p.kvh = static_cast<int>(rest / places);
-      tc_cut(a, p, static_cast<int>(rest - static_cast<int64_t>(p.kvh) * places));
-      if (p.cnt == 0) tc_next(a, p);
-      return;
-    }
-    rest -= __shfl_sync(0xffffffffu, incl, 31);
-  }
+  if (!tc_locate(a, worker * per, p.flat, p.kvh, at)) return;
+  p.tiles = a.tiles(p.flat);
+  tc_cut(a, p, at);
+  if (p.cnt == 0) tc_next(a, p);
 }
 #endif
 
@@ -273,12 +280,13 @@ cudaError_t cache_attn_init();
 // p, s: the prefix / own caches by attn_tc_kernel where their workers are set, with its maps
 struct TcMapsKV {
   CUtensorMap k, v;
+  CUtensorMap q;  // the slot weights' query tiles: [tokens][heads][d], box {64, group, tile_tokens}
 };
 cudaError_t launch_cache_attn(const CacheAttnArgs& a, const TcAttnArgs& p, const TcMapsKV& mp, const TcAttnArgs& s,
                               const TcMapsKV& ms, const TcWeightArgs& w, int d, cudaStream_t st);
 cudaError_t attn_tc_init();
 cudaError_t launch_attn_tc(const TcAttnArgs& a, int d, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st);
-cudaError_t launch_slot_weight_tc(const TcWeightArgs& a, int d, const CUtensorMap& k, cudaStream_t st);
+cudaError_t launch_slot_weight_tc(const TcWeightArgs& a, int d, const CUtensorMap& k, const CUtensorMap& q, cudaStream_t st);
 cudaError_t launch_evict(const EvictArgs& a, int num_sms, cudaStream_t st);
 
 }  // namespace fm

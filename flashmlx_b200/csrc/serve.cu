@@ -183,23 +183,16 @@ FM_DEV int seq_len(const CacheAttnArgs& a, int b) {
   return n < 0 || n > a.max_len ? 0 : n;  // reported by the merge
 }
 
-FM_DEV int64_t warp_sum64(int64_t v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 // tiles of one item of sequences [0, b), summed; whole warp, B <= a few thousand
-FM_DEV int64_t tiles_before(const CacheAttnArgs& a, int b) {
+FM_DEV int tiles_before(const CacheAttnArgs& a, int b) {
   const int lane = threadIdx.x & 31;
-  int64_t s = 0;
+  int s = 0;
   for (int i = lane; i < b; i += 32) s += (seq_len(a, i) + kAttnTile - 1) / kAttnTile;
-  return warp_sum64(s);
+  return __reduce_add_sync(0xffffffffu, s);
 }
 
-FM_DEV int64_t tiles_per_worker(const CacheAttnArgs& a, int64_t total) {
-  const int64_t per = (total + a.workers - 1) / a.workers;
-  return per < kAttnMinTiles ? kAttnMinTiles : per;
+FM_DEV int tiles_per_worker(const CacheAttnArgs& a, int total) {
+  return max(kAttnMinTiles, (total + a.workers - 1) / a.workers);
 }
 
 FM_DEV void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
@@ -235,34 +228,34 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const uint32_t ring = smem_u32(s_kv) + warp * (kAttnStages * STAGE);
-  const int64_t worker = static_cast<int64_t>(blockIdx.x) * kAttnWarps + warp;
+  const int worker = blockIdx.x * kAttnWarps + warp;
 
-  const int64_t tp = (a.split_prefix + kAttnTile - 1) / kAttnTile;  // tiles of a prefix item
-  const int np = a.nkv * a.rt_p, ns = a.nkv * a.rt_s;             // items of the prefix / of a sequence
-  const int64_t total_p = tp * np;
-  const int64_t total = total_p + ns * tiles_before(a, a.B);
-  const int64_t per = tiles_per_worker(a, total);
-  int64_t t = worker * per;
-  const int64_t t_end = min(total, t + per);
+  const int tp = (a.split_prefix + kAttnTile - 1) / kAttnTile;  // tiles of a prefix item
+  const int np = a.nkv * a.rt_p, ns = a.nkv * a.rt_s;           // items of the prefix / of a sequence
+  const int total_p = tp * np;
+  const int total = total_p + ns * tiles_before(a, a.B);
+  const int per = tiles_per_worker(a, total);
+  int t = worker * per;
+  const int t_end = min(total, t + per);
   if (t >= t_end) return;
 
   // the item of tile t: sequence (-1: the prefix), item of it, tile of the item
   int b = -1, item, tiles;
   int tile;
   if (t < total_p) {
-    item = static_cast<int>(t / tp);
-    tile = static_cast<int>(t - item * tp);
-    tiles = static_cast<int>(tp);
+    item = t / tp;
+    tile = t - item * tp;
+    tiles = tp;
   } else {
-    int64_t rest = t - total_p;
+    int rest = t - total_p;
     b = 0;
     while (true) {  // 32 sequences at a time
       const int i = b + lane;
-      const int64_t mine = i < a.B ? static_cast<int64_t>(ns) * ((seq_len(a, i) + kAttnTile - 1) / kAttnTile) : 0;
-      int64_t incl = mine;
+      const int mine = i < a.B ? ns * ((seq_len(a, i) + kAttnTile - 1) / kAttnTile) : 0;
+      int incl = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += up;
       }
       const uint32_t past = __ballot_sync(0xffffffffu, incl > rest);
@@ -277,12 +270,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
       if (b >= a.B) return;  // t < total makes this unreachable
     }
     tiles = (seq_len(a, b) + kAttnTile - 1) / kAttnTile;
-    item = static_cast<int>(rest / tiles);
-    tile = static_cast<int>(rest - static_cast<int64_t>(item) * tiles);
+    item = rest / tiles;
+    tile = rest - item * tiles;
   }
 
   while (t < t_end) {
-    const int cnt = static_cast<int>(min(static_cast<int64_t>(tiles - tile), t_end - t));
+    const int cnt = min(tiles - tile, t_end - t);
     const bool pre = b < 0;
     const int rts = pre ? a.rt_p : a.rt_s;
     const int kvh = item / rts, row0 = (item - kvh * rts) * kAttnRowTile;
@@ -402,8 +395,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
     }
     cp_async_wait<0>();
 
-    const int64_t gi = pre ? item : np + static_cast<int64_t>(b) * ns + item;
-    const int64_t slot = worker + gi;
+    const int64_t slot = worker + (pre ? item : np + static_cast<int64_t>(b) * ns + item);
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
@@ -426,118 +418,152 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
       item = 0;
       while (seq_len(a, b) == 0) ++b;  // tiles are left, so a sequence that has some follows
     }
-    tiles = b < 0 ? static_cast<int>(tp) : (seq_len(a, b) + kAttnTile - 1) / kAttnTile;
+    tiles = b < 0 ? tp : (seq_len(a, b) + kAttnTile - 1) / kAttnTile;
   }
 }
 
 // Joins the pieces of output rows: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, zeros when
-// nothing was seen; lse2 = M + log2(sum) for the slot weights.  A block takes a.merge_rows of
-// a (sequence, kv head)'s rows (fewer when there are few in all: a row's pieces are read one
-// after the other), a warp every fourth of them.
+// nothing was seen; lse2 = M + log2(sum) for the slot weights.
+namespace {
 
 template <int D>
+struct RowJoin {
+  static constexpr int V = D / 32;  // columns of a lane
+  static constexpr int U = 8;       // pieces whose loads are in flight together
+  float acc[V] = {};
+  float M = -INFINITY, S = 0.f;
+
+  // n pieces, piece i in row row0 + i * step of a part buffer
+  FM_DEV void add(const float* part_o, const float2* part_ml, int64_t row0, int step, int n) {
+    const int lane = threadIdx.x & 31;
+    for (int i0 = 0; i0 < n; i0 += U) {
+      float2 ml[U];
+      float v[U][V];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t pr = row0 + static_cast<int64_t>(min(i0 + u, n - 1)) * step;
+        ml[u] = part_ml[pr];
+        const float* po = part_o + pr * D + lane * V;
+        if (V == 4) {
+          const float4 t4 = *reinterpret_cast<const float4*>(po);
+          v[u][0] = t4.x; v[u][1] = t4.y; v[u][2 % V] = t4.z; v[u][3 % V] = t4.w;
+        } else {
+          const float2 t2 = *reinterpret_cast<const float2*>(po);
+          v[u][0] = t2.x; v[u][1] = t2.y;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i0 + u >= n || ml[u].y == 0.f) continue;  // the piece's keys are all hidden from this row
+        const float mn = fmaxf(M, ml[u].x);
+        const float wa = exp2f(M - mn), wb = exp2f(ml[u].x - mn);
+        M = mn;
+        S = S * wa + ml[u].y * wb;
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = acc[e] * wa + v[u][e] * wb;
+      }
+    }
+  }
+
+  // row r of (sequence b, kv head kvh)
+  FM_DEV void store(const CacheAttnArgs& a, int b, int kvh, int r) const {
+    const int lane = threadIdx.x & 31;
+    const float inv = S == 0.f ? 0.f : 1.f / S;
+    const int tk = r / a.group;
+    uint16_t* out = a.out + ((static_cast<int64_t>(b) * a.L + tk) * a.nh + kvh * a.group + (r - tk * a.group)) * D + lane * V;
+#pragma unroll
+    for (int i = 0; i < V; i += 2)
+      *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
+    if (a.lse2 && lane == 0)
+      a.lse2[(static_cast<int64_t>(b) * a.nkv + kvh) * a.L * a.group + r] = S == 0.f ? INFINITY : M + log2f(S);
+  }
+};
+
+}  // namespace
+
+// Every row of a (sequence, kv head): a block takes a.merge_rows of them (fewer when there are few
+// in all: a row's pieces are read one after the other), a warp every fourth.
+template <int D>
 __global__ void __launch_bounds__(128) attn_merge_kernel(const CacheAttnArgs a, const TcAttnArgs tp, const TcAttnArgs ts) {
-  constexpr int V = D / 32;  // columns of a lane
-  constexpr int U = 8;       // pieces whose loads are in flight together
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
   const int b = blockIdx.z, kvh = blockIdx.y;
   const int rows = a.L * a.group, first_row = blockIdx.x * a.merge_rows;
   if (a.lens && threadIdx.x == 0 && blockIdx.x == 0 && kvh == 0 && (a.lens[b] < 0 || a.lens[b] > a.max_len))
     report(a.err, DEVERR_BOUNDS);
   // the split kernel's cut
-  const int64_t tp16 = (a.split_prefix + kAttnTile - 1) / kAttnTile;
+  const int tp16 = (a.split_prefix + kAttnTile - 1) / kAttnTile;
   const int np = a.nkv * a.rt_p, ns = a.nkv * a.rt_s;
-  int64_t per = 1, own_first = 0, own_tiles = 0;
+  int per = 1, own_first = 0, own_tiles = 0;
   if (a.workers) {
     per = tiles_per_worker(a, tp16 * np + ns * tiles_before(a, a.B));
     own_tiles = (seq_len(a, b) + kAttnTile - 1) / kAttnTile;
-    own_first = tp16 * np + ns * tiles_before(a, b) + static_cast<int64_t>(kvh) * a.rt_s * own_tiles;
+    own_first = tp16 * np + ns * tiles_before(a, b) + kvh * a.rt_s * own_tiles;
   }
-  // the tcgen05 kernel's cuts
-  int64_t per_p = 1, tiles_p = 0, per_s = 1, first_s = 0, tiles_s = 0;  // first_s: a place
-  int flat_s = 0;
+  // the tcgen05 kernel's cuts, in places
+  constexpr int kCost = TcAttnArgs::kItemCost;
+  int per_p = 1, tiles_p = 0, per_s = 1, first_s = 0, tiles_s = 0, flat_s = 0;
   if (tp.workers) {
     tiles_p = tp.tiles(0);
-    per_p = tc_places_per_worker(tp, (tiles_p + TcAttnArgs::kItemCost) * tp.rps * tp.nkv);
+    per_p = tc_places_per_worker(tp, (tiles_p + kCost) * tp.rps * tp.nkv);
   }
   if (ts.workers) {
     flat_s = b * ts.rps + first_row / kTcRows;
     tiles_s = ts.tiles(flat_s);
     per_s = tc_places_per_worker(ts, tc_places_before(ts, ts.items()) * ts.nkv);
-    first_s = tc_places_before(ts, flat_s) * ts.nkv + kvh * (tiles_s + TcAttnArgs::kItemCost) + TcAttnArgs::kItemCost;
-    // written by the kernel itself when one worker had the item whole and a row is one stream's
-    const bool pair = rows - first_row / kTcRows * kTcRows > kTcKeys;
-    if (ts.direct && pair && tiles_s > 0 && first_s / per_s == (first_s + tiles_s - 1) / per_s) return;
+    first_s = tc_places_before(ts, flat_s) * ts.nkv + kvh * (tiles_s + kCost) + kCost;
   }
   for (int r = first_row + warp; r < min(rows, first_row + a.merge_rows); r += 4) {
-    float acc[V] = {};
-    float M = -INFINITY, S = 0.f;
-    // n pieces, piece i in row row0 + i * step of a part buffer
-    auto join = [&](const float* part_o, const float2* part_ml, int64_t row0, int64_t step, int n) {
-      for (int i0 = 0; i0 < n; i0 += U) {
-        float2 ml[U];
-        float v[U][V];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int64_t pr = row0 + min(i0 + u, n - 1) * step;
-          ml[u] = part_ml[pr];
-          const float* po = part_o + pr * D + lane * V;
-          if (V == 4) {
-            const float4 t4 = *reinterpret_cast<const float4*>(po);
-            v[u][0] = t4.x; v[u][1] = t4.y; v[u][2 % V] = t4.z; v[u][3 % V] = t4.w;
-          } else {
-            const float2 t2 = *reinterpret_cast<const float2*>(po);
-            v[u][0] = t2.x; v[u][1] = t2.y;
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (i0 + u >= n || ml[u].y == 0.f) continue;  // the piece's keys are all hidden from this row
-          const float mn = fmaxf(M, ml[u].x);
-          const float wa = exp2f(M - mn), wb = exp2f(ml[u].x - mn);
-          M = mn;
-          S = S * wa + ml[u].y * wb;
-#pragma unroll
-          for (int e = 0; e < V; ++e) acc[e] = acc[e] * wa + v[u][e] * wb;
-        }
-      }
-    };
-    auto split_join = [&](int64_t first, int64_t tiles, int64_t item, int rr) {
+    RowJoin<D> row;
+    auto split_join = [&](int first, int tiles, int64_t item, int rr) {
       if (tiles <= 0) return;
-      const int64_t w0 = first / per, w1 = (first + tiles - 1) / per;
-      join(a.part_o, a.part_ml, (w0 + item) * kAttnRowTile + rr, kAttnRowTile, static_cast<int>(w1 - w0 + 1));
+      const int w0 = first / per, w1 = (first + tiles - 1) / per;
+      row.add(a.part_o, a.part_ml, (w0 + item) * kAttnRowTile + rr, kAttnRowTile, w1 - w0 + 1);
     };
-    auto tc_join = [&](const TcAttnArgs& t, int64_t pr, int64_t first, int64_t tiles, int64_t item, int rr, bool pair) {
+    auto tc_join = [&](const TcAttnArgs& t, int pw, int first, int tiles, int64_t item, int rr) {
       if (tiles <= 0) return;
-      const int64_t w0 = first / pr, w1 = (first + tiles - 1) / pr;
-      // pair: a row is one stream's; otherwise both streams hold a piece of it
-      join(t.part_o, t.part_ml, (w0 + item) * kTcRows + rr, pair ? kTcRows : kTcKeys,
-           static_cast<int>(w1 - w0 + 1) * (pair ? 1 : 2));
+      const int w0 = first / pw, w1 = (first + tiles - 1) / pw;
+      row.add(t.part_o, t.part_ml, (w0 + item) * kTcRows + rr, kTcRows, w1 - w0 + 1);
     };
-    const int64_t rp = static_cast<int64_t>(b) * rows + r;  // the row among all sequences'
+    const int rp = b * rows + r;  // the row among all sequences'
     if (tp16 > 0) {
-      const int64_t item = kvh * a.rt_p + rp / kAttnRowTile;
-      split_join(item * tp16, tp16, item, static_cast<int>(rp % kAttnRowTile));
+      const int item = kvh * a.rt_p + rp / kAttnRowTile;
+      split_join(item * tp16, tp16, item, rp % kAttnRowTile);
     }
     if (tiles_p > 0) {
-      const int64_t flat = rp / kTcRows, item = flat * tp.nkv + kvh;
-      tc_join(tp, per_p, item * (tiles_p + TcAttnArgs::kItemCost) + TcAttnArgs::kItemCost, tiles_p, item, static_cast<int>(rp % kTcRows),
-              static_cast<int64_t>(a.B) * rows - flat * kTcRows > kTcKeys);
+      const int item = rp / kTcRows * tp.nkv + kvh;
+      tc_join(tp, per_p, item * (tiles_p + kCost) + kCost, tiles_p, item, rp % kTcRows);
     }
     if (own_tiles > 0)
       split_join(own_first + r / kAttnRowTile * own_tiles, own_tiles,
                  np + static_cast<int64_t>(b) * ns + kvh * a.rt_s + r / kAttnRowTile, r % kAttnRowTile);
-    if (tiles_s > 0)
-      tc_join(ts, per_s, first_s, tiles_s, static_cast<int64_t>(flat_s) * ts.nkv + kvh, r % kTcRows,
-              rows - r / kTcRows * kTcRows > kTcKeys);
-    const float inv = S == 0.f ? 0.f : 1.f / S;
-    const int tk = r / a.group;
-    const int64_t row = (static_cast<int64_t>(b) * a.L + tk) * a.nh + kvh * a.group + (r - tk * a.group);
-    uint16_t* out = a.out + row * D + lane * V;
-#pragma unroll
-    for (int i = 0; i < V; i += 2)
-      *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
-    if (a.lse2 && lane == 0) a.lse2[row] = S == 0.f ? INFINITY : M + log2f(S);
+    if (tiles_s > 0) tc_join(ts, per_s, first_s, tiles_s, static_cast<int64_t>(flat_s) * ts.nkv + kvh, r % kTcRows);
+    row.store(a, b, kvh, r);
+  }
+}
+
+// With attn_tc_kernel's own caches as the only source, the rows of the items that a cut between
+// two workers splits: block (w, y) takes the item over the cut before worker w + 1, if that is
+// the first cut of the item.
+template <int D>
+__global__ void __launch_bounds__(128) attn_merge_cut_kernel(const CacheAttnArgs a, const TcAttnArgs ts) {
+  constexpr int kCost = TcAttnArgs::kItemCost;
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int b = threadIdx.x; b < a.B; b += 128)
+      if (a.lens[b] < 0 || a.lens[b] > a.max_len) report(a.err, DEVERR_BOUNDS);
+  const int per = tc_places_per_worker(ts, tc_places_before(ts, ts.items()) * ts.nkv);
+  const int place = (blockIdx.x + 1) * per;
+  int flat, kvh, at;
+  if (!tc_locate(ts, place, flat, kvh, at)) return;
+  const int first = place - at + kCost, tiles = ts.tiles(flat);
+  if (first >= place || first / per != static_cast<int>(blockIdx.x)) return;
+  const int w1 = (first + tiles - 1) / per;
+  const int b = flat / ts.rps, row0 = (flat - b * ts.rps) * kTcRows;
+  const int rows = min(a.L * a.group - row0, kTcRows);
+  const int64_t slot = blockIdx.x + static_cast<int64_t>(flat) * ts.nkv + kvh;
+  for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < rows; r += 4 * gridDim.y) {
+    RowJoin<D> row;
+    row.add(ts.part_o, ts.part_ml, slot * kTcRows + r, kTcRows, w1 - static_cast<int>(blockIdx.x) + 1);
+    row.store(a, b, kvh, row0 + r);
   }
 }
 
@@ -587,7 +613,7 @@ __global__ void __launch_bounds__(128) slot_weight_kernel(const CacheAttnArgs a)
       const int r = r0 + 2 * c + e;
       if (r >= rows) continue;
       const int tr = r / a.group;
-      const float lse = a.lse2[(static_cast<int64_t>(b) * a.L + tr) * a.nh + kvh * a.group + r - tr * a.group];
+      const float lse = a.lse2[(static_cast<int64_t>(b) * a.nkv + kvh) * rows + r];
       const int lim = len - a.L + tr;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf)
@@ -608,11 +634,11 @@ __global__ void __launch_bounds__(kTcKeys) slot_weight_sum_kernel(const TcWeight
   const int b = blockIdx.z, kvh = blockIdx.y, flat = b * a.key_tiles + blockIdx.x;
   const int tiles = a.tiles(flat);
   if (tiles == 0) return;
-  const int64_t per = tc_places_per_worker(a, tc_places_before(a, a.items()) * a.nkv);
-  const int64_t first = tc_places_before(a, flat) * a.nkv + kvh * (tiles + TcWeightArgs::kItemCost) + TcWeightArgs::kItemCost;
+  const int per = tc_places_per_worker(a, tc_places_before(a, a.items()) * a.nkv);
+  const int first = tc_places_before(a, flat) * a.nkv + kvh * (tiles + TcWeightArgs::kItemCost) + TcWeightArgs::kItemCost;
   const int64_t item = static_cast<int64_t>(flat) * a.nkv + kvh;
   float sum = 0.f;
-  for (int64_t w = first / per; w <= (first + tiles - 1) / per; ++w) {
+  for (int w = first / per; w <= (first + tiles - 1) / per; ++w) {
     const float* p = a.part + (w + item) * 2 * kTcKeys + threadIdx.x;
     sum += p[0] + p[kTcKeys];
   }
@@ -663,7 +689,7 @@ CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_l
   if (B * nkv * ((rows_s + 15) / 16) < 8ll * num_sms) p.merge_rows = 4;
   p.off_lse = add(scored ? sizeof(float) * B * L * nh : 0);
   const size_t key_items = static_cast<size_t>(B) * nkv * ((max_len + kTcKeys - 1) / kTcKeys);
-  p.off_w = add(scored && p.tc_s ? (num_sms + key_items) * 2 * kTcKeys * sizeof(float) : 0);
+  p.off_w = add(scored && p.tc_s && group <= kTcKeys ? (num_sms + key_items) * 2 * kTcKeys * sizeof(float) : 0);
   return p;
 }
 
@@ -679,12 +705,16 @@ static cudaError_t launch_cache_attn_d(const CacheAttnArgs& a, const TcAttnArgs&
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
-  const dim3 rows((a.L * a.group + a.merge_rows - 1) / a.merge_rows, a.nkv, a.B);
-  attn_merge_kernel<D><<<rows, 128, 0, st>>>(a, p, s);
+  if (s.workers && s.direct) {
+    if (s.workers > 1) attn_merge_cut_kernel<D><<<dim3(s.workers - 1, 16), 128, 0, st>>>(a, s);
+  } else {
+    const dim3 rows((a.L * a.group + a.merge_rows - 1) / a.merge_rows, a.nkv, a.B);
+    attn_merge_kernel<D><<<rows, 128, 0, st>>>(a, p, s);
+  }
   e = cudaGetLastError();
   if (e != cudaSuccess || !a.acc) return e;
   if (w.workers) {
-    e = launch_slot_weight_tc(w, D, ms.k, st);
+    e = launch_slot_weight_tc(w, D, ms.k, ms.q, st);
     if (e != cudaSuccess) return e;
     slot_weight_sum_kernel<<<dim3(w.key_tiles, a.nkv, a.B), kTcKeys, 0, st>>>(w);
     return cudaGetLastError();
