@@ -14,9 +14,11 @@
 //                   visibility, online softmax, P back into TMEM over S (bf16 pairs); at the
 //                   end O out of TMEM, through the warp's own Q rows so that the stores are
 //                   whole lines
-//   warp 8          MMA issuer: S = Q K^T (both operands K-major in shared memory) and
-//                   O += P V (P in TMEM, V as loaded: keys x head, i.e. MN-major)
-//   warp 9          TMA loads of K / V tiles of 128 keys into a ring
+//   warps 8, 9      MMA issuers of streams 0 and 1: S = Q K^T (both operands K-major in shared
+//                   memory) and O += P V (P in TMEM, V as loaded: keys x head, i.e. MN-major).
+//                   One each, since an issuer's own waits and commits took ~950 cycles a step
+//                   where the products take 640
+//   warp 10         TMA loads of K / V tiles of 128 keys into a ring
 //
 // TMEM: per stream two S / P buffers of 64 columns and head_dim columns of O.  A step is 64 keys
 // of a stream; S of step n + 2 is issued right after P V of step n, into the buffer that step
@@ -24,22 +26,17 @@
 // never wait for the pipe's latency.  (With one S of 128 keys a stream -- all that fits next to
 // O -- the chain S, softmax, P V, S took 3950 cycles a tile where the products take 2048.)
 //
-// A stream's running maximum is only a reference: P is 2^(s - ref) with ref moved (and O
-// rescaled, by the stream itself) when a row's maximum passes it by more than 8, so that O
-// in TMEM is rarely touched; P stays below 2^8 and keeps its relative precision.  Past an item's
-// first step the exponentials do not wait for the maximum: it is taken alongside, and in the
-// rare case that ref has to move they are done again.  The special-function units (4
-// exponentials a cycle and scheduler) alone would take as long as the products, so a share
-// of the exponentials is computed with fused multiply-adds instead.
+// P is 2^(s - ref) with a row's ref the maximum of its first step, moved (and O rescaled, by the
+// stream itself) only when a later term passes it by more than 8: O in TMEM is rarely touched,
+// and P stays below 2^8 and keeps its relative precision.
 #include "fm_serve.cuh"
 
 namespace fm {
 namespace {
 
-constexpr int kThreads = 320;
-constexpr int kMmaWarp = 8;      // warp 9 loads
+constexpr int kThreads = 352;
+constexpr int kMmaWarp = 8;      // and 9; warp 10 loads
 constexpr int kStep = 64;        // keys of a stream's step
-constexpr int kPolyEvery = 4;    // one pair of exponentials in so many by fused multiply-adds
 
 template <int D>
 struct Shape {
@@ -50,8 +47,8 @@ struct Shape {
 };
 
 struct Bars {
-  uint64_t qfull[2], sfull[2][2], pfull[2][2], ofull, tail, done;
-  uint64_t kvfull[8], kvempty[8];
+  uint64_t qfull[2], sfull[2][2], pfull[2][2], ofull, tail, done[2];
+  uint64_t kvfull[8], kvempty[8], half[4];
   uint32_t tmem;
   int abort_flag;
 };
@@ -81,56 +78,6 @@ FM_DEV float ex2(float x) {  // 2^x, 2 ulp; results below 2^-126 are 0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// two fp32 operations an instruction
-FM_DEV uint64_t pack2(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-FM_DEV void unpack2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-FM_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-FM_DEV uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
-FM_DEV float max_nan(float a, float b) {  // NaN if either is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
-// 2^x for both halves without the special-function unit: x = n + f with n the nearest whole
-// number (the low bits of x + 1.5 * 2^23) and |f| <= 1/2, 2^f by a polynomial of degree 5 fitted
-// for the least relative error with p(0) = 1 (9e-8, 1.7e-7 with fp32 sums), n added to the
-// exponent.  x is at least -127, where the exponent's bits give exactly 0: a hidden key's
-// weight is 0 here too, and a row that sees nothing sums to 0.
-FM_DEV uint64_t ex2_poly2(uint64_t x) {
-  float lo, hi;
-  unpack2(x, lo, hi);
-  x = pack2(max_nan(lo, -127.f), max_nan(hi, -127.f));
-  const float kMagic = 12582912.f;
-  const uint64_t t = add2(x, pack2(kMagic, kMagic));
-  const uint64_t n = add2(t, pack2(-kMagic, -kMagic));
-  const uint64_t f = fma2(n, pack2(-1.f, -1.f), x);
-  uint64_t p = pack2(0.0013264727302716457f, 0.0013264727302716457f);
-  p = fma2(p, f, pack2(0.009671512728706911f, 0.009671512728706911f));
-  p = fma2(p, f, pack2(0.05550733743810932f, 0.05550733743810932f));
-  p = fma2(p, f, pack2(0.24022242084016385f, 0.24022242084016385f));
-  p = fma2(p, f, pack2(0.6931469775983554f, 0.6931469775983554f));
-  p = fma2(p, f, pack2(1.f, 1.f));
-  float pl, ph, tl, th;
-  unpack2(p, pl, ph);
-  unpack2(t, tl, th);
-  return pack2(__uint_as_float(__float_as_uint(pl) + (__float_as_uint(tl) << 23)),
-               __uint_as_float(__float_as_uint(ph) + (__float_as_uint(th) << 23)));
 }
 
 FM_DEV void tma_load_3d(uint32_t dst, const void* map, int x, int y, int z, uint64_t* bar) {
@@ -212,12 +159,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         mbar_init(&bars.pfull[i][j], 4);
       }
     }
-    mbar_init(&bars.ofull, 1);
+    mbar_init(&bars.ofull, 2);
     mbar_init(&bars.tail, 1);
-    mbar_init(&bars.done, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&bars.done[i], 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&bars.half[i], 2);
     for (int i = 0; i < NS; ++i) {
       mbar_init(&bars.kvfull[i], 1);
-      mbar_init(&bars.kvempty[i], 1);
+      mbar_init(&bars.kvempty[i], 2);
     }
     bars.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -286,11 +234,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       if (lane == 0) mbar_arrive(&bars.qfull[s]);
     };
     uint32_t g = 0;  // steps of this stream: step g is in buffer g % 2
-    int oph = 0;
+    int oph = 0, half_ph = 0;
     bool ok = true;
+    // the two streams' warps of the same rows see what the other wrote
+    auto meet = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.half[quad]);
+      const bool got = __all_sync(0xffffffffu, mbar_wait(&bars.half[quad], half_ph & 1, abort_flag, a.err));
+      ++half_ph;
+      return got;
+    };
     fetch_q(it);
     store_q(it);
-    const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2);
     while (it.cnt > 0) {
       const int b = it.flat / a.rps, row_base = (it.flat - b * a.rps) * kTcRows;
       const bool pair = rows - row_base > kTcKeys;
@@ -323,68 +278,54 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
             for (int c = 0; c < kStep; ++c) v[c] = key0 + c <= lim ? v[c] : -INFINITY;
           }
-          float mx;
           auto maximum = [&]() {
             float m4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
             for (int c = 4; c < kStep; ++c) m4[c & 3] = fmaxf(m4[c & 3], v[c]);
-            mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
+            return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;
           };
           float sum;
           auto exponentials = [&]() {
             const float base = ref == -INFINITY ? 0.f : -ref;
-            const uint64_t base2 = pack2(base, base);
-            uint64_t sum2[2] = {0ull, 0ull};
+            float sum4[4] = {0.f, 0.f, 0.f, 0.f};
             uint4 w[8];
             uint32_t* pw = reinterpret_cast<uint32_t*>(w);
 #pragma unroll
             for (int c = 0; c < kStep / 2; ++c) {
-              uint64_t x = fma2(pack2(v[2 * c], v[2 * c + 1]), scale2, base2);
-              float p0, p1;
-              if (c % kPolyEvery == kPolyEvery - 1) {
-                x = ex2_poly2(x);
-                unpack2(x, p0, p1);
-              } else {
-                unpack2(x, p0, p1);
-                p0 = ex2(p0);
-                p1 = ex2(p1);
-                x = pack2(p0, p1);
-              }
-              sum2[c & 1] = add2(sum2[c & 1], x);
+              const float p0 = ex2(fmaf(v[2 * c], a.scale_log2, base)), p1 = ex2(fmaf(v[2 * c + 1], a.scale_log2, base));
+              sum4[2 * c & 3] += p0;
+              sum4[2 * c + 1 & 3] += p1;
               pw[c] = pack_bf16x2(p0, p1);  // the tensor product's operand: one rounding to bf16
             }
             tmem_st32(t_b, w);
-            float s0, s1;
-            unpack2(add2(sum2[0], sum2[1]), s0, s1);
-            sum = s0 + s1;
+            sum = (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
           };
-          // the first step's maximum is needed before its exponentials; later ones' alongside
-          bool done = false;
-          if (n == 0) {
-            maximum();
-            ref = mx;
-            done = true;
-          }
-#pragma unroll 1
-          while (true) {
+          // ref is the maximum of the first step that a row sees anything in.  Later a row's sum says
+          // whether ref still serves: a term above 2^8 makes it larger than 2^8 (many smaller terms may
+          // too, which costs an unneeded move).  That saves the maximum, as long a job as the
+          // exponentials are; in the rare case that ref moves the step's exponentials are done again.
+          bool fresh = ref == -INFINITY && lim >= key0;
+          if (!__any_sync(0xffffffffu, fresh)) {
             exponentials();
-            if (done) break;
-            maximum();
-            if (!__any_sync(0xffffffffu, mx > ref + 8.f)) break;
-            const float nref = mx > ref + 8.f ? mx : ref;
-            // the product that last wrote O is complete (this step's S was issued after it)
+            fresh = sum > 256.f;
+          }
+          if (__any_sync(0xffffffffu, fresh)) {
+            const float nref = fresh ? fmaxf(maximum(), ref) : ref;
             const float f = ref == -INFINITY ? 0.f : ex2(ref - nref);
-            l *= f;
+            if (n > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+              // the product that last wrote O is complete (this step's S was issued after it)
+              l *= f;
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
-              float o[16];
-              tmem_ld16(t_o + c, o);
+              for (int c = 0; c < D; c += 16) {
+                float o[16];
+                tmem_ld16(t_o + c, o);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] *= f;
-              tmem_st16(t_o + c, o);
+                for (int e = 0; e < 16; ++e) o[e] *= f;
+                tmem_st16(t_o + c, o);
+              }
             }
             ref = nref;
-            done = true;
+            exponentials();
           }
           l += sum;
           tmem_wait_st();
@@ -396,7 +337,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       TcPiece nx = it;
       tc_next(a, nx);
       fetch_q(nx);
-      if (!ok || !__all_sync(0xffffffffu, mbar_wait(&bars.ofull, oph & 1, abort_flag, a.err))) break;
+      if (!ok || !__all_sync(0xffffffffu, mbar_wait(&bars.ofull, oph & 1, abort_flag, a.err))) {
+        ok = false;
+        break;
+      }
       ++oph;
       tc_fence_after();
       const bool whole = a.direct && it.cnt == it.tiles;
@@ -410,9 +354,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         if (!pair) {      // one reference for both streams' halves
           const int other = s == 0 ? static_cast<int>(S::kTileBytes) : -static_cast<int>(S::kTileBytes);
           reinterpret_cast<float2*>(stage)[lane] = make_float2(ref, l);
-          named_bar_sync(1 + quad, 64);
-          const float2 o = reinterpret_cast<const float2*>(stage + other)[lane];
-          named_bar_sync(1 + quad, 64);
+          ok = meet();
+          const volatile float* theirs = reinterpret_cast<const volatile float*>(stage + other) + 2 * lane;
+          const float2 o = make_float2(theirs[0], theirs[1]);
+          ok = ok && meet();
+          if (!ok) break;
           const float top = fmaxf(ref, o.x);
           fac = ref == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2(ref - top);
           l = l * fac + (o.x == -INFINITY ? o.y : o.y * ex2(o.x - top));
@@ -433,7 +379,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
               for (int e = 0; e < 8; ++e)
                 *reinterpret_cast<float4*>(stage + sw128_off(lane, e)) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
-            named_bar_sync(1 + quad, 64);
+            if (!meet()) {
+              ok = false;
+              break;
+            }
             if (s == 0) {
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
@@ -444,7 +393,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 o[4 * e + 3] += h.w;
               }
             }
-            named_bar_sync(1 + quad, 64);
+            if (!meet()) {
+              ok = false;
+              break;
+            }
             if (s == 1) continue;
           }
           if (whole) {
@@ -470,6 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             else *reinterpret_cast<uint4*>(a.part_o + (pr + rr) * D + c + 4 * csub) = v;
           }
         }
+        if (!ok) break;
         if (on && (pair || s == 0)) {
           if (!whole) a.part_ml[pr + lane] = make_float2(ref, l);
           else if (a.lse2) a.lse2[(static_cast<int64_t>(b) * a.nkv + it.kvh) * rows + r] = l == 0.f ? INFINITY : ref + log2f(l);
@@ -491,19 +444,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           if (ch == 0 && a.lse2) a.lse2[(static_cast<int64_t>(b) * a.nkv + kvh) * rows + r] = INFINITY;
         }
       }
-  } else if (warp == kMmaWarp) {
-    // ---------------------------------------------------------------- MMA issuer
+  } else if (warp < kMmaWarp + 2) {
+    // ---------------------------------------------------------------- MMA issuers
     // elect.sync, not a lane test: one lane chosen so lets the compiler hold the operands in uniform
     // registers (65 to 90 cycles a product otherwise, where the pipe takes 48)
     if (elect_one()) {
+      const int s = warp - kMmaWarp;
       const uint64_t q_desc = sdesc_sw128(smem_u32(s_q)), k_desc = sdesc_sw128(smem_u32(s_kv));
       const uint64_t v_desc = sdesc_mn_sw128(smem_u32(s_kv), kTcKeys * 128);
       constexpr uint32_t kTile16 = S::kTileBytes >> 4;      // in descriptor units
       constexpr uint32_t kHalf16 = kTcKeys * 128 >> 4;      // the next 64 columns of a tile
       constexpr uint32_t kStep16 = kStep * 128 >> 4;        // the next 64 keys
       const uint32_t id_s = idesc_bf16(kTcKeys, kStep), id_o = idesc_bf16(kTcKeys, D) | (1u << 16);  // B MN-major
+      const uint32_t t_s = tmem + s * kTcKeys, t_o = tmem + 2 * kTcKeys + s * D;
       int qph = 0, kslot = 0, vslot = 0, ring = 0;
-      uint32_t ring_ph = 0, g = 0;  // g: steps done by a stream, as in the streams
+      uint32_t ring_ph = 0, g = 0;  // g: steps done by the stream, as there
       bool ok = true;
       auto next_slot = [&](int& slot) {
         slot = ring;
@@ -515,54 +470,48 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         return got;
       };
       for (; ok && it.cnt > 0; tc_next(a, it)) {
+        // with one row tile a tile is one step, the stream's half of its keys
         const bool pair = rows - it.flat % a.rps * kTcRows > kTcKeys;
         const int steps = pair ? 2 * it.cnt : it.cnt;
-        // S of step n: with one row tile a tile is one step (a half of its keys per stream)
-        auto issue_s = [&](int n, int s) {
-          if (s == 0 && !(pair && (n & 1))) {
-            if (!next_slot(kslot)) return false;
-            tc_fence_after();
-          }
-          const uint64_t ad = q_desc + (pair ? s : 0) * kTile16;
+        const uint64_t ad = q_desc + (pair ? s : 0) * kTile16;
+        auto issue_s = [&](int n) {
+          const bool odd = pair && (n & 1);
+          if (!odd && !next_slot(kslot)) return false;
+          tc_fence_after();
           const uint64_t bd = k_desc + kslot * kTile16 + (pair ? n & 1 : s) * kStep16;
-          const uint32_t buf = (g + n) & 1;
-          const uint32_t d = tmem + s * kTcKeys + buf * kStep;
+          const uint32_t buf = (g + n) & 1, d = t_s + buf * kStep;
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
             umma_bf16(d, ad + (kk >> 2) * kHalf16 + 2 * (kk & 3), bd + (kk >> 2) * kHalf16 + 2 * (kk & 3), id_s, kk != 0);
           umma_commit(&bars.sfull[s][buf]);
-          if (s == 1 && !(pair && !(n & 1))) umma_commit(&bars.kvempty[kslot]);
+          if (odd || !pair) umma_commit(&bars.kvempty[kslot]);
           return true;
         };
-        for (int s = 0; ok && s < 2; ++s) ok = mbar_wait(&bars.qfull[s], qph & 1, abort_flag, a.err);
+        for (int i = 0; ok && i < 2; ++i) ok = mbar_wait(&bars.qfull[i], qph & 1, abort_flag, a.err);
         ++qph;
         tc_fence_after();
-        for (int n = 0; ok && n < min(2, steps); ++n)
-          for (int s = 0; ok && s < 2; ++s) ok = issue_s(n, s);
+        for (int n = 0; ok && n < min(2, steps); ++n) ok = issue_s(n);
 #pragma unroll 1
         for (int n = 0; ok && n < steps; ++n) {
-          const uint32_t buf = (g + n) & 1, ph = (g + n) >> 1 & 1;
+          const uint32_t buf = (g + n) & 1;
+          const bool odd = pair && (n & 1);
+          if (!odd) ok = next_slot(vslot);
+          ok = ok && mbar_wait(&bars.pfull[s][buf], (g + n) >> 1 & 1, abort_flag, a.err);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t bd = v_desc + vslot * kTile16 + (pair ? n & 1 : s) * kStep16;
+          const uint32_t at = t_s + buf * kStep;
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            if (s == 0 && !(pair && (n & 1))) ok = next_slot(vslot);
-            ok = ok && mbar_wait(&bars.pfull[s][buf], ph, abort_flag, a.err);
-            if (!ok) break;
-            tc_fence_after();
-            const uint64_t bd = v_desc + vslot * kTile16 + (pair ? n & 1 : s) * kStep16;
-            const uint32_t d = tmem + 2 * kTcKeys + s * D, at = tmem + s * kTcKeys + buf * kStep;
-#pragma unroll
-            for (int kk = 0; kk < kStep / 16; ++kk) umma_bf16_ts(d, at + 8 * kk, bd + kk * 128, id_o, n != 0 || kk != 0);
-            if (s == 1 && !(pair && !(n & 1))) umma_commit(&bars.kvempty[vslot]);
-            if (n + 2 < steps) ok = issue_s(n + 2, s);
-            if (!ok) break;
-          }
+          for (int kk = 0; kk < kStep / 16; ++kk) umma_bf16_ts(t_o, at + 8 * kk, bd + kk * 128, id_o, n != 0 || kk != 0);
+          if (odd || !pair) umma_commit(&bars.kvempty[vslot]);
+          if (n + 2 < steps) ok = issue_s(n + 2);
         }
         if (ok) umma_commit(&bars.ofull);
         g += steps;
       }
-      // every product and commit of this CTA has landed before it frees TMEM and leaves
-      umma_commit(&bars.done);
-      wait_drained(&bars.done, 0, a.err);
+      // every product and commit of this lane has landed before the CTA frees TMEM and leaves
+      umma_commit(&bars.done[s]);
+      wait_drained(&bars.done[s], 0, a.err);
     }
     __syncwarp();
   } else {
@@ -632,14 +581,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 // ------------------------------------------------------------------ slot weights
 // acc[j] of a kv head's 128 keys: S^T = K Q^T for 128 query rows at a time (keys are the TMEM
 // lanes, rows the columns), so a thread's sum over its columns of 2^(s - lse of the row) is its
-// key's weight and needs no other thread.  The two groups of 128 threads take every other row
-// tile.  Bound by the exponentials (128 x 128 a tile: 1024 cycles of the special-function units
+// key's weight and needs no other thread.  The four groups of 128 threads take every fourth row
+// tile (two groups were bound by latency: 44% of the issue slots).  Bound by the exponentials (128 x 128 a tile: 1024 cycles of the special-function units
 // against 512 of the tensor pipe), of which a third go to fused multiply-adds here.
-//   warps 0-3, 4-7  groups 0, 1     warp 8  MMA issuer     warp 9  TMA loads of K and Q
+//   warps 0-15  groups 0-3     warp 16  MMA issuer     warp 17  TMA loads of K and Q
 namespace {
-constexpr int kWThreads = 320;
-constexpr int kWStages = 4;    // Q tiles, their rows' lse, TMEM buffers
-constexpr int kWPolyEvery = 3;
+constexpr int kWThreads = 576;
+constexpr int kWMmaWarp = 16;
+constexpr int kWStages = kTcWeightParts;  // Q tiles, TMEM buffers, groups; twice as many rows' lse, which
+                                          // the sums read after the product has freed its Q tile
 
 template <int D>
 struct WShape {
@@ -648,7 +598,7 @@ struct WShape {
 };
 
 struct WBars {
-  uint64_t qfull[kWStages], sfull[kWStages], sempty[kWStages], kfull[2], kempty[2], done;
+  uint64_t qfull[kWStages], qempty[kWStages], sfull[kWStages], sempty[kWStages], kfull[2], kempty[2], done;
   uint32_t tmem;
   int abort_flag;
 };
@@ -661,7 +611,7 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
   using S = WShape<D>;
   extern __shared__ uint8_t s_raw[];
   __shared__ WBars bars;
-  __shared__ __align__(16) float s_lse[kWStages][kTcKeys];  // negated; -inf: no such row
+  __shared__ __align__(16) float s_lse[2 * kWStages][kTcKeys];  // negated; -inf: no such row
   const uint32_t pad = (1024u - (smem_u32(s_raw) & 1023u)) & 1023u;
   uint8_t* s_k = s_raw + pad;                    // [2][kTileBytes]
   uint8_t* s_q = s_k + 2 * S::kTileBytes;        // [kWStages][kTileBytes]
@@ -671,7 +621,8 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
   if (threadIdx.x == 0) {
     for (int i = 0; i < kWStages; ++i) {
       mbar_init(&bars.qfull[i], 2);  // the copy, and the rows' lse
-      mbar_init(&bars.sfull[i], 1);
+      mbar_init(&bars.qempty[i], 1);
+      mbar_init(&bars.sfull[i], 2);  // the product, and its issuer (for the loader's writes of lse)
       mbar_init(&bars.sempty[i], 4);
     }
     for (int i = 0; i < 2; ++i) {
@@ -687,7 +638,7 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
   for (uint32_t i = threadIdx.x; i < kWStages * S::kTileBytes / 16; i += kWThreads)
     reinterpret_cast<uint4*>(s_q)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async();
-  if (warp == 8) {
+  if (warp == kWMmaWarp) {
     tmem_alloc(&bars.tmem, 512);
     tmem_relinquish();
   }
@@ -700,12 +651,11 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
   const int rows = a.L * a.group;
   uint32_t t = 0;  // tiles of this CTA: tile t is in stage t % 4
 
-  if (warp < 8) {
+  if (warp < kWMmaWarp) {
     // ---------------------------------------------------------------- sums
     const int grp = warp >> 2;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int kl = (warp & 3) * 32 + lane;
-    const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2);
     bool ok = true;
     for (; ok && it.cnt > 0; tc_next(a, it)) {
       const int b = it.flat / a.key_tiles, key0 = (it.flat - b * a.key_tiles) * kTcKeys;
@@ -717,11 +667,9 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
       const int rmin = key0 + kl < len ? tk * a.group : 0x7fffffff, rmin_last = tk_last * a.group;
       float total = 0.f, low = 0.f;  // a compensated sum over tiles
       for (int i = 0; i < it.cnt; ++i, ++t) {
-        if ((t & 1) != static_cast<uint32_t>(grp)) continue;
         const uint32_t st = t % kWStages;
-        // qfull (complete by then) for the loaders' s_lse, sfull for the product
-        if (!__all_sync(0xffffffffu, mbar_wait(&bars.sfull[st], t / kWStages & 1, abort_flag, a.err) &&
-                                         mbar_wait(&bars.qfull[st], t / kWStages & 1, abort_flag, a.err))) {
+        if (st != static_cast<uint32_t>(grp)) continue;
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars.sfull[st], t / kWStages & 1, abort_flag, a.err))) {
           ok = false;
           break;
         }
@@ -729,7 +677,7 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
         const int r0 = row0 + i * tile_rows;
         // a copy past the sequence's tokens brings another's rows
         const bool masked = r0 < rmin_last || r0 + tile_rows > rows;
-        uint64_t sum2[2] = {0ull, 0ull};
+        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (int c = 0; c < kTcKeys; c += 32) {
           float v[32];
@@ -739,38 +687,28 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = r0 + c + e >= rmin && r0 + c + e < rows ? v[e] * a.scale_log2 : -INFINITY;
           }
-          const uint64_t mul = masked ? pack2(1.f, 1.f) : scale2;
-          const float4* nl = reinterpret_cast<const float4*>(&s_lse[st][c]);
+          const float mul = masked ? 1.f : a.scale_log2;
+          const float4* nl = reinterpret_cast<const float4*>(&s_lse[t % (2 * kWStages)][c]);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const float4 n4 = nl[e];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint64_t x = fma2(pack2(v[4 * e + 2 * h], v[4 * e + 2 * h + 1]), mul, h ? pack2(n4.z, n4.w) : pack2(n4.x, n4.y));
-              if ((2 * e + h) % kWPolyEvery == kWPolyEvery - 1) {
-                x = ex2_poly2(x);
-              } else {
-                float p0, p1;
-                unpack2(x, p0, p1);
-                x = pack2(ex2(p0), ex2(p1));
-              }
-              sum2[h] = add2(sum2[h], x);
-            }
+            sum4[0] += ex2(fmaf(v[4 * e], mul, n4.x));
+            sum4[1] += ex2(fmaf(v[4 * e + 1], mul, n4.y));
+            sum4[2] += ex2(fmaf(v[4 * e + 2], mul, n4.z));
+            sum4[3] += ex2(fmaf(v[4 * e + 3], mul, n4.w));
           }
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.sempty[st]);
-        float s0, s1;
-        unpack2(add2(sum2[0], sum2[1]), s0, s1);
-        const float y = (s0 + s1) - low, u = total + y;
+        const float y = ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3])) - low, u = total + y;
         low = (u - total) - y;
         total = u;
       }
       if (!ok) break;
-      a.part[((static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(it.flat) * a.nkv + it.kvh) * 2 + grp) * kTcKeys + kl] = total;
+      a.part[((static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(it.flat) * a.nkv + it.kvh) * kTcWeightParts + grp) * kTcKeys + kl] = total;
     }
-  } else if (warp == 8) {
+  } else if (warp == kWMmaWarp) {
     // ---------------------------------------------------------------- MMA issuer
     if (elect_one()) {
       const uint64_t k_desc = sdesc_sw128(smem_u32(s_k)), q_desc = sdesc_sw128(smem_u32(s_q));
@@ -783,8 +721,10 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
 #pragma unroll 1
         for (int i = 0; ok && i < it.cnt; ++i, ++t) {
           const uint32_t st = t % kWStages;
-          ok = mbar_wait(&bars.qfull[st], t / kWStages & 1, abort_flag, a.err);  // and its buffer is free
+          ok = mbar_wait(&bars.qfull[st], t / kWStages & 1, abort_flag, a.err) &&
+               mbar_wait(&bars.sempty[st], (t / kWStages & 1) ^ 1, abort_flag, a.err);
           if (!ok) break;
+          mbar_arrive(&bars.sfull[st]);
           tc_fence_after();
           const uint64_t ad = k_desc + (n & 1) * kTile16, bd = q_desc + st * kTile16;
           const uint32_t d = tmem + st * kTcKeys;
@@ -792,6 +732,7 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
           for (int kk = 0; kk < D / 16; ++kk)
             umma_bf16(d, ad + (kk >> 2) * kHalf16 + 2 * (kk & 3), bd + (kk >> 2) * kHalf16 + 2 * (kk & 3), id, kk != 0);
           umma_commit(&bars.sfull[st]);
+          umma_commit(&bars.qempty[st]);
         }
         if (ok) umma_commit(&bars.kempty[n & 1]);
       }
@@ -829,8 +770,9 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
       fetch(0);
       for (int i = 0; i < it.cnt; ++i, ++t) {
         const uint32_t st = t % kWStages;
-        // the sums of tile t - 4 were taken, so its product is complete: its stage is free
-        if (!mbar_wait_lane0(&bars.sempty[st], (t / kWStages & 1) ^ 1, abort_flag, a.err)) {
+        // the product of tile t - 4 is complete; it waited for the sums of tile t - 8, so their
+        // rows' lse are free too
+        if (!mbar_wait_lane0(&bars.qempty[st], (t / kWStages & 1) ^ 1, abort_flag, a.err)) {
           ok = false;
           break;
         }
@@ -842,7 +784,7 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
                         b * a.L + (tile0 + i) * a.tile_tokens, &bars.qfull[st]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s_lse[st][32 * e + lane] = nl[e];
+        for (int e = 0; e < 4; ++e) s_lse[t % (2 * kWStages)][32 * e + lane] = nl[e];
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.qfull[st]);
         if (i + 1 < it.cnt) fetch(i + 1);
@@ -857,7 +799,7 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kWMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }

@@ -49,6 +49,7 @@ constexpr int attn_split_smem(int d) { return kAttnWarps * kAttnStages * 2 * kAt
 
 constexpr int kTcKeys = 128;         // keys of a tile, rows of a TMEM tile
 constexpr int kTcRows = 256;         // query rows of an item
+constexpr int kTcWeightParts = 4;    // sums of a piece of slot weights
 
 struct CacheAttnArgs {
   const uint16_t* q;        // [B * L, q_ld]: nh heads of d
@@ -93,7 +94,7 @@ struct TcAttnArgs {
   float* lse2;
   uint32_t* err;
 
-  static constexpr int kItemCost = 2;  // what an item costs beside its tiles, in tiles
+  static constexpr int kItemCost = 4;  // what an item costs beside its tiles, in tiles
 #ifdef __CUDACC__
   __device__ int items() const { return nseq * rps; }
   // tiles of item flat = b * rps + rp: up to the last key that its last token sees
@@ -110,7 +111,7 @@ struct TcWeightArgs {
   const int32_t* lens;
   const float* lse2;        // [B, nkv, L * group]
   float* acc;               // [B, nkv, max_len]
-  float* part;              // [workers + items][2][128] sums of a piece's even and odd tiles
+  float* part;              // [workers + items][4][128] sums of every fourth tile of a piece
   int B, L, nh, nkv, group, max_len;
   int key_tiles;            // of max_len
   int tile_tokens;          // 128 / group

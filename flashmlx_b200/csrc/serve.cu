@@ -429,12 +429,18 @@ namespace {
 template <int D>
 struct RowJoin {
   static constexpr int V = D / 32;  // columns of a lane
-  static constexpr int U = 8;       // pieces whose loads are in flight together
   float acc[V] = {};
   float M = -INFINITY, S = 0.f;
 
   // n pieces, piece i in row row0 + i * step of a part buffer
   FM_DEV void add(const float* part_o, const float2* part_ml, int64_t row0, int step, int n) {
+    if (n <= 2) add_by<2>(part_o, part_ml, row0, step, n);
+    else add_by<8>(part_o, part_ml, row0, step, n);
+  }
+
+  // U: pieces whose loads are in flight together
+  template <int U>
+  FM_DEV void add_by(const float* part_o, const float2* part_ml, int64_t row0, int step, int n) {
     const int lane = threadIdx.x & 31;
     for (int i0 = 0; i0 < n; i0 += U) {
       float2 ml[U];
@@ -639,8 +645,8 @@ __global__ void __launch_bounds__(kTcKeys) slot_weight_sum_kernel(const TcWeight
   const int64_t item = static_cast<int64_t>(flat) * a.nkv + kvh;
   float sum = 0.f;
   for (int w = first / per; w <= (first + tiles - 1) / per; ++w) {
-    const float* p = a.part + (w + item) * 2 * kTcKeys + threadIdx.x;
-    sum += p[0] + p[kTcKeys];
+    const float* p = a.part + (w + item) * kTcWeightParts * kTcKeys + threadIdx.x;
+    sum += (p[0] + p[kTcKeys]) + (p[2 * kTcKeys] + p[3 * kTcKeys]);
   }
   const int key = blockIdx.x * kTcKeys + threadIdx.x;
   if (key < a.lens[b]) a.acc[(static_cast<int64_t>(b) * a.nkv + kvh) * a.max_len + key] += sum;
@@ -689,7 +695,7 @@ CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_l
   if (B * nkv * ((rows_s + 15) / 16) < 8ll * num_sms) p.merge_rows = 4;
   p.off_lse = add(scored ? sizeof(float) * B * L * nh : 0);
   const size_t key_items = static_cast<size_t>(B) * nkv * ((max_len + kTcKeys - 1) / kTcKeys);
-  p.off_w = add(scored && p.tc_s && group <= kTcKeys ? (num_sms + key_items) * 2 * kTcKeys * sizeof(float) : 0);
+  p.off_w = add(scored && p.tc_s && group <= kTcKeys ? (num_sms + key_items) * kTcWeightParts * kTcKeys * sizeof(float) : 0);
   return p;
 }
 
