@@ -124,6 +124,9 @@ struct fm_handle {
   size_t sv_bytes = 0;
   size_t sv_total = 0;        // bytes of all blocks
   bool sv_ready = false;      // shared-memory opt-in done
+  // the frequencies of the last rotary config (64 powers cost more host time than the launch)
+  fm_rope_config rope_cfg = {};
+  fm::RopeArgs rope_set = {};
   // kernel timing (fm_profile_enable)
   bool profile = false;
   struct Pending {
@@ -2048,8 +2051,12 @@ namespace {
 
 // cfg's frequencies in full turns per position, and the factor on cos and sin
 int rope_args(fm_handle* h, const fm_rope_config* c, fm::RopeArgs* a) {
-  std::memset(a, 0, sizeof(*a));
   if (!c) return set_err(h, FM_EINVAL, "null config");
+  if (h->rope_set.d && std::memcmp(&h->rope_cfg, c, sizeof(*c)) == 0) {
+    *a = h->rope_set;
+    return FM_OK;
+  }
+  std::memset(a, 0, sizeof(*a));
   const int r = c->rotary_dim ? c->rotary_dim : c->head_dim;
   if (c->head_dim <= 0 || r <= 0 || r % 2 || r > c->head_dim)
     return set_err(h, FM_EINVAL, "rotary_dim must be even and at most head_dim");
@@ -2093,6 +2100,8 @@ int rope_args(fm_handle* h, const fm_rope_config* c, fm::RopeArgs* a) {
   a->rotary = r;
   a->traditional = c->traditional != 0;
   a->L = 1;
+  h->rope_cfg = *c;
+  h->rope_set = *a;
   return FM_OK;
 }
 

@@ -20,6 +20,7 @@ the next `synchronize()`.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import threading
 from dataclasses import dataclass
 
@@ -32,6 +33,14 @@ __all__ = ["Handle", "default_handle", "quantized_matmul", "gather_qmm", "MoECon
            "FlashMoEError", "synchronize", "bf16_from_numpy", "u32_from_numpy", "bf16_to_numpy"]
 
 _tls = threading.local()
+
+
+def _raw_stream(device: int) -> int:
+    """The current stream's cudaStream_t, without a torch.cuda.Stream object where torch offers it."""
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
 class Handle:
@@ -48,6 +57,7 @@ class Handle:
         if st != _lib.FM_OK:
             raise FlashMoEError(st, "fm_create failed: " + self.lib.fm_status_string(st).decode())
         self.h = h
+        self._stream = None  # the stream fm_set_stream was last given (None: not by bind_stream)
 
     def close(self):
         if self.h and not getattr(self, "_borrowed", False):  # a borrowed view never destroys
@@ -67,6 +77,15 @@ class Handle:
     def bind_stream(self, stream: torch.cuda.Stream | None = None):
         s = stream if stream is not None else torch.cuda.current_stream(self.device)
         self.check(self.lib.fm_set_stream(self.h, C.c_void_p(s.cuda_stream)))
+        self._stream = s.cuda_stream
+
+    def bind_current(self):
+        """bind_stream() to torch's current stream, told to the library only when it changes (for
+        handles that nothing else binds: a call's host time is a few microseconds)."""
+        s = _raw_stream(self.device)
+        if s != self._stream or getattr(self, "_borrowed", False):
+            self.check(self.lib.fm_set_stream(self.h, s))
+            self._stream = s
 
     def set_path(self, path: int):
         self.check(self.lib.fm_set_path(self.h, path))
@@ -545,12 +564,14 @@ def argmax(logits, handle=None) -> torch.Tensor:
 # ---------------------------------------------------------------- serving over long and shared caches
 
 _BF16, _I32, _F32 = (torch.bfloat16,), (torch.int32,), (torch.float32,)
+_BF = torch.bfloat16
 _ROPE_SCALINGS = {"linear": _lib.FM_ROPE_LINEAR, "ntk": _lib.FM_ROPE_NTK, "yarn": _lib.FM_ROPE_YARN,
                   "banded": _lib.FM_ROPE_BANDED}
 
 
-def _rope_config(d, theta, rotary_dim, traditional, scaling) -> _lib.RopeConfig:
-    c = _lib.RopeConfig(int(d), int(rotary_dim or 0), int(traditional), _lib.FM_ROPE_UNSCALED, float(theta))
+@functools.lru_cache(maxsize=256)
+def _rope_config_of(d, theta, rotary_dim, traditional, scaling) -> _lib.RopeConfig:
+    c = _lib.RopeConfig(d, rotary_dim or 0, int(traditional), _lib.FM_ROPE_UNSCALED, theta)
     if rotary_dim is not None and not 0 < rotary_dim <= d:
         raise ValueError("rotary_dim must be between 2 and the head size")
     if scaling is not None:
@@ -569,31 +590,53 @@ def _rope_config(d, theta, rotary_dim, traditional, scaling) -> _lib.RopeConfig:
     return c
 
 
-def _need_heads(t, name, device):
-    """[..., heads, d] bf16 whose heads lie side by side in each token's row: the elements
-    from one token's row to the next (leading axes must be one stride apart in order)."""
+def _rope_config(d, theta, rotary_dim, traditional, scaling) -> _lib.RopeConfig:
+    return _rope_config_of(d, float(theta), rotary_dim, bool(traditional),
+                           None if scaling is None else tuple(sorted(scaling.items())))
+
+
+def _heads_ld(t, name, dev, shape, step):
+    """Checks [..., heads, d] bf16 on `dev` whose heads lie side by side in each token's row (`shape`
+    and `step` are t's sizes and strides); returns the elements from one token's row to the next
+    (leading axes must be one stride apart, in order)."""
+    if t.dtype is not _BF or t.device != dev:
+        if t.device != dev:
+            raise ValueError(f"{name} must live on {dev}")
+        raise ValueError(f"{name} has dtype {t.dtype}, expected torch.bfloat16")
+    n = len(shape)
+    if n < 3:
+        raise ValueError(f"{name} must be [..., heads, head size]")
+    h, d = shape[-2], shape[-1]
+    if (d > 1 and step[-1] != 1) or (h > 1 and step[-2] != d):
+        if t.numel():
+            raise ValueError(f"the heads of {name} must lie side by side")
+    if n == 3:
+        return step[0] if shape[0] > 1 else h * d
+    ld, many = None, 1
+    for i in range(n - 3, -1, -1):
+        if shape[i] > 1:
+            if ld is None:
+                ld = step[i]
+            elif step[i] != ld * many and t.numel():
+                raise ValueError(f"the tokens of {name} must be one stride apart")
+            many *= shape[i]
+    return h * d if ld is None else ld
+
+
+def _cuda_tensor(t, name):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor")
-    if t.device.type != "cuda" or (device is not None and t.device != device):
-        raise ValueError(f"{name} must live on {device or 'a CUDA device'}")
-    if t.dtype != torch.bfloat16:
-        raise ValueError(f"{name} has dtype {t.dtype}, expected torch.bfloat16")
-    if t.dim() < 3:
-        raise ValueError(f"{name} must be [..., heads, head size]")
-    h, d = t.shape[-2:]
-    if t.numel() == 0:
-        return h * d
-    if (d > 1 and t.stride(-1) != 1) or (h > 1 and t.stride(-2) != d):
-        raise ValueError(f"the heads of {name} must lie side by side")
-    ld, n = None, 1
-    for size, step in zip(reversed(t.shape[:-2]), reversed(t.stride()[:-2])):
-        if size > 1:
-            if ld is None:
-                ld = step
-            elif step != ld * n:
-                raise ValueError(f"the tokens of {name} must be one stride apart")
-            n *= size
-    return h * d if ld is None else ld
+    dev = t.device
+    if dev.type != "cuda":
+        raise ValueError(f"{name} must live on a CUDA device")
+    return dev
+
+
+def _packed(t, name, dtype, dev):
+    """A contiguous tensor of `dtype` on `dev`: its data pointer."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != dev or not t.is_contiguous():
+        _need(t, name, (dtype,), dev)
+    return t.data_ptr()
 
 
 def rope(x, positions, theta, rotary_dim=None, traditional=False, scaling=None, out=None, handle=None) -> torch.Tensor:
@@ -604,27 +647,27 @@ def rope(x, positions, theta, rotary_dim=None, traditional=False, scaling=None, 
     "type" and "factor": "linear", "ntk", "yarn" (original_len, beta_slow, beta_fast) or
     "banded" (original_len, low_freq, high_freq), and optionally attn_factor.  x and out may
     be views of wider rows (a fused projection's)."""
-    ld = _need_heads(x, "x", None)
-    dev = x.device
-    _need(positions, "positions", _I32, dev)
-    if tuple(positions.shape) != tuple(x.shape[:-2]):
+    dev = _cuda_tensor(x, "x")
+    shape = x.shape
+    ld = _heads_ld(x, "x", dev, shape, x.stride())
+    pos = _packed(positions, "positions", torch.int32, dev)
+    if positions.shape != shape[:-2]:
         raise ValueError("positions must have x's shape without heads and head size")
-    cfg = _rope_config(x.shape[-1], theta, rotary_dim, traditional, scaling)
-    y = out if out is not None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-    y_ld = _need_heads(y, "out", dev)
-    if y.shape != x.shape:
-        raise ValueError("out has another shape than x")
+    cfg = _rope_config(shape[-1], theta, rotary_dim, traditional, scaling)
+    if out is None:
+        out = torch.empty(shape, dtype=_BF, device=dev)
+        out_ld = shape[-2] * shape[-1]
+    else:
+        _cuda_tensor(out, "out")
+        out_ld = _heads_ld(out, "out", dev, out.shape, out.stride())
+        if out.shape != shape:
+            raise ValueError("out has another shape than x")
     h = handle or default_handle(dev.index)
-    h.bind_stream()
-    h.check(h.lib.fm_rope(h.h, C.byref(cfg), _ptr(x), ld, x.shape[-2], _ptr(positions), positions.numel(), _ptr(y), y_ld))
-    return y
-
-
-def _need_caches(cache_k, cache_v, dev, what="cache"):
-    _need(cache_k, what + "_k", _BF16, dev)
-    _need(cache_v, what + "_v", _BF16, dev)
-    if cache_v.shape != cache_k.shape:
-        raise ValueError(f"{what}_k and {what}_v must be alike")
+    h.bind_current()
+    st = h.lib.fm_rope(h.h, cfg, x.data_ptr(), ld, shape[-2], pos, positions.numel(), out.data_ptr(), out_ld)
+    if st:
+        h.check(st)
+    return out
 
 
 def rope_append(q, k, v, positions, slots, cache_k, cache_v, theta, traditional=False, scaling=None, rotary_dim=None,
@@ -633,59 +676,87 @@ def rope_append(q, k, v, positions, slots, cache_k, cache_v, theta, traditional=
     separate) with T = B * L tokens in sequence order: returns q rotated at positions [T] (in
     `out` if given, which may be q); k rotated and v go into the caches [B, n_kv, max_len, d]
     at slots [T] (a negative slot writes nothing; a sequence's slots must differ)."""
-    ld = _need_heads(q, "q", None)
-    dev = q.device
-    kv_ld = _need_heads(k, "k", dev)
-    if _need_heads(v, "v", dev) != kv_ld or v.shape != k.shape:
+    dev = _cuda_tensor(q, "q")
+    _cuda_tensor(k, "k")
+    _cuda_tensor(v, "v")
+    q_shape, k_shape, c_shape = q.shape, k.shape, cache_k.shape
+    ld = _heads_ld(q, "q", dev, q_shape, q.stride())
+    kv_ld = _heads_ld(k, "k", dev, k_shape, k.stride())
+    if _heads_ld(v, "v", dev, v.shape, v.stride()) != kv_ld or v.shape != k_shape:
         raise ValueError("k and v must have the same shape and strides")
-    _need_caches(cache_k, cache_v, dev)
-    _need(positions, "positions", _I32, dev)
-    _need(slots, "slots", _I32, dev)
-    T, d = positions.numel(), q.shape[-1]
-    if cache_k.dim() != 4 or cache_k.shape[3] != d or k.shape[-1] != d or k.shape[-2] != cache_k.shape[1]:
+    ck, cv = _packed(cache_k, "cache_k", _BF, dev), _packed(cache_v, "cache_v", _BF, dev)
+    pos, slot = _packed(positions, "positions", torch.int32, dev), _packed(slots, "slots", torch.int32, dev)
+    T, nh, d = positions.numel(), q_shape[-2], q_shape[-1]
+    if len(c_shape) != 4 or cache_v.shape != c_shape or c_shape[3] != d or k_shape[-1] != d or k_shape[-2] != c_shape[1]:
         raise ValueError("caches must be [B, n_kv, max_len, d] with k's heads and q's head size")
-    B = cache_k.shape[0]
-    if B == 0 or T % B or slots.numel() != T or q.numel() != T * q.shape[-2] * d or k.numel() != T * k.shape[-2] * d:
+    B = c_shape[0]
+    if B == 0 or T % B or slots.numel() != T or q.numel() != T * nh * d or k.numel() != T * k_shape[-2] * d:
         raise ValueError("q, k, v, positions and slots must hold the same T = B * L tokens")
     cfg = _rope_config(d, theta, rotary_dim, traditional, scaling)
-    y = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=dev)
-    y_ld = _need_heads(y, "out", dev)
-    if y.shape != q.shape:
-        raise ValueError("out has another shape than q")
+    if out is None:
+        out = torch.empty(q_shape, dtype=_BF, device=dev)
+        out_ld = nh * d
+    else:
+        _cuda_tensor(out, "out")
+        out_ld = _heads_ld(out, "out", dev, out.shape, out.stride())
+        if out.shape != q_shape:
+            raise ValueError("out has another shape than q")
     h = handle or default_handle(dev.index)
-    h.bind_stream()
-    h.check(h.lib.fm_rope_append(h.h, C.byref(cfg), _ptr(q), ld, q.shape[-2], _ptr(k), _ptr(v), kv_ld, k.shape[-2],
-                                 _ptr(positions), _ptr(slots), B, T // B, _ptr(cache_k), _ptr(cache_v),
-                                 cache_k.shape[2], _ptr(y), y_ld))
-    return y
+    h.bind_current()
+    st = h.lib.fm_rope_append(h.h, cfg, q.data_ptr(), ld, nh, k.data_ptr(), v.data_ptr(), kv_ld, k_shape[-2], pos, slot, B,
+                              T // B, ck, cv, c_shape[2], out.data_ptr(), out_ld)
+    if st:
+        h.check(st)
+    return out
 
 
-def _cache_attn(q, cache_k, lens, prefix_k, scale):
-    """Checked sizes of an attention over caches: (config, B, L, device)."""
-    ld = _need_heads(q, "q", None)
-    if q.dim() != 4:
+def _cache_attn(q, prefix_k, prefix_v, prefix_len, cache_k, cache_v, lens, acc, scale, handle):
+    dev = _cuda_tensor(q, "q")
+    q_shape = q.shape
+    ld = _heads_ld(q, "q", dev, q_shape, q.stride())
+    if len(q_shape) != 4:
         raise ValueError("q must be [B, L, n_heads, d]")
-    B, L, nh, d = q.shape
-    some = cache_k if cache_k is not None else prefix_k
-    if some is None:
-        raise ValueError("a prefix or caches are needed")
-    nkv = some.shape[1] if cache_k is not None else some.shape[0]
+    B, L, nh, d = q_shape
+    nkv = max_len = prefix_max = 0
+    pk = pv = ck = cv = n = None
     if cache_k is not None:
-        if cache_k.dim() != 4 or cache_k.shape[0] != B or cache_k.shape[3] != d:
-            raise ValueError("caches must be [B, n_kv, max_len, d] with q's batch and head size")
+        ck, cv = _packed(cache_k, "cache_k", _BF, dev), _packed(cache_v, "cache_v", _BF, dev)
+        shape = cache_k.shape
+        if len(shape) != 4 or shape[0] != B or shape[3] != d or cache_v.shape != shape:
+            raise ValueError("caches must be [B, n_kv, max_len, d] with q's batch and head size, and alike")
+        nkv, max_len = shape[1], shape[2]
         if lens is None:
             raise ValueError("lens is required with caches")
-        _need(lens, "lens", _I32, q.device)
-        if tuple(lens.shape) != (B,):
+        n = _packed(lens, "lens", torch.int32, dev)
+        if lens.shape != (B,):
             raise ValueError("lens must be [B]")
-    elif lens is not None:
-        raise ValueError("lens without caches")
-    if prefix_k is not None and (prefix_k.dim() != 3 or prefix_k.shape[0] != nkv or prefix_k.shape[2] != d):
-        raise ValueError("the prefix must be [n_kv, length, d] with the caches' heads and q's head size")
+    elif lens is not None or prefix_k is None:
+        raise ValueError("caches (or a prefix, without lens) are needed")
+    if prefix_k is not None:
+        pk, pv = _packed(prefix_k, "prefix_k", _BF, dev), _packed(prefix_v, "prefix_v", _BF, dev)
+        shape = prefix_k.shape
+        if len(shape) != 3 or shape[2] != d or prefix_v.shape != shape or (cache_k is not None and shape[0] != nkv):
+            raise ValueError("the prefix must be [n_kv, length, d] with the caches' heads and q's head size, k and v alike")
+        nkv, prefix_max = shape[0], shape[1]
+        prefix_len = prefix_max if prefix_len is None else int(prefix_len)
+        if not 0 <= prefix_len <= prefix_max:
+            raise ValueError("prefix_len is not within the prefix")
     if nkv == 0 or nh % nkv:
         raise ValueError("n_heads must be a multiple of n_kv")
-    return _lib.CacheAttnConfig(nh, nkv, d, cache_k.shape[2] if cache_k is not None else 0,
-                                prefix_k.shape[1] if prefix_k is not None else 0, ld, float(scale)), B, L
+    out = torch.empty(q_shape, dtype=_BF, device=dev)
+    cfg = _lib.CacheAttnConfig(nh, nkv, d, max_len, prefix_max, ld, scale)
+    h = handle or default_handle(dev.index)
+    h.bind_current()
+    if acc is None:
+        st = h.lib.fm_attention_prefix(h.h, cfg, q.data_ptr(), pk, pv, prefix_len or 0, ck, cv, n, B, L, out.data_ptr())
+    else:
+        a = _packed(acc, "acc", torch.float32, dev)
+        if acc.shape != cache_k.shape[:3]:
+            raise ValueError("acc must be [B, n_kv, max_len]")
+        st = h.lib.fm_attention_scored(h.h, cfg, q.data_ptr(), ck, cv, n, B, L, a, out.data_ptr())
+    if st:
+        h.check(st)
+    return out
 
 
 def attention_prefix(q, prefix_k, prefix_v, cache_k=None, cache_v=None, lens=None, prefix_len=None, scale=0.0,
@@ -695,38 +766,15 @@ def attention_prefix(q, prefix_k, prefix_v, cache_k=None, cache_v=None, lens=Non
     first prefix_len rows count (default all), and each sequence's own caches
     [B, n_kv, max_len, d] with lens [B] int32 filled slots, the L new tokens' among them:
     token l sees the prefix and the slots j <= lens[b] - L + l.  Returns [B, L, nh, d]."""
-    cfg, B, L = _cache_attn(q, cache_k, lens, prefix_k, scale)
-    dev = q.device
-    if prefix_k is not None:
-        _need_caches(prefix_k, prefix_v, dev, "prefix")
-    if cache_k is not None:
-        _need_caches(cache_k, cache_v, dev)
-    n = cfg.prefix_max if prefix_len is None else int(prefix_len)
-    if not 0 <= n <= cfg.prefix_max:
-        raise ValueError("prefix_len is not within the prefix")
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    h = handle or default_handle(dev.index)
-    h.bind_stream()
-    h.check(h.lib.fm_attention_prefix(h.h, C.byref(cfg), _ptr(q), _ptr(prefix_k), _ptr(prefix_v), n, _ptr(cache_k),
-                                      _ptr(cache_v), _ptr(lens), B, L, _ptr(out)))
-    return out
+    return _cache_attn(q, prefix_k, prefix_v, prefix_len, cache_k, cache_v, lens, None, scale, handle)
 
 
 def attention_scored(q, cache_k, cache_v, lens, acc, scale=0.0, handle=None) -> torch.Tensor:
     """attention_prefix without a prefix that also adds to acc [B, n_kv, max_len] fp32 each
     slot's attention probabilities, summed over the kv head's query heads and the L tokens."""
-    cfg, B, L = _cache_attn(q, cache_k, lens, None, scale)
-    dev = q.device
-    _need_caches(cache_k, cache_v, dev)
-    _need(acc, "acc", _F32, dev)
-    if acc.shape != cache_k.shape[:3]:
-        raise ValueError("acc must be [B, n_kv, max_len]")
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    h = handle or default_handle(dev.index)
-    h.bind_stream()
-    h.check(h.lib.fm_attention_scored(h.h, C.byref(cfg), _ptr(q), _ptr(cache_k), _ptr(cache_v), _ptr(lens), B, L,
-                                      _ptr(acc), _ptr(out)))
-    return out
+    if acc is None:
+        raise TypeError("acc must be a torch tensor")
+    return _cache_attn(q, None, None, None, cache_k, cache_v, lens, acc, scale, handle)
 
 
 def cache_evict(cache_k, cache_v, acc, lens, budget, sinks=0, recent=0, positions=None, out=None, lens_out=None,
@@ -738,39 +786,37 @@ def cache_evict(cache_k, cache_v, acc, lens, budget, sinks=0, recent=0, position
     out = (k, v, acc, positions) of [B, n_kv, M >= budget, ...] (positions may be None when
     `positions` is).  Slots that stay below n keep their places, the others below n take those
     from n on in order.  Returns the new lengths [B] (lens_out if given; it may be lens)."""
-    _need(cache_k, "cache_k", _BF16, None)
-    dev = cache_k.device
-    _need_caches(cache_k, cache_v, dev)
-    if cache_k.dim() != 4:
-        raise ValueError("caches must be [B, n_kv, max_len, d]")
-    B, nkv, max_len, d = cache_k.shape
-
-    def beside(a, p, name, rows):
-        _need(a, name + "acc", _F32, dev)
-        if tuple(a.shape) != (B, nkv, rows):
-            raise ValueError(name + "acc must be [B, n_kv, max_len]")
-        if p is not None:
-            _need(p, name + "positions", _I32, dev)
-            if p.shape != a.shape:
-                raise ValueError(name + "positions must be [B, n_kv, max_len]")
-
-    beside(acc, positions, "", max_len)
+    dev = _cuda_tensor(cache_k, "cache_k")
+    shape = cache_k.shape
+    ck, cv = _packed(cache_k, "cache_k", _BF, dev), _packed(cache_v, "cache_v", _BF, dev)
+    if len(shape) != 4 or cache_v.shape != shape:
+        raise ValueError("caches must be [B, n_kv, max_len, d] and alike")
+    B, nkv, max_len, d = shape
+    a = _packed(acc, "acc", torch.float32, dev)
+    p = None if positions is None else _packed(positions, "positions", torch.int32, dev)
+    if acc.shape != shape[:3] or (positions is not None and positions.shape != shape[:3]):
+        raise ValueError("acc and positions must be [B, n_kv, max_len]")
     if out is None:
-        out = (cache_k, cache_v, acc, positions)
-    ok, ov, oacc, opos = out
-    _need_caches(ok, ov, dev, "out")
-    if ok.dim() != 4 or (ok.shape[0], ok.shape[1], ok.shape[3]) != (B, nkv, d):
-        raise ValueError("the output caches must be [B, n_kv, length, d]")
-    beside(oacc, opos, "out ", ok.shape[2])
+        rows, ok, ov, oa, op = max_len, ck, cv, a, p
+    else:
+        out_k, out_v, out_acc, out_positions = out
+        ok, ov = _packed(out_k, "out k", _BF, dev), _packed(out_v, "out v", _BF, dev)
+        oa = _packed(out_acc, "out acc", torch.float32, dev)
+        op = None if out_positions is None else _packed(out_positions, "out positions", torch.int32, dev)
+        rows = out_k.shape[2] if out_k.dim() == 4 else -1
+        if out_k.shape != (B, nkv, rows, d) or out_v.shape != out_k.shape or out_acc.shape != (B, nkv, rows) or \
+                (out_positions is not None and out_positions.shape != (B, nkv, rows)):
+            raise ValueError("the outputs must be [B, n_kv, length, d] (k, v) and [B, n_kv, length] (acc, positions)")
+    n = _packed(lens, "lens", torch.int32, dev)
     if lens_out is None:
         lens_out = torch.empty_like(lens)
-    for t, n in ((lens, "lens"), (lens_out, "lens_out")):
-        _need(t, n, _I32, dev)
-        if tuple(t.shape) != (B,):
-            raise ValueError(f"{n} must be [B]")
-    cfg = _lib.EvictConfig(nkv, d, max_len, ok.shape[2], int(budget), int(sinks), int(recent))
+    no = _packed(lens_out, "lens_out", torch.int32, dev)
+    if lens.shape != (B,) or lens_out.shape != (B,):
+        raise ValueError("lens and lens_out must be [B]")
+    cfg = _lib.EvictConfig(nkv, d, max_len, rows, budget, sinks, recent)
     h = handle or default_handle(dev.index)
-    h.bind_stream()
-    h.check(h.lib.fm_cache_evict(h.h, C.byref(cfg), _ptr(cache_k), _ptr(cache_v), _ptr(acc), _ptr(positions),
-                                 _ptr(lens), B, _ptr(ok), _ptr(ov), _ptr(oacc), _ptr(opos), _ptr(lens_out)))
+    h.bind_current()
+    st = h.lib.fm_cache_evict(h.h, cfg, ck, cv, a, p, n, B, ok, ov, oa, op, no)
+    if st:
+        h.check(st)
     return lens_out
