@@ -2113,6 +2113,14 @@ bool overlap(const void* p, int64_t n, const void* q, int64_t m) {
   return a < b + m && b < a + n;
 }
 
+int serve_ready(fm_handle* h) {
+  if (h->sv_ready) return FM_OK;
+  const cudaError_t e = fm::serve_init();
+  if (e != cudaSuccess) return cuda_err(h, e, "serving kernels' set-up");
+  h->sv_ready = true;
+  return FM_OK;
+}
+
 size_t evict_bytes(int64_t heads, int64_t budget) { return align_up(sizeof(int32_t) * heads * 2 * budget, 256) + sizeof(int32_t) * heads * 2; }
 
 int check_cache_attn(fm_handle* h, const fm_cache_attn_config* c, int B, int L, int prefix_len) {
@@ -2146,11 +2154,8 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
   const int64_t T = static_cast<int64_t>(B) * L, cols = static_cast<int64_t>(c->n_heads) * c->head_dim;
   if (overlap(q, 2 * ((T - 1) * q_ld + cols), out, 2 * T * cols)) return set_err(h, FM_EINVAL, "out may not overlap q");
   const OnDevice on(h);
-  if (!h->sv_ready) {
-    const cudaError_t e = fm::cache_attn_init();
-    if (e != cudaSuccess) return cuda_err(h, e, "cache attention kernel set-up");
-    h->sv_ready = true;
-  }
+  rc = serve_ready(h);
+  if (rc != FM_OK) return rc;
   const int nh = c->n_heads, nkv = c->n_kv_heads, d = c->head_dim;
   const fm::CacheAttnPlan p = fm::cache_attn_plan(B, L, nh, nkv, d, prefix_len, lens != nullptr, scored, c->max_len, h->num_sms);
   const int64_t own_rows = static_cast<int64_t>(B) * nkv * c->max_len, prefix_rows = static_cast<int64_t>(nkv) * c->prefix_max;
@@ -2380,7 +2385,8 @@ int fm_cache_evict(fm_handle* h, const fm_evict_config* c, const uint16_t* cache
         if (s.n && t.n && overlap(s.p, s.n, t.p, t.n)) return set_err(h, FM_EINVAL, "the outputs may not overlap the inputs");
   }
   const OnDevice on(h);
-  const int rc = ensure_sv(h, evict_bytes(heads, budget));
+  int rc = serve_ready(h);
+  if (rc == FM_OK) rc = ensure_sv(h, evict_bytes(heads, budget));
   if (rc != FM_OK) return rc;
   fm::EvictArgs a;
   std::memset(&a, 0, sizeof(a));
@@ -2407,7 +2413,8 @@ int fm_cache_evict(fm_handle* h, const fm_evict_config* c, const uint16_t* cache
   a.counts = reinterpret_cast<int32_t*>(h->sv_ws + align_up(sizeof(int32_t) * heads * 2 * budget, 256));
   a.err = sv_err(h);
   prof_begin(h, "cache_evict");
-  const cudaError_t e = fm::launch_evict(a, h->num_sms, h->stream);
+  const bool lens_apart = !overlap(lens, 4ll * B, out_lens, 4ll * B);
+  const cudaError_t e = fm::launch_evict(a, lens_apart, h->num_sms, h->stream);
   prof_end(h);
   return e == cudaSuccess ? FM_OK : cuda_err(h, e, "cache_evict launch");
 }

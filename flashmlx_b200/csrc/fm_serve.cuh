@@ -271,13 +271,15 @@ struct EvictArgs {
   int32_t* out_lens;        // [B]
   int B, nkv, d, max_len, out_max_len, budget, sinks, recent;
   int in_place;
+  int keys_in_smem;
+  int fused;                // the select kernel makes the moves
   int32_t* list;            // [B * nkv][2][budget] destinations, sources
   int32_t* counts;          // [B * nkv][2] rows to move, slots that stay
   uint32_t* err;
 };
 
 cudaError_t launch_rope(RopeArgs a, int num_sms, cudaStream_t st);
-cudaError_t cache_attn_init();
+cudaError_t serve_init();
 // p, s: the prefix / own caches by attn_tc_kernel where their workers are set, with its maps
 struct TcMapsKV {
   CUtensorMap k, v;
@@ -288,6 +290,6 @@ cudaError_t launch_cache_attn(const CacheAttnArgs& a, const TcAttnArgs& p, const
 cudaError_t attn_tc_init();
 cudaError_t launch_attn_tc(const TcAttnArgs& a, int d, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st);
 cudaError_t launch_slot_weight_tc(const TcWeightArgs& a, int d, const CUtensorMap& k, const CUtensorMap& q, cudaStream_t st);
-cudaError_t launch_evict(const EvictArgs& a, int num_sms, cudaStream_t st);
+cudaError_t launch_evict(EvictArgs a, bool lens_apart, int num_sms, cudaStream_t st);
 
 }  // namespace fm

@@ -657,9 +657,12 @@ static cudaError_t attn_opt_in() {
   return cudaFuncSetAttribute(attn_split_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_split_smem(D));
 }
 
-cudaError_t cache_attn_init() {
+cudaError_t evict_init();
+
+cudaError_t serve_init() {
   cudaError_t e = attn_opt_in<128>();
   if (e == cudaSuccess) e = attn_opt_in<64>();
+  if (e == cudaSuccess) e = evict_init();
   return e == cudaSuccess ? attn_tc_init() : e;
 }
 
@@ -738,11 +741,14 @@ cudaError_t launch_cache_attn(const CacheAttnArgs& a, const TcAttnArgs& p, const
 // ------------------------------------------------------------------ eviction
 // evict_select_kernel (one CTA per sequence and kv head) finds the n = min(len, budget) slots
 // that stay: a radix select over 32-bit keys (protected slots the largest, then the weight's
-// order-preserving bits, NaN as -inf), 8 bits a pass, ties to the lower slot.  It leaves the
-// list of rows that move as (destination, source) pairs; evict_move_kernel moves them.
-// In place only the holes below n are filled, by the kept slots from n on, both in ascending
-// order: sources >= n, destinations < n, so no move reads what another writes.
+// order-preserving bits, NaN as -inf), 8 bits a pass, ties to the lower slot.  The keys are read
+// once, into shared memory where they fit.  It leaves the list of rows that move as
+// (destination, source) pairs, for evict_move_kernel or, when there can only be a few, for
+// itself.  In place only the holes below n are filled, by the kept slots from n on, both in
+// ascending order: sources >= n, destinations < n, so no move reads what another writes.
 constexpr int kEvictThreads = 1024;
+constexpr int kEvictSmemKeys = 40960;  // 160 KB beside the 32 KB of counts
+constexpr int kEvictFused = 64;        // moves of a head that the select kernel makes itself
 
 namespace {
 
@@ -753,39 +759,57 @@ FM_DEV uint32_t order_bits(float v) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;  // [0x007fffff, 0xff800000]
 }
 
-// inclusive scan over the CTA of one value a thread; s_w: 32 ints of shared memory
-FM_DEV int block_scan(int v, int* s_w, int* sum) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// exclusive prefix of warp w's count and the total, from every warp's count; whole warp
+FM_DEV int warps_before(const int* counts, int warp, int* total) {
+  const int lane = threadIdx.x & 31;
+  const int v = counts[lane];
+  const int before = __reduce_add_sync(0xffffffffu, lane < warp ? v : 0);
+  *total = __reduce_add_sync(0xffffffffu, v);
+  return before;
+}
+
+// rows [0, cnt) of the list, `warps` warps together, warp `w` of them: K and V rows, weights, positions
+FM_DEV void evict_rows(const EvictArgs& a, int64_t bh, const int32_t* list_dst, const int32_t* list_src, int cnt, int w,
+                       int warps) {
+  constexpr int R = 4, U = 4;  // rows of a warp at a time, loads in flight
+  const int lane = threadIdx.x & 31;
+  const int ch = a.d / 8;
+  for (int i0 = w * R; i0 < cnt; i0 += warps * R) {
+    const int n = min(R, cnt - i0), total = n * 2 * ch;
+    for (int e0 = lane; e0 < total; e0 += 32 * U) {
+      uint4 v[U];
+      uint16_t* to[U];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += up;
-  }
-  if (lane == 31) s_w[warp] = v;
-  __syncthreads();
-  if (warp == 0) {
-    int w = s_w[lane];
+      for (int u = 0; u < U; ++u) {
+        const int e = e0 + 32 * u;
+        if (e >= total) continue;
+        const int row = e / (2 * ch), c = e - row * 2 * ch;
+        const bool is_v = c >= ch;
+        const int col = (is_v ? c - ch : c) * 8;
+        v[u] = *reinterpret_cast<const uint4*>((is_v ? a.cache_v : a.cache_k) + (bh * a.max_len + list_src[i0 + row]) * a.d + col);
+        to[u] = (is_v ? a.out_v : a.out_k) + (bh * a.out_max_len + list_dst[i0 + row]) * a.d + col;
+      }
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += up;
+      for (int u = 0; u < U; ++u)
+        if (e0 + 32 * u < total) *reinterpret_cast<uint4*>(to[u]) = v[u];
     }
-    s_w[lane] = w;
+    if (lane < n) {
+      const int dst = list_dst[i0 + lane], src = list_src[i0 + lane];
+      a.out_acc[bh * a.out_max_len + dst] = a.acc[bh * a.max_len + src];
+      if (a.out_positions)
+        a.out_positions[bh * a.out_max_len + dst] = a.positions ? a.positions[bh * a.max_len + src] : src;
+    }
   }
-  __syncthreads();
-  const int before = warp ? s_w[warp - 1] : 0;
-  *sum = s_w[31];
-  __syncthreads();  // s_w may be written again
-  return v + before;
 }
 
 }  // namespace
 
 __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const EvictArgs a) {
+  extern __shared__ __align__(16) uint32_t s_keys[];  // [max_len] when they fit
   __shared__ int s_hist[256 * 32];  // [bin][lane]: a lane's own bank, no conflicts
-  __shared__ int s_w[32];
+  __shared__ int s_w[3][32];
   __shared__ int s_pick[2];
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t bh = blockIdx.x;
   const int b = static_cast<int>(bh / a.nkv);
   int len = a.lens[b];
@@ -798,10 +822,11 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
   const int32_t* pos = a.positions ? a.positions + bh * a.max_len : nullptr;
   int32_t* list_dst = a.list + bh * 2 * a.budget;
   int32_t* list_src = list_dst + a.budget;
+  if (threadIdx.x == 0 && a.fused && bh % a.nkv == 0) a.out_lens[b] = n;
   if (n == len) {  // all stay
     if (!a.in_place)
       for (int i = threadIdx.x; i < n; i += kEvictThreads) list_dst[i] = list_src[i] = i;
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && !a.fused) {
       a.counts[2 * bh] = a.in_place ? 0 : n;
       a.counts[2 * bh + 1] = n;
     }
@@ -811,112 +836,153 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
   int64_t newest = len - 1;
   if (pos) {
     int mx = INT32_MIN;
+#pragma unroll 4
     for (int i = threadIdx.x; i < len; i += kEvictThreads) mx = max(mx, pos[i]);
     mx = __reduce_max_sync(0xffffffffu, mx);
-    if (lane == 0) s_w[threadIdx.x >> 5] = mx;
+    if (lane == 0) s_w[0][warp] = mx;
     __syncthreads();
-    newest = __reduce_max_sync(0xffffffffu, s_w[lane]);
-    __syncthreads();
+    newest = __reduce_max_sync(0xffffffffu, s_w[0][lane]);
   }
-  auto key_of = [&](int i) -> uint32_t {
+  auto make_key = [&](int i) -> uint32_t {
     const int64_t p = pos ? pos[i] : i;
-    if (p < a.sinks || p > newest - a.recent) return 0xffffffffu;
-    return order_bits(acc[i]);
+    return p < a.sinks || p > newest - a.recent ? 0xffffffffu : order_bits(acc[i]);
   };
+  const bool kept_here = a.keys_in_smem;
+  auto key_of = [&](int i) -> uint32_t { return kept_here ? s_keys[i] : make_key(i); };
   // radix select: the n-th largest key and how many keys equal to it stay
   uint32_t prefix = 0;
   int want = n;  // of the keys that match the prefix so far
 #pragma unroll 1
   for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256 * 32; i += kEvictThreads) s_hist[i] = 0;
+    for (int i = threadIdx.x; i < 256 * 32 / 4; i += kEvictThreads) reinterpret_cast<int4*>(s_hist)[i] = make_int4(0, 0, 0, 0);
     __syncthreads();
-    for (int i = threadIdx.x; i < len; i += kEvictThreads) {
-      const uint32_t k = key_of(i);
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
-        atomicAdd(&s_hist[((k >> shift) & 255u) * 32 + lane], 1);
+    if (shift == 24) {
+#pragma unroll 4
+      for (int i = threadIdx.x; i < len; i += kEvictThreads) {
+        const uint32_t k = make_key(i);
+        if (kept_here) s_keys[i] = k;
+        atomicAdd(&s_hist[(k >> 24) * 32 + lane], 1);
+      }
+    } else {
+#pragma unroll 4
+      for (int i = threadIdx.x; i < len; i += kEvictThreads) {
+        const uint32_t k = key_of(i);
+        if ((k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[((k >> shift) & 255u) * 32 + lane], 1);
+      }
     }
     __syncthreads();
-    // bins from the largest down: thread t < 256 holds bin 255 - t
-    int cnt = 0;
-    if (threadIdx.x < 256)
-      for (int i = 0; i < 32; ++i) cnt += s_hist[(255 - threadIdx.x) * 32 + ((i + lane) & 31)];
-    int all;
-    const int incl = block_scan(cnt, s_w, &all);
-    if (threadIdx.x < 256 && incl >= want && incl - cnt < want) {
-      s_pick[0] = 255 - threadIdx.x;
-      s_pick[1] = want - (incl - cnt);
+    // a warp sums eight bins; bins are then walked from the largest down
+    for (int i = 0; i < 8; ++i) {
+      const int c = __reduce_add_sync(0xffffffffu, s_hist[(warp * 8 + i) * 32 + lane]);
+      if (lane == 0) s_hist[(warp * 8 + i) * 32] = c;
+    }
+    __syncthreads();
+    if (warp == 0) {  // lane l: bins 255 - 8 l down to 248 - 8 l
+      int c[8], mine = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine += c[i] = s_hist[(255 - 8 * lane - i) * 32];
+      int incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      int left = want - (incl - mine);
+      if (left > 0 && left <= mine) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (left > 0 && left <= c[i]) {
+            s_pick[0] = 255 - 8 * lane - i;
+            s_pick[1] = left;
+          }
+          left -= c[i];
+        }
+      }
     }
     __syncthreads();
     prefix |= static_cast<uint32_t>(s_pick[0]) << shift;
     want = s_pick[1];
-    __syncthreads();
   }
-  // `want` of the keys equal to `prefix` stay, the lowest slots first.  Slots in order, 1024
-  // at a time, with running counts of equals, holes and kept tails; the heads that stay are
-  // listed after the m moves when rows are copied elsewhere.
-  int eq0 = 0, hole0 = 0, tail0 = 0;
-  // holes below n: n minus the kept below n, so m is known only at the end; heads are listed
-  // from the back of the list
-  int head0 = 0;
-  for (int base = 0; base < len; base += kEvictThreads) {
-    const int i = base + threadIdx.x;
-    const uint32_t k = i < len ? key_of(i) : 0u;
-    const bool eq = i < len && k == prefix;
-    int all;
-    const int eq_incl = block_scan(eq ? 1 : 0, s_w, &all);
-    const bool kept = i < len && (k > prefix || (eq && eq0 + eq_incl <= want));
-    eq0 += all;
-    const bool hole = i < n && !kept, tail = i >= n && kept, head = i < n && kept;
-    const int hi = block_scan(hole ? 1 : 0, s_w, &all);
-    if (hole) list_dst[hole0 + hi - 1] = i;
-    hole0 += all;
-    const int ti = block_scan(tail ? 1 : 0, s_w, &all);
-    if (tail) list_src[tail0 + ti - 1] = i;
-    tail0 += all;
-    if (!a.in_place) {
-      const int ci = block_scan(head ? 1 : 0, s_w, &all);
-      if (head) list_dst[n - (head0 + ci)] = list_src[n - (head0 + ci)] = i;
-      head0 += all;
+  // `want` of the keys equal to `prefix` stay, the lowest slots first.  A warp takes a contiguous
+  // range of slots, 32 at a time; first the equal keys are counted, then the holes below n and
+  // the kept slots from n on, then the lists are written.
+  const int per = (len + 32 * 32 - 1) / (32 * 32) * 32, i0 = warp * per, i1 = min(len, i0 + per);
+  int eq = 0;
+  for (int i = i0 + lane; i - lane < i1; i += 32) eq += __popc(__ballot_sync(0xffffffffu, i < i1 && key_of(i) == prefix));
+  if (lane == 0) s_w[0][warp] = eq;
+  __syncthreads();
+  int all;
+  const int eq0 = warps_before(s_w[0], warp, &all);
+  const uint32_t below = (1u << lane) - 1;
+  int holes = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    int e = eq0, hole = 0, tail = 0, moves = 0;
+    if (pass == 1) {
+      hole = warps_before(s_w[1], warp, &moves);
+      tail = warps_before(s_w[2], warp, &all);
     }
+    for (int i = i0 + lane; i - lane < i1; i += 32) {
+      const uint32_t k = i < i1 ? key_of(i) : 0u;
+      const bool is_eq = i < i1 && k == prefix;
+      const uint32_t eqs = __ballot_sync(0xffffffffu, is_eq);
+      const bool kept = i < i1 && (k > prefix || (is_eq && e + __popc(eqs & below) < want));
+      e += __popc(eqs);
+      const bool is_hole = i < min(n, i1) && !kept, is_tail = i >= n && kept;
+      const uint32_t hm = __ballot_sync(0xffffffffu, is_hole), tm = __ballot_sync(0xffffffffu, is_tail);
+      if (pass == 1) {
+        if (is_hole) list_dst[hole + __popc(hm & below)] = i;
+        if (is_tail) list_src[tail + __popc(tm & below)] = i;
+        // copied elsewhere, the slots that keep their places follow the moves
+        if (!a.in_place && i < n && kept) {
+          const int at = moves + i - (hole + __popc(hm & below));
+          list_dst[at] = list_src[at] = i;
+        }
+      }
+      hole += __popc(hm);
+      tail += __popc(tm);
+    }
+    if (pass == 0) {
+      if (lane == 0) {
+        s_w[1][warp] = hole;
+        s_w[2][warp] = tail;
+      }
+      __syncthreads();
+    }
+    holes = moves;
   }
-  if (threadIdx.x == 0) {
-    a.counts[2 * bh] = a.in_place ? hole0 : n;
+  if (a.fused) {
+    __syncthreads();  // the lists are written (and read by this block alone)
+    evict_rows(a, bh, list_dst, list_src, holes, warp, 32);
+  } else if (threadIdx.x == 0) {
+    a.counts[2 * bh] = a.in_place ? holes : n;
     a.counts[2 * bh + 1] = n;
   }
 }
 
-// One warp a row pair: K and V rows, weight and position.
 __global__ void __launch_bounds__(256) evict_move_kernel(const EvictArgs a) {
   const int64_t bh = blockIdx.y;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cnt = a.counts[2 * bh];
   if (blockIdx.x == 0 && threadIdx.x == 0 && bh % a.nkv == 0) a.out_lens[bh / a.nkv] = a.counts[2 * bh + 1];
   const int32_t* list_dst = a.list + bh * 2 * a.budget;
-  const int32_t* list_src = list_dst + a.budget;
-  const int ch = a.d / 8;
-  for (int i = blockIdx.x * 8 + warp; i < cnt; i += gridDim.x * 8) {
-    const int dst = list_dst[i], src = list_src[i];
-    const int64_t from = (bh * a.max_len + src) * a.d, to = (bh * a.out_max_len + dst) * a.d;
-    for (int e = lane; e < 2 * ch; e += 32) {
-      const bool v = e >= ch;
-      const int c = (v ? e - ch : e) * 8;
-      *reinterpret_cast<uint4*>((v ? a.out_v : a.out_k) + to + c) =
-          *reinterpret_cast<const uint4*>((v ? a.cache_v : a.cache_k) + from + c);
-    }
-    if (lane == 0) a.out_acc[bh * a.out_max_len + dst] = a.acc[bh * a.max_len + src];
-    if (lane == 1 && a.out_positions)
-      a.out_positions[bh * a.out_max_len + dst] = a.positions ? a.positions[bh * a.max_len + src] : src;
-  }
+  evict_rows(a, bh, list_dst, list_dst + a.budget, cnt, blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8);
 }
 
-cudaError_t launch_evict(const EvictArgs& a, int num_sms, cudaStream_t st) {
+cudaError_t evict_init() {
+  return cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictSmemKeys * 4);
+}
+
+cudaError_t launch_evict(EvictArgs a, bool lens_apart, int num_sms, cudaStream_t st) {
   const int64_t heads = static_cast<int64_t>(a.B) * a.nkv;
-  evict_select_kernel<<<static_cast<unsigned>(heads), kEvictThreads, 0, st>>>(a);
+  const int64_t most = a.in_place ? std::min(a.budget, std::max(0, a.max_len - a.budget)) : a.budget;
+  a.keys_in_smem = a.max_len <= kEvictSmemKeys;
+  // a step that is a few slots over: no second launch (unless out_lens is lens, which other blocks
+  // of the sequence may not have read yet)
+  a.fused = a.in_place && most <= kEvictFused && lens_apart;
+  evict_select_kernel<<<static_cast<unsigned>(heads), kEvictThreads, a.keys_in_smem ? 4 * a.max_len : 0, st>>>(a);
   const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  const int64_t most = a.in_place ? std::min<int64_t>(a.budget, std::max(0, a.max_len - a.budget)) : a.budget;
+  if (e != cudaSuccess || a.fused) return e;
   const int64_t want = std::max<int64_t>(1, (num_sms * 8 + heads - 1) / heads);
-  const unsigned gx = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((most + 7) / 8, want)));
+  const unsigned gx = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((most + 31) / 32, want)));
   evict_move_kernel<<<dim3(gx, static_cast<unsigned>(heads)), 256, 0, st>>>(a);
   return cudaGetLastError();
 }
