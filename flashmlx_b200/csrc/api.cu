@@ -2159,6 +2159,7 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
   const int nh = c->n_heads, nkv = c->n_kv_heads, d = c->head_dim;
   const fm::CacheAttnPlan p = fm::cache_attn_plan(B, L, nh, nkv, d, prefix_len, lens != nullptr, scored, c->max_len, h->num_sms);
   const int64_t own_rows = static_cast<int64_t>(B) * nkv * c->max_len, prefix_rows = static_cast<int64_t>(nkv) * c->prefix_max;
+  if (scored && nh / nkv > fm::kTcKeys) return set_err(h, FM_EUNSUPPORTED, "more than 128 query heads to a kv head");
   // the kernels count rows and tiles in 32 bits
   const double group = nh / nkv, tiles = (c->max_len / 128 + 3.0) * nkv * B * (L * group / 256 + 1) +
                                          (prefix_len / 128 + 3.0) * nkv * (static_cast<double>(B) * L * group / 256 + 1) +
@@ -2196,6 +2197,8 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
   a.part_o = reinterpret_cast<float*>(h->sv_ws);
   a.part_ml = reinterpret_cast<float2*>(h->sv_ws + p.off_ml);
   a.lse2 = scored ? reinterpret_cast<float*>(h->sv_ws + p.off_lse) : nullptr;
+  a.scores = scored && !p.tc_s ? reinterpret_cast<float*>(h->sv_ws + p.off_scores) : nullptr;
+  a.score_ld = (static_cast<int64_t>(c->max_len) + 3) / 4 * 4;
   a.err = sv_err(h);
   fm::TcAttnArgs t[2];
   fm::TcMapsKV maps[2];
@@ -2233,7 +2236,7 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
   }
   fm::TcWeightArgs w;
   std::memset(&w, 0, sizeof(w));
-  if (scored && p.tc_s && a.group <= fm::kTcKeys) {
+  if (scored && p.tc_s) {
     w.q = q;
     w.q_ld = q_ld;
     w.lens = lens;

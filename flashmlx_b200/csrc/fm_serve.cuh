@@ -72,6 +72,8 @@ struct CacheAttnArgs {
   float* part_o;            // [slots][16][d]
   float2* part_ml;          // [slots][16] (maximum in log2 units, sum)
   float* lse2;              // [B, nkv, L * group] or null
+  float* scores;            // split, scored: [B, nkv, L * group][score_ld] scores in log2 units (-inf: hidden)
+  int64_t score_ld;         // max_len rounded up to 4
   uint32_t* err;
 };
 
@@ -253,7 +255,7 @@ struct CacheAttnPlan {
   bool tc_p = false, tc_s = false;  // the prefix / the own caches by attn_tc_kernel
   int rt_p = 0, rt_s = 0, rps_p = 0, rps_s = 0, merge_rows = 16;
   int workers = 0, workers_p = 0, workers_s = 0;
-  size_t off_ml = 0, off_po = 0, off_pml = 0, off_so = 0, off_sml = 0, off_lse = 0, off_w = 0, bytes = 0;
+  size_t off_ml = 0, off_po = 0, off_pml = 0, off_so = 0, off_sml = 0, off_lse = 0, off_w = 0, off_scores = 0, bytes = 0;
 };
 CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_len, bool own, bool scored, int max_len,
                               int num_sms);

@@ -324,6 +324,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
         qa[ks][hf + 2] = on ? *reinterpret_cast<const uint32_t*>(q + 16 * ks + 2 * c + 8) : 0u;
       }
     }
+    float* srow[2];  // where this thread's rows' scores go
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int r = row0 + g + 8 * hf;
+      srow[hf] = a.scores && r < rows ? a.scores + ((static_cast<int64_t>(b) * a.nkv + kvh) * rows + r) * a.score_ld : nullptr;
+    }
     float o[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -361,6 +367,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
             v = key <= lim[hf] ? v * a.scale_log2 : -INFINITY;
             mx = fmaxf(mx, v);
           }
+        if (srow[hf]) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const int key = (tile + j) * kAttnTile + 8 * n + 2 * c;
+            if (key + 1 < len) *reinterpret_cast<float2*>(srow[hf] + key) = make_float2(s[n][2 * hf], s[n][2 * hf + 1]);
+            else if (key < len) srow[hf][key] = s[n][2 * hf];
+          }
+        }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const float mn = fmaxf(m[hf], mx);
@@ -574,65 +588,38 @@ __global__ void __launch_bounds__(128) attn_merge_cut_kernel(const CacheAttnArgs
 }
 
 // ------------------------------------------------------------------ slot weights
-// acc[b, kvh, j] += sum over the kv head's query rows of 2^(s_rj - lse2_r), recomputing the
-// scores with keys as the product's rows: a warp holds 16 keys' fragments and walks the query
-// rows 8 at a time, so a key's sum over rows stays in a lane quad.
-template <int D>
-__global__ void __launch_bounds__(128) slot_weight_kernel(const CacheAttnArgs a) {
-  constexpr int KS = D / 16;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, c = lane & 3;
+// acc[b, kvh, j] += sum over the kv head's query rows of 2^(s_rj - lse2_r), from the scores that
+// attn_split_kernel left: 4 bytes a row and slot, where K again would be 2 * head_dim a slot
+// (16 sequences of up to 16001 slots, 32/4 heads of 128: 54 us recomputing the scores, 6 us so).
+// Four neighbouring slots a thread.
+__global__ void __launch_bounds__(256) slot_weight_kernel(const CacheAttnArgs a) {
+  __shared__ float s_lse[kAttnRowTile];
   const int b = blockIdx.z, kvh = blockIdx.y;
   int len = a.lens[b];
   if (len < 0 || len > a.max_len) len = 0;  // reported by the merge
-  const int key0 = (blockIdx.x * 4 + warp) * 16;
-  if (key0 >= len) return;
-  const uint16_t* kb = a.ck + (static_cast<int64_t>(b) * a.nkv + kvh) * a.max_len * D;
-  uint32_t ka[KS][4];
-#pragma unroll
-  for (int hf = 0; hf < 2; ++hf) {
-    const int key = key0 + g + 8 * hf;
-    const uint16_t* kr = kb + static_cast<int64_t>(min(key, len - 1)) * D;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      ka[ks][hf] = *reinterpret_cast<const uint32_t*>(kr + 16 * ks + 2 * c);
-      ka[ks][hf + 2] = *reinterpret_cast<const uint32_t*>(kr + 16 * ks + 2 * c + 8);
-    }
-  }
+  if (static_cast<int>(blockIdx.x) * 1024 >= len) return;
   const int rows = a.L * a.group;
-  float sum[2] = {0.f, 0.f};
-  // token l sees slot j iff j <= len - L + l: rows of earlier tokens see none of these keys
-  const int first = max(0, key0 - (len - a.L)) * a.group;
-  for (int r0 = first / 8 * 8; r0 < rows; r0 += 8) {
-    const int rq = min(r0 + g, rows - 1);
-    const int tk = rq / a.group;
-    const uint16_t* q = a.q + (static_cast<int64_t>(b) * a.L + tk) * a.q_ld +
-                        static_cast<int64_t>(kvh * a.group + rq - tk * a.group) * D;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      mma_bf16_16816(s, ka[ks][0], ka[ks][1], ka[ks][2], ka[ks][3],
-                     *reinterpret_cast<const uint32_t*>(q + 16 * ks + 2 * c),
-                     *reinterpret_cast<const uint32_t*>(q + 16 * ks + 2 * c + 8));
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = r0 + 2 * c + e;
-      if (r >= rows) continue;
-      const int tr = r / a.group;
-      const float lse = a.lse2[(static_cast<int64_t>(b) * a.nkv + kvh) * rows + r];
-      const int lim = len - a.L + tr;
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-        if (key0 + g + 8 * hf <= lim) sum[hf] += exp2f(s[2 * hf + e] * a.scale_log2 - lse);
-    }
+  const int64_t head = static_cast<int64_t>(b) * a.nkv + kvh;
+  if (threadIdx.x < rows) s_lse[threadIdx.x] = a.lse2[head * rows + threadIdx.x];
+  __syncthreads();
+  const int j = blockIdx.x * 1024 + threadIdx.x * 4;
+  if (j >= len) return;
+  const float* sc = a.scores + head * rows * a.score_ld + j;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r) {
+    const float4 v = *reinterpret_cast<const float4*>(sc + static_cast<int64_t>(r) * a.score_ld);
+    const float lse = s_lse[r];
+    sum.x += exp2f(v.x - lse);
+    sum.y += exp2f(v.y - lse);
+    sum.z += exp2f(v.z - lse);
+    sum.w += exp2f(v.w - lse);
   }
-#pragma unroll
-  for (int hf = 0; hf < 2; ++hf) {
-    sum[hf] += __shfl_xor_sync(0xffffffffu, sum[hf], 1);
-    sum[hf] += __shfl_xor_sync(0xffffffffu, sum[hf], 2);
-    const int key = key0 + g + 8 * hf;
-    if (c == 0 && key < len) a.acc[(static_cast<int64_t>(b) * a.nkv + kvh) * a.max_len + key] += sum[hf];
-  }
+  float* acc = a.acc + head * a.max_len + j;
+  acc[0] += sum.x;
+  if (j + 1 < len) acc[1] += sum.y;
+  if (j + 2 < len) acc[2] += sum.z;
+  if (j + 3 < len) acc[3] += sum.w;
 }
 
 // Adds the pieces of a key tile's weights, in the workers' order.
@@ -698,7 +685,8 @@ CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_l
   if (B * nkv * ((rows_s + 15) / 16) < 8ll * num_sms) p.merge_rows = 4;
   p.off_lse = add(scored ? sizeof(float) * B * L * nh : 0);
   const size_t key_items = static_cast<size_t>(B) * nkv * ((max_len + kTcKeys - 1) / kTcKeys);
-  p.off_w = add(scored && p.tc_s && group <= kTcKeys ? (num_sms + key_items) * kTcWeightParts * kTcKeys * sizeof(float) : 0);
+  p.off_scores = add(scored && !p.tc_s ? sizeof(float) * B * nkv * rows_s * (static_cast<size_t>(max_len) + 3) / 4 * 4 : 0);
+  p.off_w = add(scored && p.tc_s ? (num_sms + key_items) * kTcWeightParts * kTcKeys * sizeof(float) : 0);
   return p;
 }
 
@@ -728,8 +716,7 @@ static cudaError_t launch_cache_attn_d(const CacheAttnArgs& a, const TcAttnArgs&
     slot_weight_sum_kernel<<<dim3(w.key_tiles, a.nkv, a.B), kTcKeys, 0, st>>>(w);
     return cudaGetLastError();
   }
-  const dim3 grid((a.max_len + 63) / 64, a.nkv, a.B);
-  slot_weight_kernel<D><<<grid, 128, 0, st>>>(a);
+  slot_weight_kernel<<<dim3((a.max_len + 1023) / 1024, a.nkv, a.B), 256, 0, st>>>(a);
   return cudaGetLastError();
 }
 

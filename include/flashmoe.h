@@ -408,7 +408,7 @@ FM_API int fm_attention_prefix(fm_handle* h, const fm_cache_attn_config* cfg, co
 
 /* The same without a prefix, and acc[b, kvh, j] += the sum, over kv head kvh's query heads and
  * the L tokens, of the attention probability of slot j (fp32 [B, n_kv_heads, max_len]; slots
- * at or past lens[b] are left as they were). */
+ * at or past lens[b] are left as they were).  At most 128 query heads to a kv head. */
 FM_API int fm_attention_scored(fm_handle* h, const fm_cache_attn_config* cfg, const uint16_t* q,
                                const uint16_t* cache_k, const uint16_t* cache_v, const int32_t* lens, int B, int L,
                                float* acc, uint16_t* out);

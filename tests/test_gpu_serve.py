@@ -95,6 +95,8 @@ def test_attention_refusals():
         lambda: h.check(h.lib.fm_attention_prefix(h.h, _lib.C.byref(cfg), q.data_ptr() + 2, pk.data_ptr(), pk.data_ptr(), 4,
                                                   None, None, None, 2, 1, ck.data_ptr())),
         lambda: h.check(h.lib.fm_serve_reserve(h.h, _lib.C.byref(cfg), -1, 1)),
+        lambda: ops.attention_scored(rnd(7, 1, 1, 129, 64), ck[:1, :1].contiguous(), ck[:1, :1].contiguous(), lens[:1].contiguous(),
+                                     acc[:1, :1].contiguous()),
     ]:
         refused(call)
 
@@ -305,6 +307,7 @@ def test_attention_scale(scale):
     (1, 1100, 8, 2, 128, [1100], 1100),
     (1, 300, 2, 2, 128, [1000], 1024),
     (17, 1, 16, 16, 64, [3 * i for i in range(17)], 64),
+    (3, 2, 4, 2, 64, [1025, 7, 2050], 2051),             # an odd leading size, several blocks of slots
 ])
 def test_attention_scored(B, L, nh, nkv, d, lens, M):
     from flashmlx_b200 import ops
