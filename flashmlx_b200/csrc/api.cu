@@ -2188,6 +2188,7 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
   a.max_len = c->max_len;
   a.split_prefix = p.rt_p ? prefix_len : 0;
   a.split_own = p.rt_s > 0;
+  a.after_tc = p.tc_p || p.tc_s;
   const double scale = c->scale != 0.f ? c->scale : 1.0 / std::sqrt(static_cast<double>(d));
   a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   a.merge_rows = p.merge_rows;

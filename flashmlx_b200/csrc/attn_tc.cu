@@ -149,7 +149,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   uint8_t* s_kv = s_q + 2 * S::kTileBytes;           // [NS][kTileBytes]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &bars.abort_flag;
-  const int per = tc_places_per_worker(a, tc_places_before(a, a.items()) * a.nkv);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -179,6 +178,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
+  pdl_wait();
+  pdl_trigger();
+  const int per = tc_places_per_worker(a, tc_places_before(a, a.items()) * a.nkv);
 
   TcPiece it;
   tc_first(a, blockIdx.x, per, it);
@@ -617,7 +619,6 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
   uint8_t* s_q = s_k + 2 * S::kTileBytes;        // [kWStages][kTileBytes]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &bars.abort_flag;
-  const int per = tc_places_per_worker(a, tc_places_before(a, a.items()) * a.nkv);
   if (threadIdx.x == 0) {
     for (int i = 0; i < kWStages; ++i) {
       mbar_init(&bars.qfull[i], 2);  // the copy, and the rows' lse
@@ -646,6 +647,9 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
+  pdl_wait();
+  pdl_trigger();
+  const int per = tc_places_per_worker(a, tc_places_before(a, a.items()) * a.nkv);
   TcPiece it;
   tc_first(a, blockIdx.x, per, it);
   const int rows = a.L * a.group;
@@ -818,19 +822,13 @@ cudaError_t attn_tc_init() {
 }
 
 cudaError_t launch_slot_weight_tc(const TcWeightArgs& a, int d, const CUtensorMap& k, const CUtensorMap& q, cudaStream_t st) {
-  if (d == 128)
-    slot_weight_tc_kernel<128><<<a.workers, kWThreads, WShape<128>::kSmem, st>>>(a, k, q);
-  else
-    slot_weight_tc_kernel<64><<<a.workers, kWThreads, WShape<64>::kSmem, st>>>(a, k, q);
-  return cudaGetLastError();
+  return d == 128 ? launch_pdl(slot_weight_tc_kernel<128>, a.workers, kWThreads, WShape<128>::kSmem, st, a, k, q)
+                  : launch_pdl(slot_weight_tc_kernel<64>, a.workers, kWThreads, WShape<64>::kSmem, st, a, k, q);
 }
 
 cudaError_t launch_attn_tc(const TcAttnArgs& a, int d, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
-  if (d == 128)
-    attn_tc_kernel<128><<<a.workers, kThreads, Shape<128>::kSmem, st>>>(a, k, v);
-  else
-    attn_tc_kernel<64><<<a.workers, kThreads, Shape<64>::kSmem, st>>>(a, k, v);
-  return cudaGetLastError();
+  return d == 128 ? launch_pdl(attn_tc_kernel<128>, a.workers, kThreads, Shape<128>::kSmem, st, a, k, v)
+                  : launch_pdl(attn_tc_kernel<64>, a.workers, kThreads, Shape<64>::kSmem, st, a, k, v);
 }
 
 }  // namespace fm

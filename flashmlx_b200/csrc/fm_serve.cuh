@@ -5,6 +5,31 @@
 
 namespace fm {
 
+// The serving kernels are launched with programmatic stream serialization: a kernel may begin
+// while the one before it ends.  It touches nothing that an earlier kernel wrote before
+// pdl_wait(), which returns when the kernel before it is complete, and says with pdl_trigger()
+// that the next one may begin -- after its own wait, so that whatever came before a call's
+// first kernel is complete when its second one begins.
+#ifdef __CUDACC__
+FM_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+FM_DEV void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <class... P, class... A>
+cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = block;
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &attr;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, args...);
+}
+#endif
+
 constexpr int kRopeMaxDim = 256;  // largest head size of the rotary kernels
 
 struct RopeArgs {
@@ -41,6 +66,7 @@ struct RopeArgs {
 // order, so no two pieces share a slot -- and attn_merge_kernel joins an output row's pieces.
 constexpr int kAttnTile = 16;        // keys of a tile
 constexpr int kAttnRowTile = 16;     // query rows of an item
+constexpr int kAttnSplitRows = 64;   // up to so many query rows to a key the split kernel reads it
 constexpr int kAttnMinTiles = 4;     // least tiles of a worker's range
 constexpr int kAttnWarps = 4;        // workers of a CTA
 constexpr int kAttnBlocksPerSm = 2;
@@ -65,6 +91,7 @@ struct CacheAttnArgs {
   int B, L, nh, nkv, group, max_len;
   int split_prefix;         // prefix rows the split kernel reads (0: none, or the other kernel's)
   int split_own;            // 1: it reads the own caches
+  int after_tc;             // attn_tc_kernel was launched before it: nothing of that is needed here
   float scale_log2;         // softmax scale * log2(e)
   int merge_rows;           // rows of a merge block: 4 or 16
   int rt_p, rt_s;           // row tiles of the prefix items / of a sequence's items, per kv head

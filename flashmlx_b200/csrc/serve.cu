@@ -67,6 +67,8 @@ FM_DEV bool rope_row(const RopeArgs& a, int64_t t, int hs, RopeRow& r) {
 template <bool TRADITIONAL, bool VEC>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
   extern __shared__ float2 s_cs[];  // [tpb][rotary / 2]
+  pdl_wait();
+  pdl_trigger();
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tpb;
   const int nt = static_cast<int>(min(static_cast<int64_t>(a.tpb), a.T - t0));
   const int half = a.rotary / 2;
@@ -165,14 +167,9 @@ cudaError_t launch_rope(RopeArgs a, int num_sms, cudaStream_t st) {
   const unsigned grid = static_cast<unsigned>((a.T + a.tpb - 1) / a.tpb);
   const size_t smem = sizeof(float2) * a.tpb * (a.rotary / 2);
   const bool vec = a.traditional ? a.rotary % 8 == 0 : (a.rotary / 2) % 8 == 0;
-  if (a.traditional) {
-    if (vec) rope_kernel<true, true><<<grid, kRopeThreads, smem, st>>>(a);
-    else rope_kernel<true, false><<<grid, kRopeThreads, smem, st>>>(a);
-  } else {
-    if (vec) rope_kernel<false, true><<<grid, kRopeThreads, smem, st>>>(a);
-    else rope_kernel<false, false><<<grid, kRopeThreads, smem, st>>>(a);
-  }
-  return cudaGetLastError();
+  void (*kernel)(RopeArgs) = a.traditional ? (vec ? rope_kernel<true, true> : rope_kernel<true, false>)
+                                           : (vec ? rope_kernel<false, true> : rope_kernel<false, false>);
+  return launch_pdl(kernel, grid, kRopeThreads, smem, st, a);
 }
 
 // ------------------------------------------------------------------ attention, split over keys
@@ -229,6 +226,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
   const int g = lane >> 2, c = lane & 3;
   const uint32_t ring = smem_u32(s_kv) + warp * (kAttnStages * STAGE);
   const int worker = blockIdx.x * kAttnWarps + warp;
+  if (!a.after_tc) pdl_wait();
+  pdl_trigger();
 
   const int tp = (a.split_prefix + kAttnTile - 1) / kAttnTile;  // tiles of a prefix item
   const int np = a.nkv * a.rt_p, ns = a.nkv * a.rt_s;           // items of the prefix / of a sequence
@@ -237,7 +236,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
   const int per = tiles_per_worker(a, total);
   int t = worker * per;
   const int t_end = min(total, t + per);
-  if (t >= t_end) return;
+  if (t >= t_end) {
+    if (a.after_tc) pdl_wait();
+    return;
+  }
 
   // the item of tile t: sequence (-1: the prefix), item of it, tile of the item
   int b = -1, item, tiles;
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
       }
       rest -= __shfl_sync(0xffffffffu, incl, 31);
       b += 32;
-      if (b >= a.B) return;  // t < total makes this unreachable
+      if (b >= a.B) break;  // t < total makes this unreachable
     }
     tiles = (seq_len(a, b) + kAttnTile - 1) / kAttnTile;
     item = rest / tiles;
@@ -434,6 +436,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
     }
     tiles = b < 0 ? tp : (seq_len(a, b) + kAttnTile - 1) / kAttnTile;
   }
+  // this kernel is not complete before the one in front of it is, so the merge need wait for one
+  if (a.after_tc) pdl_wait();
 }
 
 // Joins the pieces of output rows: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, zeros when
@@ -532,6 +536,8 @@ __global__ void __launch_bounds__(128) attn_merge_kernel(const CacheAttnArgs a, 
     per_s = tc_places_per_worker(ts, tc_places_before(ts, ts.items()) * ts.nkv);
     first_s = tc_places_before(ts, flat_s) * ts.nkv + kvh * (tiles_s + kCost) + kCost;
   }
+  pdl_wait();
+  pdl_trigger();
   for (int r = first_row + warp; r < min(rows, first_row + a.merge_rows); r += 4) {
     RowJoin<D> row;
     auto split_join = [&](int first, int tiles, int64_t item, int rr) {
@@ -572,6 +578,8 @@ __global__ void __launch_bounds__(128) attn_merge_cut_kernel(const CacheAttnArgs
       if (a.lens[b] < 0 || a.lens[b] > a.max_len) report(a.err, DEVERR_BOUNDS);
   const int per = tc_places_per_worker(ts, tc_places_before(ts, ts.items()) * ts.nkv);
   const int place = (blockIdx.x + 1) * per;
+  pdl_wait();
+  pdl_trigger();
   int flat, kvh, at;
   if (!tc_locate(ts, place, flat, kvh, at)) return;
   const int first = place - at + kCost, tiles = ts.tiles(flat);
@@ -597,6 +605,8 @@ __global__ void __launch_bounds__(256) slot_weight_kernel(const CacheAttnArgs a)
   const int b = blockIdx.z, kvh = blockIdx.y;
   int len = a.lens[b];
   if (len < 0 || len > a.max_len) len = 0;  // reported by the merge
+  pdl_wait();
+  pdl_trigger();
   if (static_cast<int>(blockIdx.x) * 1024 >= len) return;
   const int rows = a.L * a.group;
   const int64_t head = static_cast<int64_t>(b) * a.nkv + kvh;
@@ -626,6 +636,8 @@ __global__ void __launch_bounds__(256) slot_weight_kernel(const CacheAttnArgs a)
 __global__ void __launch_bounds__(kTcKeys) slot_weight_sum_kernel(const TcWeightArgs a) {
   const int b = blockIdx.z, kvh = blockIdx.y, flat = b * a.key_tiles + blockIdx.x;
   const int tiles = a.tiles(flat);
+  pdl_wait();
+  pdl_trigger();
   if (tiles == 0) return;
   const int per = tc_places_per_worker(a, tc_places_before(a, a.items()) * a.nkv);
   const int first = tc_places_before(a, flat) * a.nkv + kvh * (tiles + TcWeightArgs::kItemCost) + TcWeightArgs::kItemCost;
@@ -657,10 +669,14 @@ CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_l
                               int num_sms) {
   CacheAttnPlan p;
   const int64_t group = nh / nkv, rows_s = L * group, rows_p = B * rows_s;
-  // up to one warp tile of rows the split kernel reads each key once with no row to spare for
-  // the tensor pipe's 128; above it attn_tc_kernel does
-  p.tc_p = prefix_len > 0 && rows_p > kAttnRowTile;
-  p.tc_s = own && rows_s > kAttnRowTile;
+  // Few rows to a key: attn_split_kernel, whose workers are warps, so that short pieces start and end
+  // quickly (its row tiles past the first read the keys from L2 again).  More: attn_tc_kernel.
+  // Whole calls, prefix by the one / by the other, 200 tokens of own cache: 32 rows (32
+  // sequences of 16/16 heads, 4096 shared) 39 / 48 us, 64 rows (64 sequences) 61 / 70 us, 64 rows
+  // (8 sequences of 32/4 heads, 16384 shared) 37 / 35 us, 128 rows (16 sequences, 8192) 32 / 33 us.
+  p.tc_p = prefix_len > 0 && rows_p > kAttnSplitRows;
+  // with slot weights the split kernel also leaves 4 bytes a row and slot: for one row tile only
+  p.tc_s = own && rows_s > (scored ? kAttnRowTile : kAttnSplitRows);
   if (prefix_len > 0 && !p.tc_p) p.rt_p = static_cast<int>((rows_p + kAttnRowTile - 1) / kAttnRowTile);
   if (own && !p.tc_s) p.rt_s = static_cast<int>((rows_s + kAttnRowTile - 1) / kAttnRowTile);
   if (p.rt_p || p.rt_s) p.workers = num_sms * kAttnBlocksPerSm * kAttnWarps;
@@ -696,28 +712,19 @@ static cudaError_t launch_cache_attn_d(const CacheAttnArgs& a, const TcAttnArgs&
   cudaError_t e = cudaSuccess;
   if (p.workers) e = launch_attn_tc(p, D, mp.k, mp.v, st);
   if (e == cudaSuccess && s.workers) e = launch_attn_tc(s, D, ms.k, ms.v, st);
+  if (e == cudaSuccess && a.workers)
+    e = launch_pdl(attn_split_kernel<D>, a.workers / kAttnWarps, kAttnWarps * 32, attn_split_smem(D), st, a);
   if (e != cudaSuccess) return e;
-  if (a.workers) {
-    attn_split_kernel<D><<<a.workers / kAttnWarps, kAttnWarps * 32, attn_split_smem(D), st>>>(a);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-  }
   if (s.workers && s.direct) {
-    if (s.workers > 1) attn_merge_cut_kernel<D><<<dim3(s.workers - 1, 16), 128, 0, st>>>(a, s);
+    if (s.workers > 1) e = launch_pdl(attn_merge_cut_kernel<D>, dim3(s.workers - 1, 16), 128, 0, st, a, s);
   } else {
     const dim3 rows((a.L * a.group + a.merge_rows - 1) / a.merge_rows, a.nkv, a.B);
-    attn_merge_kernel<D><<<rows, 128, 0, st>>>(a, p, s);
+    e = launch_pdl(attn_merge_kernel<D>, rows, 128, 0, st, a, p, s);
   }
-  e = cudaGetLastError();
   if (e != cudaSuccess || !a.acc) return e;
-  if (w.workers) {
-    e = launch_slot_weight_tc(w, D, ms.k, ms.q, st);
-    if (e != cudaSuccess) return e;
-    slot_weight_sum_kernel<<<dim3(w.key_tiles, a.nkv, a.B), kTcKeys, 0, st>>>(w);
-    return cudaGetLastError();
-  }
-  slot_weight_kernel<<<dim3((a.max_len + 1023) / 1024, a.nkv, a.B), 256, 0, st>>>(a);
-  return cudaGetLastError();
+  if (!w.workers) return launch_pdl(slot_weight_kernel, dim3((a.max_len + 1023) / 1024, a.nkv, a.B), 256, 0, st, a);
+  e = launch_slot_weight_tc(w, D, ms.k, ms.q, st);
+  return e == cudaSuccess ? launch_pdl(slot_weight_sum_kernel, dim3(w.key_tiles, a.nkv, a.B), kTcKeys, 0, st, w) : e;
 }
 
 cudaError_t launch_cache_attn(const CacheAttnArgs& a, const TcAttnArgs& p, const TcMapsKV& mp, const TcAttnArgs& s,
@@ -799,6 +806,8 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t bh = blockIdx.x;
   const int b = static_cast<int>(bh / a.nkv);
+  pdl_wait();
+  pdl_trigger();
   int len = a.lens[b];
   if (len < 0 || len > a.max_len) {
     if (threadIdx.x == 0) report(a.err, DEVERR_BOUNDS);
@@ -948,6 +957,8 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
 
 __global__ void __launch_bounds__(256) evict_move_kernel(const EvictArgs a) {
   const int64_t bh = blockIdx.y;
+  pdl_wait();
+  pdl_trigger();
   const int cnt = a.counts[2 * bh];
   if (blockIdx.x == 0 && threadIdx.x == 0 && bh % a.nkv == 0) a.out_lens[bh / a.nkv] = a.counts[2 * bh + 1];
   const int32_t* list_dst = a.list + bh * 2 * a.budget;
@@ -965,13 +976,12 @@ cudaError_t launch_evict(EvictArgs a, bool lens_apart, int num_sms, cudaStream_t
   // a step that is a few slots over: no second launch (unless out_lens is lens, which other blocks
   // of the sequence may not have read yet)
   a.fused = a.in_place && most <= kEvictFused && lens_apart;
-  evict_select_kernel<<<static_cast<unsigned>(heads), kEvictThreads, a.keys_in_smem ? 4 * a.max_len : 0, st>>>(a);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_pdl(evict_select_kernel, static_cast<unsigned>(heads), kEvictThreads,
+                                   a.keys_in_smem ? 4 * a.max_len : 0, st, a);
   if (e != cudaSuccess || a.fused) return e;
   const int64_t want = std::max<int64_t>(1, (num_sms * 8 + heads - 1) / heads);
   const unsigned gx = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((most + 31) / 32, want)));
-  evict_move_kernel<<<dim3(gx, static_cast<unsigned>(heads)), 256, 0, st>>>(a);
-  return cudaGetLastError();
+  return launch_pdl(evict_move_kernel, dim3(gx, static_cast<unsigned>(heads)), 256, 0, st, a);
 }
 
 }  // namespace fm
