@@ -32,7 +32,7 @@ cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem,
 
 constexpr int kRopeMaxDim = 256;  // largest head size of the rotary kernels
 
-struct RopeArgs {
+struct RopeBase {
   const uint16_t* q;        // [T, q_ld]: nq heads of d
   uint16_t* q_out;          // [T, qo_ld]
   int64_t q_ld, qo_ld;
@@ -48,8 +48,16 @@ struct RopeArgs {
   int tpb;                  // tokens of a CTA
   float factor;             // on cos and sin
   uint32_t* err;
-  double turns[kRopeMaxDim / 2];  // full turns per position of each pair
 };
+
+// with the full turns per position of each pair (the kernel's argument: half the heads' bytes where
+// they fit, since the launch copies it)
+template <int PAIRS>
+struct RopeSet : RopeBase {
+  double turns[PAIRS];
+};
+using RopeArgs = RopeSet<kRopeMaxDim / 2>;
+
 
 // Attention over caches is split over keys.  A source of keys -- the shared prefix, or the
 // sequences' own caches -- is read by one of two kernels:
@@ -307,7 +315,7 @@ struct EvictArgs {
   uint32_t* err;
 };
 
-cudaError_t launch_rope(RopeArgs a, int num_sms, cudaStream_t st);
+cudaError_t launch_rope(RopeArgs& a, int num_sms, cudaStream_t st);
 cudaError_t serve_init();
 // p, s: the prefix / own caches by attn_tc_kernel where their workers are set, with its maps
 struct TcMapsKV {

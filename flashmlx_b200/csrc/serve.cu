@@ -7,6 +7,7 @@
 // own cache (scheduler.cpp:121-168), caches bounded by max_context_len.
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 
 #include "fm_serve.cuh"
 
@@ -37,7 +38,7 @@ struct RopeRow {
   bool rot;
 };
 
-FM_DEV bool rope_row(const RopeArgs& a, int64_t t, int hs, RopeRow& r) {
+FM_DEV bool rope_row(const RopeBase& a, int64_t t, int hs, RopeRow& r) {
   if (hs < a.nq) {
     r.src = a.q + t * a.q_ld + static_cast<int64_t>(hs) * a.d;
     r.dst = a.q_out + t * a.qo_ld + static_cast<int64_t>(hs) * a.d;
@@ -64,8 +65,8 @@ FM_DEV bool rope_row(const RopeArgs& a, int64_t t, int hs, RopeRow& r) {
 
 // VEC: the rotated part splits into whole 16-byte chunks (half: rotary / 2 a multiple of 8,
 // traditional: rotary a multiple of 8); otherwise elements are taken pair by pair.
-template <bool TRADITIONAL, bool VEC>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
+template <bool TRADITIONAL, bool VEC, int PAIRS>
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeSet<PAIRS> a) {
   extern __shared__ float2 s_cs[];  // [tpb][rotary / 2]
   pdl_wait();
   pdl_trigger();
@@ -161,15 +162,24 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
   }
 }
 
-cudaError_t launch_rope(RopeArgs a, int num_sms, cudaStream_t st) {
+template <int PAIRS>
+static cudaError_t launch_rope_set(const RopeSet<PAIRS>& a, unsigned grid, cudaStream_t st) {
+  const size_t smem = sizeof(float2) * a.tpb * (a.rotary / 2);
+  const bool vec = a.traditional ? a.rotary % 8 == 0 : (a.rotary / 2) % 8 == 0;
+  void (*kernel)(RopeSet<PAIRS>) = a.traditional ? (vec ? rope_kernel<true, true, PAIRS> : rope_kernel<true, false, PAIRS>)
+                                                 : (vec ? rope_kernel<false, true, PAIRS> : rope_kernel<false, false, PAIRS>);
+  return launch_pdl(kernel, grid, kRopeThreads, smem, st, a);
+}
+
+cudaError_t launch_rope(RopeArgs& a, int num_sms, cudaStream_t st) {
   // few tokens: one per CTA (latency); many: four share the cos / sin set-up's barrier
   a.tpb = a.T >= 8ll * num_sms ? 4 : 1;
   const unsigned grid = static_cast<unsigned>((a.T + a.tpb - 1) / a.tpb);
-  const size_t smem = sizeof(float2) * a.tpb * (a.rotary / 2);
-  const bool vec = a.traditional ? a.rotary % 8 == 0 : (a.rotary / 2) % 8 == 0;
-  void (*kernel)(RopeArgs) = a.traditional ? (vec ? rope_kernel<true, true> : rope_kernel<true, false>)
-                                           : (vec ? rope_kernel<false, true> : rope_kernel<false, false>);
-  return launch_pdl(kernel, grid, kRopeThreads, smem, st, a);
+  if (a.rotary > kRopeMaxDim / 2) return launch_rope_set(a, grid, st);
+  RopeSet<kRopeMaxDim / 4> b;
+  static_cast<RopeBase&>(b) = a;
+  std::memcpy(b.turns, a.turns, sizeof(b.turns));
+  return launch_rope_set(b, grid, st);
 }
 
 // ------------------------------------------------------------------ attention, split over keys
@@ -459,34 +469,38 @@ struct RowJoin {
   // U: pieces whose loads are in flight together
   template <int U>
   FM_DEV void add_by(const float* part_o, const float2* part_ml, int64_t row0, int step, int n) {
-    const int lane = threadIdx.x & 31;
     for (int i0 = 0; i0 < n; i0 += U) {
       float2 ml[U];
       float v[U][V];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t pr = row0 + static_cast<int64_t>(min(i0 + u, n - 1)) * step;
-        ml[u] = part_ml[pr];
-        const float* po = part_o + pr * D + lane * V;
-        if (V == 4) {
-          const float4 t4 = *reinterpret_cast<const float4*>(po);
-          v[u][0] = t4.x; v[u][1] = t4.y; v[u][2 % V] = t4.z; v[u][3 % V] = t4.w;
-        } else {
-          const float2 t2 = *reinterpret_cast<const float2*>(po);
-          v[u][0] = t2.x; v[u][1] = t2.y;
-        }
-      }
+      for (int u = 0; u < U; ++u)
+        load(part_o, part_ml, row0 + static_cast<int64_t>(min(i0 + u, n - 1)) * step, ml[u], v[u]);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (i0 + u >= n || ml[u].y == 0.f) continue;  // the piece's keys are all hidden from this row
-        const float mn = fmaxf(M, ml[u].x);
-        const float wa = exp2f(M - mn), wb = exp2f(ml[u].x - mn);
-        M = mn;
-        S = S * wa + ml[u].y * wb;
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] = acc[e] * wa + v[u][e] * wb;
-      }
+      for (int u = 0; u < U; ++u)
+        if (i0 + u < n) join(ml[u], v[u]);
     }
+  }
+
+  FM_DEV void load(const float* part_o, const float2* part_ml, int64_t pr, float2& ml, float (&v)[V]) const {
+    const float* po = part_o + pr * D + (threadIdx.x & 31) * V;
+    ml = part_ml[pr];
+    if (V == 4) {
+      const float4 t4 = *reinterpret_cast<const float4*>(po);
+      v[0] = t4.x; v[1] = t4.y; v[2 % V] = t4.z; v[3 % V] = t4.w;
+    } else {
+      const float2 t2 = *reinterpret_cast<const float2*>(po);
+      v[0] = t2.x; v[1] = t2.y;
+    }
+  }
+
+  FM_DEV void join(const float2& ml, const float (&v)[V]) {
+    if (ml.y == 0.f) return;  // the piece's keys are all hidden from this row
+    const float mn = fmaxf(M, ml.x);
+    const float wa = exp2f(M - mn), wb = exp2f(ml.x - mn);
+    M = mn;
+    S = S * wa + ml.y * wb;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = acc[e] * wa + v[e] * wb;
   }
 
   // row r of (sequence b, kv head kvh)
@@ -584,14 +598,31 @@ __global__ void __launch_bounds__(128) attn_merge_cut_kernel(const CacheAttnArgs
   if (!tc_locate(ts, place, flat, kvh, at)) return;
   const int first = place - at + kCost, tiles = ts.tiles(flat);
   if (first >= place || first / per != static_cast<int>(blockIdx.x)) return;
-  const int w1 = (first + tiles - 1) / per;
+  const int w1 = (first + tiles - 1) / per, n = w1 - static_cast<int>(blockIdx.x) + 1;
   const int b = flat / ts.rps, row0 = (flat - b * ts.rps) * kTcRows;
   const int rows = min(a.L * a.group - row0, kTcRows);
-  const int64_t slot = blockIdx.x + static_cast<int64_t>(flat) * ts.nkv + kvh;
-  for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < rows; r += 4 * gridDim.y) {
-    RowJoin<D> row;
-    row.add(ts.part_o, ts.part_ml, slot * kTcRows + r, kTcRows, w1 - static_cast<int>(blockIdx.x) + 1);
-    row.store(a, b, kvh, row0 + r);
+  const int64_t slot = (blockIdx.x + static_cast<int64_t>(flat) * ts.nkv + kvh) * kTcRows;
+  constexpr int R = 4;  // rows of a warp at a time: their pieces' loads are in flight together
+  for (int r = (blockIdx.y * 4 + (threadIdx.x >> 5)) * R; r < rows; r += 4 * R * gridDim.y) {
+    RowJoin<D> row[R];
+    if (n == 2) {  // nearly every cut
+      float2 ml[R][2];
+      float v[R][2][RowJoin<D>::V];
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) row[i].load(ts.part_o, ts.part_ml, slot + u * kTcRows + min(r + i, rows - 1), ml[i][u], v[i][u]);
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) row[i].join(ml[i][u], v[i][u]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < R; ++i) row[i].add(ts.part_o, ts.part_ml, slot + min(r + i, rows - 1), kTcRows, n);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (r + i < rows) row[i].store(a, b, kvh, row0 + r + i);
   }
 }
 
@@ -716,7 +747,7 @@ static cudaError_t launch_cache_attn_d(const CacheAttnArgs& a, const TcAttnArgs&
     e = launch_pdl(attn_split_kernel<D>, a.workers / kAttnWarps, kAttnWarps * 32, attn_split_smem(D), st, a);
   if (e != cudaSuccess) return e;
   if (s.workers && s.direct) {
-    if (s.workers > 1) e = launch_pdl(attn_merge_cut_kernel<D>, dim3(s.workers - 1, 16), 128, 0, st, a, s);
+    if (s.workers > 1) e = launch_pdl(attn_merge_cut_kernel<D>, dim3(s.workers - 1, 4), 128, 0, st, a, s);
   } else {
     const dim3 rows((a.L * a.group + a.merge_rows - 1) / a.merge_rows, a.nkv, a.B);
     e = launch_pdl(attn_merge_kernel<D>, rows, 128, 0, st, a, p, s);

@@ -595,13 +595,13 @@ def _rope_config(d, theta, rotary_dim, traditional, scaling) -> _lib.RopeConfig:
                            None if scaling is None else tuple(sorted(scaling.items())))
 
 
-def _heads_ld(t, name, dev, shape, step):
-    """Checks [..., heads, d] bf16 on `dev` whose heads lie side by side in each token's row (`shape`
-    and `step` are t's sizes and strides); returns the elements from one token's row to the next
-    (leading axes must be one stride apart, in order)."""
-    if t.dtype is not _BF or t.device != dev:
-        if t.device != dev:
-            raise ValueError(f"{name} must live on {dev}")
+def _heads_ld(t, name, index, shape, step):
+    """Checks [..., heads, d] bf16 on CUDA device `index` whose heads lie side by side in each token's
+    row (`shape` and `step` are t's sizes and strides); returns the elements from one token's row
+    to the next (leading axes must be one stride apart, in order)."""
+    if t.get_device() != index:
+        raise ValueError(f"{name} must live on CUDA device {index}")
+    if t.dtype is not _BF:
         raise ValueError(f"{name} has dtype {t.dtype}, expected torch.bfloat16")
     n = len(shape)
     if n < 3:
@@ -623,19 +623,20 @@ def _heads_ld(t, name, dev, shape, step):
     return h * d if ld is None else ld
 
 
-def _cuda_tensor(t, name):
+def _cuda_index(t, name):
+    """The CUDA device a tensor is on."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor")
-    dev = t.device
-    if dev.type != "cuda":
+    index = t.get_device() if t.is_cuda else -1
+    if index < 0:
         raise ValueError(f"{name} must live on a CUDA device")
-    return dev
+    return index
 
 
-def _packed(t, name, dtype, dev):
-    """A contiguous tensor of `dtype` on `dev`: its data pointer."""
-    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != dev or not t.is_contiguous():
-        _need(t, name, (dtype,), dev)
+def _packed(t, name, dtype, index):
+    """A contiguous tensor of `dtype` on CUDA device `index`: its data pointer."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():
+        _need(t, name, (dtype,), torch.device("cuda", index))
     return t.data_ptr()
 
 
@@ -647,7 +648,7 @@ def rope(x, positions, theta, rotary_dim=None, traditional=False, scaling=None, 
     "type" and "factor": "linear", "ntk", "yarn" (original_len, beta_slow, beta_fast) or
     "banded" (original_len, low_freq, high_freq), and optionally attn_factor.  x and out may
     be views of wider rows (a fused projection's)."""
-    dev = _cuda_tensor(x, "x")
+    dev = _cuda_index(x, "x")
     shape = x.shape
     ld = _heads_ld(x, "x", dev, shape, x.stride())
     pos = _packed(positions, "positions", torch.int32, dev)
@@ -655,14 +656,14 @@ def rope(x, positions, theta, rotary_dim=None, traditional=False, scaling=None, 
         raise ValueError("positions must have x's shape without heads and head size")
     cfg = _rope_config(shape[-1], theta, rotary_dim, traditional, scaling)
     if out is None:
-        out = torch.empty_like(x) if x.is_contiguous() else torch.empty(shape, dtype=_BF, device=dev)
+        out = torch.empty_like(x) if x.is_contiguous() else torch.empty(shape, dtype=_BF, device=torch.device("cuda", dev))
         out_ld = shape[-2] * shape[-1]
     else:
-        _cuda_tensor(out, "out")
+        _cuda_index(out, "out")
         out_ld = _heads_ld(out, "out", dev, out.shape, out.stride())
         if out.shape != shape:
             raise ValueError("out has another shape than x")
-    h = handle or default_handle(dev.index)
+    h = handle or default_handle(dev)
     h.bind_current()
     st = h.lib.fm_rope(h.h, cfg, x.data_ptr(), ld, shape[-2], pos, positions.numel(), out.data_ptr(), out_ld)
     if st:
@@ -676,9 +677,9 @@ def rope_append(q, k, v, positions, slots, cache_k, cache_v, theta, traditional=
     separate) with T = B * L tokens in sequence order: returns q rotated at positions [T] (in
     `out` if given, which may be q); k rotated and v go into the caches [B, n_kv, max_len, d]
     at slots [T] (a negative slot writes nothing; a sequence's slots must differ)."""
-    dev = _cuda_tensor(q, "q")
-    _cuda_tensor(k, "k")
-    _cuda_tensor(v, "v")
+    dev = _cuda_index(q, "q")
+    if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
+        raise TypeError("k and v must be torch tensors")
     q_shape, k_shape, c_shape = q.shape, k.shape, cache_k.shape
     ld = _heads_ld(q, "q", dev, q_shape, q.stride())
     kv_ld = _heads_ld(k, "k", dev, k_shape, k.stride())
@@ -694,14 +695,14 @@ def rope_append(q, k, v, positions, slots, cache_k, cache_v, theta, traditional=
         raise ValueError("q, k, v, positions and slots must hold the same T = B * L tokens")
     cfg = _rope_config(d, theta, rotary_dim, traditional, scaling)
     if out is None:
-        out = torch.empty(q_shape, dtype=_BF, device=dev)
+        out = torch.empty(q_shape, dtype=_BF, device=torch.device("cuda", dev))
         out_ld = nh * d
     else:
-        _cuda_tensor(out, "out")
+        _cuda_index(out, "out")
         out_ld = _heads_ld(out, "out", dev, out.shape, out.stride())
         if out.shape != q_shape:
             raise ValueError("out has another shape than q")
-    h = handle or default_handle(dev.index)
+    h = handle or default_handle(dev)
     h.bind_current()
     st = h.lib.fm_rope_append(h.h, cfg, q.data_ptr(), ld, nh, k.data_ptr(), v.data_ptr(), kv_ld, k_shape[-2], pos, slot, B,
                               T // B, ck, cv, c_shape[2], out.data_ptr(), out_ld)
@@ -711,7 +712,7 @@ def rope_append(q, k, v, positions, slots, cache_k, cache_v, theta, traditional=
 
 
 def _cache_attn(q, prefix_k, prefix_v, prefix_len, cache_k, cache_v, lens, acc, scale, handle):
-    dev = _cuda_tensor(q, "q")
+    dev = _cuda_index(q, "q")
     q_shape = q.shape
     ld = _heads_ld(q, "q", dev, q_shape, q.stride())
     if len(q_shape) != 4:
@@ -743,9 +744,9 @@ def _cache_attn(q, prefix_k, prefix_v, prefix_len, cache_k, cache_v, lens, acc, 
             raise ValueError("prefix_len is not within the prefix")
     if nkv == 0 or nh % nkv:
         raise ValueError("n_heads must be a multiple of n_kv")
-    out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q_shape, dtype=_BF, device=dev)
+    out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q_shape, dtype=_BF, device=torch.device("cuda", dev))
     cfg = _lib.CacheAttnConfig(nh, nkv, d, max_len, prefix_max, ld, scale)
-    h = handle or default_handle(dev.index)
+    h = handle or default_handle(dev)
     h.bind_current()
     if acc is None:
         st = h.lib.fm_attention_prefix(h.h, cfg, q.data_ptr(), pk, pv, prefix_len or 0, ck, cv, n, B, L, out.data_ptr())
@@ -786,7 +787,7 @@ def cache_evict(cache_k, cache_v, acc, lens, budget, sinks=0, recent=0, position
     out = (k, v, acc, positions) of [B, n_kv, M >= budget, ...] (positions may be None when
     `positions` is).  Slots that stay below n keep their places, the others below n take those
     from n on in order.  Returns the new lengths [B] (lens_out if given; it may be lens)."""
-    dev = _cuda_tensor(cache_k, "cache_k")
+    dev = _cuda_index(cache_k, "cache_k")
     shape = cache_k.shape
     ck, cv = _packed(cache_k, "cache_k", _BF, dev), _packed(cache_v, "cache_v", _BF, dev)
     if len(shape) != 4 or cache_v.shape != shape:
@@ -814,7 +815,7 @@ def cache_evict(cache_k, cache_v, acc, lens, budget, sinks=0, recent=0, position
     if lens.shape != (B,) or lens_out.shape != (B,):
         raise ValueError("lens and lens_out must be [B]")
     cfg = _lib.EvictConfig(nkv, d, max_len, rows, budget, sinks, recent)
-    h = handle or default_handle(dev.index)
+    h = handle or default_handle(dev)
     h.bind_current()
     st = h.lib.fm_cache_evict(h.h, cfg, ck, cv, a, p, n, B, ok, ov, oa, op, no)
     if st:
