@@ -2319,9 +2319,9 @@ int fm_rope_append(fm_handle* h, const fm_rope_config* cfg, const uint16_t* q, i
   const int64_t out_bytes = 2 * ((T - 1) * q_out_ld + cols);
   if (!(q == q_out && q_ld == q_out_ld) && overlap(q, 2 * ((T - 1) * q_ld + cols), q_out, out_bytes))
     return set_err(h, FM_EINVAL, "q_out must be q or not overlap it");
+  const OnDevice on(h);
   rc = ensure_sv(h, 0);
   if (rc != FM_OK) return rc;
-  const OnDevice on(h);
   a.q = q;
   a.q_ld = q_ld;
   a.q_out = q_out;
@@ -2366,6 +2366,7 @@ int fm_cache_evict(fm_handle* h, const fm_evict_config* c, const uint16_t* cache
     return set_err(h, FM_EINVAL, "bad eviction config (budget >= 1, 0 <= sinks + recent <= budget)");
   if (c->head_dim % 8 || c->head_dim > 256)
     return set_err(h, FM_EUNSUPPORTED, "head_dim must be a multiple of 8, at most 256");
+  if (c->max_len > 1 << 20) return set_err(h, FM_EUNSUPPORTED, "max_len must be at most 2^20");
   const int budget = std::min(c->budget, c->max_len);
   if (c->out_max_len < budget) return set_err(h, FM_EINVAL, "out_max_len is below the budget");
   const int64_t heads = static_cast<int64_t>(B) * c->n_kv_heads;
@@ -2428,9 +2429,9 @@ int fm_serve_reserve(fm_handle* h, const fm_cache_attn_config* cfg, int B, int L
   const int rc = check_cache_attn(h, cfg, B, L, 0);
   if (rc != FM_OK) return rc;
   const OnDevice on(h);
-  const fm::CacheAttnPlan p =
-      fm::cache_attn_plan(B, L, cfg->n_heads, cfg->n_kv_heads, cfg->head_dim, cfg->prefix_max, true, true, cfg->max_len, h->num_sms);
-  return ensure_sv(h, std::max(p.bytes, evict_bytes(static_cast<int64_t>(B) * cfg->n_kv_heads, cfg->max_len)));
+  const size_t attn = fm::cache_attn_bound(B, L, cfg->n_heads, cfg->n_kv_heads, cfg->head_dim, cfg->prefix_max,
+                                           cfg->max_len, h->num_sms);
+  return ensure_sv(h, std::max(attn, evict_bytes(static_cast<int64_t>(B) * cfg->n_kv_heads, cfg->max_len)));
 }
 
 }  // extern "C"

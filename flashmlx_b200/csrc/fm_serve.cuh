@@ -72,6 +72,8 @@ using RopeArgs = RopeSet<kRopeMaxDim / 2>;
 // ragged lengths balance.  A worker's piece of an item leaves an unnormalised fp32 output,
 // its maximum (log2 units) and its sum in slot worker + item -- both only grow along the
 // order, so no two pieces share a slot -- and attn_merge_kernel joins an output row's pieces.
+// (Where whole items go to the output at once, a worker leaves at most two pieces: slots
+// 2 worker for the item that it goes on with, 2 worker + 1 for the one that it begins.)
 constexpr int kAttnTile = 16;        // keys of a tile
 constexpr int kAttnRowTile = 16;     // query rows of an item
 constexpr int kAttnSplitRows = 64;   // up to so many query rows to a key the split kernel reads it
@@ -125,7 +127,7 @@ struct TcAttnArgs {
   int direct;               // the only source: an item that one worker has whole goes to out
   float scale_log2;         // >= 0
   uint32_t q_sign;          // 0x80008000: q is negated (a negative scale)
-  float* part_o;            // [workers + items][256][d]
+  float* part_o;            // [slots][256][d]
   float2* part_ml;
   uint16_t* out;
   float* lse2;
@@ -294,6 +296,9 @@ struct CacheAttnPlan {
 };
 CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_len, bool own, bool scored, int max_len,
                               int num_sms);
+
+// At least what any call of up to B sequences of L tokens over such a prefix and caches needs.
+size_t cache_attn_bound(int B, int L, int nh, int nkv, int d, int prefix_max, int max_len, int num_sms);
 
 struct EvictArgs {
   const uint16_t* cache_k;  // [B, nkv, max_len, d]

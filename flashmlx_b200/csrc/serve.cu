@@ -601,7 +601,8 @@ __global__ void __launch_bounds__(128) attn_merge_cut_kernel(const CacheAttnArgs
   const int w1 = (first + tiles - 1) / per, n = w1 - static_cast<int>(blockIdx.x) + 1;
   const int b = flat / ts.rps, row0 = (flat - b * ts.rps) * kTcRows;
   const int rows = min(a.L * a.group - row0, kTcRows);
-  const int64_t slot = (blockIdx.x + static_cast<int64_t>(flat) * ts.nkv + kvh) * kTcRows;
+  // the first worker's piece in its slot 2 w + 1, the next ones' in their slots 2 w
+  const int64_t slot0 = (2 * static_cast<int64_t>(blockIdx.x) + 1) * kTcRows, slot1 = slot0 + kTcRows;
   constexpr int R = 4;  // rows of a warp at a time: their pieces' loads are in flight together
   for (int r = (blockIdx.y * 4 + (threadIdx.x >> 5)) * R; r < rows; r += 4 * R * gridDim.y) {
     RowJoin<D> row[R];
@@ -611,14 +612,17 @@ __global__ void __launch_bounds__(128) attn_merge_cut_kernel(const CacheAttnArgs
 #pragma unroll
       for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) row[i].load(ts.part_o, ts.part_ml, slot + u * kTcRows + min(r + i, rows - 1), ml[i][u], v[i][u]);
+        for (int u = 0; u < 2; ++u) row[i].load(ts.part_o, ts.part_ml, (u ? slot1 : slot0) + min(r + i, rows - 1), ml[i][u], v[i][u]);
 #pragma unroll
       for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int u = 0; u < 2; ++u) row[i].join(ml[i][u], v[i][u]);
     } else {
 #pragma unroll
-      for (int i = 0; i < R; ++i) row[i].add(ts.part_o, ts.part_ml, slot + min(r + i, rows - 1), kTcRows, n);
+      for (int i = 0; i < R; ++i) {
+        row[i].add(ts.part_o, ts.part_ml, slot0 + min(r + i, rows - 1), kTcRows, 1);
+        row[i].add(ts.part_o, ts.part_ml, slot1 + min(r + i, rows - 1), 2 * kTcRows, n - 1);
+      }
     }
 #pragma unroll
     for (int i = 0; i < R; ++i)
@@ -719,22 +723,38 @@ CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_l
   const size_t rows = p.workers ? (p.workers + static_cast<size_t>(nkv) * (p.rt_p + static_cast<size_t>(B) * p.rt_s)) * kAttnRowTile : 0;
   add(rows * d * sizeof(float));
   p.off_ml = add(rows * sizeof(float2));
-  auto tc = [&](bool on, int64_t nseq, int64_t item_rows, int& rps, int& workers, size_t& off_o, size_t& off_ml) {
+  auto tc = [&](bool on, bool direct, int64_t nseq, int64_t item_rows, int& rps, int& workers, size_t& off_o, size_t& off_ml) {
     if (!on) return;
     rps = static_cast<int>((item_rows + kTcRows - 1) / kTcRows);
     workers = num_sms;
-    const size_t n = (workers + static_cast<size_t>(nseq) * rps * nkv) * kTcRows;
+    const size_t n = (direct ? 2 * workers : workers + static_cast<size_t>(nseq) * rps * nkv) * kTcRows;
     off_o = add(n * d * sizeof(float));
     off_ml = add(n * sizeof(float2));
   };
-  tc(p.tc_p, 1, rows_p, p.rps_p, p.workers_p, p.off_po, p.off_pml);
-  tc(p.tc_s, B, rows_s, p.rps_s, p.workers_s, p.off_so, p.off_sml);
+  tc(p.tc_p, false, 1, rows_p, p.rps_p, p.workers_p, p.off_po, p.off_pml);
+  tc(p.tc_s, prefix_len == 0, B, rows_s, p.rps_s, p.workers_s, p.off_so, p.off_sml);
   if (B * nkv * ((rows_s + 15) / 16) < 8ll * num_sms) p.merge_rows = 4;
   p.off_lse = add(scored ? sizeof(float) * B * L * nh : 0);
   const size_t key_items = static_cast<size_t>(B) * nkv * ((max_len + kTcKeys - 1) / kTcKeys);
   p.off_scores = add(scored && !p.tc_s ? sizeof(float) * B * nkv * rows_s * (static_cast<size_t>(max_len) + 3) / 4 * 4 : 0);
   p.off_w = add(scored && p.tc_s ? (num_sms + key_items) * kTcWeightParts * kTcKeys * sizeof(float) : 0);
   return p;
+}
+
+size_t cache_attn_bound(int B, int L, int nh, int nkv, int d, int prefix_max, int max_len, int num_sms) {
+  // every part at its largest: both kernels' pieces, the log sums, the scores of one row tile, the
+  // slot weights' sums
+  const size_t group = nh / nkv, rows_s = L * group, rows_p = B * rows_s;
+  auto up = [](size_t n, size_t m) { return (n + m - 1) / m; };
+  const size_t split = num_sms * kAttnBlocksPerSm * kAttnWarps +
+                       nkv * (up(std::min<size_t>(rows_p, kAttnSplitRows), kAttnRowTile) +
+                              B * up(std::min<size_t>(rows_s, kAttnSplitRows), kAttnRowTile));
+  const size_t tc = 4 * num_sms + nkv * (up(rows_p, kTcRows) + B * up(rows_s, kTcRows));
+  const size_t piece_rows = split * kAttnRowTile + tc * kTcRows;
+  const size_t key_items = static_cast<size_t>(B) * nkv * up(max_len, kTcKeys);
+  return piece_rows * (d * sizeof(float) + sizeof(float2)) + sizeof(float) * rows_p * nkv +
+         sizeof(float) * B * nkv * std::min<size_t>(rows_s, kAttnRowTile) * (max_len + 3) +
+         (num_sms + key_items) * kTcWeightParts * kTcKeys * sizeof(float) + (prefix_max >= 0 ? 4096 : 0);
 }
 
 template <int D>
@@ -772,7 +792,9 @@ cudaError_t launch_cache_attn(const CacheAttnArgs& a, const TcAttnArgs& p, const
 // itself.  In place only the holes below n are filled, by the kept slots from n on, both in
 // ascending order: sources >= n, destinations < n, so no move reads what another writes.
 constexpr int kEvictThreads = 1024;
-constexpr int kEvictSmemKeys = 40960;  // 160 KB beside the 32 KB of counts
+constexpr int kEvictSmemKeys = 40960;  // 160 KB
+constexpr int kEvictCopies = 8;        // of the counts: a lane's own of eight, so that a warp whose keys are
+                                       // alike does not add to one word 32 times
 constexpr int kEvictFused = 64;        // moves of a head that the select kernel makes itself
 
 namespace {
@@ -830,8 +852,10 @@ FM_DEV void evict_rows(const EvictArgs& a, int64_t bh, const int32_t* list_dst, 
 }  // namespace
 
 __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const EvictArgs a) {
-  extern __shared__ __align__(16) uint32_t s_keys[];  // [max_len] when they fit
-  __shared__ int s_hist[256 * 32];  // [bin][lane]: a lane's own bank, no conflicts
+  extern __shared__ __align__(16) uint32_t s_dyn[];  // a bit per slot that stays, then the keys when they fit
+  __shared__ __align__(16) int s_hist[256 * kEvictCopies];
+  uint32_t* s_kept = s_dyn;
+  uint32_t* s_keys = s_dyn + (a.max_len + 31) / 32;
   __shared__ int s_w[3][32];
   __shared__ int s_pick[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -860,19 +884,23 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
     return;
   }
   // the newest position held
-  int64_t newest = len - 1;
+  int newest = len - 1;
   if (pos) {
     int mx = INT32_MIN;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = threadIdx.x; i < len; i += kEvictThreads) mx = max(mx, pos[i]);
     mx = __reduce_max_sync(0xffffffffu, mx);
     if (lane == 0) s_w[0][warp] = mx;
     __syncthreads();
     newest = __reduce_max_sync(0xffffffffu, s_w[0][lane]);
   }
+  // protected: below `sinks`, or one of the `recent` positions up to the newest
+  const int64_t oldest = static_cast<int64_t>(newest) - a.recent + 1;
+  const int guard = oldest < INT32_MIN ? INT32_MIN : static_cast<int>(min(oldest, static_cast<int64_t>(INT32_MAX)));
+  const bool any = a.recent > 0;  // (oldest passes the newest when none is)
   auto make_key = [&](int i) -> uint32_t {
-    const int64_t p = pos ? pos[i] : i;
-    return p < a.sinks || p > newest - a.recent ? 0xffffffffu : order_bits(acc[i]);
+    const int p = pos ? pos[i] : i;
+    return p < a.sinks || (any && p >= guard) ? 0xffffffffu : order_bits(acc[i]);
   };
   const bool kept_here = a.keys_in_smem;
   auto key_of = [&](int i) -> uint32_t { return kept_here ? s_keys[i] : make_key(i); };
@@ -881,33 +909,33 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
   int want = n;  // of the keys that match the prefix so far
 #pragma unroll 1
   for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256 * 32 / 4; i += kEvictThreads) reinterpret_cast<int4*>(s_hist)[i] = make_int4(0, 0, 0, 0);
+    if (threadIdx.x < 256 * kEvictCopies / 4) reinterpret_cast<int4*>(s_hist)[threadIdx.x] = make_int4(0, 0, 0, 0);
     __syncthreads();
     if (shift == 24) {
-#pragma unroll 4
+#pragma unroll 8
       for (int i = threadIdx.x; i < len; i += kEvictThreads) {
         const uint32_t k = make_key(i);
         if (kept_here) s_keys[i] = k;
-        atomicAdd(&s_hist[(k >> 24) * 32 + lane], 1);
+        atomicAdd(&s_hist[(k >> 24) * kEvictCopies + lane % kEvictCopies], 1);
       }
     } else {
 #pragma unroll 4
       for (int i = threadIdx.x; i < len; i += kEvictThreads) {
         const uint32_t k = key_of(i);
-        if ((k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[((k >> shift) & 255u) * 32 + lane], 1);
+        if ((k >> (shift + 8)) == (prefix >> (shift + 8))) 
+          atomicAdd(&s_hist[((k >> shift) & 255u) * kEvictCopies + lane % kEvictCopies], 1);
       }
     }
     __syncthreads();
-    // a warp sums eight bins; bins are then walked from the largest down
-    for (int i = 0; i < 8; ++i) {
-      const int c = __reduce_add_sync(0xffffffffu, s_hist[(warp * 8 + i) * 32 + lane]);
-      if (lane == 0) s_hist[(warp * 8 + i) * 32] = c;
+    if (threadIdx.x < 256) {
+      const int4 x = reinterpret_cast<const int4*>(s_hist)[2 * threadIdx.x], y = reinterpret_cast<const int4*>(s_hist)[2 * threadIdx.x + 1];
+      s_hist[kEvictCopies * threadIdx.x] = ((x.x + x.y) + (x.z + x.w)) + ((y.x + y.y) + (y.z + y.w));
     }
     __syncthreads();
-    if (warp == 0) {  // lane l: bins 255 - 8 l down to 248 - 8 l
+    if (warp == 0) {  // the bins from the largest down; lane l: 255 - 8 l to 248 - 8 l
       int c[8], mine = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mine += c[i] = s_hist[(255 - 8 * lane - i) * 32];
+      for (int i = 0; i < 8; ++i) mine += c[i] = s_hist[(255 - 8 * lane - i) * kEvictCopies];
       int incl = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -931,51 +959,65 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
     want = s_pick[1];
   }
   // `want` of the keys equal to `prefix` stay, the lowest slots first.  A warp takes a contiguous
-  // range of slots, 32 at a time; first the equal keys are counted, then the holes below n and
-  // the kept slots from n on, then the lists are written.
-  const int per = (len + 32 * 32 - 1) / (32 * 32) * 32, i0 = warp * per, i1 = min(len, i0 + per);
+  // range of 32-slot words: first the equal keys are counted, then a bit says which slots stay, and
+  // the holes below n and the kept slots from n on are counted; then a lane lists a word's.
+  const int words = (len + 31) / 32, per = (words + 31) / 32, w0 = warp * per, w1 = min(words, w0 + per);
   int eq = 0;
-  for (int i = i0 + lane; i - lane < i1; i += 32) eq += __popc(__ballot_sync(0xffffffffu, i < i1 && key_of(i) == prefix));
+  for (int w = w0; w < w1; ++w) {
+    const int i = 32 * w + lane;
+    eq += __popc(__ballot_sync(0xffffffffu, i < len && key_of(i) == prefix));
+  }
   if (lane == 0) s_w[0][warp] = eq;
   __syncthreads();
   int all;
-  const int eq0 = warps_before(s_w[0], warp, &all);
+  eq = warps_before(s_w[0], warp, &all);
   const uint32_t below = (1u << lane) - 1;
-  int holes = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    int e = eq0, hole = 0, tail = 0, moves = 0;
-    if (pass == 1) {
-      hole = warps_before(s_w[1], warp, &moves);
-      tail = warps_before(s_w[2], warp, &all);
-    }
-    for (int i = i0 + lane; i - lane < i1; i += 32) {
-      const uint32_t k = i < i1 ? key_of(i) : 0u;
-      const bool is_eq = i < i1 && k == prefix;
-      const uint32_t eqs = __ballot_sync(0xffffffffu, is_eq);
-      const bool kept = i < i1 && (k > prefix || (is_eq && e + __popc(eqs & below) < want));
-      e += __popc(eqs);
-      const bool is_hole = i < min(n, i1) && !kept, is_tail = i >= n && kept;
-      const uint32_t hm = __ballot_sync(0xffffffffu, is_hole), tm = __ballot_sync(0xffffffffu, is_tail);
-      if (pass == 1) {
-        if (is_hole) list_dst[hole + __popc(hm & below)] = i;
-        if (is_tail) list_src[tail + __popc(tm & below)] = i;
-        // copied elsewhere, the slots that keep their places follow the moves
-        if (!a.in_place && i < n && kept) {
-          const int at = moves + i - (hole + __popc(hm & below));
-          list_dst[at] = list_src[at] = i;
-        }
+  auto under_n = [&](int w) {  // the slots of word w below n
+    const int c = n - 32 * w;
+    return c >= 32 ? 0xffffffffu : c <= 0 ? 0u : (1u << c) - 1;
+  };
+  int hole = 0, tail = 0;
+  for (int w = w0; w < w1; ++w) {
+    const int i = 32 * w + lane;
+    const uint32_t k = i < len ? key_of(i) : 0u;
+    const bool is_eq = i < len && k == prefix;
+    const uint32_t eqs = __ballot_sync(0xffffffffu, is_eq);
+    const uint32_t kept = __ballot_sync(0xffffffffu, i < len && (k > prefix || (is_eq && eq + __popc(eqs & below) < want)));
+    eq += __popc(eqs);
+    if (lane == 0) s_kept[w] = kept;
+    hole += __popc(~kept & under_n(w));
+    tail += __popc(kept & ~under_n(w));
+  }
+  if (lane == 0) {
+    s_w[1][warp] = hole;
+    s_w[2][warp] = tail;
+  }
+  __syncthreads();
+  int holes;
+  hole = warps_before(s_w[1], warp, &holes);
+  tail = warps_before(s_w[2], warp, &all);
+  for (int base = w0; base < w1; base += 32) {
+    const int w = base + lane;
+    const uint32_t kept = w < w1 ? s_kept[w] : 0u, under = w < w1 ? under_n(w) : 0u;
+    uint32_t hm = ~kept & under, tm = kept & ~under, stay = a.in_place ? 0u : kept & under;
+    int hi = __popc(hm), ti = __popc(tm);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int hu = __shfl_up_sync(0xffffffffu, hi, o), tu = __shfl_up_sync(0xffffffffu, ti, o);
+      if (lane >= o) {
+        hi += hu;
+        ti += tu;
       }
-      hole += __popc(hm);
-      tail += __popc(tm);
     }
-    if (pass == 0) {
-      if (lane == 0) {
-        s_w[1][warp] = hole;
-        s_w[2][warp] = tail;
-      }
-      __syncthreads();
-    }
-    holes = moves;
+    int at = hole + hi - __popc(hm);
+    // copied elsewhere, the slots that keep their places follow the moves
+    int to = holes + 32 * w - at;
+    for (; hm; hm &= hm - 1) list_dst[at++] = 32 * w + __ffs(hm) - 1;
+    at = tail + ti - __popc(tm);
+    for (; tm; tm &= tm - 1) list_src[at++] = 32 * w + __ffs(tm) - 1;
+    for (; stay; stay &= stay - 1, ++to) list_dst[to] = list_src[to] = 32 * w + __ffs(stay) - 1;
+    hole += __shfl_sync(0xffffffffu, hi, 31);
+    tail += __shfl_sync(0xffffffffu, ti, 31);
   }
   if (a.fused) {
     __syncthreads();  // the lists are written (and read by this block alone)
@@ -997,7 +1039,8 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const EvictArgs a) {
 }
 
 cudaError_t evict_init() {
-  return cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictSmemKeys * 4);
+  return cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              kEvictSmemKeys * 4 + kEvictSmemKeys / 8);
 }
 
 cudaError_t launch_evict(EvictArgs a, bool lens_apart, int num_sms, cudaStream_t st) {
@@ -1008,7 +1051,7 @@ cudaError_t launch_evict(EvictArgs a, bool lens_apart, int num_sms, cudaStream_t
   // of the sequence may not have read yet)
   a.fused = a.in_place && most <= kEvictFused && lens_apart;
   const cudaError_t e = launch_pdl(evict_select_kernel, static_cast<unsigned>(heads), kEvictThreads,
-                                   a.keys_in_smem ? 4 * a.max_len : 0, st, a);
+                                   (a.max_len + 31) / 32 * 4 + (a.keys_in_smem ? 4 * a.max_len : 0), st, a);
   if (e != cudaSuccess || a.fused) return e;
   const int64_t want = std::max<int64_t>(1, (num_sms * 8 + heads - 1) / heads);
   const unsigned gx = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((most + 31) / 32, want)));

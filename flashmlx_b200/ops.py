@@ -640,6 +640,16 @@ def _packed(t, name, dtype, index):
     return t.data_ptr()
 
 
+def _bound(handle, index):
+    """The handle of a call on CUDA device `index`, bound to torch's current stream there."""
+    if handle is None:
+        handle = default_handle(index)
+    elif handle.device != index:
+        raise ValueError(f"the handle is of CUDA device {handle.device}, the tensors are on {index}")
+    handle.bind_current()
+    return handle
+
+
 def rope(x, positions, theta, rotary_dim=None, traditional=False, scaling=None, out=None, handle=None) -> torch.Tensor:
     """Rotary positions (mx::fast::rope with one position per token): x [..., heads, d] bf16,
     positions int32 [...] (any int32; negative ones rotate back) -> x rotated, in `out` if given
@@ -663,8 +673,7 @@ def rope(x, positions, theta, rotary_dim=None, traditional=False, scaling=None, 
         out_ld = _heads_ld(out, "out", dev, out.shape, out.stride())
         if out.shape != shape:
             raise ValueError("out has another shape than x")
-    h = handle or default_handle(dev)
-    h.bind_current()
+    h = _bound(handle, dev)
     st = h.lib.fm_rope(h.h, cfg, x.data_ptr(), ld, shape[-2], pos, positions.numel(), out.data_ptr(), out_ld)
     if st:
         h.check(st)
@@ -691,7 +700,7 @@ def rope_append(q, k, v, positions, slots, cache_k, cache_v, theta, traditional=
     if len(c_shape) != 4 or cache_v.shape != c_shape or c_shape[3] != d or k_shape[-1] != d or k_shape[-2] != c_shape[1]:
         raise ValueError("caches must be [B, n_kv, max_len, d] with k's heads and q's head size")
     B = c_shape[0]
-    if B == 0 or T % B or slots.numel() != T or q.numel() != T * nh * d or k.numel() != T * k_shape[-2] * d:
+    if T % max(B, 1) or (B == 0 and T) or slots.numel() != T or q.numel() != T * nh * d or k.numel() != T * k_shape[-2] * d:
         raise ValueError("q, k, v, positions and slots must hold the same T = B * L tokens")
     cfg = _rope_config(d, theta, rotary_dim, traditional, scaling)
     if out is None:
@@ -702,10 +711,9 @@ def rope_append(q, k, v, positions, slots, cache_k, cache_v, theta, traditional=
         out_ld = _heads_ld(out, "out", dev, out.shape, out.stride())
         if out.shape != q_shape:
             raise ValueError("out has another shape than q")
-    h = handle or default_handle(dev)
-    h.bind_current()
+    h = _bound(handle, dev)
     st = h.lib.fm_rope_append(h.h, cfg, q.data_ptr(), ld, nh, k.data_ptr(), v.data_ptr(), kv_ld, k_shape[-2], pos, slot, B,
-                              T // B, ck, cv, c_shape[2], out.data_ptr(), out_ld)
+                              T // max(B, 1), ck, cv, c_shape[2], out.data_ptr(), out_ld)
     if st:
         h.check(st)
     return out
@@ -746,8 +754,7 @@ def _cache_attn(q, prefix_k, prefix_v, prefix_len, cache_k, cache_v, lens, acc, 
         raise ValueError("n_heads must be a multiple of n_kv")
     out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q_shape, dtype=_BF, device=torch.device("cuda", dev))
     cfg = _lib.CacheAttnConfig(nh, nkv, d, max_len, prefix_max, ld, scale)
-    h = handle or default_handle(dev)
-    h.bind_current()
+    h = _bound(handle, dev)
     if acc is None:
         st = h.lib.fm_attention_prefix(h.h, cfg, q.data_ptr(), pk, pv, prefix_len or 0, ck, cv, n, B, L, out.data_ptr())
     else:
@@ -815,8 +822,7 @@ def cache_evict(cache_k, cache_v, acc, lens, budget, sinks=0, recent=0, position
     if lens.shape != (B,) or lens_out.shape != (B,):
         raise ValueError("lens and lens_out must be [B]")
     cfg = _lib.EvictConfig(nkv, d, max_len, rows, budget, sinks, recent)
-    h = handle or default_handle(dev)
-    h.bind_current()
+    h = _bound(handle, dev)
     st = h.lib.fm_cache_evict(h.h, cfg, ck, cv, a, p, n, B, ok, ov, oa, op, no)
     if st:
         h.check(st)

@@ -408,7 +408,7 @@ FM_API int fm_attention_prefix(fm_handle* h, const fm_cache_attn_config* cfg, co
 
 /* The same without a prefix, and acc[b, kvh, j] += the sum, over kv head kvh's query heads and
  * the L tokens, of the attention probability of slot j (fp32 [B, n_kv_heads, max_len]; slots
- * at or past lens[b] are left as they were).  At most 128 query heads to a kv head. */
+ * at or past lens[b] are left as they were; a slot that a new token takes should hold 0 before its first call).  At most 128 query heads to a kv head. */
 FM_API int fm_attention_scored(fm_handle* h, const fm_cache_attn_config* cfg, const uint16_t* q,
                                const uint16_t* cache_k, const uint16_t* cache_v, const int32_t* lens, int B, int L,
                                float* acc, uint16_t* out);
@@ -416,7 +416,7 @@ FM_API int fm_attention_scored(fm_handle* h, const fm_cache_attn_config* cfg, co
 typedef struct fm_evict_config {
   int n_kv_heads;
   int head_dim;     /* a multiple of 8, at most 256 */
-  int max_len;      /* slots per (sequence, kv head) of the caches, acc and positions */
+  int max_len;      /* slots per (sequence, kv head) of the caches, acc and positions; at most 2^20 */
   int out_max_len;  /* the same of the outputs */
   int budget;       /* slots that stay, >= 1 */
   int sinks;        /* positions below it stay */
@@ -438,8 +438,8 @@ FM_API int fm_cache_evict(fm_handle* h, const fm_evict_config* cfg, const uint16
                           uint16_t* out_v, float* out_acc, int32_t* out_positions, int32_t* out_lens);
 
 /* Sizes the workspace for fm_attention_prefix / fm_attention_scored calls of up to B sequences
- * of L tokens over cfg's caches and prefix_max, and for fm_cache_evict of such a batch, so
- * that later calls do not allocate. */
+ * of up to L tokens over cfg's caches and up to prefix_max rows, and for fm_cache_evict of such a
+ * batch, so that later calls do not allocate. */
 FM_API int fm_serve_reserve(fm_handle* h, const fm_cache_attn_config* cfg, int B, int L);
 
 /* Expert parallelism ------------------------------------------------------------

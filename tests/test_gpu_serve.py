@@ -372,6 +372,8 @@ def test_attention_far_into_a_large_cache():
     (1, 2, 256, 3000, [2999], 1500, 4, 100, "rand"),
     (2, 2, 64, 5000, [5000, 1025], 1024, 0, 512, "ties"),
     (1, 1, 64, 100, [100], 200, 0, 0, "rand"),           # nothing to evict
+    (1, 1, 8, 50000, [49990], 20001, 3, 77, "rand"),     # more keys than shared memory holds
+    (1, 2, 8, 4096, [4096], 4095, 0, 4095, "ties"),      # one too many, nearly all protected
 ])
 @pytest.mark.parametrize("in_place", [True, False])
 @pytest.mark.parametrize("given", [True, False])
@@ -479,9 +481,7 @@ def test_a_captured_step_follows_its_lengths():
         q = ops.rope_append(qkv[:, :nh], qkv[:, nh:nh + nkv], qkv[:, nh + nkv:], slots, slots, ck, cv, 1e6, handle=h)
         return ops.attention_prefix(q.view(B, 1, nh, d), pk, pv, ck, cv, lens, handle=h)
 
-    cfg = _lib.CacheAttnConfig(nh, nkv, d, M, P, 0, 0.0)
-    h.check(h.lib.fm_serve_reserve(h.h, _lib.C.byref(cfg), B, 1))
-    keep = ck.clone(), cv.clone()
+    keep = ck.clone(), cv.clone()  # the step before the capture sizes the workspace
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -510,6 +510,44 @@ def test_a_captured_step_follows_its_lengths():
         slots += 1
         lens += 1
     h.sync()
+
+
+@pytest.mark.parametrize("nh,nkv,d,M,P,B,L", [(32, 4, 128, 700, 300, 9, 40), (4, 4, 64, 130, 0, 33, 3), (8, 1, 64, 2000, 5000, 1, 1)])
+def test_reserved_calls_do_not_allocate(nh, nkv, d, M, P, B, L):
+    """After fm_serve_reserve no call of up to its sizes grows the workspace."""
+    from flashmlx_b200 import _lib, ops
+    h = ops.Handle()
+    cfg = _lib.CacheAttnConfig(nh, nkv, d, M, P, 0, 0.0)
+    h.check(h.lib.fm_serve_reserve(h.h, _lib.C.byref(cfg), B, L))
+    size = h.workspace_bytes()
+    ck, cv = rnd(120, B, nkv, M, d), rnd(121, B, nkv, M, d)
+    acc = torch.zeros(B, nkv, M, device="cuda")
+    pk = rnd(122, nkv, P, d) if P else None
+    for b in sorted({1, min(2, B), B // 2, B} - {0}):
+        for n in sorted({1, min(2, L), L // 2, L} - {0}):
+            q, lens = rnd(123, b, n, nh, d), i32([M] * b)
+            ops.attention_prefix(q, pk, pk, ck[:b], cv[:b], lens, handle=h)
+            ops.attention_scored(q, ck[:b], cv[:b], lens, acc[:b], handle=h)
+    if P:
+        ops.attention_prefix(rnd(124, B, L, nh, d), pk, pk, handle=h)
+    ops.cache_evict(ck, cv, acc, i32([M] * B), M - 1, handle=h)
+    h.sync()
+    assert h.workspace_bytes() == size
+
+
+def test_negative_positions_and_their_window():
+    """recent counts from the newest position, whatever its sign; at the type's lowest value too."""
+    from flashmlx_b200 import ops
+    low = -2 ** 31
+    pos = torch.tensor([low, low + 1, low + 2, low + 3, low + 4], dtype=torch.int32).view(1, 1, 5)
+    ck, cv, acc = rnd(130, 1, 1, 5, 64), rnd(131, 1, 1, 5, 64), torch.tensor([5.0, 4, 3, 2, 1]).view(1, 1, 5)
+    host = [ck.cpu().clone(), cv.cpu().clone(), acc.clone(), pos.clone()]
+    R.evict(host[0], host[1], host[2], host[3], [5], 4, 0, 4, host)
+    dev = [ck, cv, acc.cuda(), pos.cuda()]
+    ops.cache_evict(dev[0], dev[1], dev[2], i32([5]), 4, recent=4, positions=dev[3])
+    # (every position is protected: all lie below `sinks` = 0)
+    for x, y in zip(dev, host):
+        assert torch.equal(x.cpu(), y)
 
 
 def test_two_streams_with_their_own_handles():
