@@ -47,7 +47,7 @@ struct Shape {
 };
 
 struct Bars {
-  uint64_t qfull[2], sfull[2][2], pfull[2][2], ofull, tail, done[2];
+  uint64_t qfull[2], sfull[2][2], pfull[2][2], ofull, tail, done[2], otail[2];
   uint64_t kvfull[8], kvempty[8], half[4];
   uint32_t tmem;
   int abort_flag;
@@ -160,7 +160,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     }
     mbar_init(&bars.ofull, 2);
     mbar_init(&bars.tail, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&bars.done[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.done[i], 1);
+      mbar_init(&bars.otail[i], 1);
+    }
     for (int i = 0; i < 4; ++i) mbar_init(&bars.half[i], 2);
     for (int i = 0; i < NS; ++i) {
       mbar_init(&bars.kvfull[i], 1);
@@ -236,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       if (lane == 0) mbar_arrive(&bars.qfull[s]);
     };
     uint32_t g = 0;  // steps of this stream: step g is in buffer g % 2
-    int oph = 0, half_ph = 0;
+    int oph = 0, half_ph = 0, tails = 0;
     bool ok = true;
     // the two streams' warps of the same rows see what the other wrote
     auto meet = [&]() {
@@ -315,7 +318,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             const float nref = fresh ? fmaxf(maximum(), ref) : ref;
             const float f = ref == -INFINITY ? 0.f : ex2(ref - nref);
             if (n > 0 && __any_sync(0xffffffffu, f != 1.f)) {
-              // the product that last wrote O is complete (this step's S was issued after it)
+              // The product of step n - 1, which writes O, has to be complete: S of step n + 1 was
+              // issued right after it (S of this step only after that of step n - 2).  At the last
+              // step there is none, and `otail` says so.
+              uint64_t* bar = n + 1 < steps ? &bars.sfull[s][buf ^ 1] : &bars.otail[s];
+              const uint32_t ph = n + 1 < steps ? (g + 1) >> 1 & 1 : tails & 1;
+              if (!__all_sync(0xffffffffu, mbar_wait(bar, ph, abort_flag, a.err))) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
               l *= f;
 #pragma unroll 1
               for (int c = 0; c < D; c += 16) {
@@ -336,6 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.pfull[s][buf]);
       }
+      tails += steps > 1;
       TcPiece nx = it;
       tc_next(a, nx);
       fetch_q(nx);
@@ -508,6 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           for (int kk = 0; kk < kStep / 16; ++kk) umma_bf16_ts(t_o, at + 8 * kk, bd + kk * 128, id_o, n != 0 || kk != 0);
           if (odd || !pair) umma_commit(&bars.kvempty[vslot]);
           if (n + 2 < steps) ok = issue_s(n + 2);
+          else if (n + 2 == steps) umma_commit(&bars.otail[s]);
         }
         if (ok) umma_commit(&bars.ofull);
         g += steps;

@@ -283,6 +283,27 @@ def test_attention_prefix_large_scores():
     held(ops.attention_prefix(q, pk, pv, ck, cv, i32(lens)), want, tol)
 
 
+@pytest.mark.parametrize("B,nh,nkv,d,P,own", [(40, 8, 2, 64, 900, 30), (33, 16, 2, 128, 700, 0), (20, 4, 1, 128, 1300, 77)])
+def test_attention_prefix_rising_scores(B, nh, nkv, d, P, own):
+    """Scores that keep rising along the keys, by several powers of two at every tile: the running
+    reference moves again and again, in the first and the second half of a tile's keys."""
+    from flashmlx_b200 import ops
+    q = rnd(140, B, 1, nh, d).abs() * 2
+    lens = [own] * B
+    ck, cv = caches(141, B, nkv, max(own, 1), d, lens)
+    pk, pv = rnd(142, nkv, P, d), rnd(143, nkv, P, d)
+    ramp = torch.arange(P, device="cuda")[None, :, None] / 160.0 + torch.randint(0, 2, (nkv, P, 1), device="cuda",
+                                                                             generator=torch.Generator("cuda").manual_seed(1)) * 0.3
+    pk = (pk * 0.1 + ramp / d ** 0.5).to(BF)
+    want, tol, _, _ = R.attention(q, ck, cv, lens, pk, pv)
+    held(ops.attention_prefix(q, pk, pv, ck, cv, i32(lens)), want, tol)
+    acc = torch.zeros(1, nkv, P, device="cuda")  # the same keys as one sequence's own, 17 tokens
+    q1 = rnd(144, 1, 17, nh, d).abs() * 2
+    want, tol, a, at = R.attention(q1, pk[None], pv[None], [P], acc=acc)
+    held(ops.attention_scored(q1, pk[None].contiguous(), pv[None].contiguous(), i32([P]), acc), want, tol)
+    held(acc, a, at)
+
+
 @pytest.mark.parametrize("scale", [0.25, -0.1])
 def test_attention_scale(scale):
     from flashmlx_b200 import ops
