@@ -29,6 +29,10 @@
 // P is 2^(s - ref) with a row's ref the maximum of its first step, moved (and O rescaled, by the
 // stream itself) only when a later term passes it by more than 8: O in TMEM is rarely touched,
 // and P stays below 2^8 and keeps its relative precision.
+//
+// Bound: the exponentials of the two streams, which fall into step (64 keys: ~1200 of 1700 cycles
+// with both at the special-function units, 1063 at their rate).  A prompt of 4096 tokens, 32/4 heads of
+// 128: 147 us, 0.93 PFLOP/s; 64 sequences' rows over 32768 shared keys: 46 us.
 #include "fm_serve.cuh"
 
 namespace fm {
