@@ -666,7 +666,7 @@ def rope(x, positions, theta, rotary_dim=None, traditional=False, scaling=None, 
         raise ValueError("positions must have x's shape without heads and head size")
     cfg = _rope_config(shape[-1], theta, rotary_dim, traditional, scaling)
     if out is None:
-        out = torch.empty_like(x) if x.is_contiguous() else torch.empty(shape, dtype=_BF, device=torch.device("cuda", dev))
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
         out_ld = shape[-2] * shape[-1]
     else:
         _cuda_index(out, "out")
@@ -704,7 +704,7 @@ def rope_append(q, k, v, positions, slots, cache_k, cache_v, theta, traditional=
         raise ValueError("q, k, v, positions and slots must hold the same T = B * L tokens")
     cfg = _rope_config(d, theta, rotary_dim, traditional, scaling)
     if out is None:
-        out = torch.empty(q_shape, dtype=_BF, device=torch.device("cuda", dev))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         out_ld = nh * d
     else:
         _cuda_index(out, "out")
@@ -752,7 +752,7 @@ def _cache_attn(q, prefix_k, prefix_v, prefix_len, cache_k, cache_v, lens, acc, 
             raise ValueError("prefix_len is not within the prefix")
     if nkv == 0 or nh % nkv:
         raise ValueError("n_heads must be a multiple of n_kv")
-    out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q_shape, dtype=_BF, device=torch.device("cuda", dev))
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     cfg = _lib.CacheAttnConfig(nh, nkv, d, max_len, prefix_max, ld, scale)
     h = _bound(handle, dev)
     if acc is None:
