@@ -2210,6 +2210,7 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
     fm::TcAttnArgs& s = t[i];
     s.q = q;
     s.q_ld = q_ld;
+    s.v = i ? cv : pv;
     s.lens = i ? lens : nullptr;
     s.nseq = i ? B : 1;
     s.L = i ? L : B * L;

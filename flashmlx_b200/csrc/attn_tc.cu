@@ -55,6 +55,8 @@ struct Bars {
   uint64_t kvfull[8], kvempty[8], half[4];
   uint32_t tmem;
   int abort_flag;
+  uint32_t hidden[8];  // [i % 8] == i + 1: of the CTA's piece i, values were set to zero (the loader is
+                       // at most four pieces ahead: the ring holds eight tiles)
 };
 
 FM_DEV void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
@@ -174,6 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       mbar_init(&bars.kvempty[i], 2);
     }
     bars.abort_flag = 0;
+    for (int i = 0; i < 8; ++i) bars.hidden[i] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_proxy_async();
   }
@@ -360,6 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         ok = false;
         break;
       }
+      const bool spoiled = *const_cast<const volatile uint32_t*>(&bars.hidden[oph & 7]) == static_cast<uint32_t>(oph) + 1;
       ++oph;
       tc_fence_after();
       const bool whole = a.direct && it.cnt == it.tiles;
@@ -418,6 +422,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
               break;
             }
             if (s == 1) continue;
+          }
+          if (spoiled) {  // the values that the loader took out, for the rows that see them
+            const uint16_t* vr = a.v + (static_cast<int64_t>(b) * a.nkv + it.kvh) * a.head_rows * D + c;
+            const int last = min(lim, (it.tile + it.cnt) * kTcKeys - 1);
+#pragma unroll 1
+            for (int k = max(tc_seen_by_all(a, it.flat, len) + 1, it.tile * kTcKeys); k <= last; ++k) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 8) {
+                const uint4 x = *reinterpret_cast<const uint4*>(vr + static_cast<int64_t>(k) * D + e);
+                add_not_finite(x.x, o[e], o[e + 1]);
+                add_not_finite(x.y, o[e + 2], o[e + 3]);
+                add_not_finite(x.z, o[e + 4], o[e + 5]);
+                add_not_finite(x.w, o[e + 6], o[e + 7]);
+              }
+            }
           }
           if (whole) {
 #pragma unroll
@@ -539,10 +558,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     // ---------------------------------------------------------------- K / V loader
     int kc = 0, tph = 0;
     bool ok = true;
-    for (; ok && it.cnt > 0; tc_next(a, it)) {
+    uint32_t piece = 0;
+    for (; ok && it.cnt > 0; tc_next(a, it), ++piece) {
       const int b = it.flat / a.rps;
       const bool pair = rows - (it.flat - b * a.rps) * kTcRows > kTcKeys;
-      const int len = tc_len(a, b);
+      const int len = tc_len(a, b), sees = tc_seen_by_all(a, it.flat, len);
       const int y0 = (b * a.nkv + it.kvh) * a.head_rows;
       auto load = [&](const CUtensorMap* map, int j, bool v) {
         const int slot = kc % NS;
@@ -550,8 +570,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         ++kc;
         uint8_t* dst = s_kv + slot * S::kTileBytes;
         const int key0 = (it.tile + j) * kTcKeys;
-        // rows of V past the length may hold anything, and 0 * NaN is NaN: they become zeros
-        const bool ragged = v && key0 + kTcKeys > len;
+        // Rows of V past the length may hold anything, and 0 * NaN is NaN: they become zeros.  So
+        // do infinities and NaN in the rows that some of the item's tokens do not see (the streams
+        // add them to the other tokens' output).
+        const int first = max(sees + 1 - key0, 0), held = min(len - key0, kTcKeys);
+        const bool ragged = v && (held < kTcKeys || first < held);
         uint64_t* bar = ragged ? &bars.tail : &bars.kvfull[slot];
         if (elect_one()) {
           mbar_arrive_expect_tx(bar, S::kTileBytes);
@@ -563,12 +586,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         if (ragged) {
           if (!__all_sync(0xffffffffu, wait_drained(&bars.tail, tph & 1, a.err))) return false;
           ++tph;
-          const int first = len - key0;
-          for (int e = lane; e < (kTcKeys - first) * 8; e += 32)
+          auto chunk = [&](int row, int e, int h) {
+            return reinterpret_cast<uint4*>(dst + h * (kTcKeys * 128) + (row + (e >> 3)) * 128 + (e & 7) * 16);
+          };
+          bool bad = false;
+          for (int e = lane; e < (held - first) * 8; e += 32)
 #pragma unroll
-            for (int h = 0; h < S::kHalf; ++h)
-              *reinterpret_cast<uint4*>(dst + h * (kTcKeys * 128) + (first + (e >> 3)) * 128 + (e & 7) * 16) =
-                  make_uint4(0, 0, 0, 0);
+            for (int h = 0; h < S::kHalf; ++h) {
+              uint4* p = chunk(first, e, h);
+              const uint4 x = *p;
+              const uint4 y = make_uint4(finite_or_zero(x.x), finite_or_zero(x.y), finite_or_zero(x.z), finite_or_zero(x.w));
+              if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
+                bad = true;
+                *p = y;
+              }
+            }
+          if (__any_sync(0xffffffffu, bad) && lane == 0)
+            *const_cast<volatile uint32_t*>(&bars.hidden[piece & 7]) = piece + 1;
+          for (int e = lane; e < (kTcKeys - held) * 8; e += 32)
+#pragma unroll
+            for (int h = 0; h < S::kHalf; ++h) *chunk(held, e, h) = make_uint4(0, 0, 0, 0);
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars.kvfull[slot]);
@@ -603,8 +640,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 // acc[j] of a kv head's 128 keys: S^T = K Q^T for 128 query rows at a time (keys are the TMEM
 // lanes, rows the columns), so a thread's sum over its columns of 2^(s - lse of the row) is its
 // key's weight and needs no other thread.  The four groups of 128 threads take every fourth row
-// tile (two groups were bound by latency: 44% of the issue slots).  Bound by the exponentials (128 x 128 a tile: 1024 cycles of the special-function units
-// against 512 of the tensor pipe), of which a third go to fused multiply-adds here.
+// tile (two groups were bound by latency: 44% of the issue slots).  Bound by the
+// exponentials (128 x 128 a tile: 1024 cycles of the special-function units against 512 of the
+// tensor pipe).
 //   warps 0-15  groups 0-3     warp 16  MMA issuer     warp 17  TMA loads of K and Q
 namespace {
 constexpr int kWThreads = 576;

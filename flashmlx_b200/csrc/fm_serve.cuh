@@ -58,7 +58,6 @@ struct RopeSet : RopeBase {
 };
 using RopeArgs = RopeSet<kRopeMaxDim / 2>;
 
-
 // Attention over caches is split over keys.  A source of keys -- the shared prefix, or the
 // sequences' own caches -- is read by one of two kernels:
 //
@@ -118,6 +117,7 @@ struct CacheAttnArgs {
 struct TcAttnArgs {
   const uint16_t* q;        // [nseq * L, q_ld]
   int64_t q_ld;
+  const uint16_t* v;        // [nseq, nkv, head_rows, d], as its map
   const int32_t* lens;      // [nseq], or null: const_len keys each
   int nseq, L, nh, nkv, group, max_len, const_len;
   int causal;               // token l sees the keys j <= len - L + l; 0: all
@@ -170,6 +170,24 @@ struct TcWeightArgs {
 FM_DEV int tc_len(const TcAttnArgs& a, int b) {
   const int n = a.lens ? a.lens[b] : a.const_len;
   return n < 0 || n > a.max_len ? 0 : n;  // reported by the merge
+}
+
+// the last key that every row of item `flat` sees, -1: none
+FM_DEV int tc_seen_by_all(const TcAttnArgs& a, int flat, int len) {
+  return a.causal ? max(len - a.L + flat % a.rps * kTcRows / a.group, -1) : len - 1;
+}
+
+// a bf16 pair with infinities and NaN (an exponent of ones) as zeros
+FM_DEV uint32_t finite_or_zero(uint32_t w) {
+  const uint32_t m = ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+  return w & ~((m >> 15) * 0xffffu);
+}
+
+// those infinities and NaN of a bf16 pair added to a pair of fp32 sums
+FM_DEV void add_not_finite(uint32_t w, float& lo, float& hi) {
+  const uint32_t bad = w & ~finite_or_zero(w);
+  if (bad & 0x7f80u) lo += __uint_as_float(bad << 16);
+  if (bad & 0x7f800000u) hi += __uint_as_float(bad & 0xffff0000u);
 }
 
 __device__ __forceinline__ int TcAttnArgs::tiles(int flat) const {

@@ -229,6 +229,16 @@ FM_DEV void cp_async16_or_zero(uint32_t dst, const void* src, int n) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
+FM_DEV void lds128(uint32_t addr, uint4& v) {
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+}
+FM_DEV void sts128(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+FM_DEV void lds32(uint32_t addr, uint32_t& v) {
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+}
+
 }  // namespace
 
 template <int D>
@@ -344,6 +354,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
         qa[ks][hf + 2] = on ? *reinterpret_cast<const uint32_t*>(q + 16 * ks + 2 * c + 8) : 0u;
       }
     }
+    const int sees = pre ? len - 1 : max(len - a.L + row0 / a.group, -1);  // the last slot that every row sees
     float* srow[2];  // where this thread's rows' scores go
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
@@ -416,6 +427,42 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attn_split_kernel(const Cache
         o[n][1] *= al[0];
         o[n][2] *= al[1];
         o[n][3] *= al[1];
+      }
+      // Infinities and NaN of V in slots that some of the rows do not see: 0 times them is NaN, so
+      // they become zeros and the rows that do see them get them added.
+      if (min((tile + j + 1) * kAttnTile, len) - 1 > sees) {
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < kAttnTile * CH / 32; ++i) {
+          const int e = i * 32 + lane;
+          uint4 x;
+          lds128(sv + e * 16, x);
+          bad |= (tile + j) * kAttnTile + e / CH > sees &&
+                 (x.x != finite_or_zero(x.x) || x.y != finite_or_zero(x.y) || x.z != finite_or_zero(x.z) || x.w != finite_or_zero(x.w));
+        }
+        if (__any_sync(0xffffffffu, bad)) {
+#pragma unroll 1
+          for (int r = 0; r < kAttnTile; ++r) {
+            const int key = (tile + j) * kAttnTile + r;
+            if (key <= sees) continue;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              uint32_t x;
+              lds32(sv + r * ROW + ((n ^ (r & 7)) << 4) + 4 * c, x);
+              if (key <= lim[0]) add_not_finite(x, o[n][0], o[n][1]);
+              if (key <= lim[1]) add_not_finite(x, o[n][2], o[n][3]);
+            }
+          }
+          __syncwarp();
+#pragma unroll 1
+          for (int e = lane; e < kAttnTile * CH; e += 32) {
+            if ((tile + j) * kAttnTile + e / CH <= sees) continue;
+            uint4 x;
+            lds128(sv + e * 16, x);
+            sts128(sv + e * 16, make_uint4(finite_or_zero(x.x), finite_or_zero(x.y), finite_or_zero(x.z), finite_or_zero(x.w)));
+          }
+          __syncwarp();
+        }
       }
 #pragma unroll
       for (int n = 0; n < NT; n += 2) {

@@ -398,8 +398,8 @@ typedef struct fm_cache_attn_config {
  * already in the caches) over a prefix that all share, prefix_k / prefix_v
  * [n_kv_heads, prefix_max, head_dim] rows [0, prefix_len), and each sequence's own cache:
  * token l of sequence b sees the whole prefix and the slots j <= lens[b] - L + l, lens[b]
- * counting the new tokens.  A token that sees nothing (no prefix, and lens[b] too short) gives
- * zeros.  out is [B * L, n_heads * head_dim].  prefix_len may be 0 (prefix pointers NULL); lens
+ * counting the new tokens.  A slot reaches only the tokens that see it, whatever it holds (infinities
+ * and NaN too).  A token that sees nothing (no prefix, and lens[b] too short) gives zeros.  out is [B * L, n_heads * head_dim].  prefix_len may be 0 (prefix pointers NULL); lens
  * NULL means no own caches (cache pointers NULL). */
 FM_API int fm_attention_prefix(fm_handle* h, const fm_cache_attn_config* cfg, const uint16_t* q,
                                const uint16_t* prefix_k, const uint16_t* prefix_v, int prefix_len,
@@ -408,7 +408,8 @@ FM_API int fm_attention_prefix(fm_handle* h, const fm_cache_attn_config* cfg, co
 
 /* The same without a prefix, and acc[b, kvh, j] += the sum, over kv head kvh's query heads and
  * the L tokens, of the attention probability of slot j (fp32 [B, n_kv_heads, max_len]; slots
- * at or past lens[b] are left as they were; a slot that a new token takes should hold 0 before its first call).  At most 128 query heads to a kv head. */
+ * at or past lens[b] are left as they were; a slot that a new token takes should hold 0 before
+ * its first call).  At most 128 query heads to a kv head. */
 FM_API int fm_attention_scored(fm_handle* h, const fm_cache_attn_config* cfg, const uint16_t* q,
                                const uint16_t* cache_k, const uint16_t* cache_v, const int32_t* lens, int B, int L,
                                float* acc, uint16_t* out);

@@ -304,6 +304,59 @@ def test_attention_prefix_rising_scores(B, nh, nkv, d, P, own):
     held(acc, a, at)
 
 
+@pytest.mark.parametrize("B,L,nh,nkv,d,P,lens,M", [
+    (2, 4, 8, 2, 64, 40, [50, 128], 130),                # up to 64 rows to a key
+    (3, 17, 2, 2, 128, 0, [64, 17, 5], 70),
+    (2, 16, 8, 2, 128, 33, [333, 21], 340),
+    (1, 70, 1, 1, 64, 0, [200], 200),                    # up to 128
+    (3, 30, 8, 2, 128, 0, [300, 30, 128], 310),
+    (2, 40, 8, 2, 128, 50, [300, 129], 300),             # up to 256
+    (2, 300, 4, 2, 64, 100, [700, 320], 701),            # several row tiles
+    (1, 600, 8, 1, 128, 0, [2000], 2000),
+    (1, 515, 3, 3, 128, 0, [515], 530),
+    (40, 150, 4, 2, 64, 0, [150 + 3 * i for i in range(40)], 300),
+])
+def test_attention_hides_values_that_are_not_finite(B, L, nh, nkv, d, P, lens, M):
+    """Infinities and NaN in V reach the tokens that see their slot, in their column, and no other;
+    NaN in the last token's K spoils that token alone."""
+    from flashmlx_b200 import ops
+    q = rnd(150 + L, B, L, nh, d)
+    ck, cv = caches(151, B, nkv, M, d, lens)
+    pk = pv = None
+    if P:
+        pk, pv = rnd(153, nkv, P, d), rnd(154, nkv, P, d)
+    finite = cv.clone()
+    group, extra = nh // nkv, torch.zeros(B, L, nh, d, dtype=torch.float64)
+    values = [float("nan"), float("inf"), -float("inf")]
+    for b, n in enumerate(lens):
+        for i, slot in enumerate(sorted({n - 1, n - 2, n - L // 2, n - 2 * L // 3, n - L + 1, n - L, n - L - 1})):
+            if not 0 <= slot < n:
+                continue
+            for h in range(nkv):
+                for col in {(5 * i + 3 * h) % d, (d // 2 + 7 * i) % d, d - 1 - i}:
+                    x = values[(i + h + col) % 3]
+                    cv[b, h, slot, col], finite[b, h, slot, col] = x, 0.0
+                    extra[b, max(slot - (n - L), 0):, h * group:(h + 1) * group, col] += x
+    acc = torch.zeros(B, nkv, M, device="cuda")
+    want, tol, a, at = R.attention(q, ck, finite, lens, pk, pv, acc=acc if not P else None)
+    spoiled = ~torch.isfinite(extra)
+
+    def check(out, keep=slice(None)):
+        out = out.cpu().double()
+        assert torch.equal(out[:, keep][spoiled[:, keep]].nan_to_num(nan=7.0), extra[:, keep][spoiled[:, keep]].nan_to_num(nan=7.0))
+        held(torch.where(spoiled, want, out)[:, keep], want[:, keep], tol[:, keep])
+
+    check(ops.attention_prefix(q, pk, pv, ck, cv, i32(lens)))
+    if not P:
+        check(ops.attention_scored(q, ck, cv, i32(lens), acc))
+        held(acc, a, at)
+    for b, n in enumerate(lens):  # stale memory where a padding token was not written
+        ck[b, :, n - 1] = float("nan")
+    out = ops.attention_prefix(q, pk, pv, ck, cv, i32(lens))
+    check(out, slice(0, L - 1))
+    assert torch.isnan(out[:, L - 1]).all()
+
+
 @pytest.mark.parametrize("scale", [0.25, -0.1])
 def test_attention_scale(scale):
     from flashmlx_b200 import ops
