@@ -2113,6 +2113,15 @@ bool overlap(const void* p, int64_t n, const void* q, int64_t m) {
   return a < b + m && b < a + n;
 }
 
+// T rows of n (m) bf16 from p (q) on, ld_p (ld_q) elements apart, share memory; rows of one
+// stride that interleave (the parts of a fused projection) do not
+bool rows_overlap(const uint16_t* p, int64_t ld_p, int64_t n, const uint16_t* q, int64_t ld_q, int64_t m, int64_t T) {
+  if (!overlap(p, 2 * ((T - 1) * ld_p + n), q, 2 * ((T - 1) * ld_q + m))) return false;
+  if (ld_p != ld_q) return true;
+  const int64_t at = ((q - p) % ld_p + ld_p) % ld_p;  // q's column in p's rows
+  return at < n || at + m > ld_p;
+}
+
 int serve_ready(fm_handle* h) {
   if (h->sv_ready) return FM_OK;
   const cudaError_t e = fm::serve_init();
@@ -2152,7 +2161,15 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
     return set_err(h, FM_EINVAL, "q, the caches and out must be 16-byte aligned");
   const int64_t q_ld = c->q_ld ? c->q_ld : static_cast<int64_t>(c->n_heads) * c->head_dim;
   const int64_t T = static_cast<int64_t>(B) * L, cols = static_cast<int64_t>(c->n_heads) * c->head_dim;
-  if (overlap(q, 2 * ((T - 1) * q_ld + cols), out, 2 * T * cols)) return set_err(h, FM_EINVAL, "out may not overlap q");
+  const int64_t out_bytes = 2 * T * cols, cache_rows = static_cast<int64_t>(B) * c->n_kv_heads * c->max_len,
+                pre_bytes = 2ll * c->n_kv_heads * c->prefix_max * c->head_dim, own_bytes = lens ? 2 * cache_rows * c->head_dim : 0;
+  const struct { const void* p; int64_t n; } in[] = {
+      {q, 2 * ((T - 1) * q_ld + cols)}, {pk, prefix_len ? pre_bytes : 0}, {pv, prefix_len ? pre_bytes : 0},
+      {ck, own_bytes}, {cv, own_bytes}};
+  for (const auto& s : in)
+    if (s.n && (overlap(s.p, s.n, out, out_bytes) || (scored && overlap(s.p, s.n, acc, 4 * cache_rows))))
+      return set_err(h, FM_EINVAL, "out and acc may not overlap the inputs");
+  if (scored && overlap(out, out_bytes, acc, 4 * cache_rows)) return set_err(h, FM_EINVAL, "out may not overlap acc");
   const OnDevice on(h);
   rc = serve_ready(h);
   if (rc != FM_OK) return rc;
@@ -2282,7 +2299,7 @@ int fm_rope(fm_handle* h, const fm_rope_config* cfg, const uint16_t* x, int64_t 
   const int64_t cols = static_cast<int64_t>(n_heads) * a.d;
   if (!rows_ok(x, x_ld, cols) || !rows_ok(y, y_ld, cols))
     return set_err(h, FM_EINVAL, "rows must be 16-byte aligned, their strides multiples of 8 of at least n_heads * head_dim");
-  if (!(x == y && x_ld == y_ld) && overlap(x, 2 * ((T - 1) * x_ld + cols), y, 2 * ((T - 1) * y_ld + cols)))
+  if (!(x == y && x_ld == y_ld) && rows_overlap(x, x_ld, cols, y, y_ld, cols, T))
     return set_err(h, FM_EINVAL, "y must be x or not overlap it");
   const OnDevice on(h);
   a.q = x;
@@ -2317,9 +2334,16 @@ int fm_rope_append(fm_handle* h, const fm_rope_config* cfg, const uint16_t* q, i
   if (!rows_ok(q, q_ld, cols) || !rows_ok(q_out, q_out_ld, cols) || !rows_ok(k, kv_ld, kv_cols) ||
       !rows_ok(v, kv_ld, kv_cols) || !aligned16(cache_k) || !aligned16(cache_v))
     return set_err(h, FM_EINVAL, "rows must be 16-byte aligned, their strides multiples of 8 of at least their heads * head_dim");
-  const int64_t out_bytes = 2 * ((T - 1) * q_out_ld + cols);
-  if (!(q == q_out && q_ld == q_out_ld) && overlap(q, 2 * ((T - 1) * q_ld + cols), q_out, out_bytes))
+  if (!(q == q_out && q_ld == q_out_ld) && rows_overlap(q, q_ld, cols, q_out, q_out_ld, cols, T))
     return set_err(h, FM_EINVAL, "q_out must be q or not overlap it");
+  if (rows_overlap(k, kv_ld, kv_cols, q_out, q_out_ld, cols, T) || rows_overlap(v, kv_ld, kv_cols, q_out, q_out_ld, cols, T))
+    return set_err(h, FM_EINVAL, "q_out may not overlap k or v");
+  const int64_t cache_bytes = 2 * kv_cols * B * max_len, kv_bytes = 2 * ((T - 1) * kv_ld + kv_cols);
+  bool clash = overlap(cache_k, cache_bytes, cache_v, cache_bytes);
+  for (const uint16_t* cache : {cache_k, cache_v})
+    clash |= overlap(cache, cache_bytes, q, 2 * ((T - 1) * q_ld + cols)) || overlap(cache, cache_bytes, k, kv_bytes) ||
+             overlap(cache, cache_bytes, v, kv_bytes) || overlap(cache, cache_bytes, q_out, 2 * ((T - 1) * q_out_ld + cols));
+  if (clash) return set_err(h, FM_EINVAL, "the caches may overlap neither each other nor the rows");
   const OnDevice on(h);
   rc = ensure_sv(h, 0);
   if (rc != FM_OK) return rc;
@@ -2379,16 +2403,19 @@ int fm_cache_evict(fm_handle* h, const fm_evict_config* c, const uint16_t* cache
     return set_err(h, FM_EINVAL, "caches must be 16-byte aligned");
   const bool in_place = out_k == cache_k;
   const int64_t in = heads * c->max_len, to = heads * c->out_max_len, d2 = 2 * static_cast<int64_t>(c->head_dim);
-  if (in_place) {
-    if (out_v != cache_v || out_acc != acc || out_positions != positions || c->out_max_len != c->max_len)
-      return set_err(h, FM_EINVAL, "in place, every output must be its input and out_max_len max_len");
-  } else {
-    const struct { const void* p; int64_t n; } src[] = {{cache_k, in * d2}, {cache_v, in * d2}, {acc, in * 4},
-                                                        {positions, positions ? in * 4 : 0}},
-        dst[] = {{out_k, to * d2}, {out_v, to * d2}, {out_acc, to * 4}, {out_positions, out_positions ? to * 4 : 0}};
-    for (const auto& s : src)
-      for (const auto& t : dst)
-        if (s.n && t.n && overlap(s.p, s.n, t.p, t.n)) return set_err(h, FM_EINVAL, "the outputs may not overlap the inputs");
+  const struct { const void* p; int64_t n; } src[] = {{cache_k, in * d2}, {cache_v, in * d2}, {acc, in * 4},
+                                                      {positions, positions ? in * 4 : 0}},
+      dst[] = {{out_k, to * d2}, {out_v, to * d2}, {out_acc, to * 4}, {out_positions, out_positions ? to * 4 : 0}};
+  if (in_place && (out_v != cache_v || out_acc != acc || out_positions != positions || c->out_max_len != c->max_len))
+    return set_err(h, FM_EINVAL, "in place, every output must be its input and out_max_len max_len");
+  for (int i = 0; i < 4; ++i) {
+    if (!dst[i].n) continue;
+    for (int j = 0; j < 4; ++j) {
+      if (!in_place && src[j].n && overlap(src[j].p, src[j].n, dst[i].p, dst[i].n))
+        return set_err(h, FM_EINVAL, "the outputs may not overlap the inputs");
+      if (j < i && dst[j].n && overlap(dst[j].p, dst[j].n, dst[i].p, dst[i].n))
+        return set_err(h, FM_EINVAL, "the outputs may not overlap each other");
+    }
   }
   const OnDevice on(h);
   int rc = serve_ready(h);

@@ -610,8 +610,6 @@ def _heads_ld(t, name, index, shape, step):
     if (d > 1 and step[-1] != 1) or (h > 1 and step[-2] != d):
         if t.numel():
             raise ValueError(f"the heads of {name} must lie side by side")
-    if n == 3:
-        return step[0] if shape[0] > 1 else h * d
     ld, many = None, 1
     for i in range(n - 3, -1, -1):
         if shape[i] > 1:
@@ -620,7 +618,11 @@ def _heads_ld(t, name, index, shape, step):
             elif step[i] != ld * many and t.numel():
                 raise ValueError(f"the tokens of {name} must be one stride apart")
             many *= shape[i]
-    return h * d if ld is None else ld
+    if ld is None:
+        return h * d
+    if ld < h * d and t.numel():
+        raise ValueError(f"the tokens of {name} may not share memory")
+    return ld
 
 
 def _cuda_index(t, name):
@@ -631,6 +633,14 @@ def _cuda_index(t, name):
     if index < 0:
         raise ValueError(f"{name} must live on a CUDA device")
     return index
+
+
+def _int32(value, name):
+    """A Python integer that a C int holds (ctypes would cut it)."""
+    value = int(value)
+    if not -2 ** 31 <= value < 2 ** 31:
+        raise ValueError(f"{name} does not fit 32 bits")
+    return value
 
 
 def _packed(t, name, dtype, index):
@@ -753,7 +763,9 @@ def _cache_attn(q, prefix_k, prefix_v, prefix_len, cache_k, cache_v, lens, acc, 
     if nkv == 0 or nh % nkv:
         raise ValueError("n_heads must be a multiple of n_kv")
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    cfg = _lib.CacheAttnConfig(nh, nkv, d, max_len, prefix_max, ld, scale)
+    cfg = _lib.CacheAttnConfig(nh, nkv, d, max_len, prefix_max, _int32(ld, "q's stride"), scale)
+    if cfg.scale == 0.0 != scale:
+        raise ValueError("scale is too small")
     h = _bound(handle, dev)
     if acc is None:
         st = h.lib.fm_attention_prefix(h.h, cfg, q.data_ptr(), pk, pv, prefix_len or 0, ck, cv, n, B, L, out.data_ptr())
@@ -773,7 +785,8 @@ def attention_prefix(q, prefix_k, prefix_v, cache_k=None, cache_v=None, lens=Non
     (rotated; a view of wider rows may be given), prefix_k / prefix_v [n_kv, P, d] of which the
     first prefix_len rows count (default all), and each sequence's own caches
     [B, n_kv, max_len, d] with lens [B] int32 filled slots, the L new tokens' among them:
-    token l sees the prefix and the slots j <= lens[b] - L + l.  Returns [B, L, nh, d]."""
+    token l sees the prefix and the slots j <= lens[b] - L + l.  scale 0: 1/sqrt(d).  Returns
+    [B, L, nh, d].  Calls whose execution may overlap on several streams need a handle each."""
     return _cache_attn(q, prefix_k, prefix_v, prefix_len, cache_k, cache_v, lens, None, scale, handle)
 
 
@@ -821,7 +834,7 @@ def cache_evict(cache_k, cache_v, acc, lens, budget, sinks=0, recent=0, position
     no = _packed(lens_out, "lens_out", torch.int32, dev)
     if lens.shape != (B,) or lens_out.shape != (B,):
         raise ValueError("lens and lens_out must be [B]")
-    cfg = _lib.EvictConfig(nkv, d, max_len, rows, budget, sinks, recent)
+    cfg = _lib.EvictConfig(nkv, d, max_len, rows, _int32(budget, "budget"), _int32(sinks, "sinks"), _int32(recent, "recent"))
     h = _bound(handle, dev)
     st = h.lib.fm_cache_evict(h.h, cfg, ck, cv, a, p, n, B, ok, ov, oa, op, no)
     if st:

@@ -376,7 +376,8 @@ typedef struct fm_rope_config {
 FM_API int fm_rope(fm_handle* h, const fm_rope_config* cfg, const uint16_t* x, int64_t x_ld, int n_heads,
                    const int32_t* positions, int64_t T, uint16_t* y, int64_t y_ld);
 
-/* A step's q, k and v, T = B * L tokens: q_out[t] = q[t] rotated at positions[t] (q_out may be q),
+/* A step's q, k and v, T = B * L tokens: q_out[t] = q[t] rotated at positions[t] (q_out may be q;
+ * it may overlap neither k nor v, but rows of one fused buffer may interleave),
  * k[t] rotated and v[t] as it is into slot slots[t] of sequence t / L's caches.  slots[t] < 0
  * writes nothing to the caches (a padding token).  The slots of one sequence must differ. */
 FM_API int fm_rope_append(fm_handle* h, const fm_rope_config* cfg, const uint16_t* q, int64_t q_ld, int n_heads,

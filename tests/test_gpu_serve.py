@@ -120,6 +120,63 @@ def test_evict_refusals():
         refused(call)
 
 
+def test_tokens_that_share_memory_are_refused():
+    """A token's rows expanded over the batch have a stride of zero, which is no packed row."""
+    from flashmlx_b200 import ops
+    one, ck, cv, lens = rnd(10, 1, 1, 4, 64), rnd(11, 3, 2, 16, 64), rnd(12, 3, 2, 16, 64), i32([3, 4, 5])
+    acc = torch.zeros(3, 2, 16, device="cuda")
+    q = one.expand(3, 1, 4, 64)
+    for call in [
+        lambda: ops.attention_prefix(q, None, None, ck, cv, lens), lambda: ops.attention_scored(q, ck, cv, lens, acc),
+        lambda: ops.attention_prefix(one.expand(3, 2, 4, 64), None, None, ck, cv, lens),
+        lambda: ops.attention_prefix(q, ck[0], cv[0]), lambda: ops.rope(one[0].expand(3, 4, 64), lens, 1e4),
+        lambda: ops.rope(rnd(13, 3, 4, 64), lens, 1e4, out=one[0].expand(3, 4, 64)),
+        lambda: ops.attention_prefix(rnd(14, 1000).as_strided((3, 1, 4, 64), (128, 128, 64, 1)), None, None, ck, cv, lens),
+    ]:
+        refused(call)
+
+
+def test_overlapping_memory_is_refused():
+    from flashmlx_b200 import _lib, ops
+    qkv, ck, cv, at = rnd(15, 2, 8, 64), rnd(16, 2, 2, 16, 64), rnd(17, 2, 2, 16, 64), i32([0, 1])
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    rows = ck.view(2, 32, 64)
+    for call in [
+        lambda: ops.rope_append(q, k, v, at, at, ck, ck, 1e4), lambda: ops.rope_append(q, k, v, at, at, ck, cv, 1e4, out=qkv[:, 1:5]),
+        lambda: ops.rope_append(k, k, v, at, at, ck, cv, 1e4, out=k), lambda: ops.rope_append(q, k, v, at, at, ck, cv, 1e4, out=qkv[:, 4:]),
+        lambda: ops.rope_append(q, rows[:, :2], rows[:, 2:4], at, at, ck, cv, 1e4),
+        lambda: ops.rope_append(q, k, v, at, at, ck, cv, 1e4, out=rows[:, :4]),
+        lambda: ops.rope(qkv[:, :4], at, 1e4, out=qkv[:, 2:6]),
+    ]:
+        refused(call, _lib.FM_EINVAL)
+    want = ops.rope(q, at, 1e4)
+    assert torch.equal(ops.rope(q, at, 1e4, out=qkv[:, 4:]), want) and torch.equal(qkv[:, 4:], want)  # rows that interleave
+    h, lens = ops.default_handle(), i32([3, 4])
+    acc = torch.zeros(2, 2, 16, device="cuda")
+    cfg = _lib.CacheAttnConfig(4, 2, 64, 16, 16, 0, 0.0)
+    x = rnd(18, 2, 1, 4, 64)
+    for out, a in [(ck, acc), (cv, acc), (x, acc), (acc, acc), (rnd(19, 2, 1, 4, 64), ck), (rnd(19, 2, 1, 4, 64), cv)]:
+        refused(lambda: h.check(h.lib.fm_attention_scored(h.h, _lib.C.byref(cfg), x.data_ptr(), ck.data_ptr(), cv.data_ptr(),
+                                                          lens.data_ptr(), 2, 1, a.data_ptr(), out.data_ptr())), _lib.FM_EINVAL)
+    refused(lambda: h.check(h.lib.fm_attention_prefix(h.h, _lib.C.byref(cfg), x.data_ptr(), ck.data_ptr(), cv.data_ptr(), 16,
+                                                      None, None, None, 2, 1, cv.data_ptr())), _lib.FM_EINVAL)
+    refused(lambda: ops.cache_evict(ck, ck, acc, lens, 3), _lib.FM_EINVAL)
+    new = rnd(20, 2, 2, 16, 64)
+    refused(lambda: ops.cache_evict(ck, cv, acc, lens, 3, out=(new, new, torch.zeros_like(acc), None)), _lib.FM_EINVAL)
+
+
+def test_numbers_beyond_their_c_types_are_refused():
+    from flashmlx_b200 import ops
+    ck, cv, acc, lens = rnd(21, 2, 2, 16, 64), rnd(22, 2, 2, 16, 64), torch.zeros(2, 2, 16, device="cuda"), i32([9, 16])
+    for call in [
+        lambda: ops.cache_evict(ck, cv, acc, lens, 2 ** 32 + 5), lambda: ops.cache_evict(ck, cv, acc, lens, 5, recent=2 ** 32),
+        lambda: ops.cache_evict(ck, cv, acc, lens, 5, sinks=2 ** 32),
+        lambda: ops.attention_prefix(rnd(23, 2, 1, 4, 64), None, None, ck, cv, lens, scale=1e-60),
+        lambda: ops.attention_prefix(rnd(23, 2, 1, 4, 64), None, None, ck, cv, lens, scale=1e60),
+    ]:
+        refused(call)
+
+
 # ------------------------------------------------------------------ rotary positions
 YARN = {"type": "yarn", "factor": 4.0, "original_len": 4096, "beta_slow": 1.0, "beta_fast": 32.0}
 BANDED = {"type": "banded", "factor": 8.0, "original_len": 8192, "low_freq": 1.0, "high_freq": 4.0}
@@ -583,6 +640,62 @@ def test_a_captured_step_follows_its_lengths():
         held(out, want, tol, f"replay {i}")
         slots += 1
         lens += 1
+    h.sync()
+
+
+def test_a_captured_step_between_copies_and_forks():
+    """The calls begin while what is in front of them ends; a clear, a copy or another stream's
+    kernel in front is waited for, in a graph and out of it."""
+    from flashmlx_b200 import ops
+    B, nh, nkv, d, M = 3, 32, 4, 128, 4000
+    h = ops.Handle()
+    ck, cv, k2, v2 = (torch.zeros(B, nkv, M, d, dtype=BF, device="cuda") for _ in range(4))
+    src_k, src_v, q = rnd(160, B, nkv, M, d), rnd(161, B, nkv, M, d), rnd(162, B, 6, nh, d)
+    lens, want_lens = torch.zeros(B, dtype=torch.int32, device="cuda"), i32([4000, 17, 2100])
+    acc, a2 = (torch.ones(B, nkv, M, device="cuda") for _ in range(2))
+    other = torch.cuda.Stream()
+
+    def step():
+        here = torch.cuda.current_stream()
+        other.wait_stream(here)
+        with torch.cuda.stream(other):
+            cv.copy_(src_v)
+        ck.copy_(src_k)
+        acc.zero_()
+        lens.copy_(want_lens)
+        here.wait_stream(other)
+        out = ops.attention_scored(q, ck, cv, lens, acc, handle=h)
+        a2.copy_(acc)
+        n = ops.cache_evict(ck, cv, acc, lens, 1000, sinks=4, recent=100, handle=h)
+        k2.copy_(ck), v2.copy_(cv)
+        ck.zero_(), cv.zero_()
+        return out, n
+
+    want, tol, a, at = R.attention(q, src_k, src_v, want_lens.tolist(), acc=torch.zeros_like(acc))
+    runs = []
+
+    def check(out, n):
+        torch.cuda.synchronize()
+        held(out, want, tol)
+        held(a2, a, at)
+        assert n.tolist() == [1000, 17, 1000]
+        runs.append([t.clone() for t in (out, a2, k2, v2, acc)])
+        assert all(torch.equal(x, y) for x, y in zip(runs[0], runs[-1]))
+
+    check(*step())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, n = step()
+    for _ in range(3):
+        for t in (lens, acc, k2, v2, a2, out):
+            t.zero_()
+        g.replay()
+        check(out, n)
     h.sync()
 
 
