@@ -15,18 +15,25 @@ FM_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 FM_DEV void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <class... P, class... A>
-cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A&... args) {
+cudaError_t launch_pdl_cluster(void (*kernel)(P...), int ctas, dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A&... args) {
   cudaLaunchConfig_t c = {};
   c.gridDim = grid;
   c.blockDim = block;
   c.dynamicSmemBytes = smem;
   c.stream = st;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  c.attrs = &attr;
-  c.numAttrs = 1;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {static_cast<unsigned>(ctas), 1, 1};
+  c.attrs = attr;
+  c.numAttrs = ctas > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&c, kernel, args...);
+}
+
+template <class... P, class... A>
+cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A&... args) {
+  return launch_pdl_cluster(kernel, 1, grid, block, smem, st, args...);
 }
 #endif
 
@@ -331,6 +338,8 @@ struct EvictArgs {
   int32_t* out_lens;        // [B]
   int B, nkv, d, max_len, out_max_len, budget, sinks, recent;
   int in_place;
+  int ctas;                 // of the cluster that selects in a head
+  int words;                // 32-slot words of a CTA, at most
   int keys_in_smem;
   int fused;                // the select kernel makes the moves
   int32_t* list;            // [B * nkv][2][budget] destinations, sources

@@ -840,7 +840,7 @@ cudaError_t launch_cache_attn(const CacheAttnArgs& a, const TcAttnArgs& p, const
 }
 
 // ------------------------------------------------------------------ eviction
-// evict_select_kernel (one CTA per sequence and kv head) finds the n = min(len, budget) slots
+// evict_select_kernel (a CTA or a cluster per sequence and kv head) finds the n = min(len, budget) slots
 // that stay: a radix select over 32-bit keys (protected slots the largest, then the weight's
 // order-preserving bits, NaN as -inf), 8 bits a pass, ties to the lower slot.  The keys are read
 // once, into shared memory where they fit.  It leaves the list of rows that move as
@@ -852,6 +852,11 @@ constexpr int kEvictSmemKeys = 40960;  // 160 KB
 constexpr int kEvictCopies = 8;        // of the counts: a lane's own of eight, so that a warp whose keys are
                                        // alike does not add to one word 32 times
 constexpr int kEvictFused = 64;        // moves of a head that the select kernel makes itself
+// Long caches of few heads: a cluster of up to four CTAs shares a head's slots, since one SM's passes
+// take longer than what the cluster adds (barriers between the passes, ~4 us): 8 heads of 4096
+// slots 14 alone / 19 us together, 32 heads of 16384 30 / 28, 16 heads of 65536 112 / 38 (whole calls).
+constexpr int kEvictMaxCtas = 4;       // (eight: 57 us for the last of these)
+constexpr int kEvictLong = 16384;      // slots of a head, at least
 
 namespace {
 
@@ -867,6 +872,39 @@ FM_DEV int warps_before(const int* counts, int warp, int* total) {
   const int lane = threadIdx.x & 31;
   const int v = counts[lane];
   const int before = __reduce_add_sync(0xffffffffu, lane < warp ? v : 0);
+  *total = __reduce_add_sync(0xffffffffu, v);
+  return before;
+}
+
+FM_DEV uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+FM_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+FM_DEV uint32_t in_cta(const void* p, int rank) {  // the address of p in another CTA of the cluster
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+FM_DEV int ld_cluster(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+FM_DEV int4 ld_cluster4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// every CTA of the cluster's *p, after a cluster barrier: the sum of those before `rank`, and of all; whole warp
+FM_DEV int ctas_before(const int* p, int rank, int ctas, int* total) {
+  const int lane = threadIdx.x & 31;
+  const int v = lane < ctas ? ld_cluster(in_cta(p, lane)) : 0;
+  const int before = __reduce_add_sync(0xffffffffu, lane < rank ? v : 0);
   *total = __reduce_add_sync(0xffffffffu, v);
   return before;
 }
@@ -907,21 +945,26 @@ FM_DEV void evict_rows(const EvictArgs& a, int64_t bh, const int32_t* list_dst, 
 
 }  // namespace
 
+template <bool CLUSTER>
 __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const EvictArgs a) {
   extern __shared__ __align__(16) uint32_t s_dyn[];  // a bit per slot that stays, then the keys when they fit
   __shared__ __align__(16) int s_hist[256 * kEvictCopies];
+  __shared__ __align__(16) int s_cnt[CLUSTER ? 2 : 1][256];  // this CTA's counts, by the pass's parity: the next
+                                                             // pass's barrier says that all have read them
+  __shared__ int s_ex[4];                                    // newest, equal keys, holes, tail for the cluster
   uint32_t* s_kept = s_dyn;
-  uint32_t* s_keys = s_dyn + (a.max_len + 31) / 32;
+  uint32_t* s_keys = s_dyn + a.words;
   __shared__ int s_w[3][32];
   __shared__ int s_pick[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t bh = blockIdx.x;
+  const int ctas = CLUSTER ? a.ctas : 1, rank = CLUSTER ? static_cast<int>(cluster_rank()) : 0;
+  const int64_t bh = blockIdx.x / ctas;
   const int b = static_cast<int>(bh / a.nkv);
   pdl_wait();
   pdl_trigger();
   int len = a.lens[b];
   if (len < 0 || len > a.max_len) {
-    if (threadIdx.x == 0) report(a.err, DEVERR_BOUNDS);
+    if (threadIdx.x == 0 && rank == 0) report(a.err, DEVERR_BOUNDS);
     len = 0;
   }
   const int n = min(len, a.budget);
@@ -929,26 +972,35 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
   const int32_t* pos = a.positions ? a.positions + bh * a.max_len : nullptr;
   int32_t* list_dst = a.list + bh * 2 * a.budget;
   int32_t* list_src = list_dst + a.budget;
-  if (threadIdx.x == 0 && a.fused && bh % a.nkv == 0) a.out_lens[b] = n;
+  if (threadIdx.x == 0 && rank == 0 && a.fused && bh % a.nkv == 0) a.out_lens[b] = n;
   if (n == len) {  // all stay
     if (!a.in_place)
-      for (int i = threadIdx.x; i < n; i += kEvictThreads) list_dst[i] = list_src[i] = i;
-    if (threadIdx.x == 0 && !a.fused) {
+      for (int i = rank * kEvictThreads + threadIdx.x; i < n; i += ctas * kEvictThreads) list_dst[i] = list_src[i] = i;
+    if (threadIdx.x == 0 && rank == 0 && !a.fused) {
       a.counts[2 * bh] = a.in_place ? 0 : n;
       a.counts[2 * bh + 1] = n;
     }
     return;
   }
+  // this CTA's slots [lo, hi): whole 32-slot words
+  const int words = (len + 31) / 32, share = (words + ctas - 1) / ctas;
+  const int first_word = min(words, rank * share), last_word = min(words, first_word + share);
+  const int lo = 32 * first_word, hi = min(len, 32 * last_word);
   // the newest position held
   int newest = len - 1;
   if (pos) {
     int mx = INT32_MIN;
 #pragma unroll 8
-    for (int i = threadIdx.x; i < len; i += kEvictThreads) mx = max(mx, pos[i]);
+    for (int i = lo + threadIdx.x; i < hi; i += kEvictThreads) mx = max(mx, pos[i]);
     mx = __reduce_max_sync(0xffffffffu, mx);
     if (lane == 0) s_w[0][warp] = mx;
     __syncthreads();
     newest = __reduce_max_sync(0xffffffffu, s_w[0][lane]);
+    if (CLUSTER) {
+      if (threadIdx.x == 0) s_ex[0] = newest;
+      cluster_sync();
+      newest = __reduce_max_sync(0xffffffffu, lane < ctas ? ld_cluster(in_cta(&s_ex[0], lane)) : INT32_MIN);
+    }
   }
   // protected: below `sinks`, or one of the `recent` positions up to the newest
   const int64_t oldest = static_cast<int64_t>(newest) - a.recent + 1;
@@ -959,7 +1011,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
     return p < a.sinks || (any && p >= guard) ? 0xffffffffu : order_bits(acc[i]);
   };
   const bool kept_here = a.keys_in_smem;
-  auto key_of = [&](int i) -> uint32_t { return kept_here ? s_keys[i] : make_key(i); };
+  auto key_of = [&](int i) -> uint32_t { return kept_here ? s_keys[i - lo] : make_key(i); };
   // radix select: the n-th largest key and how many keys equal to it stay
   uint32_t prefix = 0;
   int want = n;  // of the keys that match the prefix so far
@@ -969,29 +1021,37 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
     __syncthreads();
     if (shift == 24) {
 #pragma unroll 8
-      for (int i = threadIdx.x; i < len; i += kEvictThreads) {
+      for (int i = lo + threadIdx.x; i < hi; i += kEvictThreads) {
         const uint32_t k = make_key(i);
-        if (kept_here) s_keys[i] = k;
+        if (kept_here) s_keys[i - lo] = k;
         atomicAdd(&s_hist[(k >> 24) * kEvictCopies + lane % kEvictCopies], 1);
       }
     } else {
 #pragma unroll 4
-      for (int i = threadIdx.x; i < len; i += kEvictThreads) {
+      for (int i = lo + threadIdx.x; i < hi; i += kEvictThreads) {
         const uint32_t k = key_of(i);
-        if ((k >> (shift + 8)) == (prefix >> (shift + 8))) 
+        if ((k >> (shift + 8)) == (prefix >> (shift + 8)))
           atomicAdd(&s_hist[((k >> shift) & 255u) * kEvictCopies + lane % kEvictCopies], 1);
       }
     }
     __syncthreads();
     if (threadIdx.x < 256) {
       const int4 x = reinterpret_cast<const int4*>(s_hist)[2 * threadIdx.x], y = reinterpret_cast<const int4*>(s_hist)[2 * threadIdx.x + 1];
-      s_hist[kEvictCopies * threadIdx.x] = ((x.x + x.y) + (x.z + x.w)) + ((y.x + y.y) + (y.z + y.w));
+      s_cnt[CLUSTER ? shift >> 3 & 1 : 0][threadIdx.x] = ((x.x + x.y) + (x.z + x.w)) + ((y.x + y.y) + (y.z + y.w));
     }
-    __syncthreads();
+    if (CLUSTER) cluster_sync();
+    else __syncthreads();
     if (warp == 0) {  // the bins from the largest down; lane l: 255 - 8 l to 248 - 8 l
-      int c[8], mine = 0;
+      const int* bins = &s_cnt[CLUSTER ? shift >> 3 & 1 : 0][248 - 8 * lane];
+      int c[8] = {}, mine = 0;
+      for (int r = 0; r < ctas; ++r) {
+        const int4 x = CLUSTER ? ld_cluster4(in_cta(bins + 4, r)) : *reinterpret_cast<const int4*>(bins + 4);
+        const int4 y = CLUSTER ? ld_cluster4(in_cta(bins, r)) : *reinterpret_cast<const int4*>(bins);
+        c[0] += x.w, c[1] += x.z, c[2] += x.y, c[3] += x.x;
+        c[4] += y.w, c[5] += y.z, c[6] += y.y, c[7] += y.x;
+      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mine += c[i] = s_hist[(255 - 8 * lane - i) * kEvictCopies];
+      for (int i = 0; i < 8; ++i) mine += c[i];
       int incl = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -1017,7 +1077,8 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
   // `want` of the keys equal to `prefix` stay, the lowest slots first.  A warp takes a contiguous
   // range of 32-slot words: first the equal keys are counted, then a bit says which slots stay, and
   // the holes below n and the kept slots from n on are counted; then a lane lists a word's.
-  const int words = (len + 31) / 32, per = (words + 31) / 32, w0 = warp * per, w1 = min(words, w0 + per);
+  const int per = (last_word - first_word + 31) / 32;
+  const int w0 = min(last_word, first_word + warp * per), w1 = min(last_word, w0 + per);
   int eq = 0;
   for (int w = w0; w < w1; ++w) {
     const int i = 32 * w + lane;
@@ -1027,6 +1088,11 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
   __syncthreads();
   int all;
   eq = warps_before(s_w[0], warp, &all);
+  if (CLUSTER) {
+    if (threadIdx.x == 0) s_ex[1] = all;
+    cluster_sync();
+    eq += ctas_before(&s_ex[1], rank, ctas, &all);
+  }
   const uint32_t below = (1u << lane) - 1;
   auto under_n = [&](int w) {  // the slots of word w below n
     const int c = n - 32 * w;
@@ -1040,7 +1106,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
     const uint32_t eqs = __ballot_sync(0xffffffffu, is_eq);
     const uint32_t kept = __ballot_sync(0xffffffffu, i < len && (k > prefix || (is_eq && eq + __popc(eqs & below) < want)));
     eq += __popc(eqs);
-    if (lane == 0) s_kept[w] = kept;
+    if (lane == 0) s_kept[w - first_word] = kept;
     hole += __popc(~kept & under_n(w));
     tail += __popc(kept & ~under_n(w));
   }
@@ -1052,9 +1118,18 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
   int holes;
   hole = warps_before(s_w[1], warp, &holes);
   tail = warps_before(s_w[2], warp, &all);
+  if (CLUSTER) {
+    if (threadIdx.x == 0) {
+      s_ex[2] = holes;
+      s_ex[3] = all;
+    }
+    cluster_sync();
+    hole += ctas_before(&s_ex[2], rank, ctas, &holes);
+    tail += ctas_before(&s_ex[3], rank, ctas, &all);
+  }
   for (int base = w0; base < w1; base += 32) {
     const int w = base + lane;
-    const uint32_t kept = w < w1 ? s_kept[w] : 0u, under = w < w1 ? under_n(w) : 0u;
+    const uint32_t kept = w < w1 ? s_kept[w - first_word] : 0u, under = w < w1 ? under_n(w) : 0u;
     uint32_t hm = ~kept & under, tm = kept & ~under, stay = a.in_place ? 0u : kept & under;
     int hi = __popc(hm), ti = __popc(tm);
 #pragma unroll
@@ -1075,10 +1150,12 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
     hole += __shfl_sync(0xffffffffu, hi, 31);
     tail += __shfl_sync(0xffffffffu, ti, 31);
   }
+  // (a CTA leaves after the others' last reads of its shared memory)
+  if (CLUSTER) cluster_sync();
   if (a.fused) {
-    __syncthreads();  // the lists are written (and read by this block alone)
-    evict_rows(a, bh, list_dst, list_src, holes, warp, 32);
-  } else if (threadIdx.x == 0) {
+    if (!CLUSTER) __syncthreads();  // the lists are written (and read by this block or cluster alone)
+    evict_rows(a, bh, list_dst, list_src, holes, rank * 32 + warp, ctas * 32);
+  } else if (threadIdx.x == 0 && rank == 0) {
     a.counts[2 * bh] = a.in_place ? holes : n;
     a.counts[2 * bh + 1] = n;
   }
@@ -1095,19 +1172,25 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const EvictArgs a) {
 }
 
 cudaError_t evict_init() {
-  return cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              kEvictSmemKeys * 4 + kEvictSmemKeys / 8);
+  const int smem = kEvictSmemKeys * 4 + kEvictSmemKeys / 8;
+  const cudaError_t e = cudaFuncSetAttribute(evict_select_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  return e == cudaSuccess ? cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : e;
 }
 
 cudaError_t launch_evict(EvictArgs a, bool lens_apart, int num_sms, cudaStream_t st) {
   const int64_t heads = static_cast<int64_t>(a.B) * a.nkv;
   const int64_t most = a.in_place ? std::min(a.budget, std::max(0, a.max_len - a.budget)) : a.budget;
-  a.keys_in_smem = a.max_len <= kEvictSmemKeys;
+  a.ctas = 1;
+  if (a.max_len >= kEvictLong)
+    while (a.ctas < kEvictMaxCtas && heads * a.ctas * 2 <= num_sms) a.ctas *= 2;
+  a.words = ((a.max_len + 31) / 32 + a.ctas - 1) / a.ctas;
+  a.keys_in_smem = a.words * 32 <= kEvictSmemKeys;
   // a step that is a few slots over: no second launch (unless out_lens is lens, which other blocks
   // of the sequence may not have read yet)
   a.fused = a.in_place && most <= kEvictFused && lens_apart;
-  const cudaError_t e = launch_pdl(evict_select_kernel, static_cast<unsigned>(heads), kEvictThreads,
-                                   (a.max_len + 31) / 32 * 4 + (a.keys_in_smem ? 4 * a.max_len : 0), st, a);
+  const cudaError_t e = launch_pdl_cluster(a.ctas > 1 ? evict_select_kernel<true> : evict_select_kernel<false>, a.ctas,
+                                           static_cast<unsigned>(heads * a.ctas), kEvictThreads,
+                                           a.words * 4 * (a.keys_in_smem ? 33 : 1), st, a);
   if (e != cudaSuccess || a.fused) return e;
   const int64_t want = std::max<int64_t>(1, (num_sms * 8 + heads - 1) / heads);
   const unsigned gx = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((most + 31) / 32, want)));

@@ -505,6 +505,11 @@ def test_attention_far_into_a_large_cache():
     (1, 1, 64, 100, [100], 200, 0, 0, "rand"),           # nothing to evict
     (1, 1, 8, 50000, [49990], 20001, 3, 77, "rand"),     # more keys than shared memory holds
     (1, 2, 8, 4096, [4096], 4095, 0, 4095, "ties"),      # one too many, nearly all protected
+    (2, 3, 16, 16384, [16384, 9001], 2048, 4, 512, "odd"),  # heads that several CTAs share
+    (3, 1, 8, 9000, [100, 8999, 33], 50, 0, 0, "zeros"),
+    (1, 1, 8, 200000, [199999], 70001, 3, 77, "ties"),
+    (1, 1, 8, 100000, [100000], 3, 1, 2, "rand"),
+    (5, 8, 8, 16500, [16500, 4097, 0, 2049, 1], 2048, 10, 0, "rand"),
 ])
 @pytest.mark.parametrize("in_place", [True, False])
 @pytest.mark.parametrize("given", [True, False])
@@ -543,6 +548,19 @@ def test_cache_evict(B, nkv, d, M, lens, budget, sinks, recent, weights, in_plac
             if b is not None:
                 assert torch.equal(a.cpu().nan_to_num(nan=-7.0), b.nan_to_num(nan=-7.0))
         assert lens_t.tolist() == lens
+
+
+@pytest.mark.parametrize("B,nkv,M,lens,budget", [(2, 2, 16400, [16400, 16395], 16390), (40, 1, 16384, [16384] * 39 + [5], 16383),
+                                                 (3, 2, 60, [60, 3, 41], 40)])
+def test_evict_a_few_slots_into_new_lengths(B, nkv, M, lens, budget):
+    """In place with lens_out apart from lens: a few moves, made by the kernel that selects."""
+    from flashmlx_b200 import ops
+    dev = [rnd(170, B, nkv, M, 64), rnd(171, B, nkv, M, 64), torch.rand(B, nkv, M, generator=torch.Generator().manual_seed(3)).cuda()]
+    host = [t.cpu().clone() for t in dev]
+    want = R.evict(*host, None, lens, budget, 4, 16, [*host, None])
+    assert ops.cache_evict(*dev, i32(lens), budget, sinks=4, recent=16).tolist() == want
+    for x, y in zip(dev, host):
+        assert torch.equal(x.cpu(), y)
 
 
 def test_evict_reports_a_length_past_the_cache():
