@@ -109,7 +109,7 @@ struct CacheAttnArgs {
   int split_own;            // 1: it reads the own caches
   int after_tc;             // attn_tc_kernel was launched before it: nothing of that is needed here
   float scale_log2;         // softmax scale * log2(e)
-  int merge_rows;           // rows of a merge block: 4 or 16
+  int merge_rows;           // rows of a merge block: 1, 4 or 16
   int rt_p, rt_s;           // row tiles of the prefix items / of a sequence's items, per kv head
   int workers;
   float* part_o;            // [slots][16][d]
