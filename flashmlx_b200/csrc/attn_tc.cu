@@ -46,8 +46,9 @@ template <int D>
 struct Shape {
   static constexpr int kHalf = D / 64;                       // 64-column halves of a row
   static constexpr uint32_t kTileBytes = kTcKeys * D * 2;    // a K, V or 128-row Q tile
-  static constexpr int kSlots = D == 128 ? 5 : 8;            // ring of K / V tiles
-  static constexpr uint32_t kSmem = 1024 + (2 + kSlots) * kTileBytes;
+  static constexpr int kSlots = D == 128 ? 4 : 8;            // ring of K / V tiles
+  static constexpr uint32_t kStage = 32 * 128;               // a warp's: 32 rows of 128 bytes
+  static constexpr uint32_t kSmem = 1024 + (2 + kSlots) * kTileBytes + kMmaWarp * kStage;
 };
 
 struct Bars {
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t t_s = tmem + lanes + s * kTcKeys, t_o = tmem + lanes + 2 * kTcKeys + s * D;
     uint8_t* q_tile = s_q + s * S::kTileBytes;
-    uint8_t* stage = q_tile + quad * 32 * 128;  // the warp's own Q rows (their first 64 columns)
+    uint8_t* stage = s_kv + NS * S::kTileBytes + warp * S::kStage;
     constexpr int CPR = D / 8, RPI = 32 / CPR;  // 16-byte chunks of a row, rows a warp brings at once
     uint4 qv[32 / RPI];
     // ---- Q: stream s brings tile s (with one tile of rows stream 0 alone)
@@ -366,6 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       const bool spoiled = *const_cast<const volatile uint32_t*>(&bars.hidden[oph & 7]) == static_cast<uint32_t>(oph) + 1;
       ++oph;
       tc_fence_after();
+      store_q(nx);  // S of the next piece's first steps while this one's O leaves
       const bool whole = a.direct && it.cnt == it.tiles;
       if (live) {
         const int64_t row = (tok0 + tk) * a.nh + it.kvh * a.group + (r - tk * a.group);
@@ -376,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const int rsub = lane >> 3, csub = lane & 7;
         float fac = 1.f;  // on this stream's O
         if (!pair) {      // one reference for both streams' halves
-          const int other = s == 0 ? static_cast<int>(S::kTileBytes) : -static_cast<int>(S::kTileBytes);
+          const int other = s == 0 ? 4 * static_cast<int>(S::kStage) : -4 * static_cast<int>(S::kStage);
           reinterpret_cast<float2*>(stage)[lane] = make_float2(ref, l);
           ok = meet();
           const volatile float* theirs = reinterpret_cast<const volatile float*>(stage + other) + 2 * lane;
@@ -410,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             if (s == 0) {
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
-                const float4 h = *reinterpret_cast<const float4*>(stage + S::kTileBytes + sw128_off(lane, e));
+                const float4 h = *reinterpret_cast<const float4*>(stage + 4 * S::kStage + sw128_off(lane, e));
                 o[4 * e] += h.x;
                 o[4 * e + 1] += h.y;
                 o[4 * e + 2] += h.z;
@@ -469,7 +471,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         __syncwarp();
       }
       it = nx;
-      store_q(it);
     }
     // items whose rows see nothing are in no worker's range
     if (ok && a.direct)

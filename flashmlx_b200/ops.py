@@ -610,6 +610,8 @@ def _heads_ld(t, name, index, shape, step):
     if (d > 1 and step[-1] != 1) or (h > 1 and step[-2] != d):
         if t.numel():
             raise ValueError(f"the heads of {name} must lie side by side")
+    if n == 3 and shape[0] > 1 and step[0] >= h * d:
+        return step[0]
     ld, many = None, 1
     for i in range(n - 3, -1, -1):
         if shape[i] > 1:
