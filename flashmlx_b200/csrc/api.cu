@@ -2239,6 +2239,8 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
     s.causal = i;
     s.head_rows = i ? c->max_len : c->prefix_max;
     s.rps = i ? p.rps_s : p.rps_p;
+    s.by_rps = fm::Divisor::of(s.rps);
+    s.by_group = fm::Divisor::of(s.group);
     s.workers = i ? p.workers_s : p.workers_p;
     s.direct = i && prefix_len == 0;
     s.scale_log2 = std::fabs(a.scale_log2);

@@ -209,27 +209,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     uint4 qv[32 / RPI];
     // ---- Q: stream s brings tile s (with one tile of rows stream 0 alone)
     auto fetch_q = [&](const TcPiece& p) {
-      const int b = p.flat / a.rps, row_base = (p.flat - b * a.rps) * kTcRows;
+      const int b = a.by_rps.divide(p.flat), row_base = (p.flat - b * a.rps) * kTcRows;
       const bool mine = p.cnt > 0 && (s == 0 || rows - row_base > kTcKeys);
       const uint16_t* q = a.q + static_cast<int64_t>(b) * a.L * a.q_ld + static_cast<int64_t>(p.kvh) * a.group * D + lane % CPR * 8;
-      int r = row_base + s * kTcKeys + quad * 32 + lane / CPR;
-      int tk = r / a.group, gq = r - tk * a.group;
+      const int r0 = row_base + s * kTcKeys + quad * 32 + lane / CPR;
 #pragma unroll
       for (int i = 0; i < 32 / RPI; ++i) {
+        const int r = r0 + i * RPI, tk = a.by_group.divide(r);
         qv[i] = make_uint4(0, 0, 0, 0);
-        if (mine && r < rows) qv[i] = *reinterpret_cast<const uint4*>(q + tk * a.q_ld + gq * D);
-        r += RPI;
-        gq += RPI;
-        while (gq >= a.group) {
-          gq -= a.group;
-          ++tk;
-        }
+        if (mine && r < rows) qv[i] = *reinterpret_cast<const uint4*>(q + tk * a.q_ld + (r - tk * a.group) * D);
       }
     };
     // both streams arrive for every piece, so that neither falls behind by a phase of `ofull`
     auto store_q = [&](const TcPiece& p) {
       if (p.cnt <= 0) return;
-      if (s == 0 || rows - p.flat % a.rps * kTcRows > kTcKeys) {
+      if (s == 0 || rows - (p.flat - a.by_rps.divide(p.flat) * a.rps) * kTcRows > kTcKeys) {
         const int ch = lane % CPR;
 #pragma unroll
         for (int i = 0; i < 32 / RPI; ++i) {
@@ -260,14 +254,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     fetch_q(it);
     store_q(it);
     while (it.cnt > 0) {
-      const int b = it.flat / a.rps, row_base = (it.flat - b * a.rps) * kTcRows;
+      const int b = a.by_rps.divide(it.flat), row_base = (it.flat - b * a.rps) * kTcRows;
       const bool pair = rows - row_base > kTcKeys;
       const int len = tc_len(a, b);
       const int64_t tok0 = static_cast<int64_t>(b) * a.L;
       const int rl = quad * 32 + lane;
       const int r = row_base + (pair ? s * kTcKeys : 0) + rl;
       const bool on = r < rows;
-      const int tk = on ? r / a.group : 0;
+      const int tk = on ? a.by_group.divide(r) : 0;
       const int lim = !on ? -1 : a.causal ? len - a.L + tk : len - 1;  // the last key this row sees
       const bool live = row_base + (pair ? s * kTcKeys : 0) + quad * 32 < rows;
       const int steps = pair ? 2 * it.cnt : it.cnt;
@@ -476,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     if (ok && a.direct)
       for (int f = blockIdx.x; f < a.items(); f += gridDim.x) {
         if (a.tiles(f) > 0) continue;
-        const int b = f / a.rps, row_base = (f - b * a.rps) * kTcRows, n = min(rows - row_base, kTcRows);
+        const int b = a.by_rps.divide(f), row_base = (f - b * a.rps) * kTcRows, n = min(rows - row_base, kTcRows);
         for (int i = threadIdx.x; i < n * a.nkv * (D / 8); i += kMmaWarp * 32) {
           const int ch = i % (D / 8), rk = i / (D / 8), kvh = rk / n, r = row_base + rk - kvh * n, tk = r / a.group;
           *reinterpret_cast<uint4*>(a.out + ((static_cast<int64_t>(b) * a.L + tk) * a.nh + kvh * a.group + r - tk * a.group) * D +
@@ -511,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       };
       for (; ok && it.cnt > 0; tc_next(a, it)) {
         // with one row tile a tile is one step, the stream's half of its keys
-        const bool pair = rows - it.flat % a.rps * kTcRows > kTcKeys;
+        const bool pair = rows - (it.flat - a.by_rps.divide(it.flat) * a.rps) * kTcRows > kTcKeys;
         const int steps = pair ? 2 * it.cnt : it.cnt;
         const uint64_t ad = q_desc + (pair ? s : 0) * kTile16;
         auto issue_s = [&](int n) {
@@ -561,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     bool ok = true;
     uint32_t piece = 0;
     for (; ok && it.cnt > 0; tc_next(a, it), ++piece) {
-      const int b = it.flat / a.rps;
+      const int b = a.by_rps.divide(it.flat);
       const bool pair = rows - (it.flat - b * a.rps) * kTcRows > kTcKeys;
       const int len = tc_len(a, b), sees = tc_seen_by_all(a, it.flat, len);
       const int y0 = (b * a.nkv + it.kvh) * a.head_rows;

@@ -120,6 +120,21 @@ struct CacheAttnArgs {
   uint32_t* err;
 };
 
+// n / d for 0 <= n < 2^31 by a multiplication: with 2^s >= d and m = ceil(2^(31 + s) / d),
+// m d - 2^(31 + s) < d <= 2^s, so n m / 2^(31 + s) passes n / d by less than 1 / d.
+struct Divisor {
+  uint32_t m, s;
+
+  static Divisor of(uint32_t d) {
+    uint32_t s = 0;
+    while ((uint64_t(1) << s) < d) ++s;
+    return {static_cast<uint32_t>(((uint64_t(1) << (31 + s)) + d - 1) / d), 31 + s};
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ int divide(int n) const { return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(n)) * m >> s); }
+#endif
+};
+
 // One source of keys for attn_tc_kernel: nseq sequences of L query tokens.
 struct TcAttnArgs {
   const uint16_t* q;        // [nseq * L, q_ld]
@@ -130,6 +145,7 @@ struct TcAttnArgs {
   int causal;               // token l sees the keys j <= len - L + l; 0: all
   int head_rows;            // rows of K / V from one (sequence, kv head) to the next
   int rps;                  // items per (sequence, kv head)
+  Divisor by_rps, by_group;
   int workers;              // 0: this source is not read here
   int direct;               // the only source: an item that one worker has whole goes to out
   float scale_log2;         // >= 0
@@ -181,7 +197,7 @@ FM_DEV int tc_len(const TcAttnArgs& a, int b) {
 
 // the last key that every row of item `flat` sees, -1: none
 FM_DEV int tc_seen_by_all(const TcAttnArgs& a, int flat, int len) {
-  return a.causal ? max(len - a.L + flat % a.rps * kTcRows / a.group, -1) : len - 1;
+  return a.causal ? max(len - a.L + a.by_group.divide((flat - a.by_rps.divide(flat) * a.rps) * kTcRows), -1) : len - 1;
 }
 
 // a bf16 pair with infinities and NaN (an exponent of ones) as zeros
@@ -198,12 +214,10 @@ FM_DEV void add_not_finite(uint32_t w, float& lo, float& hi) {
 }
 
 __device__ __forceinline__ int TcAttnArgs::tiles(int flat) const {
-  const int b = flat / rps, rp = flat - b * rps;
+  const int b = by_rps.divide(flat), rp = flat - b * rps;
   const int len = tc_len(*this, b);
   int seen = len;
-  if (causal) {
-    seen = len - L + min((rp * kTcRows + kTcRows - 1) / group, L - 1) + 1;
-  }
+  if (causal) seen = len - L + min(by_group.divide(rp * kTcRows + kTcRows - 1), L - 1) + 1;
   return seen <= 0 ? 0 : (seen + kTcKeys - 1) / kTcKeys;
 }
 
