@@ -9,16 +9,17 @@
 // with fewer both have the same rows and a stream takes half of each tile's keys; their halves
 // are joined in shared memory when the piece ends.
 //
-//   warps 0-3, 4-7  stream 0, 1: Q rows to shared memory (the next piece's are already in
-//                   registers when a piece ends); per 64 keys S out of TMEM, scale and
+//   warps 0-3, 4-7  stream 0, 1: Q rows to shared memory (the next piece's come in while a
+//                   piece's last product runs, and are stored before its O leaves, so that the
+//                   next S are computed meanwhile); per 64 keys S out of TMEM, scale and
 //                   visibility, online softmax, P back into TMEM over S (bf16 pairs); at the
-//                   end O out of TMEM, through the warp's own Q rows so that the stores are
-//                   whole lines
+//                   end O out of TMEM, through shared memory so that the stores are whole lines
 //   warps 8, 9      MMA issuers of streams 0 and 1: S = Q K^T (both operands K-major in shared
 //                   memory) and O += P V (P in TMEM, V as loaded: keys x head, i.e. MN-major).
 //                   One each, since an issuer's own waits and commits took ~950 cycles a step
 //                   where the products take 640
-//   warp 10         TMA loads of K / V tiles of 128 keys into a ring
+//   warp 10         TMA loads of K / V tiles of 128 keys into a ring (four tiles of 128 columns:
+//                   a fifth would take the room of the stage that O leaves through)
 //
 // TMEM: per stream two S / P buffers of 64 columns and head_dim columns of O.  A step is 64 keys
 // of a stream; S of step n + 2 is issued right after P V of step n, into the buffer that step
@@ -32,7 +33,7 @@
 //
 // Bound: the exponentials of the two streams, which fall into step (64 keys: ~1200 of 1700 cycles
 // with both at the special-function units, 1063 at their rate).  A prompt of 4096 tokens, 32/4 heads of
-// 128: 147 us, 0.93 PFLOP/s; 64 sequences' rows over 32768 shared keys: 46 us.
+// 128: 146 us, 0.94 PFLOP/s; 64 sequences' rows over 32768 shared keys: 45 us.
 #include "fm_serve.cuh"
 
 namespace fm {
