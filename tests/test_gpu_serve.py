@@ -563,6 +563,42 @@ def test_evict_a_few_slots_into_new_lengths(B, nkv, M, lens, budget):
         assert torch.equal(x.cpu(), y)
 
 
+@pytest.mark.parametrize("in_place", [True, False])
+def test_a_captured_eviction_follows_its_inputs(in_place):
+    """Heads that a cluster shares, in a graph replayed over other lengths and weights."""
+    from flashmlx_b200 import ops
+    B, nkv, M, budget, d = 2, 2, 16384, 700, 8
+    h = ops.Handle()
+    k, v = rnd(180, B, nkv, M, d), rnd(181, B, nkv, M, d)
+    acc, lens = torch.zeros(B, nkv, M, device="cuda"), i32([M, M])
+    dev = [k.clone(), v.clone(), acc.clone()]
+    out = dev if in_place else [torch.zeros(B, nkv, budget, d, dtype=BF, device="cuda") for _ in range(2)] + \
+        [torch.zeros(B, nkv, budget, device="cuda")]
+
+    def step():
+        for x, y in zip(dev, (k, v, acc)):
+            x.copy_(y)
+        return ops.cache_evict(*dev, lens, budget, sinks=4, recent=50, out=None if in_place else (*out, None), handle=h)
+
+    step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        n = step()
+    for i, now in enumerate([[M, 9000], [3, 16001], [701, 0]]):
+        acc.copy_(torch.rand(B, nkv, M, generator=torch.Generator().manual_seed(i)))
+        lens.copy_(i32(now))
+        for x in out if not in_place else []:
+            x.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        host = [x.cpu().clone() for x in (k, v, acc)]
+        to = host if in_place else [torch.zeros(x.shape, dtype=x.dtype) for x in out]
+        assert n.tolist() == R.evict(*host, None, now, budget, 4, 50, [*to, None])
+        for x, y in zip(out, to):
+            assert torch.equal(x.cpu(), y), f"replay {i}"
+    h.sync()
+
+
 def test_evict_reports_a_length_past_the_cache():
     from flashmlx_b200 import _lib, ops
     ck, cv, acc = rnd(72, 2, 1, 16, 64), rnd(73, 2, 1, 16, 64), torch.rand(2, 1, 16, device="cuda")
