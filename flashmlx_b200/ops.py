@@ -46,6 +46,8 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 class Handle:
     """One libflashmoe handle (device workspace + stream binding)."""
 
+    _stream = None  # the stream fm_set_stream was last given (None: not by bind_stream)
+
     def __init__(self, device: int | None = None):
         self.lib = _lib.load()
         if device is None:
@@ -57,7 +59,6 @@ class Handle:
         if st != _lib.FM_OK:
             raise FlashMoEError(st, "fm_create failed: " + self.lib.fm_status_string(st).decode())
         self.h = h
-        self._stream = None  # the stream fm_set_stream was last given (None: not by bind_stream)
 
     def close(self):
         if self.h and not getattr(self, "_borrowed", False):  # a borrowed view never destroys

@@ -78,3 +78,31 @@ def test_unknown_scalings_are_refused(scaling):
     from flashmlx_b200 import ops
     with pytest.raises(ValueError):
         ops._rope_config(64, 1e4, None, False, scaling)
+
+
+def test_handles_are_bound_to_the_current_stream(monkeypatch):
+    """An own handle is told a stream when it changes, a decoder's borrowed view every time (others
+    bind the handle behind it)."""
+    from flashmlx_b200 import ops
+
+    class Lib:
+        told = []
+
+        def fm_set_stream(self, h, s):
+            self.told.append(s)
+            return _lib.FM_OK
+
+    now = [7]
+    monkeypatch.setattr(ops, "_raw_stream", lambda device: now[0])
+    for borrowed, want in [(False, [7, 9]), (True, [7, 7, 9])]:
+        h = ops.Handle.__new__(ops.Handle)  # as Decoder.handle() makes one
+        h.lib, h.h, h.device, h._borrowed = Lib(), None, 0, borrowed
+        h.lib.told = []
+        now[0] = 7
+        assert ops._bound(h, 0) is h and ops._bound(h, 0) is h
+        now[0] = 9
+        ops._bound(h, 0)
+        assert h.lib.told == want
+        with pytest.raises(ValueError):
+            ops._bound(h, 1)
+        h._borrowed, h.h = True, None  # nothing to destroy
