@@ -2144,6 +2144,10 @@ int check_cache_attn(fm_handle* h, const fm_cache_attn_config* c, int B, int L, 
   if (prefix_len > c->prefix_max) return set_err(h, FM_EINVAL, "prefix_len exceeds prefix_max");
   if (static_cast<int64_t>(B) * L > 0x7fffffffLL / c->n_heads || c->n_kv_heads > 65535 || B > 65535)
     return set_err(h, FM_EUNSUPPORTED, "too many tokens or heads");
+  // cache rows are 32-bit coordinates of the tensor maps
+  if (static_cast<int64_t>(B) * c->n_kv_heads * c->max_len > 0x7fffff00LL ||
+      static_cast<int64_t>(c->n_kv_heads) * c->prefix_max > 0x7fffff00LL)
+    return set_err(h, FM_EUNSUPPORTED, "too many cache rows");
   return FM_OK;
 }
 
@@ -2177,12 +2181,8 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
   const fm::CacheAttnPlan p = fm::cache_attn_plan(B, L, nh, nkv, d, prefix_len, lens != nullptr, scored, c->max_len, h->num_sms);
   const int64_t own_rows = static_cast<int64_t>(B) * nkv * c->max_len, prefix_rows = static_cast<int64_t>(nkv) * c->prefix_max;
   if (scored && nh / nkv > fm::kTcKeys) return set_err(h, FM_EUNSUPPORTED, "more than 128 query heads to a kv head");
-  // the kernels count rows and tiles in 32 bits
-  const double group = nh / nkv, tiles = (c->max_len / 128 + 3.0) * nkv * B * (L * group / 256 + 1) +
-                                         (prefix_len / 128 + 3.0) * nkv * (static_cast<double>(B) * L * group / 256 + 1) +
-                                         (c->max_len + 16.0) * nkv * B / 8 + prefix_len / 8.0 * nkv;
-  if (own_rows > 0x7fffff00LL || prefix_rows > 0x7fffff00LL || tiles > 1e9)
-    return set_err(h, FM_EUNSUPPORTED, "too many rows");
+  if (!fm::cache_attn_fits(p, B, L, nh, nkv, prefix_len, c->max_len, scored))
+    return set_err(h, FM_EUNSUPPORTED, "too many rows and keys");
   rc = ensure_sv(h, p.bytes);
   if (rc != FM_OK) return rc;
   fm::CacheAttnArgs a;

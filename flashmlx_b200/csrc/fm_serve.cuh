@@ -73,13 +73,15 @@ using RopeArgs = RopeSet<kRopeMaxDim / 2>;
 //   attn_tc_kernel (attn_tc.cu), a worker a CTA, for many: items of 256 query rows (of the heads
 //     that share a kv head, neighbouring tokens together), tiles of 128 keys, tcgen05.
 //
-// The host refuses calls of 2^31 / 2 tiles or rows.
+// The kernels count these places in 32 bits (and a worker's range may reach past the last), so the
+// host refuses calls that could have more than kMaxPlaces in one kernel (cache_attn_fits).
 // Either way the tiles of all items, in order, are cut into one contiguous range per worker, so
 // ragged lengths balance.  A worker's piece of an item leaves an unnormalised fp32 output,
 // its maximum (log2 units) and its sum in slot worker + item -- both only grow along the
 // order, so no two pieces share a slot -- and attn_merge_kernel joins an output row's pieces.
 // (Where whole items go to the output at once, a worker leaves at most two pieces: slots
 // 2 worker for the item that it goes on with, 2 worker + 1 for the one that it begins.)
+constexpr double kMaxPlaces = 1 << 30;
 constexpr int kAttnTile = 16;        // keys of a tile
 constexpr int kAttnRowTile = 16;     // query rows of an item
 constexpr int kAttnSplitRows = 64;   // up to so many query rows to a key the split kernel reads it
@@ -338,6 +340,9 @@ CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_l
 
 // At least what any call of up to B sequences of L tokens over such a prefix and caches needs.
 size_t cache_attn_bound(int B, int L, int nh, int nkv, int d, int prefix_max, int max_len, int num_sms);
+
+// Whether every count of the plan's kernels fits their 32 bits (group at most kTcKeys when scored).
+bool cache_attn_fits(const CacheAttnPlan& p, int B, int L, int nh, int nkv, int prefix_len, int max_len, bool scored);
 
 struct EvictArgs {
   const uint16_t* cache_k;  // [B, nkv, max_len, d]

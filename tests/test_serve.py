@@ -106,3 +106,57 @@ def test_handles_are_bound_to_the_current_stream(monkeypatch):
         with pytest.raises(ValueError):
             ops._bound(h, 1)
         h._borrowed, h.h = True, None  # nothing to destroy
+
+
+# ------------------------------------------------------------------ the plan of attention over caches
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    """The library's own planning code, built alone for the host: plan(lines) -> answers."""
+    from flashmlx_b200 import build
+    exe = tmp_path_factory.mktemp("plan") / "serve_plan"
+    subprocess.check_call([build.nvcc(), *build.ARCH, "-std=c++17", "-I", build.INCLUDE, "-I", build.CSRC,
+                           os.path.join(ROOT, "tests", "cpp", "serve_plan.cu"),
+                           os.path.join(build.CSRC, "serve_plan.cu"), "-o", str(exe)])
+
+    def ask(lines):
+        r = subprocess.run([str(exe)], input="\n".join(lines) + "\n", capture_output=True, text=True, timeout=600)
+        assert r.returncode == 0, r.stderr
+        return r.stdout.split("\n")[:-1]
+
+    return ask
+
+
+def _weight_places(B, L, group, nkv, max_len):
+    """Places of the slot weights' order (full caches, a causal prompt): every 128 keys take 2 and a
+    place for each tile of 128 // group whole tokens from the first that sees them on."""
+    tokens = 128 // group
+    tiles = -(-L // tokens)
+    n = 0
+    for key0 in range(0, max_len, 128):
+        n += tiles - max(key0 - (max_len - L), 0) // tokens + 2
+    return n * nkv * B
+
+
+@pytest.mark.parametrize("B,L,group,nkv,max_len", [
+    (1, 70000, 71, 1, 2 ** 22), (1, 160000, 43, 1, 2 ** 22), (3, 100000, 65, 2, 2 ** 20), (1, 800000, 127, 1, 800000),
+    (1, 70000, 100, 1, 2 ** 23)])
+def test_slot_weights_beyond_their_32_bit_counts_are_refused(plan, B, L, group, nkv, max_len):
+    assert _weight_places(B, L, group, nkv, max_len) >= 2 ** 31
+    assert plan([f"fits {B} {L} {group * nkv} {nkv} 64 0 1 1 {max_len}"]) == ["0"]
+
+
+@pytest.mark.parametrize("B,L,nh,nkv,prefix,own,scored,max_len", [
+    (1, 1, 1, 1, 0, 1, 1, 1), (64, 1, 32, 4, 131072, 1, 0, 131072), (16, 1, 32, 4, 0, 1, 1, 131072),
+    (1, 131072, 32, 4, 0, 1, 1, 131072), (1, 100000, 128, 1, 0, 1, 1, 100000), (4, 32768, 71, 1, 0, 1, 1, 65536),
+    (65535, 1, 8, 8, 0, 1, 0, 4096), (2, 8192, 64, 8, 1048576, 1, 0, 8192), (1, 1, 16, 16, 2 ** 27, 0, 0, 0)])
+def test_large_calls_are_accepted(plan, B, L, nh, nkv, prefix, own, scored, max_len):
+    assert plan([f"fits {B} {L} {nh} {nkv} 128 {prefix} {own} {scored} {max_len}"]) == ["1"]
+
+
+def test_counts_of_the_other_kernels_beyond_32_bits_are_refused(plan):
+    full = 0x7fffff00
+    lines = [f"fits 1 2000000 1 1 64 0 1 0 {2 ** 28}",      # tcgen05, own caches: 7813 items of 2^21 tiles
+             f"fits 500 4000 1 1 64 {2 ** 28} 0 0 0",       # tcgen05, prefix
+             f"fits 1 64 1 1 64 0 1 0 {full}",              # split: four row tiles of 2^27 tiles, accepted
+             f"fits 2 32 1 1 64 {full} 1 0 {full // 2}"]    # split, both sources: 2^29 + 2^28
+    assert plan(lines) == ["0", "0", "1", "1"]
