@@ -246,6 +246,13 @@ int ensure_ws(fm_handle* h, size_t bytes) {
   return FM_OK;
 }
 
+// Clears the control bytes at p before it returns: the next call's reports, on whatever stream, come
+// after it (the legacy stream, which other work may hold up, orders no non-blocking stream).
+cudaError_t clear_ctrl(fm_handle* h, void* p) {
+  const cudaError_t e = cudaMemsetAsync(p, 0, kCtrlBytes, h->stream);
+  return e == cudaSuccess ? cudaStreamSynchronize(h->stream) : e;
+}
+
 // the status of a non-zero device error word
 int device_status(fm_handle* h, uint32_t word) {
   if (word & fm::DEVERR_TIMEOUT) return set_err(h, FM_ETIMEOUT, "a bounded device-side wait ran out");
@@ -285,10 +292,10 @@ int ensure_sv(fm_handle* h, size_t bytes) {
     return set_err(h, FM_ENOMEM, std::string("workspace allocation failed: ") + cudaGetErrorString(e));
   }
   if (h->sv_blocks.empty()) {
-    e = cudaMemset(p, 0, kCtrlBytes);
+    e = cudaMemsetAsync(p, 0, kCtrlBytes, h->stream);
     if (e != cudaSuccess) {
       cudaFree(p);
-      return cuda_err(h, e, "cudaMemset");
+      return cuda_err(h, e, "cudaMemsetAsync");
     }
   }
   h->sv_blocks.push_back(p);
@@ -1002,12 +1009,13 @@ int fm_sync_status(fm_handle* h) {
     uint32_t sv = 0;
     e = cudaMemcpy(&sv, h->sv_blocks[0], sizeof(sv), cudaMemcpyDeviceToHost);
     if (e != cudaSuccess) return cuda_err(h, e, "cudaMemcpy(error word)");
-    if (sv) cudaMemset(h->sv_blocks[0], 0, kCtrlBytes);
+    if (sv && (e = clear_ctrl(h, h->sv_blocks[0])) != cudaSuccess) return cuda_err(h, e, "clearing the error word");
     if (sv && !word) return device_status(h, sv);
     word |= sv;
   }
   if (word == 0) return FM_OK;
-  cudaMemset(h->ws, 0, kCtrlBytes);  // clear the error word and the grid-sync counters
+  // the error word and the grid-sync counters
+  if ((e = clear_ctrl(h, h->ws)) != cudaSuccess) return cuda_err(h, e, "clearing the error word");
   return device_status(h, word);
 }
 

@@ -808,3 +808,21 @@ def test_two_streams_with_their_own_handles():
                 got.append(ops.attention_prefix(q, None, None, ck, cv, n, handle=h))
     torch.cuda.synchronize()
     assert all(torch.equal(x, one) for x in got)
+
+
+def test_the_first_report_outlasts_the_default_streams_work():
+    """A handle's first serving call sets up its error word: on the call's stream, so that work queued on
+    the default stream, which does not order other streams, cannot delay it past the report."""
+    from flashmlx_b200 import _lib, ops
+    h, side = ops.Handle(), torch.cuda.Stream()
+    ck, cv, x, out = rnd(23, 1, 2, 8, 64), rnd(24, 1, 2, 8, 64), rnd(25, 2, 2, 64), rnd(26, 2, 2, 64)
+    at, slots = i32([0, 1]), i32([8, 3])
+    ops.rope_append(x, x, x, at, at, ck, cv, 1e4, out=out)  # the kernel is loaded
+    torch.cuda.synchronize()
+    torch.cuda._sleep(400_000_000)  # 0.2 s of the default stream
+    with torch.cuda.stream(side):
+        ops.rope_append(x, x, x, at, slots, ck, cv, 1e4, out=out, handle=h)
+    with pytest.raises(_lib.FlashMoEError) as e:
+        h.sync()
+    assert e.value.status == _lib.FM_EDEVICE
+    h.sync()  # reported once
