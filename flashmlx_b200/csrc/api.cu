@@ -124,6 +124,8 @@ struct fm_handle {
   size_t sv_bytes = 0;
   size_t sv_total = 0;        // bytes of all blocks
   bool sv_ready = false;      // shared-memory opt-in done
+  fm::StreamOrder sv_order;   // the workspace has one user at a time
+  cudaEvent_t sv_event = nullptr;
   // the frequencies of the last rotary config (64 powers cost more host time than the launch)
   fm_rope_config rope_cfg = {};
   fm::RopeArgs rope_set = {};
@@ -292,16 +294,50 @@ int ensure_sv(fm_handle* h, size_t bytes) {
     return set_err(h, FM_ENOMEM, std::string("workspace allocation failed: ") + cudaGetErrorString(e));
   }
   if (h->sv_blocks.empty()) {
-    e = cudaMemsetAsync(p, 0, kCtrlBytes, h->stream);
+    e = clear_ctrl(h, p);
     if (e != cudaSuccess) {
       cudaFree(p);
-      return cuda_err(h, e, "cudaMemsetAsync");
+      return cuda_err(h, e, "clearing the error word");
     }
   }
   h->sv_blocks.push_back(p);
   h->sv_ws = p + kCtrlBytes;
   h->sv_bytes = want - kCtrlBytes;
   h->sv_total += want;
+  return FM_OK;
+}
+
+// the stream calls of StreamOrder
+struct StreamCalls {
+  fm_handle* h;
+  cudaError_t capturing(cudaStream_t s, bool* yes) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    cudaError_t e = cudaStreamIsCapturing(s, &cap);
+    // the legacy stream while a stream that it would wait for is being captured
+    const bool implicit = e == cudaErrorStreamCaptureImplicit;
+    if (implicit) {
+      cudaGetLastError();
+      e = cudaSuccess;
+    }
+    *yes = implicit || cap != cudaStreamCaptureStatusNone;
+    return e;
+  }
+  cudaError_t wait(cudaStream_t now, cudaStream_t s) {
+    cudaError_t e = cudaSuccess;
+    if (!h->sv_event) e = cudaEventCreateWithFlags(&h->sv_event, cudaEventDisableTiming);
+    if (e == cudaSuccess) e = cudaEventRecord(h->sv_event, s);
+    return e == cudaSuccess ? cudaStreamWaitEvent(now, h->sv_event, 0) : e;
+  }
+};
+
+// Before a call uses the workspace: calls on other streams are waited for.
+int own_sv(fm_handle* h) {
+  const cudaError_t e = h->sv_order.join(h->stream, StreamCalls{h});
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return cuda_err(h, e, "ordering the handle's streams");
+  }
+  h->sv_order.mark();
   return FM_OK;
 }
 
@@ -916,12 +952,14 @@ int fm_destroy(fm_handle* h) {
   if (h->ws) cudaFree(h->ws);
   if (h->ep_ws) cudaFree(h->ep_ws);
   for (uint8_t* b : h->sv_blocks) cudaFree(b);
+  if (h->sv_event) cudaEventDestroy(h->sv_event);
   delete h;
   return FM_OK;
 }
 
 int fm_set_stream(fm_handle* h, void* stream) {
   if (!h) return FM_EINVAL;
+  h->sv_order.rebind(h->stream, static_cast<cudaStream_t>(stream));
   h->stream = static_cast<cudaStream_t>(stream);
   return FM_OK;
 }
@@ -1000,8 +1038,15 @@ int fm_profile_report(fm_handle* h, fm_kernel_time* out, int capacity, int* coun
 
 int fm_sync_status(fm_handle* h) {
   if (!h) return FM_EINVAL;
-  cudaError_t e = cudaStreamSynchronize(h->stream);
+  cudaError_t e;
+  {
+    const OnDevice on(h);
+    e = h->sv_order.join(h->stream, StreamCalls{h});  // reports of calls on other streams too
+  }
+  if (e != cudaSuccess) return cuda_err(h, e, "ordering the handle's streams");
+  e = cudaStreamSynchronize(h->stream);
   if (e != cudaSuccess) return cuda_err(h, e, "cudaStreamSynchronize");
+  h->sv_order.settle();
   uint32_t word = 0;
   e = cudaMemcpy(&word, h->ws, sizeof(word), cudaMemcpyDeviceToHost);
   if (e != cudaSuccess) return cuda_err(h, e, "cudaMemcpy(error word)");
@@ -2192,6 +2237,7 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
   if (!fm::cache_attn_fits(p, B, L, nh, nkv, prefix_len, c->max_len, scored))
     return set_err(h, FM_EUNSUPPORTED, "too many rows and keys");
   rc = ensure_sv(h, p.bytes);
+  if (rc == FM_OK) rc = own_sv(h);
   if (rc != FM_OK) return rc;
   fm::CacheAttnArgs a;
   std::memset(&a, 0, sizeof(a));
@@ -2374,6 +2420,7 @@ int fm_rope_append(fm_handle* h, const fm_rope_config* cfg, const uint16_t* q, i
   a.L = L;
   a.max_len = max_len;
   a.err = sv_err(h);
+  h->sv_order.mark();  // (of the workspace it takes the error word alone)
   prof_begin(h, "rope_append");
   const cudaError_t e = fm::launch_rope(a, h->num_sms, h->stream);
   prof_end(h);
@@ -2430,6 +2477,7 @@ int fm_cache_evict(fm_handle* h, const fm_evict_config* c, const uint16_t* cache
   const OnDevice on(h);
   int rc = serve_ready(h);
   if (rc == FM_OK) rc = ensure_sv(h, evict_bytes(heads, budget));
+  if (rc == FM_OK) rc = own_sv(h);
   if (rc != FM_OK) return rc;
   fm::EvictArgs a;
   std::memset(&a, 0, sizeof(a));

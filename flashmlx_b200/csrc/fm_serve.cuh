@@ -1,6 +1,9 @@
 // fm_serve.cuh -- arguments of the serving kernels (serve.cu).
 #pragma once
 
+#include <algorithm>
+#include <vector>
+
 #include "fm_internal.cuh"
 
 namespace fm {
@@ -340,6 +343,48 @@ CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_l
 
 // At least what any call of up to B sequences of L tokens over such a prefix and caches needs.
 size_t cache_attn_bound(int B, int L, int nh, int nkv, int d, int prefix_max, int max_len, int num_sms);
+
+// One handle's serving calls share a workspace, so a call on another stream than the calls before it
+// waits for them.  Streams are followed, not calls: `busy` says that calls were made on the bound
+// stream, `behind` holds the streams whose calls the bound one has yet to wait for.  What a capture
+// records runs later, and its replays are the caller's to order: in a capture nothing is waited for,
+// and a stream that is being captured stays `behind`.  Cuda has the two stream calls, so that tests
+// can do without a device.
+class StreamOrder {
+ public:
+  // the handle is bound to `now` instead of `before`
+  void rebind(cudaStream_t before, cudaStream_t now) {
+    if (before == now) return;
+    if (busy_ && std::find(behind_.begin(), behind_.end(), before) == behind_.end()) behind_.push_back(before);
+    busy_ = false;
+  }
+
+  // a call on the bound stream
+  void mark() { busy_ = true; }
+
+  // what stream `now`, the bound one, does next waits for the calls on the others
+  template <class Cuda>
+  cudaError_t join(cudaStream_t now, Cuda&& cuda) {
+    if (behind_.empty()) return cudaSuccess;
+    bool capturing = false;
+    cudaError_t e = cuda.capturing(now, &capturing);
+    if (capturing) return e;
+    for (size_t i = 0; i < behind_.size() && e == cudaSuccess;) {
+      const cudaStream_t s = behind_[i];
+      if (s != now && (e = cuda.capturing(s, &capturing)) == cudaSuccess && !capturing) e = cuda.wait(now, s);
+      if (s == now || (e == cudaSuccess && !capturing)) behind_.erase(behind_.begin() + i);
+      else ++i;
+    }
+    return e;
+  }
+
+  // the bound stream was synchronized after join()
+  void settle() { busy_ = false; }
+
+ private:
+  std::vector<cudaStream_t> behind_;
+  bool busy_ = false;
+};
 
 // Whether every count of the plan's kernels fits their 32 bits (group at most kTcKeys when scored).
 bool cache_attn_fits(const CacheAttnPlan& p, int B, int L, int nh, int nkv, int prefix_len, int max_len, bool scored);

@@ -789,13 +789,16 @@ def attention_prefix(q, prefix_k, prefix_v, cache_k=None, cache_v=None, lens=Non
     first prefix_len rows count (default all), and each sequence's own caches
     [B, n_kv, max_len, d] with lens [B] int32 filled slots, the L new tokens' among them:
     token l sees the prefix and the slots j <= lens[b] - L + l.  scale 0: 1/sqrt(d).  Returns
-    [B, L, nh, d].  Calls whose execution may overlap on several streams need a handle each."""
+    [B, L, nh, d].  Calls of one handle (the thread's default one without `handle`) on several
+    streams wait for one another; those that are to overlap, and replays of captured calls that
+    may, need a handle each."""
     return _cache_attn(q, prefix_k, prefix_v, prefix_len, cache_k, cache_v, lens, None, scale, handle)
 
 
 def attention_scored(q, cache_k, cache_v, lens, acc, scale=0.0, handle=None) -> torch.Tensor:
     """attention_prefix without a prefix that also adds to acc [B, n_kv, max_len] fp32 each
-    slot's attention probabilities, summed over the kv head's query heads and the L tokens."""
+    slot's attention probabilities, summed over the kv head's query heads and the L tokens.
+    Streams and handles as for attention_prefix."""
     if acc is None:
         raise TypeError("acc must be a torch tensor")
     return _cache_attn(q, None, None, None, cache_k, cache_v, lens, acc, scale, handle)
@@ -809,7 +812,8 @@ def cache_evict(cache_k, cache_v, acc, lens, budget, sinks=0, recent=0, position
     [B, n_kv, max_len] int32, a slot's index without them).  In place, or into
     out = (k, v, acc, positions) of [B, n_kv, M >= budget, ...] (positions may be None when
     `positions` is).  Slots that stay below n keep their places, the others below n take those
-    from n on in order.  Returns the new lengths [B] (lens_out if given; it may be lens)."""
+    from n on in order.  Returns the new lengths [B] (lens_out if given; it may be lens).
+    Streams and handles as for attention_prefix."""
     dev = _cuda_index(cache_k, "cache_k")
     shape = cache_k.shape
     ck, cv = _packed(cache_k, "cache_k", _BF, dev), _packed(cache_v, "cache_v", _BF, dev)

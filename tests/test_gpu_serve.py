@@ -826,3 +826,67 @@ def test_the_first_report_outlasts_the_default_streams_work():
         h.sync()
     assert e.value.status == _lib.FM_EDEVICE
     h.sync()  # reported once
+
+
+def test_streams_that_share_a_handle_take_turns():
+    """Without a handle given, calls on two streams share the default handle's workspace: the later
+    call waits for the earlier one, whatever held that up."""
+    from flashmlx_b200 import ops
+    lens = [3000, 500, 2100, 77]
+    n = i32(lens)
+    data = []
+    for i in range(2):
+        q, acc = rnd(190 + i, 4, 6, 8, 128), torch.rand(4, 2, 3000, generator=torch.Generator().manual_seed(i)).cuda()
+        data.append((q, *caches(192 + 2 * i, 4, 2, 3000, 128, lens), acc))
+
+    def work(q, ck, cv, acc):
+        ck, cv, acc = ck.clone(), cv.clone(), acc.clone()
+        out = ops.attention_scored(q, ck, cv, n, acc)
+        weights = acc.clone()
+        new = ops.cache_evict(ck, cv, acc, n, 1500, sinks=4, recent=64)
+        return [out, weights, ck, cv, acc, new]
+
+    want = [work(*d) for d in data]
+    ops.synchronize()
+    streams, ends, got = [torch.cuda.Stream() for _ in range(2)], [], []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            if i == 0:
+                torch.cuda._sleep(400_000_000)  # 0.2 s
+            got.append(work(*data[i % 2]))
+            ends.append(torch.cuda.Event())
+            ends[-1].record()
+    assert not ends[1].query()  # behind the first stream's sleep
+    ops.synchronize()
+    assert all(e.query() for e in ends)
+    for i, g in enumerate(got):
+        for x, y in zip(g, want[i % 2]):
+            assert torch.equal(x.nan_to_num(nan=-7.0), y.nan_to_num(nan=-7.0)), i
+
+
+def test_a_captured_call_on_its_own_stream_between_eager_ones():
+    """The default handle: eager calls before, in between (on another stream) and after a capture, whose
+    own calls wait for nothing."""
+    from flashmlx_b200 import _lib, ops
+    lens = [300, 20, 150]
+    q, (ck, cv), n = rnd(200, 3, 1, 8, 64), caches(201, 3, 2, 300, 64, lens), i32(lens)
+    want = ops.attention_prefix(q, None, None, ck, cv, n)
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    between, h, cfg = torch.zeros_like(q), ops.default_handle(), _lib.CacheAttnConfig(8, 2, 64, 300, 0, 0, 0.0)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        out = ops.attention_prefix(q, None, None, ck, cv, n)
+        with torch.cuda.stream(side):
+            h.bind_current()  # (torch allocates on no other stream during a capture)
+            h.check(h.lib.fm_attention_prefix(h.h, _lib.C.byref(cfg), q.data_ptr(), None, None, 0, ck.data_ptr(), cv.data_ptr(),
+                                              n.data_ptr(), 3, 1, between.data_ptr()))
+        again = ops.attention_prefix(q, None, None, ck, cv, n)
+    after = ops.attention_prefix(q, None, None, ck, cv, n)
+    ops.synchronize()
+    assert torch.equal(after, want)
+    for t in (out, again):
+        t.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(again, want) and torch.equal(between, want)
+    ops.synchronize()

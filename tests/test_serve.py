@@ -160,3 +160,22 @@ def test_counts_of_the_other_kernels_beyond_32_bits_are_refused(plan):
              f"fits 1 64 1 1 64 0 1 0 {full}",              # split: four row tiles of 2^27 tiles, accepted
              f"fits 2 32 1 1 64 {full} 1 0 {full // 2}"]    # split, both sources: 2^29 + 2^28
     assert plan(lines) == ["0", "0", "1", "1"]
+
+
+@pytest.mark.parametrize("steps,waits", [
+    ("c c c", "| | |"),                                       # one stream: nothing
+    ("c b1 c b1 c b2 c b1 c", "| | 1<0 | | 2<1 | 1<2"),       # each change waits once
+    ("b1 b2 c b1 c", "| | 1<2"),                              # a stream without calls is not waited for
+    ("c b1 b2 b3 c b0 c", "| | 3<0 | 0<3"),                   # bound over, the calls stay to be waited for
+    ("c b1 b0 c b1 c", "| | | 1<0"),                          # back again: its own calls
+    ("c b1 +1 c c -1 c b0 c", "| | | | 1<0 | 0<1"),           # a capture waits for nothing; the first call after it does
+    ("c b1 +1 c b2 c -1 b0 c", "| | | 2<0 | 0<1 0<2"),        # a stream being captured is waited for later
+    ("c +0 c b1 c -0 c c", "| | | | 1<0 |"),                  # the stream of earlier calls is captured itself
+    ("c b1 s b2 c", "| | 1<0 |"),                             # synchronized: nothing is in flight
+    ("c b1 +0 s b2 c -0 c", "| | | | 2<0"),
+    ("c b1 c b2 f2 c c b1 c c", "| | 1<0 | 2<1 | | error | 1<2"),
+    ("c b1 f1 c c", "| | error | 1<0"),                       # an error leaves it to be waited for
+])
+def test_calls_of_a_handle_on_several_streams_wait_for_one_another(plan, steps, waits):
+    n = steps.split()
+    assert plan([f"order {len(n)} {steps}"])[0].split() == waits.split()
