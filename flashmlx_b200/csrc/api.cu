@@ -2211,15 +2211,17 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
   int rc = check_cache_attn(h, c, B, L, prefix_len);
   if (rc != FM_OK) return rc;
   if (B == 0 || L == 0) return FM_OK;
-  if (!q || !out || (prefix_len > 0 && (!pk || !pv)) || (lens && (!ck || !cv)) || (scored && (!acc || !lens)))
+  const bool own = lens && c->max_len > 0;  // caches without slots may be null: no token sees anything there
+  if (!q || !out || (prefix_len > 0 && (!pk || !pv)) || (own && (!ck || !cv || (scored && !acc))) || (scored && !lens))
     return set_err(h, FM_EINVAL, "null pointer");
+  scored &= own;
   if (!aligned16(q) || !aligned16(out) || (prefix_len > 0 && (!aligned16(pk) || !aligned16(pv))) ||
-      (lens && (!aligned16(ck) || !aligned16(cv))))
+      (own && (!aligned16(ck) || !aligned16(cv))))
     return set_err(h, FM_EINVAL, "q, the caches and out must be 16-byte aligned");
   const int64_t q_ld = c->q_ld ? c->q_ld : static_cast<int64_t>(c->n_heads) * c->head_dim;
   const int64_t T = static_cast<int64_t>(B) * L, cols = static_cast<int64_t>(c->n_heads) * c->head_dim;
   const int64_t out_bytes = 2 * T * cols, cache_rows = static_cast<int64_t>(B) * c->n_kv_heads * c->max_len,
-                pre_bytes = 2ll * c->n_kv_heads * c->prefix_max * c->head_dim, own_bytes = lens ? 2 * cache_rows * c->head_dim : 0;
+                pre_bytes = 2ll * c->n_kv_heads * c->prefix_max * c->head_dim, own_bytes = own ? 2 * cache_rows * c->head_dim : 0;
   const struct { const void* p; int64_t n; } in[] = {
       {q, 2 * ((T - 1) * q_ld + cols)}, {pk, prefix_len ? pre_bytes : 0}, {pv, prefix_len ? pre_bytes : 0},
       {ck, own_bytes}, {cv, own_bytes}};
@@ -2231,7 +2233,7 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
   rc = serve_ready(h);
   if (rc != FM_OK) return rc;
   const int nh = c->n_heads, nkv = c->n_kv_heads, d = c->head_dim;
-  const fm::CacheAttnPlan p = fm::cache_attn_plan(B, L, nh, nkv, d, prefix_len, lens != nullptr, scored, c->max_len, h->num_sms);
+  const fm::CacheAttnPlan p = fm::cache_attn_plan(B, L, nh, nkv, d, prefix_len, own, scored, c->max_len, h->num_sms);
   const int64_t own_rows = static_cast<int64_t>(B) * nkv * c->max_len, prefix_rows = static_cast<int64_t>(nkv) * c->prefix_max;
   if (scored && nh / nkv > fm::kTcKeys) return set_err(h, FM_EUNSUPPORTED, "more than 128 query heads to a kv head");
   if (!fm::cache_attn_fits(p, B, L, nh, nkv, prefix_len, c->max_len, scored))

@@ -582,8 +582,6 @@ __global__ void __launch_bounds__(128) attn_merge_kernel(const CacheAttnArgs a, 
   const int warp = threadIdx.x >> 5;
   const int b = blockIdx.z, kvh = blockIdx.y;
   const int rows = a.L * a.group, first_row = blockIdx.x * a.merge_rows;
-  if (a.lens && threadIdx.x == 0 && blockIdx.x == 0 && kvh == 0 && (a.lens[b] < 0 || a.lens[b] > a.max_len))
-    report(a.err, DEVERR_BOUNDS);
   // the split kernel's cut
   const int tp16 = (a.split_prefix + kAttnTile - 1) / kAttnTile;
   const int np = a.nkv * a.rt_p, ns = a.nkv * a.rt_s;
@@ -608,6 +606,9 @@ __global__ void __launch_bounds__(128) attn_merge_kernel(const CacheAttnArgs a, 
   }
   pdl_wait();
   pdl_trigger();
+  // (here, since with caches of no slots this kernel may be the call's first)
+  if (a.lens && threadIdx.x == 0 && blockIdx.x == 0 && kvh == 0 && (a.lens[b] < 0 || a.lens[b] > a.max_len))
+    report(a.err, DEVERR_BOUNDS);
   __shared__ __align__(16) float s_acc[SHARED ? 3 : 1][SHARED ? D : 4];
   __shared__ float2 s_ml[3];
   constexpr int kEvery = SHARED ? 4 : 1;

@@ -394,7 +394,7 @@ typedef struct fm_cache_attn_config {
   int n_heads;
   int n_kv_heads;  /* divides n_heads */
   int head_dim;    /* 64 or 128 */
-  int max_len;     /* slots per (sequence, kv head) of the caches */
+  int max_len;     /* slots per (sequence, kv head) of the caches; at 0 their pointers may be NULL */
   int prefix_max;  /* rows per kv head of the prefix buffers */
   int q_ld;        /* elements from one token's q row to the next; 0 = n_heads * head_dim */
   float scale;     /* softmax scale; 0 = 1/sqrt(head_dim) */

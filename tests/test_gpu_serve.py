@@ -890,3 +890,22 @@ def test_a_captured_call_on_its_own_stream_between_eager_ones():
     torch.cuda.synchronize()
     assert torch.equal(out, want) and torch.equal(again, want) and torch.equal(between, want)
     ops.synchronize()
+
+
+@pytest.mark.parametrize("L", [1, 5, 40])
+@pytest.mark.parametrize("P", [0, 33])
+def test_caches_without_slots(L, P):
+    """max_len 0: every token sees the prefix alone, or nothing; a length above it is reported."""
+    from flashmlx_b200 import _lib, ops
+    q, empty, lens = rnd(210, 3, L, 8, 64), torch.empty(3, 2, 0, 64, dtype=BF, device="cuda"), i32([0, 0, 0])
+    pk, pv = (rnd(211, 2, P, 64), rnd(212, 2, P, 64)) if P else (None, None)
+    out = ops.attention_prefix(q, pk, pv, empty, empty, lens)
+    assert torch.equal(out, ops.attention_prefix(q, pk, pv) if P else torch.zeros_like(q))
+    if not P:
+        acc = torch.empty(3, 2, 0, device="cuda")
+        assert torch.equal(ops.attention_scored(q, empty, empty, lens, acc), torch.zeros_like(q))
+    ops.synchronize()
+    assert torch.equal(ops.attention_prefix(q, pk, pv, empty, empty, i32([0, 1, 0])), out)
+    with pytest.raises(_lib.FlashMoEError) as e:
+        ops.synchronize()
+    assert e.value.status == _lib.FM_EDEVICE
