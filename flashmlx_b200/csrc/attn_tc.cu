@@ -740,6 +740,11 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
           float v[32];
           tmem_ld32_async(tmem + lanes + st * kTcKeys + c, v);
           tmem_wait_ld();
+          if (c + 32 > tile_rows) {  // columns past the tile's rows: zeros, but NaN where a key is infinite
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c + e >= tile_rows) v[e] = 0.f;
+          }
           if (masked) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = r0 + c + e >= rmin && r0 + c + e < rows ? v[e] * a.scale_log2 : -INFINITY;

@@ -909,3 +909,23 @@ def test_caches_without_slots(L, P):
     with pytest.raises(_lib.FlashMoEError) as e:
         ops.synchronize()
     assert e.value.status == _lib.FM_EDEVICE
+
+
+@pytest.mark.parametrize("B,L,nh,nkv,d,lens", [
+    (2, 40, 6, 2, 64, [300, 129]), (1, 50, 7, 1, 128, [200]), (1, 30, 65, 1, 64, [150]), (1, 3, 3, 1, 64, [90]),
+    (2, 64, 8, 2, 128, [128, 260])])
+def test_slots_of_minus_infinite_score_weigh_nothing(B, L, nh, nkv, d, lens):
+    """A key of -infinity in one column scores -infinity with queries that are positive there: the call is as
+    without the slot, whose weight stays (groups that do not fill a tile of 128 rows among them)."""
+    from flashmlx_b200 import ops
+    q, M, at = rnd(220 + L, B, L, nh, d).abs() + 0.125, max(lens) + 1, 20
+    ck, cv = caches(221, B, nkv, M, d, lens)
+    ck[:, :, at, 3] = -float("inf")
+    acc = torch.rand(B, nkv, M, generator=torch.Generator().manual_seed(9)).cuda()
+    first = acc.clone()
+    keep = [i for i in range(M) if i != at]
+    want, tol, a, at_tol = R.attention(q, ck[:, :, keep], cv[:, :, keep], [n - 1 for n in lens], acc=acc[:, :, keep])
+    out = ops.attention_scored(q, ck, cv, i32(lens), acc)
+    held(out, want, tol, "out")
+    held(acc[:, :, keep], a, at_tol, "acc")
+    assert torch.equal(acc[:, :, at], first[:, :, at])
