@@ -745,19 +745,28 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
             for (int e = 0; e < 32; ++e)
               if (c + e >= tile_rows) v[e] = 0.f;
           }
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = r0 + c + e >= rmin && r0 + c + e < rows ? v[e] * a.scale_log2 : -INFINITY;
-          }
-          const float mul = masked ? 1.f : a.scale_log2;
           const float4* nl = reinterpret_cast<const float4*>(&s_lse[t % (2 * kWStages)][c]);
+          if (masked) {  // after lse, which may be NaN: such a row has no weight on what it does not see
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float4 n4 = nl[e];
-            sum4[0] += ex2(fmaf(v[4 * e], mul, n4.x));
-            sum4[1] += ex2(fmaf(v[4 * e + 1], mul, n4.y));
-            sum4[2] += ex2(fmaf(v[4 * e + 2], mul, n4.z));
-            sum4[3] += ex2(fmaf(v[4 * e + 3], mul, n4.w));
+            for (int e = 0; e < 8; ++e) {
+              const float4 n4 = nl[e];
+              const float n[4] = {n4.x, n4.y, n4.z, n4.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int r = r0 + c + 4 * e + i;
+                const float x = fmaf(v[4 * e + i], a.scale_log2, n[i]);
+                sum4[i] += ex2(r >= rmin && r < rows ? x : -INFINITY);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float4 n4 = nl[e];
+              sum4[0] += ex2(fmaf(v[4 * e], a.scale_log2, n4.x));
+              sum4[1] += ex2(fmaf(v[4 * e + 1], a.scale_log2, n4.y));
+              sum4[2] += ex2(fmaf(v[4 * e + 2], a.scale_log2, n4.z));
+              sum4[3] += ex2(fmaf(v[4 * e + 3], a.scale_log2, n4.w));
+            }
           }
         }
         tc_fence_before();

@@ -719,6 +719,7 @@ __global__ void __launch_bounds__(128) attn_merge_cut_kernel(const CacheAttnArgs
 // Four neighbouring slots a thread.
 __global__ void __launch_bounds__(256) slot_weight_kernel(const CacheAttnArgs a) {
   __shared__ float s_lse[kAttnRowTile];
+  __shared__ int s_lim[kAttnRowTile];  // the last slot that the row sees (whose lse may be NaN)
   const int b = blockIdx.z, kvh = blockIdx.y;
   int len = a.lens[b];
   if (len < 0 || len > a.max_len) len = 0;  // reported by the merge
@@ -727,20 +728,36 @@ __global__ void __launch_bounds__(256) slot_weight_kernel(const CacheAttnArgs a)
   if (static_cast<int>(blockIdx.x) * 1024 >= len) return;
   const int rows = a.L * a.group;
   const int64_t head = static_cast<int64_t>(b) * a.nkv + kvh;
-  if (threadIdx.x < rows) s_lse[threadIdx.x] = a.lse2[head * rows + threadIdx.x];
+  if (threadIdx.x < rows) {
+    s_lse[threadIdx.x] = a.lse2[head * rows + threadIdx.x];
+    s_lim[threadIdx.x] = len - a.L + static_cast<int>(threadIdx.x) / a.group;
+  }
   __syncthreads();
   const int j = blockIdx.x * 1024 + threadIdx.x * 4;
   if (j >= len) return;
   const float* sc = a.scores + head * rows * a.score_ld + j;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (min(static_cast<int>(blockIdx.x) * 1024 + 1023, len - 1) <= len - a.L) {  // every row sees the block's slots
 #pragma unroll 8
-  for (int r = 0; r < rows; ++r) {
-    const float4 v = *reinterpret_cast<const float4*>(sc + static_cast<int64_t>(r) * a.score_ld);
-    const float lse = s_lse[r];
-    sum.x += exp2f(v.x - lse);
-    sum.y += exp2f(v.y - lse);
-    sum.z += exp2f(v.z - lse);
-    sum.w += exp2f(v.w - lse);
+    for (int r = 0; r < rows; ++r) {
+      const float4 v = *reinterpret_cast<const float4*>(sc + static_cast<int64_t>(r) * a.score_ld);
+      const float lse = s_lse[r];
+      sum.x += exp2f(v.x - lse);
+      sum.y += exp2f(v.y - lse);
+      sum.z += exp2f(v.z - lse);
+      sum.w += exp2f(v.w - lse);
+    }
+  } else {
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
+      const float4 v = *reinterpret_cast<const float4*>(sc + static_cast<int64_t>(r) * a.score_ld);
+      const float lse = s_lse[r];
+      const int lim = s_lim[r];
+      sum.x += j <= lim ? exp2f(v.x - lse) : 0.f;
+      sum.y += j + 1 <= lim ? exp2f(v.y - lse) : 0.f;
+      sum.z += j + 2 <= lim ? exp2f(v.z - lse) : 0.f;
+      sum.w += j + 3 <= lim ? exp2f(v.w - lse) : 0.f;
+    }
   }
   float* acc = a.acc + head * a.max_len + j;
   acc[0] += sum.x;

@@ -929,3 +929,23 @@ def test_slots_of_minus_infinite_score_weigh_nothing(B, L, nh, nkv, d, lens):
     held(out, want, tol, "out")
     held(acc[:, :, keep], a, at_tol, "acc")
     assert torch.equal(acc[:, :, at], first[:, :, at])
+
+
+@pytest.mark.parametrize("B,L,nh,nkv,d,lens", [
+    (2, 4, 8, 2, 64, [100, 37]), (1, 2, 4, 4, 128, [700]), (2, 40, 8, 2, 64, [300, 129]), (1, 200, 6, 2, 128, [260])])
+def test_a_token_of_nan_weighs_only_on_slots_that_it_sees(B, L, nh, nkv, d, lens):
+    from flashmlx_b200 import ops
+    M = max(lens)
+    q = rnd(230 + L, B, L, nh, d)
+    ck, cv = caches(231, B, nkv, M, d, lens)
+    clean, acc = q.clone(), torch.zeros(B, nkv, M, device="cuda")
+    q[0, 0, 0, 5], clean[0, 0, 0, 5] = float("nan"), 0.0
+    want, tol, a, at = R.attention(clean, ck, cv, lens, acc=acc)
+    out = ops.attention_scored(q, ck, cv, i32(lens), acc)
+    assert torch.isnan(out[0, 0, 0]).all()
+    out[0, 0, 0] = want[0, 0, 0].to(BF).cuda()
+    held(out, want, tol, "out")
+    seen = lens[0] - L + 1  # slots that the first token sees
+    assert torch.isnan(acc[0, 0, :seen]).all()
+    acc[0, 0, :seen] = a[0, 0, :seen].float().cuda()
+    held(acc, a, at, "acc")
