@@ -949,3 +949,68 @@ def test_a_token_of_nan_weighs_only_on_slots_that_it_sees(B, L, nh, nkv, d, lens
     assert torch.isnan(acc[0, 0, :seen]).all()
     acc[0, 0, :seen] = a[0, 0, :seen].float().cuda()
     held(acc, a, at, "acc")
+
+
+def test_a_capture_right_after_the_reservation():
+    """fm_serve_reserve is enough: the handle's first calls may be captured ones."""
+    from flashmlx_b200 import _lib, ops
+    B, L, nh, nkv, d, M, P, lens = 3, 40, 8, 2, 128, 600, 200, [600, 41, 333]
+    h, cfg = ops.Handle(), _lib.CacheAttnConfig(8, 2, 128, 600, 200, 0, 0.0)
+    q, (ck, cv), n = rnd(240, B, L, nh, d), caches(241, B, nkv, M, d, lens), i32(lens)
+    pk, pv, acc = rnd(243, nkv, P, d), rnd(244, nkv, P, d), torch.zeros(B, nkv, M, device="cuda")
+    one, at = q[:, :1].contiguous(), torch.arange(B, dtype=torch.int32, device="cuda")
+    h.check(h.lib.fm_serve_reserve(h.h, _lib.C.byref(cfg), B, L))
+
+    def step(handle):
+        r = ops.rope(one[:, 0], at, 1e4, handle=handle)
+        outs = [r, ops.attention_prefix(q, pk, pv, ck, cv, n, handle=handle), ops.attention_scored(q, ck, cv, n, acc, handle=handle),
+                ops.attention_scored(one, ck, cv, n, acc, handle=handle), ops.attention_prefix(one, pk, pv, ck, cv, n, handle=handle)]
+        a = acc.clone()
+        k, v = ck.clone(), cv.clone()
+        return outs + [a, ops.cache_evict(k, v, a, n, 300, sinks=2, recent=20, handle=handle), k, v]
+
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step(h)
+    acc.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    acc.zero_()
+    for x, y in zip(got, step(None)):
+        assert torch.equal(x.nan_to_num(nan=-7.0), y.nan_to_num(nan=-7.0))
+    h.sync()
+
+
+@pytest.mark.parametrize("M,lens,lo", [(40, [40, 33], -10), (300, [300, 290], 5), (3000, [2999, 1600], -1500), (17000, [17000, 9000], 100)])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_the_recent_window_counts_from_the_newest_position(M, lens, lo, in_place):
+    """Positions on both sides of 0, or all at or above the sinks, in a shuffled order; the recent slots are the
+    lightest, so that only the window keeps them, and the sinks the next lightest."""
+    from flashmlx_b200 import ops
+    B, nkv, d, sinks, recent = len(lens), 2, 8, 6, 9
+    g = torch.Generator().manual_seed(M)
+    pos = torch.stack([torch.randperm(M, generator=g) + lo for _ in range(B * nkv)]).view(B, nkv, M).int()
+    acc = 1.0 + torch.rand(B, nkv, M, generator=g)
+    for b, n in enumerate(lens):
+        for h in range(nkv):
+            newest = int(pos[b, h, :n].max())
+            acc[b, h, pos[b, h] > newest - recent] = 0.0
+            acc[b, h, pos[b, h] < sinks] = 0.5
+    budget = M - lo if lo < 0 else M // 2  # (below 0 all positions are the sinks')
+    budget = min(budget, min(lens) - 1)
+    dev = [rnd(250, B, nkv, M, d), rnd(251, B, nkv, M, d), acc.cuda(), pos.cuda()]
+    host = [t.cpu().clone() for t in dev]
+    out = dev if in_place else [torch.zeros(B, nkv, budget, *t.shape[3:], dtype=t.dtype, device="cuda") for t in dev]
+    to = host if in_place else [torch.zeros(t.shape, dtype=t.dtype) for t in out]
+    want = R.evict(*host, lens, budget, sinks, recent, to)
+    got = ops.cache_evict(*dev[:3], i32(lens), budget, sinks=sinks, recent=recent, positions=dev[3],
+                          out=None if in_place else tuple(out))
+    assert got.tolist() == want
+    for x, y in zip(out, to):
+        assert torch.equal(x.cpu(), y)
+    for b in range(B):  # the window's slots are among those that stay
+        for h in range(nkv):
+            held_at = set(to[3][b, h, :want[b]].tolist())
+            top = int(pos[b, h, :lens[b]].max())
+            here = set(pos[b, h, :lens[b]].tolist())
+            assert {p for p in here if p > top - recent} <= held_at
