@@ -366,9 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       const bool whole = a.direct && it.cnt == it.tiles;
       if (live) {
         const int64_t row = (tok0 + tk) * a.nh + it.kvh * a.group + (r - tk * a.group);
-        const int64_t slot = a.direct ? 2 * static_cast<int64_t>(blockIdx.x) + (it.tile == 0)
-                                      : blockIdx.x + static_cast<int64_t>(it.flat) * a.nkv + it.kvh;
-        const int64_t pr = slot * kTcRows + (pair ? s * kTcKeys : 0) + quad * 32;
+        const int64_t pr = tc_slot(a, blockIdx.x, it) * kTcRows + (pair ? s * kTcKeys : 0) + quad * 32;
         const uint32_t on_rows = __ballot_sync(0xffffffffu, on);
         const int rsub = lane >> 3, csub = lane & 7;
         float fac = 1.f;  // on this stream's O
@@ -777,7 +775,7 @@ __global__ void __launch_bounds__(kWThreads, 1) slot_weight_tc_kernel(const __gr
         total = u;
       }
       if (!ok) break;
-      a.part[((static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(it.flat) * a.nkv + it.kvh) * kTcWeightParts + grp) * kTcKeys + kl] = total;
+      a.part[(tc_slot(a, blockIdx.x, it) * kTcWeightParts + grp) * kTcKeys + kl] = total;
     }
   } else if (warp == kWMmaWarp) {
     // ---------------------------------------------------------------- MMA issuer

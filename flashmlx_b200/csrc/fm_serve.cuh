@@ -6,6 +6,8 @@
 
 #include "fm_internal.cuh"
 
+#define FM_HD __host__ __device__ __forceinline__
+
 namespace fm {
 
 // The serving kernels are launched with programmatic stream serialization: a kernel may begin
@@ -135,9 +137,7 @@ struct Divisor {
     while ((uint64_t(1) << s) < d) ++s;
     return {static_cast<uint32_t>(((uint64_t(1) << (31 + s)) + d - 1) / d), 31 + s};
   }
-#ifdef __CUDACC__
-  __device__ __forceinline__ int divide(int n) const { return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(n)) * m >> s); }
-#endif
+  FM_HD int divide(int n) const { return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(n)) * m >> s); }
 };
 
 // One source of keys for attn_tc_kernel: nseq sequences of L query tokens.
@@ -162,11 +162,9 @@ struct TcAttnArgs {
   uint32_t* err;
 
   static constexpr int kItemCost = 4;  // what an item costs beside its tiles, in tiles
-#ifdef __CUDACC__
-  __device__ int items() const { return nseq * rps; }
+  FM_HD int items() const { return nseq * rps; }
   // tiles of item flat = b * rps + rp: up to the last key that its last token sees
-  __device__ int tiles(int flat) const;
-#endif
+  FM_HD int tiles(int flat) const;
 };
 
 // The slot weights by slot_weight_tc_kernel (attn_tc.cu): an item is a kv head's 128 keys, its
@@ -187,24 +185,22 @@ struct TcWeightArgs {
   uint32_t* err;
 
   static constexpr int kItemCost = 2;
-#ifdef __CUDACC__
-  __device__ int items() const { return B * key_tiles; }
-  __device__ int first_tile(int key0, int len) const;  // of the rows that see key0
-  __device__ int tiles(int flat) const;
-#endif
+  FM_HD int items() const { return B * key_tiles; }
+  FM_HD int first_tile(int key0, int len) const;  // of the rows that see key0
+  FM_HD int tiles(int flat) const;
 };
 
-#ifdef __CUDACC__
-FM_DEV int tc_len(const TcAttnArgs& a, int b) {
+FM_HD int tc_len(const TcAttnArgs& a, int b) {
   const int n = a.lens ? a.lens[b] : a.const_len;
   return n < 0 || n > a.max_len ? 0 : n;  // reported by the merge
 }
 
 // the last key that every row of item `flat` sees, -1: none
-FM_DEV int tc_seen_by_all(const TcAttnArgs& a, int flat, int len) {
+FM_HD int tc_seen_by_all(const TcAttnArgs& a, int flat, int len) {
   return a.causal ? max(len - a.L + a.by_group.divide((flat - a.by_rps.divide(flat) * a.rps) * kTcRows), -1) : len - 1;
 }
 
+#ifdef __CUDACC__
 // a bf16 pair with infinities and NaN (an exponent of ones) as zeros
 FM_DEV uint32_t finite_or_zero(uint32_t w) {
   const uint32_t m = ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
@@ -217,8 +213,9 @@ FM_DEV void add_not_finite(uint32_t w, float& lo, float& hi) {
   if (bad & 0x7f80u) lo += __uint_as_float(bad << 16);
   if (bad & 0x7f800000u) hi += __uint_as_float(bad & 0xffff0000u);
 }
+#endif
 
-__device__ __forceinline__ int TcAttnArgs::tiles(int flat) const {
+FM_HD int TcAttnArgs::tiles(int flat) const {
   const int b = by_rps.divide(flat), rp = flat - b * rps;
   const int len = tc_len(*this, b);
   int seen = len;
@@ -226,11 +223,11 @@ __device__ __forceinline__ int TcAttnArgs::tiles(int flat) const {
   return seen <= 0 ? 0 : (seen + kTcKeys - 1) / kTcKeys;
 }
 
-__device__ __forceinline__ int TcWeightArgs::first_tile(int key0, int len) const {
+FM_HD int TcWeightArgs::first_tile(int key0, int len) const {
   return max(key0 - (len - L), 0) / tile_tokens;  // token key0 - (len - L) is the first that sees key0
 }
 
-__device__ __forceinline__ int TcWeightArgs::tiles(int flat) const {
+FM_HD int TcWeightArgs::tiles(int flat) const {
   const int b = flat / key_tiles, key0 = (flat - b * key_tiles) * kTcKeys;
   const int len = lens[b];
   if (len < 0 || len > max_len || key0 >= len) return 0;
@@ -240,28 +237,47 @@ __device__ __forceinline__ int TcWeightArgs::tiles(int flat) const {
 // An item's start and end cost a worker about as much as kItemCost tiles, so the order has that
 // many empty places before each item's tiles and ranges are cut by places.
 template <class A>
-FM_DEV int tc_item_places(const A& a, int flat) {
+FM_HD int tc_item_places(const A& a, int flat) {
   const int n = a.tiles(flat);
   return n ? n + A::kItemCost : 0;
 }
 
-// places of one kv head of items [0, n), summed by the whole warp
+// places of one kv head of items [0, n), summed by the whole warp (on the host, for tests of the cut, by
+// one thread)
 template <class A>
-FM_DEV int tc_places_before(const A& a, int n) {
+FM_HD int tc_places_before(const A& a, int n) {
   int s = 0;
+#ifdef __CUDA_ARCH__
   for (int i = threadIdx.x & 31; i < n; i += 32) s += tc_item_places(a, i);
   return __reduce_add_sync(0xffffffffu, s);
+#else
+  for (int i = 0; i < n; ++i) s += tc_item_places(a, i);
+  return s;
+#endif
 }
 
 template <class A>
-FM_DEV int tc_places_per_worker(const A& a, int total) {
+FM_HD int tc_places_per_worker(const A& a, int total) {
   return max(1, (total + a.workers - 1) / a.workers);
 }
 
 // The item (flat, kvh) that place `place` falls into, and which of its places; false past the
 // end.  Whole warp.
 template <class A>
-FM_DEV bool tc_locate(const A& a, int place, int& flat, int& kvh, int& at) {
+FM_HD bool tc_locate(const A& a, int place, int& flat, int& kvh, int& at) {
+#ifndef __CUDA_ARCH__
+  int rest = place;
+  for (flat = 0; flat < a.items(); ++flat) {
+    const int places = tc_item_places(a, flat);
+    if (rest < places * a.nkv) {
+      kvh = rest / places;
+      at = rest - kvh * places;
+      return true;
+    }
+    rest -= places * a.nkv;
+  }
+  return false;
+#else
   const int lane = threadIdx.x & 31;
   int rest = place;
   for (int base = 0; base < a.items(); base += 32) {
@@ -286,6 +302,7 @@ FM_DEV bool tc_locate(const A& a, int place, int& flat, int& kvh, int& at) {
     rest -= __shfl_sync(0xffffffffu, incl, 31);
   }
   return false;
+#endif
 }
 
 // A worker's piece in hand: tiles [tile, tile + cnt) of item (flat, kvh); cnt 0 at the end.
@@ -296,7 +313,7 @@ struct TcPiece {
 
 // the piece of the range that begins at place `at` of item (flat, kvh)
 template <class A>
-FM_DEV void tc_cut(const A&, TcPiece& p, int at) {
+FM_HD void tc_cut(const A&, TcPiece& p, int at) {
   const int end = at + p.left;  // in the item's places
   p.tile = max(at - A::kItemCost, 0);
   p.cnt = max(min(end - A::kItemCost, p.tiles) - p.tile, 0);
@@ -305,7 +322,7 @@ FM_DEV void tc_cut(const A&, TcPiece& p, int at) {
 
 // the next item's piece; ends with cnt 0
 template <class A>
-FM_DEV void tc_next(const A& a, TcPiece& p) {
+FM_HD void tc_next(const A& a, TcPiece& p) {
   p.cnt = 0;
   while (p.left > 0 && p.cnt == 0) {
     if (++p.kvh == a.nkv) {
@@ -320,7 +337,7 @@ FM_DEV void tc_next(const A& a, TcPiece& p) {
 }
 
 template <class A>
-FM_DEV void tc_first(const A& a, int worker, int per, TcPiece& p) {  // whole warp
+FM_HD void tc_first(const A& a, int worker, int per, TcPiece& p) {  // whole warp
   int at;
   p.left = per;
   p.cnt = 0;
@@ -329,7 +346,14 @@ FM_DEV void tc_first(const A& a, int worker, int per, TcPiece& p) {  // whole wa
   tc_cut(a, p, at);
   if (p.cnt == 0) tc_next(a, p);
 }
-#endif
+
+// the slot of a worker's piece
+FM_HD int64_t tc_slot(const TcAttnArgs& a, int worker, const TcPiece& p) {
+  return a.direct ? 2 * static_cast<int64_t>(worker) + (p.tile == 0) : worker + static_cast<int64_t>(p.flat) * a.nkv + p.kvh;
+}
+FM_HD int64_t tc_slot(const TcWeightArgs& a, int worker, const TcPiece& p) {
+  return worker + static_cast<int64_t>(p.flat) * a.nkv + p.kvh;
+}
 
 // Which kernel reads what, and the workspace.
 struct CacheAttnPlan {

@@ -179,3 +179,15 @@ def test_counts_of_the_other_kernels_beyond_32_bits_are_refused(plan):
 def test_calls_of_a_handle_on_several_streams_wait_for_one_another(plan, steps, waits):
     n = steps.split()
     assert plan([f"order {len(n)} {steps}"])[0].split() == waits.split()
+
+
+@pytest.mark.parametrize("seed", [random.Random(s).randrange(2 ** 31) for s in range(8)])
+def test_attention_work_is_cut_without_gaps(plan, seed):
+    """Random calls: every tile of every item belongs to one worker, every piece has a slot of its own inside the
+    planned workspace, where the kernels that join an item's pieces look for it; the reservation covers
+    the plan."""
+    assert plan([f"cut {seed} 400"]) == ["ok"]
+
+
+def test_division_by_multiplication_is_exact(plan):
+    assert plan(["divide 200000"]) == ["ok"]
