@@ -124,6 +124,7 @@ struct fm_handle {
   size_t sv_bytes = 0;
   size_t sv_total = 0;        // bytes of all blocks
   bool sv_ready = false;      // shared-memory opt-in done
+  fm::EvictClusters sv_clusters;
   fm::StreamOrder sv_order;   // the workspace has one user at a time
   cudaEvent_t sv_event = nullptr;
   // the frequencies of the last rotary config (64 powers cost more host time than the launch)
@@ -2177,7 +2178,7 @@ bool rows_overlap(const uint16_t* p, int64_t ld_p, int64_t n, const uint16_t* q,
 
 int serve_ready(fm_handle* h) {
   if (h->sv_ready) return FM_OK;
-  const cudaError_t e = fm::serve_init();
+  const cudaError_t e = fm::serve_init(&h->sv_clusters);
   if (e != cudaSuccess) return cuda_err(h, e, "serving kernels' set-up");
   h->sv_ready = true;
   return FM_OK;
@@ -2507,7 +2508,7 @@ int fm_cache_evict(fm_handle* h, const fm_evict_config* c, const uint16_t* cache
   a.err = sv_err(h);
   prof_begin(h, "cache_evict");
   const bool lens_apart = !overlap(lens, 4ll * B, out_lens, 4ll * B);
-  const cudaError_t e = fm::launch_evict(a, lens_apart, h->num_sms, h->stream);
+  const cudaError_t e = fm::launch_evict(a, lens_apart, h->sv_clusters, h->num_sms, h->stream);
   prof_end(h);
   return e == cudaSuccess ? FM_OK : cuda_err(h, e, "cache_evict launch");
 }

@@ -436,7 +436,12 @@ struct EvictArgs {
 };
 
 cudaError_t launch_rope(RopeArgs& a, int num_sms, cudaStream_t st);
-cudaError_t serve_init();
+// How many clusters of two and of four CTAs of the selecting kernel run at a time.
+struct EvictClusters {
+  int twos = 0, fours = 0;
+};
+int evict_ctas(int64_t heads, int max_len, const EvictClusters& c);  // CTAs that share a head
+cudaError_t serve_init(EvictClusters* c);
 // p, s: the prefix / own caches by attn_tc_kernel where their workers are set, with its maps
 struct TcMapsKV {
   CUtensorMap k, v;
@@ -447,6 +452,6 @@ cudaError_t launch_cache_attn(const CacheAttnArgs& a, const TcAttnArgs& p, const
 cudaError_t attn_tc_init();
 cudaError_t launch_attn_tc(const TcAttnArgs& a, int d, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st);
 cudaError_t launch_slot_weight_tc(const TcWeightArgs& a, int d, const CUtensorMap& k, const CUtensorMap& q, cudaStream_t st);
-cudaError_t launch_evict(EvictArgs a, bool lens_apart, int num_sms, cudaStream_t st);
+cudaError_t launch_evict(EvictArgs a, bool lens_apart, const EvictClusters& clusters, int num_sms, cudaStream_t st);
 
 }  // namespace fm

@@ -790,12 +790,12 @@ static cudaError_t attn_opt_in() {
   return cudaFuncSetAttribute(attn_split_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_split_smem(D));
 }
 
-cudaError_t evict_init();
+cudaError_t evict_init(EvictClusters* c);
 
-cudaError_t serve_init() {
+cudaError_t serve_init(EvictClusters* c) {
   cudaError_t e = attn_opt_in<128>();
   if (e == cudaSuccess) e = attn_opt_in<64>();
-  if (e == cudaSuccess) e = evict_init();
+  if (e == cudaSuccess) e = evict_init(c);
   return e == cudaSuccess ? attn_tc_init() : e;
 }
 
@@ -838,11 +838,6 @@ constexpr int kEvictSmemKeys = 40960;  // 160 KB
 constexpr int kEvictCopies = 8;        // of the counts: a lane's own of eight, so that a warp whose keys are
                                        // alike does not add to one word 32 times
 constexpr int kEvictFused = 64;        // moves of a head that the select kernel makes itself
-// Long caches of few heads: a cluster of up to four CTAs shares a head's slots, since one SM's passes
-// take longer than what the cluster adds (barriers between the passes, ~4 us): 8 heads of 4096
-// slots 14 alone / 19 us together, 32 heads of 16384 30 / 28, 16 heads of 65536 112 / 38 (whole calls).
-constexpr int kEvictMaxCtas = 4;       // (eight: 57 us for the last of these)
-constexpr int kEvictLong = 16384;      // slots of a head, at least
 
 namespace {
 
@@ -1157,18 +1152,29 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const EvictArgs a) {
   evict_rows(a, bh, list_dst, list_dst + a.budget, cnt, blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8);
 }
 
-cudaError_t evict_init() {
+cudaError_t evict_init(EvictClusters* c) {
   const int smem = kEvictSmemKeys * 4 + kEvictSmemKeys / 8;
-  const cudaError_t e = cudaFuncSetAttribute(evict_select_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  return e == cudaSuccess ? cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : e;
+  cudaError_t e = cudaFuncSetAttribute(evict_select_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  for (int ctas : {2, 4}) {
+    cudaLaunchConfig_t l = {};
+    l.gridDim = dim3(ctas);
+    l.blockDim = dim3(kEvictThreads);
+    l.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {static_cast<unsigned>(ctas), 1, 1};
+    l.attrs = &attr;
+    l.numAttrs = 1;
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(ctas == 2 ? &c->twos : &c->fours, evict_select_kernel<true>, &l);
+  }
+  return e;
 }
 
-cudaError_t launch_evict(EvictArgs a, bool lens_apart, int num_sms, cudaStream_t st) {
+cudaError_t launch_evict(EvictArgs a, bool lens_apart, const EvictClusters& clusters, int num_sms, cudaStream_t st) {
   const int64_t heads = static_cast<int64_t>(a.B) * a.nkv;
   const int64_t most = a.in_place ? std::min(a.budget, std::max(0, a.max_len - a.budget)) : a.budget;
-  a.ctas = 1;
-  if (a.max_len >= kEvictLong)
-    while (a.ctas < kEvictMaxCtas && heads * a.ctas * 2 <= num_sms) a.ctas *= 2;
+  a.ctas = evict_ctas(heads, a.max_len, clusters);
   a.words = ((a.max_len + 31) / 32 + a.ctas - 1) / a.ctas;
   a.keys_in_smem = a.words * 32 <= kEvictSmemKeys;
   // a step that is a few slots over: no second launch (unless out_lens is lens, which other blocks

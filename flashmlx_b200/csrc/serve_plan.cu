@@ -69,6 +69,24 @@ size_t cache_attn_bound(int B, int L, int nh, int nkv, int d, int prefix_max, in
          (num_sms + key_items) * kTcWeightParts * kTcKeys * sizeof(float) + (prefix_max >= 0 ? 4096 : 0);
 }
 
+// Long caches of few heads: a cluster of four or two CTAs shares a head's slots, since one SM's passes take
+// longer than what a cluster adds (barriers between the passes, ~4 us).  GPU time of one / two / four CTAs a
+// head, 32 heads of 128, inputs out of cache; in place with one row to move, and cut to 2048 elsewhere:
+//   10240 slots  17.3 / 21.3 / 19.9 us  and  40.2 / 42.3 / 41.3 us
+//   12288        19.7 / 23.0 / 19.9          43.0 / 43.9 / 41.8
+//   14336        22.7 / 24.5 / 21.2          46.0 / 45.4 / 42.2
+//   16384        20.6 / 21.3 / 21.2          43.5 / 42.4 / 42.2
+//   18432        23.2 / 23.1 / 22.7          46.4 / 44.0 / 43.8
+//   24576        28.7 / 27.7 / 24.6          51.8 / 49.0 / 46.1
+// (Eight CTAs of 16 heads of 65536: 57 where four take 38 and one 112.)  Only as many clusters as run at a
+// time: SMs come in groups that clusters do not span, so that 33 of four fit 148 SMs, and 34 heads of 20480
+// take 41 us in two rounds of them, 25 in clusters of two.
+constexpr int kEvictFours = 14336, kEvictTwos = 18432;
+
+int evict_ctas(int64_t heads, int max_len, const EvictClusters& c) {
+  return max_len >= kEvictFours && heads <= c.fours ? 4 : max_len >= kEvictTwos && heads <= c.twos ? 2 : 1;
+}
+
 bool cache_attn_fits(const CacheAttnPlan& p, int B, int L, int nh, int nkv, int prefix_len, int max_len, bool scored) {
   // as many as a kernel's order has places when every length is max_len and nothing is hidden; in
   // doubles, which the products of the largest sizes cannot pass

@@ -253,6 +253,11 @@ int main() {
       if (std::scanf("%d %d %d %d %d %d %d %d %d", &B, &L, &nh, &nkv, &d, &prefix, &own, &scored, &max_len) != 9) return 1;
       const fm::CacheAttnPlan p = fm::cache_attn_plan(B, L, nh, nkv, d, prefix, own != 0, scored != 0, max_len, 148);
       std::printf("%d\n", fm::cache_attn_fits(p, B, L, nh, nkv, prefix, max_len, scored != 0));
+    } else if (!std::strcmp(what, "evict")) {
+      int heads, max_len;
+      fm::EvictClusters c;
+      if (std::scanf("%d %d %d %d", &heads, &max_len, &c.twos, &c.fours) != 4) return 1;
+      std::printf("%d\n", fm::evict_ctas(heads, max_len, c));
     } else if (!std::strcmp(what, "order")) {
       if (!order()) return 1;
     } else if (!std::strcmp(what, "cut")) {

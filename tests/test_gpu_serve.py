@@ -1014,3 +1014,63 @@ def test_the_recent_window_counts_from_the_newest_position(M, lens, lo, in_place
             top = int(pos[b, h, :lens[b]].max())
             here = set(pos[b, h, :lens[b]].tolist())
             assert {p for p in here if p > top - recent} <= held_at
+
+
+@pytest.mark.parametrize("B,nkv,M,lens,budget,recent", [
+    (2, 3, 18500, [18500, 9001], 2048, 512), (5, 8, 20000, [20000, 4097, 0, 2049, 1], 2048, 0),  # four, two CTAs a head
+    (1, 1, 40000, [39990], 20001, 77), (38, 2, 18432, [18432 - 450 * i for i in range(38)], 2000, 99),  # one: too many heads
+    (2, 2, 19000, [19000, 18890], 18875, 16), (17, 2, 18600, [18600] * 16 + [5], 18480, 16)])  # a few moves
+@pytest.mark.parametrize("how", ["in place", "lens is lens_out", "elsewhere"])
+def test_evict_long_caches(B, nkv, M, lens, budget, recent, how):
+    from flashmlx_b200 import ops
+    g, d = torch.Generator().manual_seed(M), 8
+    acc = (torch.rand(B, nkv, M, generator=g) * 500).floor()
+    pos = torch.stack([torch.randperm(3 * M, generator=g)[:M] for _ in range(B * nkv)]).view(B, nkv, M).int()
+    dev = [rnd(260, B, nkv, M, d), rnd(261, B, nkv, M, d), acc.cuda(), pos.cuda()]
+    host = [t.cpu().clone() for t in dev]
+    inside = how != "elsewhere"
+    out = dev if inside else [torch.zeros(B, nkv, budget, *t.shape[3:], dtype=t.dtype, device="cuda") for t in dev]
+    to = host if inside else [torch.zeros(t.shape, dtype=t.dtype) for t in out]
+    want = R.evict(*host, lens, budget, 4, recent, to)
+    n = i32(lens)
+    got = ops.cache_evict(*dev[:3], n, budget, sinks=4, recent=recent, positions=dev[3], out=None if inside else tuple(out),
+                          lens_out=n if how == "lens is lens_out" else None)
+    assert got.tolist() == want
+    for x, y in zip(out, to):
+        assert torch.equal(x.cpu(), y)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_a_captured_eviction_of_a_long_cache(in_place):
+    """The cluster's kernel in a graph replayed over other lengths and weights."""
+    from flashmlx_b200 import ops
+    B, nkv, M, budget, d = 2, 2, 20000, 700, 8
+    h = ops.Handle()
+    k, v = rnd(280, B, nkv, M, d), rnd(281, B, nkv, M, d)
+    acc, lens = torch.zeros(B, nkv, M, device="cuda"), i32([M, M])
+    dev = [k.clone(), v.clone(), acc.clone()]
+    out = dev if in_place else [torch.zeros(B, nkv, budget, d, dtype=BF, device="cuda") for _ in range(2)] + \
+        [torch.zeros(B, nkv, budget, device="cuda")]
+
+    def step():
+        for x, y in zip(dev, (k, v, acc)):
+            x.copy_(y)
+        return ops.cache_evict(*dev, lens, budget, sinks=4, recent=50, out=None if in_place else (*out, None), handle=h)
+
+    step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        n = step()
+    for i, now in enumerate([[M, 9000], [3, 19001], [701, 0]]):
+        acc.copy_(torch.rand(B, nkv, M, generator=torch.Generator().manual_seed(i)))
+        lens.copy_(i32(now))
+        for x in out if not in_place else []:
+            x.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        host = [x.cpu().clone() for x in (k, v, acc)]
+        to = host if in_place else [torch.zeros(x.shape, dtype=x.dtype) for x in out]
+        assert n.tolist() == R.evict(*host, None, now, budget, 4, 50, [*to, None])
+        for x, y in zip(out, to):
+            assert torch.equal(x.cpu(), y), f"replay {i}"
+    h.sync()

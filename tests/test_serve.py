@@ -191,3 +191,10 @@ def test_attention_work_is_cut_without_gaps(plan, seed):
 
 def test_division_by_multiplication_is_exact(plan):
     assert plan(["divide 200000"]) == ["ok"]
+
+
+def test_evictions_share_a_head_among_as_many_ctas_as_run_at_a_time(plan):
+    """148 SMs hold 74 clusters of two and 33 of four: the 34th head would wait for a second round."""
+    lines = [f"evict {heads} {n} 74 33" for heads, n in [(1, 14335), (1, 14336), (33, 2 ** 20), (34, 18431), (34, 18432), (74, 20480), (75, 20480)]]
+    assert plan(lines) == ["1", "4", "4", "1", "2", "2", "1"]
+    assert plan(["evict 1 20480 0 0", "evict 5 20480 5 4"]) == ["1", "2"]
