@@ -837,7 +837,11 @@ constexpr int kEvictThreads = 1024;
 constexpr int kEvictSmemKeys = 40960;  // 160 KB
 constexpr int kEvictCopies = 8;        // of the counts: a lane's own of eight, so that a warp whose keys are
                                        // alike does not add to one word 32 times
-constexpr int kEvictFused = 64;        // moves of a head that the select kernel makes itself
+// Where no head can have more moves than this, the select kernel makes them itself.  In place, rows of
+// 128, inputs out of cache, GPU time with two launches / one: 32 heads that move one row 12.9 / 10.9 us
+// whatever the limit, that move as many as it allows 64: 15.0 / 13.7, 128: 15.9 / 15.4, 256: 16.5 / 18.6,
+// 512: 18.6 / 24.4 (128 of 4 heads: 14.8 / 14.5, of 128 heads 18.8 / 16.9, of 512 heads 61.4 / 60.8).
+constexpr int kEvictFused = 128;
 
 namespace {
 

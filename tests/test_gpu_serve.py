@@ -1040,6 +1040,24 @@ def test_evict_long_caches(B, nkv, M, lens, budget, recent, how):
         assert torch.equal(x.cpu(), y)
 
 
+@pytest.mark.parametrize("slack", [1, 63, 64, 65, 127, 128, 129, 300])
+@pytest.mark.parametrize("heads", [(3, 2), (40, 4)])
+def test_evict_up_to_the_slack_of_a_cache(slack, heads):
+    """Around the number of moves that the selecting kernel makes itself: all of them, and one."""
+    from flashmlx_b200 import ops
+    (B, nkv), budget, d = heads, 400, 16
+    M = budget + slack
+    lens = [budget + slack if i % 2 == 0 else budget + 1 for i in range(B)]
+    acc = torch.rand(B, nkv, M, generator=torch.Generator().manual_seed(slack))
+    acc[:, :, budget:] += 1.0  # the late slots stay, so that all of them move
+    dev = [rnd(270, B, nkv, M, d), rnd(271, B, nkv, M, d), acc.cuda()]
+    host = [t.cpu().clone() for t in dev]
+    want = R.evict(*host, None, lens, budget, 2, 0, [*host, None])
+    assert ops.cache_evict(*dev, i32(lens), budget, sinks=2).tolist() == want
+    for x, y in zip(dev, host):
+        assert torch.equal(x.cpu(), y)
+
+
 @pytest.mark.parametrize("in_place", [True, False])
 def test_a_captured_eviction_of_a_long_cache(in_place):
     """The cluster's kernel in a graph replayed over other lengths and weights."""
