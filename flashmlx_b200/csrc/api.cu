@@ -275,6 +275,14 @@ struct OnDevice {
   }
 };
 
+// A capture on another stream (of any thread) goes on although this scope allocates and waits: nothing of it
+// is part of that capture.
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 // The serving calls' workspace: at least `bytes`, and their error word (sv_err).  Blocks are
 // never freed before fm_destroy, and each is at least half as large again as the last.
 int ensure_sv(fm_handle* h, size_t bytes) {
@@ -289,6 +297,7 @@ int ensure_sv(fm_handle* h, size_t bytes) {
     return set_err(h, FM_EINVAL, "the workspace would have to grow during a capture: reserve it first");
   const size_t want = ws_alloc_bytes(std::max(bytes, h->sv_bytes + h->sv_bytes / 2) + kCtrlBytes);
   uint8_t* p = nullptr;
+  const RelaxedCapture relaxed;
   e = cudaMalloc(&p, want);
   if (e != cudaSuccess) {
     cudaGetLastError();

@@ -1092,3 +1092,26 @@ def test_a_captured_eviction_of_a_long_cache(in_place):
         for x, y in zip(out, to):
             assert torch.equal(x.cpu(), y), f"replay {i}"
     h.sync()
+
+
+def test_a_workspace_grows_beside_a_capture():
+    """An eager call on another stream allocates its handle's workspace while torch captures: the capture goes on."""
+    from flashmlx_b200 import _lib, ops
+    lens = [300, 20, 150]
+    q, (ck, cv), n = rnd(290, 3, 1, 8, 64), caches(291, 3, 2, 300, 64, lens), i32(lens)
+    want = ops.attention_prefix(q, None, None, ck, cv, n)
+    side, g, out, x = torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.zeros_like(q), torch.zeros(4, device="cuda")
+    h, cfg = ops.Handle(), _lib.CacheAttnConfig(8, 2, 64, 300, 0, 0, 0.0)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        x.add_(1.0)
+        with torch.cuda.stream(side):
+            h.bind_current()
+            st = h.lib.fm_attention_prefix(h.h, _lib.C.byref(cfg), q.data_ptr(), None, None, 0, ck.data_ptr(), cv.data_ptr(),
+                                           n.data_ptr(), 3, 1, out.data_ptr())
+        x.add_(1.0)
+    h.check(st)
+    h.sync()
+    assert torch.equal(out, want)
+    g.replay()
+    assert x.tolist() == [2.0] * 4
