@@ -10,6 +10,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <mutex>
 #include <cstdio>
@@ -2195,12 +2196,14 @@ int serve_ready(fm_handle* h) {
 
 size_t evict_bytes(int64_t heads, int64_t budget) { return align_up(sizeof(int32_t) * heads * 2 * budget, 256) + sizeof(int32_t) * heads * 2; }
 
+constexpr double kLog2e = 1.4426950408889634;
+
 int check_cache_attn(fm_handle* h, const fm_cache_attn_config* c, int B, int L, int prefix_len) {
   if (!c) return set_err(h, FM_EINVAL, "null config");
   if (c->n_heads <= 0 || c->n_kv_heads <= 0 || c->n_heads % c->n_kv_heads || c->max_len < 0 || c->prefix_max < 0)
     return set_err(h, FM_EINVAL, "bad attention config");
   if (c->head_dim != 64 && c->head_dim != 128) return set_err(h, FM_EUNSUPPORTED, "head_dim must be 64 or 128");
-  if (!std::isfinite(c->scale)) return set_err(h, FM_EINVAL, "bad scale");
+  if (!(std::fabs(c->scale * kLog2e) <= FLT_MAX)) return set_err(h, FM_EINVAL, "bad scale");  // (0 times infinity is NaN)
   if (c->q_ld < 0 || c->q_ld % 8 || (c->q_ld > 0 && c->q_ld < static_cast<int64_t>(c->n_heads) * c->head_dim))
     return set_err(h, FM_EINVAL, "q_ld must be 0 or a multiple of 8 of at least n_heads * head_dim");
   if (B < 0 || L < 0 || prefix_len < 0) return set_err(h, FM_EINVAL, "negative B, L or prefix_len");
@@ -2273,7 +2276,7 @@ int cache_attn(fm_handle* h, const fm_cache_attn_config* c, const uint16_t* q, c
   a.split_own = p.rt_s > 0;
   a.after_tc = p.tc_p || p.tc_s;
   const double scale = c->scale != 0.f ? c->scale : 1.0 / std::sqrt(static_cast<double>(d));
-  a.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  a.scale_log2 = static_cast<float>(scale * kLog2e);
   a.merge_rows = p.merge_rows;
   a.rt_p = p.rt_p;
   a.rt_s = p.rt_s;

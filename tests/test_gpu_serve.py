@@ -1115,3 +1115,14 @@ def test_a_workspace_grows_beside_a_capture():
     assert torch.equal(out, want)
     g.replay()
     assert x.tolist() == [2.0] * 4
+
+
+def test_scales_whose_scores_have_no_number_are_refused():
+    """The scale times log2(e) has to be a number: beyond, a score of 0 would be 0 times infinity."""
+    from flashmlx_b200 import _lib, ops
+    q, (ck, cv), n = torch.zeros(2, 1, 4, 64, dtype=BF, device="cuda"), caches(292, 2, 2, 16, 64, [9, 16]), i32([9, 16])
+    for scale in (3.0e38, -2.4e38):
+        refused(lambda: ops.attention_prefix(q, None, None, ck, cv, n, scale=scale), _lib.FM_EINVAL)
+    out = ops.attention_prefix(q, None, None, ck, cv, n, scale=2.3e38)  # scores of 0: the mean of the values
+    want, tol, _, _ = R.attention(q, ck, cv, [9, 16])
+    held(out, want, tol)
