@@ -2530,8 +2530,7 @@ int fm_serve_reserve(fm_handle* h, const fm_cache_attn_config* cfg, int B, int L
   const int rc = check_cache_attn(h, cfg, B, L, 0);
   if (rc != FM_OK) return rc;
   const OnDevice on(h);
-  const size_t attn = fm::cache_attn_bound(B, L, cfg->n_heads, cfg->n_kv_heads, cfg->head_dim, cfg->prefix_max,
-                                           cfg->max_len, h->num_sms);
+  const size_t attn = fm::cache_attn_bound(B, L, cfg->n_heads, cfg->n_kv_heads, cfg->head_dim, cfg->max_len, h->num_sms);
   return ensure_sv(h, std::max(attn, evict_bytes(static_cast<int64_t>(B) * cfg->n_kv_heads, cfg->max_len)));
 }
 

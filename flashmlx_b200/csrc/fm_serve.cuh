@@ -365,8 +365,8 @@ struct CacheAttnPlan {
 CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_len, bool own, bool scored, int max_len,
                               int num_sms);
 
-// At least what any call of up to B sequences of L tokens over such a prefix and caches needs.
-size_t cache_attn_bound(int B, int L, int nh, int nkv, int d, int prefix_max, int max_len, int num_sms);
+// At least what any call of up to B sequences of L tokens over such caches and any prefix needs.
+size_t cache_attn_bound(int B, int L, int nh, int nkv, int d, int max_len, int num_sms);
 
 // One handle's serving calls share a workspace, so a call on another stream than the calls before it
 // waits for them.  Streams are followed, not calls: `busy` says that calls were made on the bound

@@ -53,9 +53,9 @@ CacheAttnPlan cache_attn_plan(int B, int L, int nh, int nkv, int d, int prefix_l
   return p;
 }
 
-size_t cache_attn_bound(int B, int L, int nh, int nkv, int d, int prefix_max, int max_len, int num_sms) {
-  // every part at its largest: both kernels' pieces, the log sums, the scores of one row tile, the
-  // slot weights' sums
+size_t cache_attn_bound(int B, int L, int nh, int nkv, int d, int max_len, int num_sms) {
+  // every part at its largest: both kernels' pieces (which the number of keys does not change), the log sums,
+  // the scores of one row tile, the slot weights' sums, and 4096 for the parts' alignment
   const size_t group = nh / nkv, rows_s = L * group, rows_p = B * rows_s;
   auto up = [](size_t n, size_t m) { return (n + m - 1) / m; };
   const size_t split = num_sms * kAttnBlocksPerSm * kAttnWarps +
@@ -66,7 +66,7 @@ size_t cache_attn_bound(int B, int L, int nh, int nkv, int d, int prefix_max, in
   const size_t key_items = static_cast<size_t>(B) * nkv * up(max_len, kTcKeys);
   return piece_rows * (d * sizeof(float) + sizeof(float2)) + sizeof(float) * rows_p * nkv +
          sizeof(float) * B * nkv * std::min<size_t>(rows_s, kAttnRowTile) * (max_len + 3) +
-         (num_sms + key_items) * kTcWeightParts * kTcKeys * sizeof(float) + (prefix_max >= 0 ? 4096 : 0);
+         (num_sms + key_items) * kTcWeightParts * kTcKeys * sizeof(float) + 4096;
 }
 
 // Long caches of few heads: a cluster of four or two CTAs shares a head's slots, since one SM's passes take

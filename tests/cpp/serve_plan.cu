@@ -216,7 +216,7 @@ bool cuts() {
       EXPECT(p.bytes >= p.off_w + slots * fm::kTcWeightParts * fm::kTcKeys * 4)
       if (!cut(w, slots, false)) return false;
     }
-    EXPECT(fm::cache_attn_bound(B, L, nh, nkv, d, prefix, max_len, sms) >= p.bytes)
+    EXPECT(fm::cache_attn_bound(B, L, nh, nkv, d, max_len, sms) >= p.bytes)
   }
   std::printf("ok\n");
   return true;
