@@ -33,7 +33,8 @@
 //
 // Bound: the exponentials of the two streams, which fall into step (64 keys: ~1200 of 1700 cycles
 // with both at the special-function units, 1063 at their rate).  A prompt of 4096 tokens, 32/4 heads of
-// 128: 146 us, 0.94 PFLOP/s; 64 sequences' rows over 32768 shared keys: 45 us.
+// 128: 146 us, 0.94 PFLOP/s; 64 sequences' rows over 32768 shared keys: 45 us, of which a worker has 11,000
+// cycles before its first S (3200 launch and cut, 3900 Q, 3900 S), 30 steps of ~1750, 8500 for O.
 #include "fm_serve.cuh"
 
 namespace fm {
@@ -303,7 +304,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
               const float p0 = ex2(fmaf(v[2 * c], a.scale_log2, base)), p1 = ex2(fmaf(v[2 * c + 1], a.scale_log2, base));
               sum4[2 * c & 3] += p0;
               sum4[2 * c + 1 & 3] += p1;
-              pw[c] = pack_bf16x2(p0, p1);  // the tensor product's operand: one rounding to bf16
+              // the tensor product's operand, one rounding to bf16: outputs are off by 0.0023 (root mean
+              // square) where P in fp32 gives 0.0017, their own rounding; two parts would double P V
+              pw[c] = pack_bf16x2(p0, p1);
             }
             tmem_st32(t_b, w);
             sum = (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);

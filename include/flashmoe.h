@@ -405,8 +405,9 @@ typedef struct fm_cache_attn_config {
  * [n_kv_heads, prefix_max, head_dim] rows [0, prefix_len), and each sequence's own cache:
  * token l of sequence b sees the whole prefix and the slots j <= lens[b] - L + l, lens[b]
  * counting the new tokens.  A slot reaches only the tokens that see it, whatever it holds (infinities
- * and NaN too).  A token that sees nothing (no prefix, and lens[b] too short) gives zeros.  out is [B * L, n_heads * head_dim].  prefix_len may be 0 (prefix pointers NULL); lens
- * NULL means no own caches (cache pointers NULL). */
+ * and NaN too).  A token that sees nothing (no prefix, and lens[b] too short) gives zeros.  out
+ * is [B * L, n_heads * head_dim].  prefix_len may be 0 (prefix pointers NULL); lens NULL means no
+ * own caches (cache pointers NULL). */
 FM_API int fm_attention_prefix(fm_handle* h, const fm_cache_attn_config* cfg, const uint16_t* q,
                                const uint16_t* prefix_k, const uint16_t* prefix_v, int prefix_len,
                                const uint16_t* cache_k, const uint16_t* cache_v, const int32_t* lens, int B, int L,
@@ -437,7 +438,8 @@ typedef struct fm_evict_config {
  * below n take the slots that stay from n on, both in ascending order -- so a step that is
  * one slot over moves one row.  k, v, acc and position of a slot move together; out_lens[b]
  * = n (out_lens may be lens).  In place when the outputs are the inputs (out_max_len ==
- * max_len then); otherwise every slot that stays is copied into the outputs, which may not
+ * max_len then; one launch where out_lens is apart from lens and max_len - budget at most 128,
+ * else two); otherwise every slot that stays is copied into the outputs, which may not
  * overlap the inputs.  Slots from n on are left as they were.  out_positions may be NULL when
  * positions is. */
 FM_API int fm_cache_evict(fm_handle* h, const fm_evict_config* cfg, const uint16_t* cache_k, const uint16_t* cache_v,
@@ -446,7 +448,9 @@ FM_API int fm_cache_evict(fm_handle* h, const fm_evict_config* cfg, const uint16
 
 /* Sizes the workspace for fm_attention_prefix / fm_attention_scored calls of up to B sequences
  * of up to L tokens over cfg's caches and up to prefix_max rows, and for fm_cache_evict of such a
- * batch, so that later calls do not allocate. */
+ * batch, so that later calls do not allocate.  fm_attention_scored of up to 16 query rows to a kv
+ * head (L * n_heads / n_kv_heads) keeps 4 bytes for each of them and each of the B * n_kv_heads *
+ * max_len slots, whatever lens: 64 sequences of 131072 slots with 32 heads take 1 GiB. */
 FM_API int fm_serve_reserve(fm_handle* h, const fm_cache_attn_config* cfg, int B, int L);
 
 /* Expert parallelism ------------------------------------------------------------
