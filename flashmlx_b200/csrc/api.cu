@@ -321,17 +321,16 @@ int ensure_sv(fm_handle* h, size_t bytes) {
 // the stream calls of StreamOrder
 struct StreamCalls {
   fm_handle* h;
-  cudaError_t capturing(cudaStream_t s, bool* yes) {
+  // the capture that s is part of, 0: none
+  cudaError_t capture(cudaStream_t s, uint64_t* id) {
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    cudaError_t e = cudaStreamIsCapturing(s, &cap);
-    // the legacy stream while a stream that it would wait for is being captured
-    const bool implicit = e == cudaErrorStreamCaptureImplicit;
-    if (implicit) {
-      cudaGetLastError();
-      e = cudaSuccess;
-    }
-    *yes = implicit || cap != cudaStreamCaptureStatusNone;
-    return e;
+    unsigned long long n = 0;
+    const cudaError_t e = cudaStreamGetCaptureInfo(s, &cap, &n);
+    *id = cap == cudaStreamCaptureStatusNone ? 0 : n;
+    if (e != cudaErrorStreamCaptureImplicit) return e;
+    cudaGetLastError();  // the legacy stream, while a stream that it would wait for is being captured
+    *id = ~0ull;
+    return cudaSuccess;
   }
   cudaError_t wait(cudaStream_t now, cudaStream_t s) {
     cudaError_t e = cudaSuccess;

@@ -371,9 +371,9 @@ size_t cache_attn_bound(int B, int L, int nh, int nkv, int d, int max_len, int n
 // One handle's serving calls share a workspace, so a call on another stream than the calls before it
 // waits for them.  Streams are followed, not calls: `busy` says that calls were made on the bound
 // stream, `behind` holds the streams whose calls the bound one has yet to wait for.  What a capture
-// records runs later, and its replays are the caller's to order: in a capture nothing is waited for,
-// and a stream that is being captured stays `behind`.  Cuda has the two stream calls, so that tests
-// can do without a device.
+// records runs later, and its replays are the caller's to order: a stream waits only for streams of its
+// own capture (whose branches a replay would run side by side), and one that is being captured stays
+// `behind`.  Cuda has the two stream calls, so that tests can do without a device.
 class StreamOrder {
  public:
   // the handle is bound to `now` instead of `before`
@@ -390,13 +390,13 @@ class StreamOrder {
   template <class Cuda>
   cudaError_t join(cudaStream_t now, Cuda&& cuda) {
     if (behind_.empty()) return cudaSuccess;
-    bool capturing = false;
-    cudaError_t e = cuda.capturing(now, &capturing);
-    if (capturing) return e;
+    uint64_t mine = 0, its = 0;
+    cudaError_t e = cuda.capture(now, &mine);
     for (size_t i = 0; i < behind_.size() && e == cudaSuccess;) {
       const cudaStream_t s = behind_[i];
-      if (s != now && (e = cuda.capturing(s, &capturing)) == cudaSuccess && !capturing) e = cuda.wait(now, s);
-      if (s == now || (e == cudaSuccess && !capturing)) behind_.erase(behind_.begin() + i);
+      if (s != now) e = cuda.capture(s, &its);
+      if (e == cudaSuccess && s != now && its == mine) e = cuda.wait(now, s);
+      if (s == now || (e == cudaSuccess && its == 0 && mine == 0)) behind_.erase(behind_.begin() + i);
       else ++i;
     }
     return e;

@@ -346,9 +346,9 @@ FM_API int fm_argmax(fm_handle* h, const uint16_t* logits, int64_t T, int64_t V,
  * before the capture).  Calls of one handle share the workspace, so calls of it on several
  * streams wait for one another: on a stream bound by fm_set_stream, the first of these calls
  * (or fm_sync_status) waits on the GPU for those made on the streams bound before, which must
- * exist until then unless fm_sync_status came in between.  Captured calls run at a replay, which no
- * call waits for: replays must overlap neither calls of the handle nor other replays of graphs
- * captured from it.  What is to overlap needs a handle each.  A handle is used by one thread at a
+ * exist until then unless fm_sync_status came in between.  So do calls on branches of one capture.
+ * Captured calls run at a replay, which no call waits for: replays must overlap neither calls of the
+ * handle nor other replays of graphs captured from it.  What is to overlap needs a handle each.  A handle is used by one thread at a
  * time. */
 #define FM_ROPE_UNSCALED 0 /* theta^(-2i/r) */
 #define FM_ROPE_LINEAR 1   /* every frequency / factor (position interpolation) */

@@ -17,10 +17,10 @@ cudaStream_t stream(int i) { return reinterpret_cast<cudaStream_t>(static_cast<i
 
 // the calls that StreamOrder makes, written down
 struct Calls {
-  std::set<cudaStream_t> captured;
+  std::map<cudaStream_t, uint64_t> captured;
   int fails = 0;  // the n-th next wait fails
-  cudaError_t capturing(cudaStream_t s, bool* yes) {
-    *yes = captured.count(s) > 0;
+  cudaError_t capture(cudaStream_t s, uint64_t* id) {
+    *id = captured.count(s) ? captured[s] : 0;
     return cudaSuccess;
   }
   cudaError_t wait(cudaStream_t now, cudaStream_t s) {
@@ -30,10 +30,11 @@ struct Calls {
   }
 };
 
-// order <n>, n steps: b<stream> bind, c call (join, mark), s sync (join, settle), +<stream> / -<stream> a
-// capture begins / ends, f<n> the n-th next wait fails; answers the waits of the calls
+// order <n>, n steps: b<stream> bind, c call (join, mark), s sync (join, settle), +<stream> a capture begins,
+// *<stream> the stream joins the last one, -<stream> it is captured no longer, f<n> the n-th next wait
+// fails; answers the waits of the calls
 bool order() {
-  int n, now = 0;
+  int n, now = 0, captures = 0;
   fm::StreamOrder o;
   Calls cuda;
   if (std::scanf("%d", &n) != 1) return false;
@@ -51,7 +52,9 @@ bool order() {
       else if (what[0] == 'c') o.mark();
       else o.settle();
     } else if (what[0] == '+') {
-      cuda.captured.insert(stream(to));
+      cuda.captured[stream(to)] = ++captures;
+    } else if (what[0] == '*') {
+      cuda.captured[stream(to)] = captures;
     } else if (what[0] == '-') {
       cuda.captured.erase(stream(to));
     } else {

@@ -1126,3 +1126,43 @@ def test_scales_whose_scores_have_no_number_are_refused():
     out = ops.attention_prefix(q, None, None, ck, cv, n, scale=2.3e38)  # scores of 0: the mean of the values
     want, tol, _, _ = R.attention(q, ck, cv, [9, 16])
     held(out, want, tol)
+
+
+def test_branches_of_a_capture_that_share_a_handle_take_turns():
+    """Two streams forked inside a capture, calls on both without a handle given: a replay runs them one after the
+    other."""
+    from flashmlx_b200 import ops
+    lens = [3000, 500, 2100, 77]
+    n, data = i32(lens), []
+    for i in range(2):
+        q, acc = rnd(300 + i, 4, 6, 8, 128), torch.rand(4, 2, 3000, generator=torch.Generator().manual_seed(i)).cuda()
+        data.append((q, *caches(302 + 2 * i, 4, 2, 3000, 128, lens), acc))
+
+    def work(q, ck, cv, acc):
+        ck, cv, acc = ck.clone(), cv.clone(), acc.clone()
+        out = ops.attention_scored(q, ck, cv, n, acc)
+        weights = acc.clone()
+        return [out, weights, ops.cache_evict(ck, cv, acc, n, 1500, sinks=4, recent=64), ck, cv, acc]
+
+    want = [work(*d) for d in data]
+    ops.synchronize()
+    g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g):
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        got = []
+        for _ in range(2):
+            got.append((0, work(*data[0])))
+            with torch.cuda.stream(side):
+                got.append((1, work(*data[1])))
+        here.wait_stream(side)
+    for _ in range(3):
+        for _, outs in got:
+            for t in outs:
+                t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        for i, outs in got:
+            for x, y in zip(outs, want[i]):
+                assert torch.equal(x.nan_to_num(nan=-7.0), y.nan_to_num(nan=-7.0))
+    ops.synchronize()

@@ -173,6 +173,8 @@ def test_counts_of_the_other_kernels_beyond_32_bits_are_refused(plan):
     ("c +0 c b1 c -0 c c", "| | | | 1<0 |"),                  # the stream of earlier calls is captured itself
     ("c b1 s b2 c", "| | 1<0 |"),                             # synchronized: nothing is in flight
     ("c b1 +0 s b2 c -0 c", "| | | | 2<0"),
+    ("+1 *2 b1 c b2 c c b1 c -1 -2 b2 c", "| | 2<1 | 2<1 | 1<2 | 2<1"),  # branches of one capture
+    ("c b1 +1 c b2 +2 c b1 c -1 -2 c", "| | | | | 1<0 1<2"),    # two captures at a time
     ("c b1 c b2 f2 c c b1 c c", "| | 1<0 | 2<1 | | error | 1<2"),
     ("c b1 f1 c c", "| | error | 1<0"),                       # an error leaves it to be waited for
 ])
